@@ -340,6 +340,96 @@ int tq_attention_fwd_kv_noalloc(const uint16_t* q_rot, const float* q_proj,
                                 int64_t smk, void* out, int32_t out_dtype, int64_t sob,
                                 int64_t soh, int64_t sos, void* stream);
 
+/* ---- Pages of a compressed cache, and drafted tokens over them.  No counterpart in the reference,
+ * which keeps no cache between steps (patch.py:81).
+ *
+ * A layer's pool holds num_pages pages of page_size positions (a power of two from 32 to 2^20): six
+ * planes in the order key codes, key signs, key rn, key vn, value codes, value vn, each
+ * [num_pages, H, page_size] rows of the widths above, 16-byte aligned.  Calls over several layers
+ * take each plane as [layers, num_pages, H, page_size] rows.  Position j of sequence b is row
+ * j % page_size of page block_table[b * ld_table + j / page_size]; a row of the table holds
+ * table_width entries.  Tables, lengths and paths are int32 on the device and checked there before
+ * use: a row whose page is outside the pool (-1: no page) is neither read nor written. */
+
+/* Rows [B, H, S] of six contiguous planes to positions start[b] + s of the sequences (a negative
+ * start writes nothing for that sequence). */
+int tq_page_write(void* const* pool, void* const* rows, int32_t B, int32_t H, int32_t S,
+                  int32_t d, int32_t key_code_bits, int32_t val_bits, int64_t num_pages,
+                  int32_t page_size, const int32_t* block_table, int64_t ld_table,
+                  int32_t table_width, const int32_t* start, void* stream);
+
+/* Positions s < min(S, lengths[b]) to rows [B, H, S] of six contiguous planes; zeros behind, and
+ * where a position has no page. */
+int tq_page_read(void* const* pool, void* const* rows, int32_t B, int32_t H, int32_t S, int32_t d,
+                 int32_t key_code_bits, int32_t val_bits, int64_t num_pages, int32_t page_size,
+                 const int32_t* block_table, int64_t ld_table, int32_t table_width,
+                 const int32_t* lengths, void* stream);
+
+/* Page dst[i] := page src[i] in every layer, i < n.  No page may be both a source and a target, and
+ * none a target twice; pairs with an index outside the pool are left out. */
+int tq_page_copy(void* const* pool, int32_t layers, int32_t H, int32_t d, int32_t key_code_bits,
+                 int32_t val_bits, int64_t num_pages, int32_t page_size, const int32_t* src,
+                 const int32_t* dst, int32_t n, void* stream);
+
+/* The accepted path of T <= 64 drafted tokens at positions lengths[b] + i: position lengths[b] +
+ * path[b, i] moves to lengths[b] + i for i < count[b], in every layer (all rows of a sequence are
+ * read before the first is written); new_lengths[b] = lengths[b] + count[b].  Sequences with a
+ * negative length are left alone. */
+int tq_page_keep(void* const* pool, int32_t layers, int32_t B, int32_t H, int32_t T, int32_t d,
+                 int32_t key_code_bits, int32_t val_bits, int64_t num_pages, int32_t page_size,
+                 const int32_t* block_table, int64_t ld_table, int32_t table_width,
+                 const int32_t* lengths, const int32_t* path, const int32_t* count,
+                 int32_t* new_lengths, void* stream);
+
+/* Attention of T <= 64 drafted tokens per sequence over its pages: node i of sequence b is row
+ * lengths[b] + i (already written) and sees the lengths[b] cached positions, its ancestors and
+ * itself.  parents[b * ld_parents + i] is an earlier node or -1 (NULL: i - 1, a chain); any other
+ * value leaves the node without a place: it sees nothing (its output is zero) and nothing sees it.
+ * T = 1 is a decoding step.  A sequence whose length is negative or does not leave room for T
+ * positions in its table row gets zeros; a position without a page is not attended.  Scores,
+ * softmax and output as in tq_attention_fwd over the prepared queries [B, Hq, T, d] of
+ * tq_query_prep.  head_dim 64 or 128, bits 2-4 (value bits = bits), at most 2^24 positions per
+ * table row; queries, code planes, val_pit_split and workspace 16-byte aligned.  The keys are split over
+ * blocks by the lengths found on the device; the workspace (tq_tree_workspace_size bytes) holds the
+ * parts, and may be reused by the next call on the stream. */
+int tq_tree_attention(const uint16_t* q_rot, const float* q_proj, const uint8_t* key_codes,
+                      const uint8_t* key_signs, const uint16_t* key_rn, const uint16_t* key_vn,
+                      const uint16_t* key_centroids_f16, int32_t bits, const uint8_t* val_codes,
+                      const uint16_t* val_vn, const float* val_centroids,
+                      const uint16_t* val_pit_split, int64_t num_pages, int32_t page_size,
+                      const int32_t* block_table, int64_t ld_table, int32_t table_width,
+                      const int32_t* lengths, const int32_t* parents, int64_t ld_parents, int32_t B,
+                      int32_t Hq, int32_t Hkv, int32_t T, int32_t d, float coeff, float scale,
+                      void* out, int32_t out_dtype, int64_t sob, int64_t soh, int64_t sos,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of tq_tree_attention on the current device (0: shape not taken). */
+int64_t tq_tree_workspace_size(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t table_width,
+                               int32_t page_size, int32_t d, int32_t bits);
+
+/* Verification of drafted tokens.  Node 0 of a sequence is the last emitted token, node i > 0 a
+ * drafted child of parents[b * ld_parents + i] < i (NULL: i - 1); target_probs[b, c, :] (element
+ * strides stb, stt, 1) is the target's distribution p_c after node c.
+ *   without draft_probs, the children of c are tried in index order, and child i is accepted iff
+ *     uniforms[b, i] * (1 - sum of p_c over the earlier children's tokens) < p_c(tokens[b, i]);
+ *     a token that repeats an earlier sibling is rejected;
+ *   with draft_probs[b, c, :] (strides sdb, sdt, 1; c < T - 1; a chain, parents NULL), the
+ *     distribution q_c that token c + 1 was drawn from: accepted iff uniforms[b, i] * q(x) < p(x).
+ * From the root on, the walk goes to the first accepted child until a node has none.  path[b, :]:
+ * its nodes (the root first), then -1; count[b]: how many; next_token[b]: the first x with
+ * w(0) + ... + w(x) > uniforms[b, 0] * sum(w), w being what is left at the last node: p_c without
+ * the rejected tokens, or (p_c - q_c)+, or p_c where nothing was rejected.  Where nothing is left of
+ * a distribution it is drawn from p_c; where that has no positive entry either, next_token is -1.
+ * Sums are float64.  Nodes with other parents are never reached.  T <= 64, V < 2^30. */
+int tq_verify_drafts(const int64_t* tokens, const void* target_probs, int32_t dtype, int64_t stb,
+                     int64_t stt, const void* draft_probs, int64_t sdb, int64_t sdt,
+                     const float* uniforms, const int32_t* parents, int64_t ld_parents, int32_t B,
+                     int32_t T, int32_t V, int32_t* path, int32_t* count, int64_t* next_token,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of tq_verify_drafts. */
+int64_t tq_verify_workspace_size(int32_t B, int32_t V);
+
 /* TQ_NOALLOC_SCRATCH_BYTES as built into the library.  Utility; no reference counterpart. */
 int64_t tq_noalloc_scratch_bytes(void);
 

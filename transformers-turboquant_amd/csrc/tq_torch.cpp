@@ -21,6 +21,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <tuple>
+#include <utility>
 
 #include "tq_api.h"
 
@@ -780,6 +781,347 @@ Tensor cache_attend_meta(const Tensor& k, const Tensor& v, const Tensor& q, cons
                         mask, out_dtype, workspace);
 }
 
+// ---------------------------------------------------------------- pages of a compressed cache
+// A layer's pool: the six planes [pages, H, page_size, (width)], or with `stacked` every layer's,
+// [layers, pages, H, page_size, (width)].  Checked as a whole: dtypes, contiguity, one geometry.
+struct Pool {
+  const Tensor *kcodes, *ksigns, *krn, *kvn, *vcodes, *vvn;
+  int64_t layers = 1, pages = 0, H = 0, P = 0, D = 0, key_code_bits = 0, val_bits = 0;
+
+  void check(const Checker& c, bool stacked) {
+    const int64_t lead = stacked ? 1 : 0;
+    TORCH_CHECK(kvn->dim() == 3 + lead, c.op, ": pool norm planes must be [", stacked ? "layers, " : "",
+                "pages, H, page_size], got ", kvn->sizes());
+    layers = stacked ? kvn->size(0) : 1;
+    pages = kvn->size(lead);
+    H = kvn->size(lead + 1);
+    P = kvn->size(lead + 2);
+    TORCH_CHECK(P >= 32 && P <= (1 << 20) && (P & (P - 1)) == 0, c.op,
+                ": page_size must be a power of two from 32 to 2^20, got ", P);
+    TORCH_CHECK(pages >= 1 && H >= 1 && pages < (int64_t{1} << 31), c.op, ": a pool needs pages and heads, got ", kvn->sizes());
+    auto wide = [&](const Tensor& t, const char* name) {
+      TORCH_CHECK(t.dim() == 4 + lead && t.size(-1) >= 1, c.op, ": ", name, " must be [", stacked ? "layers, " : "",
+                  "pages, H, page_size, bytes], got ", t.sizes());
+      c.plane(t, name, at::kByte, layers * pages * H * P, t.size(-1));
+      TORCH_CHECK(t.sizes().slice(0, 3 + lead) == kvn->sizes(), c.op, ": ", name, " ", t.sizes(),
+                  " has another geometry than the norms ", kvn->sizes());
+    };
+    wide(*kcodes, "pool key codes");
+    wide(*ksigns, "pool key signs");
+    wide(*vcodes, "pool value codes");
+    const std::pair<const Tensor*, const char*> norms[] = {
+        {krn, "pool residual norms"}, {kvn, "pool key norms"}, {vvn, "pool value norms"}};
+    for (const auto& n : norms) {
+      c.plane(*n.first, n.second, at::kHalf, layers * pages * H * P);
+      TORCH_CHECK(n.first->sizes() == kvn->sizes(), c.op, ": ", n.second, " ", n.first->sizes(),
+                  " has another geometry than ", kvn->sizes());
+    }
+    D = ksigns->size(-1) * 8;
+    key_code_bits = kcodes->size(-1) * 8 / D;
+    val_bits = vcodes->size(-1) * 8 / D;
+    TORCH_CHECK(D <= 256 && key_code_bits >= 1 && key_code_bits <= 8 && val_bits >= 1 && val_bits <= 8 &&
+                    out_cols(D, key_code_bits) == kcodes->size(-1) && out_cols(D, val_bits) == vcodes->size(-1),
+                c.op, ": rows of ", kcodes->size(-1), ", ", ksigns->size(-1), " and ", vcodes->size(-1),
+                " bytes are no codes of one head_dim");
+  }
+  void pointers(void* (&p)[6]) const {
+    const Tensor* t[6] = {kcodes, ksigns, krn, kvn, vcodes, vvn};
+    for (int i = 0; i < 6; ++i) p[i] = t[i]->data_ptr();
+  }
+};
+
+void check_index(const Checker& c, const Tensor& t, const char* name, at::IntArrayRef shape) {
+  c.same_device(t, name);
+  TORCH_CHECK(t.scalar_type() == at::kInt, c.op, ": ", name, " must be int32, got ", t.scalar_type());
+  TORCH_CHECK(t.sizes() == shape, c.op, ": ", name, " must be ", shape, ", got ", t.sizes());
+  TORCH_CHECK(t.is_contiguous(), c.op, ": ", name, " must be contiguous");
+}
+void check_table(const Checker& c, const Tensor& table) {
+  TORCH_CHECK(table.dim() == 2, c.op, ": block_table must be [B, pages of a sequence], got ", table.sizes());
+  check_index(c, table, "block_table", table.sizes());
+}
+int32_t i32(int64_t v) { return static_cast<int32_t>(v); }
+
+void page_write_meta(const Tensor& kcodes, const Tensor& ksigns, const Tensor& krn, const Tensor& kvn, const Tensor& vcodes,
+                     const Tensor& vvn, const Tensor& pkcodes, const Tensor& pksigns, const Tensor& pkrn, const Tensor& pkvn,
+                     const Tensor& pvcodes, const Tensor& pvvn, const Tensor& table, const Tensor& start, int64_t S) {
+  const Checker c{"tq::page_write", pkvn.device()};
+  Pool pool{&pkcodes, &pksigns, &pkrn, &pkvn, &pvcodes, &pvvn};
+  pool.check(c, false);
+  check_table(c, table);
+  check_index(c, start, "start", {table.size(0)});
+  TORCH_CHECK(S >= 0 && S < (int64_t{1} << 31), c.op, ": bad row count ", S);
+  const int64_t rows = table.size(0) * pool.H * S;
+  auto same = [&](const Tensor& t, const char* name, at::ScalarType dt, int64_t width) {
+    c.plane(t, name, dt, rows, width);
+    TORCH_CHECK(t.numel() == rows * width, c.op, ": ", name, " holds ", t.numel(), " elements, expected ", rows * width);
+  };
+  same(kcodes, "key codes", at::kByte, pkcodes.size(-1));
+  same(ksigns, "key signs", at::kByte, pksigns.size(-1));
+  same(krn, "residual norms", at::kHalf, 1);
+  same(kvn, "key norms", at::kHalf, 1);
+  same(vcodes, "value codes", at::kByte, pvcodes.size(-1));
+  same(vvn, "value norms", at::kHalf, 1);
+}
+
+void page_write(const Tensor& kcodes, const Tensor& ksigns, const Tensor& krn, const Tensor& kvn, const Tensor& vcodes,
+                const Tensor& vvn, const Tensor& pkcodes, const Tensor& pksigns, const Tensor& pkrn, const Tensor& pkvn,
+                const Tensor& pvcodes, const Tensor& pvvn, const Tensor& table, const Tensor& start, int64_t S) {
+  page_write_meta(kcodes, ksigns, krn, kvn, vcodes, vvn, pkcodes, pksigns, pkrn, pkvn, pvcodes, pvvn, table, start, S);
+  const c10::DeviceGuard g(pkvn.device());
+  const Checker c{"tq::page_write", pkvn.device()};
+  Pool pool{&pkcodes, &pksigns, &pkrn, &pkvn, &pvcodes, &pvvn};
+  pool.check(c, false);
+  void* pp[6];
+  pool.pointers(pp);
+  void* rows[6] = {kcodes.data_ptr(), ksigns.data_ptr(), krn.data_ptr(), kvn.data_ptr(), vcodes.data_ptr(), vvn.data_ptr()};
+  check_status(tq_page_write(pp, rows, i32(table.size(0)), i32(pool.H), i32(S), i32(pool.D), i32(pool.key_code_bits),
+                             i32(pool.val_bits), pool.pages, i32(pool.P), ptr<int32_t>(table), table.size(1),
+                             i32(table.size(1)), ptr<int32_t>(start), stream_of(pkvn)),
+               "PagePool.write");
+}
+
+using Planes6 = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
+
+Planes6 page_read_meta(const Tensor& pkcodes, const Tensor& pksigns, const Tensor& pkrn, const Tensor& pkvn,
+                       const Tensor& pvcodes, const Tensor& pvvn, const Tensor& table, const Tensor& lengths, int64_t S) {
+  const Checker c{"tq::page_read", pkvn.device()};
+  Pool pool{&pkcodes, &pksigns, &pkrn, &pkvn, &pvcodes, &pvvn};
+  pool.check(c, false);
+  check_table(c, table);
+  check_index(c, lengths, "lengths", {table.size(0)});
+  TORCH_CHECK(S >= 0 && S < (int64_t{1} << 31), c.op, ": bad row count ", S);
+  const int64_t B = table.size(0);
+  auto rows = [&](const Tensor& p) { return at::empty({B, pool.H, S, p.size(-1)}, p.options()); };
+  auto norms = [&](const Tensor& p) { return at::empty({B, pool.H, S}, p.options()); };
+  return {rows(pkcodes), rows(pksigns), norms(pkrn), norms(pkvn), rows(pvcodes), norms(pvvn)};
+}
+
+Planes6 page_read(const Tensor& pkcodes, const Tensor& pksigns, const Tensor& pkrn, const Tensor& pkvn,
+                  const Tensor& pvcodes, const Tensor& pvvn, const Tensor& table, const Tensor& lengths, int64_t S) {
+  Planes6 out = page_read_meta(pkcodes, pksigns, pkrn, pkvn, pvcodes, pvvn, table, lengths, S);
+  const c10::DeviceGuard g(pkvn.device());
+  const Checker c{"tq::page_read", pkvn.device()};
+  Pool pool{&pkcodes, &pksigns, &pkrn, &pkvn, &pvcodes, &pvvn};
+  pool.check(c, false);
+  void* pp[6];
+  pool.pointers(pp);
+  void* rows[6] = {std::get<0>(out).data_ptr(), std::get<1>(out).data_ptr(), std::get<2>(out).data_ptr(),
+                   std::get<3>(out).data_ptr(), std::get<4>(out).data_ptr(), std::get<5>(out).data_ptr()};
+  check_status(tq_page_read(pp, rows, i32(table.size(0)), i32(pool.H), i32(S), i32(pool.D), i32(pool.key_code_bits),
+                            i32(pool.val_bits), pool.pages, i32(pool.P), ptr<int32_t>(table), table.size(1),
+                            i32(table.size(1)), ptr<int32_t>(lengths), stream_of(pkvn)),
+               "PagePool.read");
+  return out;
+}
+
+void page_copy_meta(const Tensor& pkcodes, const Tensor& pksigns, const Tensor& pkrn, const Tensor& pkvn,
+                    const Tensor& pvcodes, const Tensor& pvvn, const Tensor& src, const Tensor& dst) {
+  const Checker c{"tq::page_copy", pkvn.device()};
+  Pool pool{&pkcodes, &pksigns, &pkrn, &pkvn, &pvcodes, &pvvn};
+  pool.check(c, true);
+  TORCH_CHECK(src.dim() == 1, c.op, ": src must be [n] page indices, got ", src.sizes());
+  check_index(c, src, "src", src.sizes());
+  check_index(c, dst, "dst", src.sizes());
+}
+
+void page_copy(const Tensor& pkcodes, const Tensor& pksigns, const Tensor& pkrn, const Tensor& pkvn,
+               const Tensor& pvcodes, const Tensor& pvvn, const Tensor& src, const Tensor& dst) {
+  page_copy_meta(pkcodes, pksigns, pkrn, pkvn, pvcodes, pvvn, src, dst);
+  const c10::DeviceGuard g(pkvn.device());
+  const Checker c{"tq::page_copy", pkvn.device()};
+  Pool pool{&pkcodes, &pksigns, &pkrn, &pkvn, &pvcodes, &pvvn};
+  pool.check(c, true);
+  void* pp[6];
+  pool.pointers(pp);
+  check_status(tq_page_copy(pp, i32(pool.layers), i32(pool.H), i32(pool.D), i32(pool.key_code_bits), i32(pool.val_bits),
+                            pool.pages, i32(pool.P), ptr<int32_t>(src), ptr<int32_t>(dst), i32(src.numel()), stream_of(pkvn)),
+               "PagePool.copy");
+}
+
+Tensor page_keep_meta(const Tensor& pkcodes, const Tensor& pksigns, const Tensor& pkrn, const Tensor& pkvn,
+                      const Tensor& pvcodes, const Tensor& pvvn, const Tensor& table, const Tensor& lengths,
+                      const Tensor& path, const Tensor& count) {
+  const Checker c{"tq::page_keep", pkvn.device()};
+  Pool pool{&pkcodes, &pksigns, &pkrn, &pkvn, &pvcodes, &pvvn};
+  pool.check(c, true);
+  check_table(c, table);
+  const int64_t B = table.size(0);
+  check_index(c, lengths, "lengths", {B});
+  TORCH_CHECK(path.dim() == 2 && path.size(1) >= 1 && path.size(1) <= 64, c.op,
+              ": path must be [B, T] with 1 to 64 drafted tokens, got ", path.sizes());
+  check_index(c, path, "path", {B, path.size(1)});
+  check_index(c, count, "count", {B});
+  return at::empty({B}, lengths.options());
+}
+
+Tensor page_keep(const Tensor& pkcodes, const Tensor& pksigns, const Tensor& pkrn, const Tensor& pkvn,
+                 const Tensor& pvcodes, const Tensor& pvvn, const Tensor& table, const Tensor& lengths,
+                 const Tensor& path, const Tensor& count) {
+  Tensor out = page_keep_meta(pkcodes, pksigns, pkrn, pkvn, pvcodes, pvvn, table, lengths, path, count);
+  const c10::DeviceGuard g(pkvn.device());
+  const Checker c{"tq::page_keep", pkvn.device()};
+  Pool pool{&pkcodes, &pksigns, &pkrn, &pkvn, &pvcodes, &pvvn};
+  pool.check(c, true);
+  void* pp[6];
+  pool.pointers(pp);
+  check_status(tq_page_keep(pp, i32(pool.layers), i32(table.size(0)), i32(pool.H), i32(path.size(1)), i32(pool.D),
+                            i32(pool.key_code_bits), i32(pool.val_bits), pool.pages, i32(pool.P), ptr<int32_t>(table),
+                            table.size(1), i32(table.size(1)), ptr<int32_t>(lengths), ptr<int32_t>(path),
+                            ptr<int32_t>(count), ptr<int32_t>(out), stream_of(pkvn)),
+               "PagePool.keep");
+  return out;
+}
+
+// ---------------------------------------------------------------- drafted tokens
+// Checks shared by the prepared and the raw form; sizes from q [B, Hq, T, D] (q_rot has q's).
+Tensor check_tree(const Checker& c, const Tensor& q, Pool& pool, const Tensor& kcent16, int64_t bits, const Tensor& vcent32,
+                  const Tensor& vpit, const Tensor& table, const Tensor& lengths, const c10::optional<Tensor>& parents,
+                  at::ScalarType out_dtype) {
+  TORCH_CHECK(q.dim() == 4, c.op, ": queries must be [B, Hq, T, D], got ", q.sizes());
+  const int64_t B = q.size(0), Hq = q.size(1), T = q.size(2), D = q.size(3);
+  TORCH_CHECK(is_act(out_dtype), c.op, ": out_dtype must be float32, float16 or bfloat16");
+  pool.check(c, false);
+  TORCH_CHECK(D == 64 || D == 128, c.op, ": head_dim ", D, " not supported (64 or 128)");
+  TORCH_CHECK(bits >= 2 && bits <= 4 && pool.D == D && pool.key_code_bits == bits - 1 && pool.val_bits == bits, c.op,
+              ": the pool holds rows of head_dim ", pool.D, " with ", pool.key_code_bits, " key code and ", pool.val_bits,
+              " value bits; expected head_dim ", D, " with ", bits - 1, " and ", bits, " (2 to 4 bits)");
+  TORCH_CHECK(Hq >= pool.H && Hq % pool.H == 0, c.op, ": ", Hq, " query heads are not a multiple of ", pool.H, " kv heads");
+  TORCH_CHECK(T >= 1 && T <= 64, c.op, ": 1 to 64 drafted tokens, got ", T);
+  check_table(c, table);
+  TORCH_CHECK(table.size(0) == B, c.op, ": block_table has ", table.size(0), " rows for ", B, " sequences");
+  TORCH_CHECK(table.size(1) * pool.P >= T && table.size(1) * pool.P <= (int64_t{1} << 24), c.op, ": a row of ", table.size(1),
+              " pages of ", pool.P, " positions must hold the ", T, " drafted tokens and at most 2^24 positions");
+  check_index(c, lengths, "lengths", {B});
+  if (parents.has_value() && parents->defined()) {
+    if (parents->dim() == 1) check_index(c, *parents, "parents", {T});
+    else check_index(c, *parents, "parents", {B, T});
+  }
+  c.table(kcent16, "key centroids", at::kHalf, int64_t{1} << (bits - 1));
+  c.table(vcent32, "value centroids", at::kFloat, int64_t{1} << bits);
+  c.table(vpit, "split Pi_v^T", at::kHalf, 2 * D * D);
+  return at::empty({B, T, Hq, D}, q.options().dtype(out_dtype));
+}
+
+Tensor tree_attention_meta(const Tensor& q_rot, const Tensor& q_proj, const Tensor& kcodes, const Tensor& ksigns,
+                           const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits, const Tensor& vcodes,
+                           const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit, const Tensor& table,
+                           const Tensor& lengths, const c10::optional<Tensor>& parents, double coeff, double scale,
+                           at::ScalarType out_dtype) {
+  const Checker c{"tq::tree_attention", q_rot.device()};
+  TORCH_CHECK(q_rot.scalar_type() == at::kHalf && q_proj.scalar_type() == at::kFloat && q_rot.is_contiguous() &&
+                  q_proj.is_contiguous() && q_proj.sizes() == q_rot.sizes(),
+              c.op, ": q_rot must be float16 and q_proj float32, contiguous and of one shape (tq::query_prep)");
+  c.same_device(q_proj, "q_proj");
+  Pool pool{&kcodes, &ksigns, &krn, &kvn, &vcodes, &vvn};
+  return check_tree(c, q_rot, pool, kcent16, bits, vcent32, vpit, table, lengths, parents, out_dtype);
+}
+
+Tensor tree_attention(const Tensor& q_rot, const Tensor& q_proj, const Tensor& kcodes, const Tensor& ksigns,
+                      const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits, const Tensor& vcodes,
+                      const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit, const Tensor& table,
+                      const Tensor& lengths, const c10::optional<Tensor>& parents, double coeff, double scale,
+                      at::ScalarType out_dtype) {
+  Tensor out = tree_attention_meta(q_rot, q_proj, kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn, vcent32, vpit, table,
+                                   lengths, parents, coeff, scale, out_dtype);
+  const c10::DeviceGuard g(q_rot.device());
+  const int32_t B = i32(q_rot.size(0)), Hq = i32(q_rot.size(1)), T = i32(q_rot.size(2)), D = i32(q_rot.size(3));
+  const int32_t Hkv = i32(kvn.size(1)), P = i32(kvn.size(2)), W = i32(table.size(1));
+  const int64_t bytes = tq_tree_workspace_size(B, Hq, Hkv, T, W, P, D, i32(bits));
+  Tensor ws = at::empty({bytes}, q_rot.options().dtype(at::kByte));
+  const bool tree = parents.has_value() && parents->defined();
+  check_status(tq_tree_attention(ptr<uint16_t>(q_rot), ptr<float>(q_proj), ptr<uint8_t>(kcodes), ptr<uint8_t>(ksigns),
+                                 ptr<uint16_t>(krn), ptr<uint16_t>(kvn), ptr<uint16_t>(kcent16), i32(bits),
+                                 ptr<uint8_t>(vcodes), ptr<uint16_t>(vvn), ptr<float>(vcent32), ptr<uint16_t>(vpit),
+                                 kvn.size(0), P, ptr<int32_t>(table), W, W, ptr<int32_t>(lengths),
+                                 tree ? ptr<int32_t>(*parents) : nullptr, tree && parents->dim() == 2 ? T : 0, B, Hq, Hkv, T,
+                                 D, static_cast<float>(coeff), static_cast<float>(scale), out.data_ptr(),
+                                 dtype_code(out_dtype), out.stride(0), out.stride(2), out.stride(1), ws.data_ptr(), bytes,
+                                 stream_of(out)),
+               "tree_attention");
+  return out;
+}
+
+Tensor tree_attend_meta(const Tensor& q, const Tensor& pi_split, const Tensor& s_eff16, const Tensor& kcodes,
+                        const Tensor& ksigns, const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits,
+                        const Tensor& vcodes, const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit,
+                        const Tensor& table, const Tensor& lengths, const c10::optional<Tensor>& parents, double coeff,
+                        double scale, at::ScalarType out_dtype) {
+  const Checker c{"tq::tree_attend", q.device()};
+  Pool pool{&kcodes, &ksigns, &krn, &kvn, &vcodes, &vvn};
+  Tensor out = check_tree(c, q, pool, kcent16, bits, vcent32, vpit, table, lengths, parents, out_dtype);
+  c.table(pi_split, "split Pi", at::kHalf, 2 * q.size(3) * q.size(3));
+  c.table(s_eff16, "f16 S_eff", at::kHalf, q.size(3) * q.size(3));
+  return out;
+}
+
+Tensor tree_attend(const Tensor& q, const Tensor& pi_split, const Tensor& s_eff16, const Tensor& kcodes,
+                   const Tensor& ksigns, const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits,
+                   const Tensor& vcodes, const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit, const Tensor& table,
+                   const Tensor& lengths, const c10::optional<Tensor>& parents, double coeff, double scale,
+                   at::ScalarType out_dtype) {
+  auto qp = query_prep(q, pi_split, s_eff16);
+  return tree_attention(std::get<0>(qp), std::get<1>(qp), kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn, vcent32, vpit,
+                        table, lengths, parents, coeff, scale, out_dtype);
+}
+
+using Verified = std::tuple<Tensor, Tensor, Tensor>;
+
+Verified verify_drafts_meta(const Tensor& tokens, const Tensor& target, const Tensor& uniforms,
+                            const c10::optional<Tensor>& parents, const c10::optional<Tensor>& draft) {
+  const Checker c{"tq::verify_drafts", target.device()};
+  TORCH_CHECK(target.dim() == 3 && is_act(target.scalar_type()), c.op,
+              ": target_probs must be float32, float16 or bfloat16 [B, T, V], got ", target.scalar_type(), " ", target.sizes());
+  const int64_t B = target.size(0), T = target.size(1), V = target.size(2);
+  TORCH_CHECK(T >= 1 && T <= 64, c.op, ": 1 to 64 nodes, got ", T);
+  TORCH_CHECK(V >= 1 && V < (int64_t{1} << 30) && B <= 65535, c.op, ": 1 to 2^30 tokens and at most 65535 sequences, got ",
+              target.sizes());
+  TORCH_CHECK(V == 1 || target.stride(2) == 1, c.op, ": target_probs must be contiguous along the vocabulary");
+  c.same_device(tokens, "tokens");
+  TORCH_CHECK(tokens.scalar_type() == at::kLong && tokens.dim() == 2 && tokens.size(0) == B && tokens.size(1) == T &&
+                  tokens.is_contiguous(),
+              c.op, ": tokens must be contiguous int64 [", B, ", ", T, "], got ", tokens.scalar_type(), " ", tokens.sizes());
+  c.same_device(uniforms, "uniforms");
+  TORCH_CHECK(uniforms.scalar_type() == at::kFloat && uniforms.dim() == 2 && uniforms.size(0) == B && uniforms.size(1) == T &&
+                  uniforms.is_contiguous(),
+              c.op, ": uniforms must be contiguous float32 [", B, ", ", T, "], got ", uniforms.scalar_type(), " ",
+              uniforms.sizes());
+  const bool tree = parents.has_value() && parents->defined(), drawn = draft.has_value() && draft->defined();
+  TORCH_CHECK(!(tree && drawn), c.op,
+              ": tokens drawn from a draft distribution form a chain; a tree (parents) holds chosen candidates");
+  if (tree) {
+    if (parents->dim() == 1) check_index(c, *parents, "parents", {T});
+    else check_index(c, *parents, "parents", {B, T});
+  }
+  if (drawn) {
+    c.same_device(*draft, "draft_probs");
+    TORCH_CHECK(draft->scalar_type() == target.scalar_type() && draft->dim() == 3 && draft->size(0) == B &&
+                    draft->size(1) == T - 1 && draft->size(2) == V && (V == 1 || draft->stride(2) == 1),
+                c.op, ": draft_probs must be ", target.scalar_type(), " [", B, ", ", T - 1, ", ", V,
+                "], contiguous along the vocabulary, got ", draft->scalar_type(), " ", draft->sizes());
+  }
+  return {at::empty({B, T}, tokens.options().dtype(at::kInt)), at::empty({B}, tokens.options().dtype(at::kInt)),
+          at::empty({B}, tokens.options())};
+}
+
+Verified verify_drafts(const Tensor& tokens, const Tensor& target, const Tensor& uniforms,
+                       const c10::optional<Tensor>& parents, const c10::optional<Tensor>& draft) {
+  Verified out = verify_drafts_meta(tokens, target, uniforms, parents, draft);
+  const c10::DeviceGuard g(target.device());
+  const int32_t B = i32(target.size(0)), T = i32(target.size(1)), V = i32(target.size(2));
+  const int64_t bytes = tq_verify_workspace_size(B, V);
+  Tensor ws = at::empty({bytes}, tokens.options().dtype(at::kByte));
+  const bool tree = parents.has_value() && parents->defined(), drawn = draft.has_value() && draft->defined() && T > 1;
+  check_status(tq_verify_drafts(ptr<int64_t>(tokens), target.data_ptr(), dtype_code(target.scalar_type()), target.stride(0),
+                                target.stride(1), drawn ? draft->data_ptr() : nullptr, drawn ? draft->stride(0) : 0,
+                                drawn ? draft->stride(1) : 0, ptr<float>(uniforms),
+                                tree ? ptr<int32_t>(*parents) : nullptr, tree && parents->dim() == 2 ? T : 0, B, T, V,
+                                ptr<int32_t>(std::get<0>(out)), ptr<int32_t>(std::get<1>(out)), ptr<int64_t>(std::get<2>(out)),
+                                ws.data_ptr(), bytes, stream_of(target)),
+               "verify_drafts");
+  return out;
+}
+
 int64_t workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t d, int64_t bits) {
   return tq_attention_workspace_size(static_cast<int32_t>(B), static_cast<int32_t>(Hq), static_cast<int32_t>(Hkv),
                                      static_cast<int32_t>(Sq), static_cast<int32_t>(Sk), static_cast<int32_t>(d),
@@ -821,6 +1163,23 @@ TORCH_LIBRARY(tq, m) {
         "Tensor(b!) ksigns, Tensor(c!) krn, Tensor(d!) kvn, Tensor(e!) vcodes, Tensor(f!) vvn, int pos, "
         "Tensor kcent16, Tensor vcent, Tensor vpit, float coeff, float scale, bool causal, Tensor? mask, "
         "ScalarType out_dtype, int workspace) -> Tensor");
+  m.def("page_write(Tensor kcodes, Tensor ksigns, Tensor krn, Tensor kvn, Tensor vcodes, Tensor vvn, "
+        "Tensor(a!) pkcodes, Tensor(b!) pksigns, Tensor(c!) pkrn, Tensor(d!) pkvn, Tensor(e!) pvcodes, "
+        "Tensor(f!) pvvn, Tensor block_table, Tensor start, int S) -> ()");
+  m.def("page_read(Tensor pkcodes, Tensor pksigns, Tensor pkrn, Tensor pkvn, Tensor pvcodes, Tensor pvvn, "
+        "Tensor block_table, Tensor lengths, int S) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("page_copy(Tensor(a!) pkcodes, Tensor(b!) pksigns, Tensor(c!) pkrn, Tensor(d!) pkvn, Tensor(e!) pvcodes, "
+        "Tensor(f!) pvvn, Tensor src, Tensor dst) -> ()");
+  m.def("page_keep(Tensor(a!) pkcodes, Tensor(b!) pksigns, Tensor(c!) pkrn, Tensor(d!) pkvn, Tensor(e!) pvcodes, "
+        "Tensor(f!) pvvn, Tensor block_table, Tensor lengths, Tensor path, Tensor count) -> Tensor");
+  m.def("tree_attention(Tensor q_rot, Tensor q_proj, Tensor kcodes, Tensor ksigns, Tensor krn, Tensor kvn, "
+        "Tensor kcent, int bits, Tensor vcodes, Tensor vvn, Tensor vcent, Tensor vpit, Tensor block_table, "
+        "Tensor lengths, Tensor? parents, float coeff, float scale, ScalarType out_dtype) -> Tensor");
+  m.def("tree_attend(Tensor q, Tensor pi_split, Tensor s_eff, Tensor kcodes, Tensor ksigns, Tensor krn, Tensor kvn, "
+        "Tensor kcent, int bits, Tensor vcodes, Tensor vvn, Tensor vcent, Tensor vpit, Tensor block_table, "
+        "Tensor lengths, Tensor? parents, float coeff, float scale, ScalarType out_dtype) -> Tensor");
+  m.def("verify_drafts(Tensor tokens, Tensor target_probs, Tensor uniforms, Tensor? parents, Tensor? draft_probs) "
+        "-> (Tensor, Tensor, Tensor)");
   m.def("workspace_size(int B, int Hq, int Hkv, int Sq, int Sk, int d, int bits) -> int", &workspace_size);
 }
 
@@ -839,6 +1198,13 @@ TORCH_LIBRARY_IMPL(tq, CUDA, m) {
   m.impl("attend", &attend);
   m.impl("attend_scores", &attend_scores);
   m.impl("cache_attend", &cache_attend);
+  m.impl("page_write", &page_write);
+  m.impl("page_read", &page_read);
+  m.impl("page_copy", &page_copy);
+  m.impl("page_keep", &page_keep);
+  m.impl("tree_attention", &tree_attention);
+  m.impl("tree_attend", &tree_attend);
+  m.impl("verify_drafts", &verify_drafts);
 }
 
 // the same checks on tensor metadata, returning empty outputs of the right shapes
@@ -857,4 +1223,11 @@ TORCH_LIBRARY_IMPL(tq, Meta, m) {
   m.impl("attend", &attend_meta);
   m.impl("attend_scores", &attend_scores_meta);
   m.impl("cache_attend", &cache_attend_meta);
+  m.impl("page_write", &page_write_meta);
+  m.impl("page_read", &page_read_meta);
+  m.impl("page_copy", &page_copy_meta);
+  m.impl("page_keep", &page_keep_meta);
+  m.impl("tree_attention", &tree_attention_meta);
+  m.impl("tree_attend", &tree_attend_meta);
+  m.impl("verify_drafts", &verify_drafts_meta);
 }
