@@ -63,28 +63,88 @@ __device__ __forceinline__ int64_t page_row(const PagePlanes& a, int b, int h, i
 }
 
 // ---------------------------------------------------------------- rows in and out
-// WRITE: rows [B, H, S] of the source planes to positions start[b] + s; otherwise positions
-// s < length[b] to rows [B, H, S] of the target planes, zeros behind.  A thread moves one piece; a
-// plane's pieces are taken in row order, so both sides are read and written in runs.
+// WRITE: rows [B, H, S] of the source planes to positions at[b] + s; otherwise positions s < at[b]
+// to rows [B, H, S] of the target planes, zeros behind.  A block takes a stretch of one (sequence,
+// head, plane).  Code planes move in pieces of a row; the rows of a page are contiguous, so both sides
+// run through in order.  Norm planes (2 bytes a row) move in groups of 8 rows that lie together in
+// a page; the flat side of a group starts anywhere, so it is accessed as unaligned 16 bytes.
+constexpr int kRowSteps = 4;  // pieces of a thread, loaded together
 template <bool WRITE>
-__global__ void __launch_bounds__(256) page_rows_kernel(PagePlanes a, const int32_t* at, int B, int S) {
-  const int p = blockIdx.y;
+__device__ __forceinline__ void code_pieces(const PagePlanes& a, int p, int b, int h, int64_t flat_row, int from, int S) {
   const uint32_t unit = a.unit[p], per = a.width[p] / unit;
-  const int64_t n = static_cast<int64_t>(B) * a.H * S * per;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t r = i / per;
-    const uint32_t piece = static_cast<uint32_t>(i - r * per);
-    const int64_t bh = r / S;
-    const int s = static_cast<int>(r - bh * S), b = static_cast<int>(bh / a.H), h = static_cast<int>(bh - static_cast<int64_t>(b) * a.H);
-    uint8_t* const flat = a.rows[p] + i * unit;
-    if constexpr (WRITE) {
-      const int64_t row = page_row(a, b, h, static_cast<int64_t>(at[b]) + s);
-      if (at[b] >= 0 && row >= 0) copy_piece(a.pool[p] + row * a.width[p] + piece * unit, flat, unit);
-    } else {
-      const int64_t row = s < at[b] ? page_row(a, b, h, s) : -1;
-      if (row >= 0) copy_piece(flat, a.pool[p] + row * a.width[p] + piece * unit, unit);
-      else zero_piece(flat, unit);
+  const uint32_t n = static_cast<uint32_t>(S) * per, i0 = blockIdx.x * (256 * kRowSteps) + threadIdx.x;
+  uint8_t* const flat = a.rows[p] + flat_row * a.width[p];
+  uint8_t* pool[kRowSteps];
+#pragma unroll
+  for (int k = 0; k < kRowSteps; ++k) {
+    const uint32_t i = i0 + k * 256, s = i / per;
+    pool[k] = nullptr;
+    if (i < n && (WRITE || static_cast<int>(s) < from)) {
+      const int64_t row = page_row(a, b, h, static_cast<int64_t>(WRITE ? from : 0) + s);
+      if (row >= 0) pool[k] = a.pool[p] + row * a.width[p] + (i - s * per) * unit;
     }
+  }
+  if (unit == 16) {  // the usual widths: every load in flight before the first store
+    uint4 v[kRowSteps];
+#pragma unroll
+    for (int k = 0; k < kRowSteps; ++k) {
+      const int64_t i = i0 + k * 256;
+      v[k] = uint4{0, 0, 0, 0};
+      if (pool[k]) v[k] = *reinterpret_cast<const uint4*>(WRITE ? flat + i * 16 : pool[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kRowSteps; ++k) {
+      const int64_t i = i0 + k * 256;
+      if (WRITE && pool[k]) *reinterpret_cast<uint4*>(pool[k]) = v[k];
+      if (!WRITE && i < n) *reinterpret_cast<uint4*>(flat + i * 16) = v[k];
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < kRowSteps; ++k) {
+    const int64_t i = i0 + k * 256;
+    if (WRITE && pool[k]) copy_piece(pool[k], flat + i * unit, unit);
+    if (!WRITE && i < n) {
+      if (pool[k]) copy_piece(flat + i * unit, pool[k], unit);
+      else zero_piece(flat + i * unit, unit);
+    }
+  }
+}
+
+template <bool WRITE>
+__device__ __forceinline__ void norm_groups(const PagePlanes& a, int p, int b, int h, int64_t flat_row, int from, int S) {
+  const int64_t first = WRITE ? from : 0;  // position of flat row 0
+  const int64_t pos = ((first >> 3) + blockIdx.x * 256 + threadIdx.x) << 3;
+  if (pos >= first + S) return;
+  const int64_t row = page_row(a, b, h, pos);  // a page holds whole groups
+  uint16_t* const flat = reinterpret_cast<uint16_t*>(a.rows[p]) + flat_row + (pos - first);
+  uint16_t* const pool = reinterpret_cast<uint16_t*>(a.pool[p]) + (row >= 0 ? row : 0);
+  const int64_t live = WRITE ? first + S : min(static_cast<int64_t>(from), first + S);
+  if (row >= 0 && pos >= first && pos + 8 <= live) {
+    uint4 v;
+    __builtin_memcpy(&v, WRITE ? flat : pool, 16);
+    __builtin_memcpy(WRITE ? pool : flat, &v, 16);
+    return;
+  }
+  for (int j = 0; j < 8; ++j) {
+    if (pos + j < first || pos + j >= first + S) continue;
+    if constexpr (WRITE) {
+      if (row >= 0) pool[j] = flat[j];
+    } else {
+      flat[j] = row >= 0 && pos + j < live ? pool[j] : 0;
+    }
+  }
+}
+
+template <bool WRITE>
+__global__ void __launch_bounds__(256) page_rows_kernel(PagePlanes a, const int32_t* at, int64_t BH, int S) {
+  const int p = blockIdx.y;
+  for (int64_t bh = blockIdx.z; bh < BH; bh += gridDim.z) {
+    const int b = static_cast<int>(bh / a.H), h = static_cast<int>(bh - static_cast<int64_t>(b) * a.H);
+    const int from = at[b];
+    if (WRITE && from < 0) continue;
+    if (p == 2 || p == 3 || p == 5) norm_groups<WRITE>(a, p, b, h, bh * S, from, S);
+    else code_pieces<WRITE>(a, p, b, h, bh * S, from, S);
   }
 }
 
@@ -108,55 +168,70 @@ __global__ void __launch_bounds__(256) page_copy_kernel(PagePlanes a, const int3
 
 // ---------------------------------------------------------------- an accepted path
 // Position lengths[b] + path[b, i] moves to lengths[b] + i for i < count[b].  Source and target
-// rows overlap, so a block takes one (sequence, head, layer) and holds every moved row in LDS
-// before it writes the first.  Rows that stay where they are (path[i] == i, the root always)
-// are not touched.
-constexpr int kKeepThreads = 128;
-__global__ void __launch_bounds__(kKeepThreads) page_keep_kernel(PagePlanes a, const int32_t* lengths, const int32_t* path,
-                                                                 const int32_t* count, int T, int32_t* new_lengths) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t held[];
+// rows overlap, so a block (one wave: one sequence, head and layer) has every row in registers
+// before it writes the first.  A piece of a row only meets the same piece of other rows, so rows too
+// many for the registers go in several passes over stretches of pieces.  Rows that stay where
+// they are (path[i] == i, the root always) are not touched.
+// U: bytes of a code piece (8 where every code width is a multiple, else 1); the three norms are
+// pieces of their own.
+constexpr int kKeepPieces = 4;  // of a lane
+template <int U>
+__global__ void __launch_bounds__(64) page_keep_kernel(PagePlanes a, const int32_t* lengths, const int32_t* path,
+                                                       const int32_t* count, int T, int32_t* new_lengths) {
   __shared__ int64_t s_from[64], s_to[64];
-  const int h = blockIdx.x, b = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x;
+  const int h = blockIdx.x, b = blockIdx.y, layer = blockIdx.z, i = threadIdx.x;
   const int n = min(max(count[b], 0), T);
   const int64_t at = lengths[b];
-  if (tid == 0 && h == 0 && layer == 0) new_lengths[b] = static_cast<int32_t>(at) + (at >= 0 ? n : 0);
+  if (i == 0 && h == 0 && layer == 0) new_lengths[b] = static_cast<int32_t>(at) + (at >= 0 ? n : 0);
   int64_t from = -1, to = -1;
-  if (tid < n && at >= 0) {
-    const int k = path[static_cast<int64_t>(b) * T + tid];
-    if (k >= 0 && k < T && k != tid) {
+  if (i < n && at >= 0) {
+    const int k = path[static_cast<int64_t>(b) * T + i];
+    if (k >= 0 && k < T && k != i) {
       from = page_row(a, b, h, at + k);
-      to = page_row(a, b, h, at + tid);
-      if (from < 0 || to < 0) from = -1;
+      to = page_row(a, b, h, at + i);
+      if (to < 0) from = -1;
     }
   }
-  const uint64_t moved = __ballot(from >= 0);  // n <= 64: the rows are the first wave's lanes
-  __shared__ int s_n;
-  if (tid < 64) {
-    if (from >= 0) {
-      const int k = __popcll(moved & ((1ull << tid) - 1));
-      s_from[k] = from;
-      s_to[k] = to;
-    }
-    if (tid == 0) s_n = __popcll(moved);
+  const uint64_t moved = __ballot(from >= 0);
+  const uint32_t m = __popcll(moved);
+  if (m == 0) return;
+  if (from >= 0) {
+    const int k = __popcll(moved & ((1ull << i) - 1));
+    s_from[k] = from;
+    s_to[k] = to;
   }
   __syncthreads();
-  const int m = s_n;
-  if (m == 0) return;
+  const uint32_t c0 = a.width[0] / U, c1 = c0 + a.width[1] / U, c2 = c1 + a.width[4] / U;  // pieces of the code planes
+  const uint32_t per = c2 + 3, span = 64 * kKeepPieces / m < per ? 64 * kKeepPieces / m : per;
+  for (uint32_t q0 = 0; q0 < per; q0 += span) {
+    const uint32_t width = per - q0 < span ? per - q0 : span;
+    uint8_t* dst[kKeepPieces];
+    uint2 v[kKeepPieces];
+    bool norm[kKeepPieces];
 #pragma unroll
-  for (int pass = 0; pass < 2; ++pass) {
-    uint32_t off = 0;
-#pragma unroll
-    for (int p = 0; p < kPlanes; ++p) {
-      const uint32_t w = a.width[p], unit = a.unit[p], per = w / unit;
-      uint8_t* const base = a.pool[p] + layer * a.layer[p];
-      for (uint32_t i = tid; i < m * per; i += kKeepThreads) {
-        const uint32_t r = i / per, piece = (i - r * per) * unit;
-        if (pass == 0) copy_piece(held + off + r * w + piece, base + s_from[r] * w + piece, unit);
-        else copy_piece(base + s_to[r] * w + piece, held + off + r * w + piece, unit);
+    for (int k = 0; k < kKeepPieces; ++k) {
+      const uint32_t x = i + 64 * k, r = x / width, q = q0 + (x - r * width);
+      dst[k] = nullptr;
+      norm[k] = q >= c2;
+      if (r < m) {
+        const int p = q < c0 ? 0 : q < c1 ? 1 : q < c2 ? 4 : q == c2 ? 2 : q == c2 + 1 ? 3 : 5;
+        const uint32_t w = a.width[p], off = norm[k] ? 0 : (q - (p == 0 ? 0 : p == 1 ? c0 : c1)) * U;
+        uint8_t* const base = a.pool[p] + layer * a.layer[p] + off;
+        const uint8_t* const src = base + s_from[r] * w;
+        dst[k] = base + s_to[r] * w;
+        if (norm[k]) v[k].x = *reinterpret_cast<const uint16_t*>(src);
+        else if constexpr (U == 8) v[k] = *reinterpret_cast<const uint2*>(src);
+        else v[k].x = *src;
       }
-      off += (m * w + 15) / 16 * 16;
     }
     __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kKeepPieces; ++k) {
+      if (!dst[k]) continue;
+      if (norm[k]) *reinterpret_cast<uint16_t*>(dst[k]) = static_cast<uint16_t>(v[k].x);
+      else if constexpr (U == 8) *reinterpret_cast<uint2*>(dst[k]) = v[k];
+      else *dst[k] = static_cast<uint8_t>(v[k].x);
+    }
   }
 }
 
@@ -204,14 +279,17 @@ static int rows_call(const char* what, void* const* pool, void* const* rows, int
   PagePlanes a{};
   const int st = fill(what, a, pool, rows, H, num_pages, page_size, d, key_code_bits, val_bits, table, ld_table, table_width);
   if (st != TQ_OK) return st;
-  int64_t most = 0;
+  TQ_REQUIRE(static_cast<int64_t>(S) * 256 < (int64_t(1) << 31), "%s: at most 2^23 rows per head in one call, got %d", what, S);
+  uint32_t most = 0;  // pieces of the widest plane
   for (int p = 0; p < kPlanes; ++p) {
-    const int64_t n = static_cast<int64_t>(B) * H * S * (a.width[p] / a.unit[p]);
+    const uint32_t n = static_cast<uint32_t>(S) * (a.width[p] / a.unit[p]);
     most = n > most ? n : most;
   }
-  const int64_t blocks = (most + 255) / 256;
-  const dim3 grid(static_cast<unsigned>(blocks < 65536 ? blocks : 65536), kPlanes);
-  page_rows_kernel<WRITE><<<grid, 256, 0, s>>>(a, at, B, S);
+  const int64_t BH = static_cast<int64_t>(B) * H;
+  // enough blocks for the norm groups too: S / 8 groups and one more where the first begins inside
+  const uint32_t nx = (most + 256 * kRowSteps - 1) / (256 * kRowSteps), ng = (static_cast<uint32_t>(S) / 8 + 2 + 255) / 256;
+  const dim3 grid(nx > ng ? nx : ng, kPlanes, static_cast<unsigned>(BH < 65535 ? BH : 65535));
+  page_rows_kernel<WRITE><<<grid, 256, 0, s>>>(a, at, BH, S);
   return launch_status(what);
 }
 
@@ -267,9 +345,11 @@ int tq_page_keep(void* const* pool, int32_t layers, int32_t B, int32_t H, int32_
   const int st = fill("tq_page_keep", a, pool, nullptr, H, num_pages, page_size, d, key_code_bits, val_bits, block_table,
                       ld_table, table_width);
   if (st != TQ_OK) return st;
-  uint32_t lds = 0;  // every row but the root can move: at most 34 KB (head_dim 256, 8 bits)
-  for (int p = 0; p < kPlanes; ++p) lds += (T * a.width[p] + 15) / 16 * 16;
-  page_keep_kernel<<<dim3(H, B, layers), kKeepThreads, lds, as_stream(stream)>>>(a, lengths, path, count, T, new_lengths);
+  const dim3 grid(H, B, layers);
+  if (a.width[0] % 8 == 0 && a.width[1] % 8 == 0 && a.width[4] % 8 == 0)
+    page_keep_kernel<8><<<grid, 64, 0, as_stream(stream)>>>(a, lengths, path, count, T, new_lengths);
+  else
+    page_keep_kernel<1><<<grid, 64, 0, as_stream(stream)>>>(a, lengths, path, count, T, new_lengths);
   return launch_status("tq_page_keep");
 }
 
