@@ -11,9 +11,9 @@
 // drawn from what is left at that node, w: the first x with w_0 + ... + w_x > u_0 sum(w).
 //
 // The walk needs a few probabilities per node (one lane each), the draw one row of the vocabulary
-// (two for a chain), so the work is latency and one pass over that row: the row is cut into chunks
-// summed by a block each (every block repeats the walk: cheaper than a launch that only walks),
-// then one block per sequence finds the chunk and searches it.  Probabilities and sums are
+// (two for a chain), so the work is latency and one pass over that row: the row is cut into tiles of
+// 2048 entries, summed over many blocks (every block repeats the walk: cheaper than a launch that only
+// walks), then one block per sequence finds the tile and searches it.  Probabilities and sums are
 // float64: the token is decided by a comparison of sums over up to ~10^5 terms, and in float32
 // their rounding would move the border of a few tokens in a hundred thousand by more than the
 // token's own probability.
@@ -23,6 +23,8 @@ namespace tq {
 
 constexpr int kVerifyThreads = 256;
 constexpr int kMaxNodes = 64;  // a node is a lane
+constexpr int kTile = kVerifyThreads * 8;  // vocabulary entries summed together
+constexpr int kLeftWords = 3 + kMaxNodes;
 
 struct VerifyArgs {
   const int64_t* tokens;  // [B, T]
@@ -34,12 +36,24 @@ struct VerifyArgs {
   const int32_t* parents; // [B, T] (ld_parents = T), [T] (0), or null: a chain
   int64_t ld_parents;
   int B, T, V;
-  int chunk, nchunk;      // vocabulary entries per block, chunks per row
-  double* sums;           // [B, nchunk, 2]: of w, of p
+  int ntile, per;         // tiles of a row, tiles per block
+  double* sums;           // [B, 2, ntile]: of w, of p
+  int64_t* left;          // [B, kLeftWords]: stop, nrej, residual, the rejected tokens
   int32_t* path;          // [B, T]
   int32_t* count;         // [B]
   int64_t* next;          // [B]
 };
+
+// lane l's value, l the same in every lane
+__device__ __forceinline__ int lane_value(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
+__device__ __forceinline__ int64_t lane_value(int64_t v, int l) {
+  const uint64_t u = static_cast<uint64_t>(v);
+  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(lane_value(static_cast<int>(u), l))) |
+                              (static_cast<uint64_t>(static_cast<uint32_t>(lane_value(static_cast<int>(u >> 32), l))) << 32));
+}
+__device__ __forceinline__ double lane_value(double v, int l) {
+  return __builtin_bit_cast(double, lane_value(__builtin_bit_cast(int64_t, v), l));
+}
 
 // what is left to draw from after the walk
 struct Left {
@@ -72,15 +86,15 @@ __device__ __forceinline__ Left walk(const VerifyArgs& a, int b, int64_t* s_rej,
       // a candidate that repeats an earlier sibling has nothing left to accept
       bool again = false;
       for (int j = 0; j < a.T; ++j) {
-        const int pj = __shfl(par, j, 64);
-        const int64_t tj = __shfl(tok, j, 64);
+        const int pj = lane_value(par, j);
+        const int64_t tj = lane_value(tok, j);
         again = again || (j < i && pj == par && tj == tok);
       }
       if (again) p = 0.0;
       double rem = 1.0;
       for (int j = 0; j < a.T; ++j) {
-        const int pj = __shfl(par, j, 64);
-        const double qj = __shfl(p, j, 64);
+        const int pj = lane_value(par, j);
+        const double qj = lane_value(p, j);
         if (j < i && pj == par) rem -= qj;
       }
       bar = u * rem;
@@ -166,83 +180,112 @@ __device__ __forceinline__ const void* row_at(const void* base, int64_t i) {
   return static_cast<const uint8_t*>(base) + i * (DT == TQ_F32 ? 4 : 2);
 }
 
+// inclusive sum over the wave
+__device__ __forceinline__ double wave_scan(double v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int sh = 1; sh < 64; sh <<= 1) {
+    const double t = __shfl_up(v, sh, 64);
+    if (lane >= sh) v += t;
+  }
+  return v;
+}
+
+// The sums of w and of p over each tile of a row; a block takes a.per consecutive tiles.
 template <int DT>
 __global__ void __launch_bounds__(kVerifyThreads) verify_sum_kernel(VerifyArgs a) {
   __shared__ int64_t s_rej[kMaxNodes];
   __shared__ int s_left[3];
-  __shared__ double s_part[2][kVerifyThreads / 64];
-  const int b = blockIdx.y, c = blockIdx.x, tid = threadIdx.x;
-  const Left l = walk<DT>(a, b, s_rej, s_left, c == 0);
+  __shared__ double s_part[2][2][kVerifyThreads / 64];
+  const int b = blockIdx.y, tid = threadIdx.x;
+  const Left l = walk<DT>(a, b, s_rej, s_left, blockIdx.x == 0);
+  if (blockIdx.x == 0) {  // the outcome, for the draw
+    int64_t* const left = a.left + static_cast<int64_t>(b) * kLeftWords;
+    if (tid < 3) left[tid] = s_left[tid];
+    if (tid < l.nrej) left[3 + tid] = s_rej[tid];
+  }
   const void* prow = row_at<DT>(a.target, b * a.tb + l.stop * a.tt);
   const void* qrow = l.residual ? row_at<DT>(a.draft, b * a.db + l.stop * a.dt) : nullptr;
-  const int end = min(a.V, (c + 1) * a.chunk);
-  double sw = 0.0, sp = 0.0;
-  for (int x = c * a.chunk + tid * 8; x < end; x += kVerifyThreads * 8) {
-    double w[8], p[8];
-    weights8<DT>(a, prow, qrow, l, s_rej, x, w, p);
+  const int end = min(a.ntile, static_cast<int>(blockIdx.x + 1) * a.per);
+  for (int t = blockIdx.x * a.per, odd = 0; t < end; ++t, odd ^= 1) {
+    double sw = 0.0, sp = 0.0;
+    const int x = t * kTile + tid * 8;
+    if (x < a.V) {
+      double w[8], p[8];
+      weights8<DT>(a, prow, qrow, l, s_rej, x, w, p);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      sw += w[j];
-      sp += p[j];
+      for (int j = 0; j < 8; ++j) {
+        sw += w[j];
+        sp += p[j];
+      }
     }
-  }
-  sw = wave_sum(sw);
-  sp = wave_sum(sp);
-  if ((tid & 63) == 0) {
-    s_part[0][tid >> 6] = sw;
-    s_part[1][tid >> 6] = sp;
-  }
-  __syncthreads();
-  if (tid < 2) {
-    double t = 0.0;
+    sw = wave_sum(sw);
+    sp = wave_sum(sp);
+    if ((tid & 63) == 0) {
+      s_part[odd][0][tid >> 6] = sw;
+      s_part[odd][1][tid >> 6] = sp;
+    }
+    __syncthreads();  // the next tile writes the other half: one barrier per tile suffices
+    if (tid < 2) {
+      double v = 0.0;
 #pragma unroll
-    for (int k = 0; k < kVerifyThreads / 64; ++k) t += s_part[tid][k];
-    a.sums[(static_cast<int64_t>(b) * a.nchunk + c) * 2 + tid] = t;
+      for (int k = 0; k < kVerifyThreads / 64; ++k) v += s_part[odd][tid][k];
+      a.sums[(static_cast<int64_t>(b) * 2 + tid) * a.ntile + t] = v;
+    }
   }
 }
 
+// One block per sequence: the first wave scans the tiles' sums for the one in which the running sum
+// passes u_0 sum(w), then the block scans that tile, 8 entries a thread.
 template <int DT>
 __global__ void __launch_bounds__(kVerifyThreads) verify_pick_kernel(VerifyArgs a) {
   __shared__ int64_t s_rej[kMaxNodes];
-  __shared__ int s_left[3];
-  __shared__ double s_sum[kVerifyThreads];
-  __shared__ double s_before;
-  __shared__ int s_chunk, s_last, s_mode;
-  const int b = blockIdx.x, tid = threadIdx.x;
-  Left l = walk<DT>(a, b, s_rej, s_left, false);
-  const double u = static_cast<double>(a.uniforms[static_cast<int64_t>(b) * a.T]);
-  if (tid == 0) {
-    const double* s = a.sums + static_cast<int64_t>(b) * a.nchunk * 2;
+  __shared__ double s_wave[kVerifyThreads / 64];
+  __shared__ double s_bar;
+  __shared__ int s_tile, s_mode, s_last;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t* const left = a.left + static_cast<int64_t>(b) * kLeftWords;
+  Left l{static_cast<int>(left[0]), static_cast<int>(left[1]), left[2] != 0};
+  if (tid < l.nrej) s_rej[tid] = left[3 + tid];
+  if (wave == 0) {
     // nothing left (p and q equal to rounding, or every candidate's mass gone): draw from p itself
-    int which = 0;
     double total = 0.0;
-    for (; which < 2; ++which) {
-      total = 0.0;
-      for (int c = 0; c < a.nchunk; ++c) total += s[2 * c + which];
+    int mode = 0;
+    const double* s = a.sums + static_cast<int64_t>(b) * 2 * a.ntile;
+    for (; mode < 2; ++mode, s += a.ntile) {
+      double v = 0.0;
+      for (int t = lane; t < a.ntile; t += 64) v += s[t];
+      total = wave_sum(v);
       if (total > 0.0) break;
     }
-    s_mode = which;
-    s_chunk = -1;
-    if (which < 2) {
-      double run = 0.0;
-      int last = 0;
-      double last_run = 0.0;
-      const double bar = u * total;
-      for (int c = 0; c < a.nchunk; ++c) {
-        const double v = s[2 * c + which];
-        if (v > 0.0) {
-          last = c;
-          last_run = run;
-          if (run + v > bar) break;
+    int tile = -1;
+    double bar = 0.0;
+    if (mode < 2) {
+      const double goal = static_cast<double>(a.uniforms[static_cast<int64_t>(b) * a.T]) * total;
+      double run = 0.0;  // of the steps before
+      for (int t0 = 0; t0 < a.ntile; t0 += 64) {
+        const double v = t0 + lane < a.ntile ? s[t0 + lane] : 0.0;
+        const double upto = wave_scan(v) + run;
+        const uint64_t some = __ballot(v > 0.0), over = __ballot(v > 0.0 && upto > goal);
+        if (some) {  // the tile that passes the goal, or the last one with any weight
+          const int at = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
+          tile = t0 + at;
+          bar = goal - (lane_value(upto, at) - lane_value(v, at));
         }
-        run += v;
+        if (over) break;
+        run = lane_value(upto, 63);
       }
-      s_chunk = last;
-      s_before = bar - last_run;  // what the chunk's own running sum has to exceed
+    }
+    if (lane == 0) {
+      s_tile = tile;
+      s_mode = mode;
+      s_bar = bar;
     }
   }
+  if (tid == 0) s_last = -1;
   __syncthreads();
-  if (s_chunk < 0) {
+  const int tile = s_tile;
+  if (tile < 0) {
     if (tid == 0) a.next[b] = -1;
     return;
   }
@@ -252,70 +295,55 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_pick_kernel(VerifyArgs 
   }
   const void* prow = row_at<DT>(a.target, b * a.tb + l.stop * a.tt);
   const void* qrow = l.residual ? row_at<DT>(a.draft, b * a.db + l.stop * a.dt) : nullptr;
-  const int beg = s_chunk * a.chunk, end = min(a.V, beg + a.chunk);
-  // each thread sums a run of `per` entries, one thread then searches the runs and its own entries
-  const int per = ((end - beg + kVerifyThreads - 1) / kVerifyThreads + 7) / 8 * 8;
-  const int mine = beg + tid * per, stop = min(end, mine + per);
-  double sum = 0.0;
-  for (int x = mine; x < stop; x += 8) {
-    double w[8], p[8];
+  const int x = tile * kTile + tid * 8;
+  double w[8], sum = 0.0;
+  if (x < a.V) {
+    double p[8];
     weights8<DT>(a, prow, qrow, l, s_rej, x, w, p);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (x + j < stop) sum += w[j];
+    for (int j = 0; j < 8; ++j) sum += w[j];
   }
-  s_sum[tid] = sum;
+  const double upto = wave_scan(sum);
+  if (lane == 63) s_wave[wave] = upto;
   __syncthreads();
-  if (tid == 0) {
-    double run = 0.0, at = 0.0;
-    int who = -1;
-    for (int t = 0; t < kVerifyThreads; ++t) {
-      if (s_sum[t] > 0.0) {
-        who = t;
-        at = run;
-        if (run + s_sum[t] > s_before) break;
-      }
-      run += s_sum[t];
-    }
-    s_last = who;
-    s_before -= at;
-  }
+  double before = 0.0;
+  for (int k = 0; k < wave; ++k) before += s_wave[k];
+  // the first thread whose entries pass the bar, or the last one with any weight
+  const uint64_t some = __ballot(sum > 0.0), over = __ballot(sum > 0.0 && before + upto > s_bar);
+  if (lane == 0 && some)
+    atomicMax(&s_last, over ? (1 << 20) - (tid + __builtin_ctzll(over)) : tid + 63 - __builtin_clzll(some));
   __syncthreads();
-  if (tid == s_last) {
+  const int key = s_last, who = key >= (1 << 19) ? (1 << 20) - key : key;
+  if (tid == who) {
+    const double bar = s_bar - (before + (upto - sum));
     double run = 0.0;
-    int64_t pick = -1;
+    int pick = -1;
     bool done = false;
-    for (int x = mine; x < stop && !done; x += 8) {
-      double w[8], p[8];
-      weights8<DT>(a, prow, qrow, l, s_rej, x, w, p);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (!done && x + j < stop && w[j] > 0.0) {
-          run += w[j];
-          pick = x + j;
-          done = run > s_before;
-        }
+    for (int j = 0; j < 8; ++j) {
+      if (!done && w[j] > 0.0) {
+        run += w[j];
+        pick = x + j;
+        done = run > bar;
       }
     }
     a.next[b] = pick;
   }
 }
 
-// chunks of a row: about 512 blocks in all, of at least 2048 entries (8 per thread)
-static void plan_verify(int B, int V, int* chunk, int* nchunk) {
-  int n = 512 / (B > 0 ? B : 1);
-  if (n > 64) n = 64;
-  if (n < 1) n = 1;
-  int c = (V + n - 1) / n;
-  if (c < 2048) c = 2048;
-  c = (c + 7) / 8 * 8;
-  *chunk = c;
-  *nchunk = (V + c - 1) / c;
+// A row's tiles go to blocks so that about 1024 blocks work in all (4 per compute unit); each block repeats
+// the walk, so a block takes at least one tile and as many as that leaves.
+static void plan_verify(int B, int V, int* ntile, int* per) {
+  const int n = (V + kTile - 1) / kTile;
+  int blocks = 1024 / (B > 0 ? B : 1);
+  if (blocks < 1) blocks = 1;
+  *ntile = n;
+  *per = n > blocks ? (n + blocks - 1) / blocks : 1;
 }
 
 template <int DT>
 static void launch_verify(const VerifyArgs& a, hipStream_t s) {
-  verify_sum_kernel<DT><<<dim3(a.nchunk, a.B), kVerifyThreads, 0, s>>>(a);
+  verify_sum_kernel<DT><<<dim3((a.ntile + a.per - 1) / a.per, a.B), kVerifyThreads, 0, s>>>(a);
   verify_pick_kernel<DT><<<dim3(a.B), kVerifyThreads, 0, s>>>(a);
 }
 
@@ -327,9 +355,9 @@ extern "C" {
 
 int64_t tq_verify_workspace_size(int32_t B, int32_t V) {
   if (B <= 0 || V <= 0) return 0;
-  int chunk, nchunk;
-  plan_verify(B, V, &chunk, &nchunk);
-  return static_cast<int64_t>(B) * nchunk * 2 * 8;
+  int ntile, per;
+  plan_verify(B, V, &ntile, &per);
+  return static_cast<int64_t>(B) * (2 * static_cast<int64_t>(ntile) + kLeftWords) * 8;
 }
 
 int tq_verify_drafts(const int64_t* tokens, const void* target_probs, int32_t dtype, int64_t stb, int64_t stt,
@@ -362,8 +390,9 @@ int tq_verify_drafts(const int64_t* tokens, const void* target_probs, int32_t dt
   a.B = B;
   a.T = T;
   a.V = V;
-  plan_verify(B, V, &a.chunk, &a.nchunk);
+  plan_verify(B, V, &a.ntile, &a.per);
   a.sums = static_cast<double*>(workspace);
+  a.left = static_cast<int64_t*>(workspace) + static_cast<int64_t>(B) * 2 * a.ntile;
   a.path = path;
   a.count = count;
   a.next = next_token;
