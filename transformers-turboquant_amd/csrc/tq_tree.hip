@@ -18,10 +18,11 @@
 // the matrix products do, which is why the decoded operands are shared by the column tiles.
 //
 // Lengths live on the device (a captured graph replays with other lengths), so the split of the
-// keys is made there: all sequences are cut into chunks of one common number of rounds (a
-// round: 32 keys per wave), chosen so that about `slots` chunks exist in all; long
-// sequences get many, short ones few.  A chunk leaves its (maximum, sum, O) in a record; the
-// merge joins a sequence's records, normalises and applies Pi_v.
+// keys is made there: the rounds (32 keys per wave of a block) of all sequences, one after another,
+// are dealt in equal stretches to `slots` blocks per column group and kv head, as many as the device
+// holds at once.  A stretch may end inside a sequence and cover several; each (block,
+// sequence) part leaves its (maximum, sum, O) in a record, and the merge joins a sequence's records,
+// normalises and applies Pi_v.
 #include "tq_decode.h"
 
 namespace tq {
@@ -42,10 +43,9 @@ struct TreeArgs {
   int64_t num_pages;
   int lg_page, maxpos;  // maxpos: positions a table row can hold
   int B, Hq, Hkv, T, G, C;
-  int slots;            // chunks aimed at, over all sequences
-  int nrec;             // records (blocks along x)
+  int slots;            // blocks along x: stretches of the rounds of all sequences
   float coeff, scale;
-  float *part_o, *part_ml;  // records [nrec, Hkv, C, D], [nrec, Hkv, C, 2]
+  float *part_o, *part_ml;  // records [slots + B, Hkv, C, D], [slots + B, Hkv, C, 2]
   const uint16_t* vpit;
   void* out;
   int out_dtype;
@@ -58,60 +58,79 @@ __device__ __forceinline__ int tree_keys(const TreeArgs& a, int b) {
   const int n = a.lengths[b];
   return n >= 0 && n <= a.maxpos - a.T ? n + a.T : 0;
 }
-// Every wave of a block computes the same, 64 sequences per step (one per lane).
+// Inclusive sum over the wave through DPP (shifts within rows of 16 lanes, then row 0's sum into
+// row 1 and row 2's into row 3, then lane 31's into the upper half): no LDS round trips.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int scan64(int v) {
+  v = dpp_add<0x111, 0xF>(v);
+  v = dpp_add<0x112, 0xF>(v);
+  v = dpp_add<0x114, 0xF>(v);
+  v = dpp_add<0x118, 0xF>(v);
+  v = dpp_add<0x142, 0xA>(v);
+  return dpp_add<0x143, 0xC>(v);
+}
+
+// Every wave of a block computes the same, 64 sequences per step (one per lane).  Block k of
+// n = min(slots, R) has the rounds [begin(k), begin(k + 1)) of the R in all: R / n of them, the first
+// R % n blocks one more.  Walking along the rounds, every step to the next part moves to the next
+// block, the next sequence or both, so k + b is a different number for every part, and the
+// parts of one sequence have consecutive ones: the record.
 template <int RK>
 struct TreeSplit {
-  int chunk;  // rounds per chunk
+  int r0, upto0;    // of sequence `lane`: its rounds, and their sum up to it
+  int total;        // rounds of all sequences
+  int blocks;       // that have any: every one of them at least a round
+  int each, extra;  // rounds of a block, blocks with one more
   __device__ __forceinline__ static int rounds(const TreeArgs& a, int b) {
-    return b < a.B ? (tree_keys(a, b) + RK - 1) / RK : 0;
+    return b < a.B ? static_cast<int>(static_cast<unsigned>(tree_keys(a, b) + RK - 1) / RK) : 0;
   }
   __device__ __forceinline__ explicit TreeSplit(const TreeArgs& a) {
     const int lane = threadIdx.x & 63;
-    int total = 0;
-    for (int b = lane; b < a.B; b += 64) total += rounds(a, b);
-#pragma unroll
-    for (int sh = 32; sh >= 1; sh >>= 1) total += __shfl_xor(total, sh, 64);
-    chunk = __builtin_amdgcn_readfirstlane(max(1, (total + a.slots - 1) / a.slots));
+    r0 = rounds(a, lane);
+    upto0 = scan64(r0);
+    total = __builtin_amdgcn_readlane(upto0, 63);
+    for (int b0 = 64; b0 < a.B; b0 += 64) total += __builtin_amdgcn_readlane(scan64(rounds(a, b0 + lane)), 63);
+    blocks = min(a.slots, total);
+    each = blocks ? static_cast<unsigned>(total) / static_cast<unsigned>(blocks) : 0;
+    extra = total - each * blocks;
   }
-  __device__ __forceinline__ static int scan(int v) {  // inclusive sum over the wave
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int sh = 1; sh < 64; sh <<= 1) {
-      const int t = __shfl_up(v, sh, 64);
-      if (lane >= sh) v += t;
-    }
-    return v;
+  __device__ __forceinline__ int begin(int k) const { return k * each + min(k, extra); }
+  __device__ __forceinline__ int block_of(int round) const {
+    const unsigned big = extra * (each + 1), x = round;
+    return x < big ? x / static_cast<unsigned>(each + 1) : extra + (x - big) / static_cast<unsigned>(each);
   }
-  // the sequence of record `rec` and its chunk within the sequence; false behind the last record
-  __device__ __forceinline__ bool find(const TreeArgs& a, int rec, int& b, int& k) const {
-    const int lane = threadIdx.x & 63;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-      const int c = (rounds(a, b0 + lane) + chunk - 1) / chunk;
-      const int upto = scan(c);
-      const uint64_t m = __ballot(rec < upto);
+  // the sequence of round x < total, its first round and its number of rounds
+  __device__ __forceinline__ void sequence_at(const TreeArgs& a, int x, int& b, int& first, int& n) const {
+    int r = r0, upto = upto0;
+    for (int b0 = 0;; b0 += 64) {
+      const uint64_t m = __ballot(x < upto);
       if (m) {
         const int l = __builtin_ctzll(m);
-        b = __builtin_amdgcn_readfirstlane(b0 + l);
-        k = __builtin_amdgcn_readfirstlane(rec - __shfl(upto - c, l, 64));
-        return true;
-      }
-      rec -= __builtin_amdgcn_readfirstlane(__shfl(upto, 63, 64));
-    }
-    return false;
-  }
-  // first record of sequence b and how many it has
-  __device__ __forceinline__ void records(const TreeArgs& a, int b, int& first, int& n) const {
-    const int lane = threadIdx.x & 63;
-    first = 0;
-    for (int b0 = 0;; b0 += 64) {
-      const int c = (rounds(a, b0 + lane) + chunk - 1) / chunk;
-      const int upto = scan(c);
-      if (b < b0 + 64) {
-        first = __builtin_amdgcn_readfirstlane(first + __shfl(upto - c, b - b0, 64));
-        n = __builtin_amdgcn_readfirstlane(__shfl(c, b - b0, 64));
+        b = b0 + l;
+        n = __builtin_amdgcn_readlane(r, l);
+        first = __builtin_amdgcn_readlane(upto, l) - n;
         return;
       }
-      first += __shfl(upto, 63, 64);
+      const int run = __builtin_amdgcn_readlane(upto, 63);
+      r = rounds(a, b0 + 64 + static_cast<int>(threadIdx.x & 63));
+      upto = scan64(r) + run;
+    }
+  }
+  // first round and number of rounds of sequence b
+  __device__ __forceinline__ void rounds_of(const TreeArgs& a, int b, int& first, int& n) const {
+    int r = r0, upto = upto0;
+    for (int b0 = 0;; b0 += 64) {
+      if (b < b0 + 64) {
+        n = __builtin_amdgcn_readlane(r, b - b0);
+        first = __builtin_amdgcn_readlane(upto, b - b0) - n;
+        return;
+      }
+      const int run = __builtin_amdgcn_readlane(upto, 63);
+      r = rounds(a, b0 + 64 + static_cast<int>(threadIdx.x & 63));
+      upto = scan64(r) + run;
     }
   }
 };
@@ -126,8 +145,7 @@ __device__ __forceinline__ uint64_t tree_ancestors(const TreeArgs& a, int b) {
   const bool placed = par >= -1 && par < i;
   uint64_t seen = placed ? 1ull << i : 0;
   int up = placed ? par : -1;
-#pragma unroll
-  for (int k = 0; k < 6; ++k) {
+  for (int reach = 1; reach < a.T; reach <<= 1) {
     const int src = up < 0 ? i : up;
     const uint64_t s = __shfl(seen, src, 64);
     const int u = __shfl(up, src, 64);
@@ -140,6 +158,8 @@ __device__ __forceinline__ uint64_t tree_ancestors(const TreeArgs& a, int b) {
 }
 
 // ---------------------------------------------------------------- attention
+// One object, so that the lookup tables lie at LDS address 0: a lookup's byte offset then is its
+// address (elsewhere every lookup pays an addition, 86 of ~330 VALU instructions a slab).
 template <int D, int BITS, int NT, int NW>
 struct TreeSmem {
   using L = SmallLuts<BITS>;
@@ -148,13 +168,26 @@ struct TreeSmem {
   static constexpr int OFF_K = 0, OFF_S = NK * KC, OFF_V = OFF_S + NK * SC, OFF_N = OFF_V + NK * VC;
   static constexpr int NRM = NK * 4;
   static constexpr int SLOT = OFF_N + 3 * NRM;
-  static constexpr int R = 2;
-  static constexpr int QF = 3 * (D / 32);  // query fragments of a column tile: q_rot, q_proj hi, lo
-  static constexpr int QBYTES = NT > 1 ? NT * QF * 1024 : 0;
+  static constexpr int R = NT == 1 || BITS == 4 ? 3 : 4;  // slabs of a wave in flight: two blocks fit a compute unit
   static constexpr int RING = NW * R * SLOT;
-  static constexpr int MERGE = NW * 16 * (D + 2) * 4;
-  static constexpr int MAIN = RING + QBYTES > MERGE ? RING + QBYTES : MERGE;
+  static constexpr int LDM = D + 4;  // floats of a column in the merge of the waves: O, maximum, sum
+  static constexpr int MERGE = NW * 16 * LDM * 4;
+  // the lo parts of q_proj stay in LDS where the registers would not hold them next to O
+  static constexpr bool LO_LDS = D == 128;
+  uint8_t luts[(L::BYTES + 15) / 16 * 16];
+  __attribute__((aligned(16))) uint8_t area[RING > MERGE ? RING : MERGE];
+  __attribute__((aligned(16))) float fac[NW][3][NK];  // a slab's fa vn_k, fb rn_k, vn_v / vcap
+  __attribute__((aligned(16))) uint8_t lo[LO_LDS ? NT * (D / 32) * 1024 : 16];
+  uint64_t anc[64];
 };
+
+// (f16(x0 y0), f16(x1 y1)), one rounding each
+__device__ __forceinline__ uint32_t mul2_f16(float x0, float y0, float x1, float y1) {
+  uint32_t r;
+  asm("v_fma_mixlo_f16 %0, %1, %2, 0" : "=&v"(r) : "v"(x0), "v"(y0));
+  asm("v_fma_mixhi_f16 %0, %1, %2, 0" : "+v"(r) : "v"(x1), "v"(y1));
+  return r;
+}
 
 template <int D, int BITS, int NT, int NW>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NT == 1 ? 3 : 2)))
@@ -171,181 +204,176 @@ tree_attn_kernel(TreeArgs a) {
   constexpr int VW32 = (VB == 3) ? 2 : 1;
   constexpr int NK = SM::NK, RK = NW * NK;
   constexpr int OFF_K = SM::OFF_K, OFF_S = SM::OFF_S, OFF_V = SM::OFF_V, OFF_N = SM::OFF_N, NRM = SM::NRM;
-  constexpr int SLOT = SM::SLOT, R = SM::R, QF = SM::QF;
+  constexpr int SLOT = SM::SLOT, R = SM::R;
+  constexpr bool LO_LDS = SM::LO_LDS;
   constexpr float LOG2E = 1.4426950408889634f;
   constexpr float TAU = 8.0f;  // a column's reference moves when a score exceeds it by more (log2 units)
   // weights are 2^(s - m + PUP) <= 2^(TAU + PUP): keys down to ~2^-31 of the heaviest still reach
   // the f16 operand P, whose subnormals end at 2^-24, and p vn / vcap stays below the f16 maximum
   constexpr float PUP = 6.0f;
 
-  __shared__ __attribute__((aligned(16))) uint8_t luts[L::BYTES];
-  __shared__ __attribute__((aligned(16))) uint8_t area[SM::MAIN];
-  __shared__ __attribute__((aligned(16))) float fac[NW][3][NK];  // a slab's fa vn_k, fb rn_k, vn_v / vcap
-  __shared__ uint64_t s_anc[64];
-  __shared__ float s_max[NW];
+  __shared__ __attribute__((aligned(16))) SM sm;
+  uint8_t* const luts = sm.luts;
+  uint8_t* const area = sm.area;
   const uint8_t* tS = luts + L::SGN_OFF;
   const uint8_t* tK = luts + L::KEY_OFF;
   const uint8_t* tV = luts + L::VAL_OFF;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, lg = lane >> 4;
-  const int rec = blockIdx.x, ct0 = blockIdx.y * (16 * NT), hkv = blockIdx.z;
+  const int ct0 = blockIdx.y * (16 * NT), hkv = blockIdx.z;
   const TreeSplit<RK> split(a);
-  int b = 0, part = 0;
-  if (!split.find(a, rec, b, part)) return;  // block-uniform
-  const int nkeys = tree_keys(a, b), nctx = nkeys - a.T;
-  const int kbeg = part * split.chunk * RK, kend = min(nkeys, kbeg + split.chunk * RK);
+  if (static_cast<int>(blockIdx.x) >= split.blocks) return;  // block-uniform
+  int x = split.begin(blockIdx.x);
+  const int x_end = split.begin(blockIdx.x + 1);
 
   {
     DecodeArgs t{};
     t.kcent = a.kcent;
     t.vcent = a.vcent;
-    for (int i = tid; i < 256; i += 64 * NW) build_small_luts<BITS, true>(t, luts, i);
+    build_small_luts<BITS, true>(t, luts, tid);
   }
-  const uint64_t anc_lane = tree_ancestors(a, b);
-  if (wave == 0) s_anc[lane] = anc_lane;
-  // drafted tokens that some node sees; the rows of the others count as empty
-  uint64_t live = anc_lane;
-#pragma unroll
-  for (int sh = 32; sh >= 1; sh >>= 1) live |= __shfl_xor(live, sh, 64);
-
-  // ---- the block's queries as B fragments.  q_proj (f32) enters as f16 hi + lo parts, scaled
-  // together by a power of two that keeps both in range (qproj_split_scale)
-  auto qrow_of = [&](int c) {
-    return ((static_cast<int64_t>(b) * a.Hq + hkv * a.G + c % a.G) * a.T + c / a.G) * D;
-  };
-  float qmax = 0.f;
-  for (int c = wave; c < 16 * NT; c += NW) {
-    if (ct0 + c < a.C) {
-      const float* q = a.q_proj + qrow_of(ct0 + c);
-#pragma unroll
-      for (int e = 0; e < D / 64; ++e) qmax = fmaxf(qmax, fabsf(q[e * 64 + lane]));
-    }
-  }
-  qmax = wave_max(qmax);
-  if (lane == 0) s_max[wave] = qmax;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < NW; ++w) qmax = fmaxf(qmax, s_max[w]);
-  const float qs = qproj_split_scale(qmax);
   const float fa = a.scale * LOG2E;
-  const float fb = a.coeff * fa / qs;
-
-  uint64_t anc[NT];  // of the lane's column in each tile
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int c = ct0 + 16 * t + l16;
-    anc[t] = c < a.C ? s_anc[c / a.G] : 0;
-  }
-  half8 qreg[NT == 1 ? QF : 1];
-  uint8_t* const qlds = area + SM::RING;
-  auto fragments = [&](int t, half8 (&f)[QF]) {
-    const int c = ct0 + 16 * t + l16;
-    const int64_t row = c < a.C ? qrow_of(c) : 0;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int d0 = lg * (D / 4) + ks * 8;
-      half8 hi = half8{}, lo = half8{}, r = half8{};
-      if (c < a.C) {
-        split8s(a.q_proj + row + d0, qs, hi, lo);
-        r = *reinterpret_cast<const half8*>(a.q_rot + row + d0);
-      }
-      f[ks] = r;
-      f[KS + ks] = hi;
-      f[2 * KS + ks] = lo;
-    }
-  };
-  if constexpr (NT == 1) {
-    fragments(0, qreg);
-  } else {
-    for (int t = wave; t < NT; t += NW) {
-      half8 f[QF];
-      fragments(t, f);
-#pragma unroll
-      for (int i = 0; i < QF; ++i) *reinterpret_cast<half8*>(qlds + ((t * QF + i) * 64 + lane) * 16) = f[i];
-    }
-  }
-  auto qfrag = [&](int t, int f) -> half8 {
-    if constexpr (NT == 1) return qreg[f];
-    else return *reinterpret_cast<const half8*>(qlds + ((t * QF + f) * 64 + lane) * 16);
-  };
-
-  // ---- the stream
   const int vbit = l16 * VFB, vbase = (vbit >> 5) * 4, vshift = vbit & 31;
   uint8_t* const mine = area + wave * (R * SLOT);
   const uint32_t mine_lds = lds_offset(mine);
-  constexpr int NKD = (NK * KC + 1023) / 1024, NSD = (NK * SC + 1023) / 1024, NVD = (NK * VC + 1023) / 1024;
-  constexpr int NDMA = NKD + NSD + NVD + 3;
-  auto copy_plane = [&](const i32x4& r, uint32_t dst, int bytes, int nrounds) {
-    const uint32_t lo = lane * 16;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      if (c >= nrounds) break;
-      if ((c + 1) * 1024 <= bytes || lane * 16 < bytes - c * 1024) dma16(r, dst + c * 1024, lo + c * 1024);
-    }
-  };
-  // rows of a slab that exist: up to the chunk's last key, none where its page is not in the pool.
-  // A slab's 32 keys lie in one page (pages hold 32 or more, slabs start at multiples of 32).
-  auto page_of = [&](int kb) -> int {
-    const int p = a.table[b * a.ld_table + (kb >> a.lg_page)];
-    return __builtin_amdgcn_readfirstlane(p);
-  };
-  auto issue = [&](int kb, int slot) {
-    const int page = page_of(kb);
-    const bool in = page >= 0 && page < a.num_pages;
-    const int64_t row = in ? ((static_cast<int64_t>(page) * a.Hkv + hkv) << a.lg_page) + (kb & ((1 << a.lg_page) - 1)) : 0;
-    const int rows = in ? min(NK, kend - kb) : 0;
-    const uint32_t dst = mine_lds + slot * SLOT;
-    wait_lds();  // earlier reads of this slot have landed
-    copy_plane(rows_desc(a.kcodes + row * KC, KC, 0, rows), dst + OFF_K, NK * KC, NKD);
-    copy_plane(rows_desc(a.ksigns + row * SC, SC, 0, rows), dst + OFF_S, NK * SC, NSD);
-    copy_plane(rows_desc(a.vcodes + row * VC, VC, 0, rows), dst + OFF_V, NK * VC, NVD);
-    if (lane < 32) {
-      dma_u16(rows_desc(a.kvn + row, 2, 0, rows), dst + OFF_N, lane * 2);
-      dma_u16(rows_desc(a.krn + row, 2, 0, rows), dst + OFF_N + NRM, lane * 2);
-      dma_u16(rows_desc(a.vvn + row, 2, 0, rows), dst + OFF_N + 2 * NRM, lane * 2);
-    }
-  };
-  auto wait_slot = [&](int later) {
-    if (later >= 1) wait_vm<NDMA>();
-    else wait_vm<0>();
-  };
+  float (*fw)[NK] = sm.fac[wave];
 
-  float m_run[NT], l_run[NT];
-  // value norms enter P as vn / vcap <= 1; vcap is a power of two that only grows (O is rescaled
-  // when it does) and multiplies O back at the end
-  float vcap = 0x1p-24f, inv_vcap = 0x1p24f;
-  float4v oacc[NT][DB];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    m_run[t] = -INFINITY;
-    l_run[t] = 0.f;
-#pragma unroll
-    for (int db = 0; db < DB; ++db) oacc[t][db] = float4v{0.f, 0.f, 0.f, 0.f};
-  }
-  float (*fw)[NK] = fac[wave];
+  // ---- one part after the other: the rounds of this block's stretch that belong to one sequence
+  while (x < x_end) {
+    int b, first, n;
+    split.sequence_at(a, x, b, first, n);
+    const int rec = static_cast<int>(blockIdx.x) + b;
+    const int nkeys = tree_keys(a, b), nctx = nkeys - a.T;
+    const int kbeg = (x - first) * RK, kend = min(nkeys, (min(x_end, first + n) - first) * RK);
+    x = min(x_end, first + n);
 
-  auto slab = [&](const uint8_t* src, int ks0) {
-    const int page = page_of(ks0);
-    const int rows = page >= 0 && page < a.num_pages ? min(NK, kend - ks0) : 0;
-    const bool edge = rows < NK || ks0 + NK > nctx;  // wave-uniform: a visibility to look up
-    // ---- per-key factors, one value per lane and pass; keys that nobody sees get zeros
+    const uint64_t anc_lane = tree_ancestors(a, b);
+    if (wave == 0) sm.anc[lane] = anc_lane;
+    const uint64_t live = __ballot(anc_lane != 0);  // tokens with a place: some node sees them
+    __syncthreads();  // tables and ancestors in place; the previous part's merge is done with the area
+
+    // ---- the stream
+    constexpr int NKD = (NK * KC + 1023) / 1024, NSD = (NK * SC + 1023) / 1024, NVD = (NK * VC + 1023) / 1024;
+    constexpr int NDMA = NKD + NSD + NVD + 3;
+    auto copy_plane = [&](const i32x4& r, uint32_t dst, int bytes, int nrounds) {
+      const uint32_t lo = lane * 16;
 #pragma unroll
-    for (int i0 = 0; i0 < 3 * NK; i0 += 64) {
-      const int i = i0 + lane, which = i / NK, k = i % NK;
-      float v = (i < 3 * NK)
-          ? h2f(static_cast<uint16_t>(*reinterpret_cast<const uint32_t*>(src + OFF_N + which * NRM + k * 4)))
-          : 0.f;
-      if (edge) {
-        const int t = ks0 + k - nctx;
-        if (k >= rows || (t >= 0 && !((live >> (t & 63)) & 1))) v = 0.f;
+      for (int c = 0; c < 4; ++c) {
+        if (c >= nrounds) break;
+        if ((c + 1) * 1024 <= bytes || lane * 16 < bytes - c * 1024) dma16(r, dst + c * 1024, lo + c * 1024);
       }
-      if (i0 + 63 >= 2 * NK) {  // this pass holds value norms: keep them <= vcap
-        const float vv = (which == 2) ? v : 0.f;
-        if (__any(vv > vcap)) {
-          float t = fminf(vv, 65504.f);
+    };
+    // A slab's 32 keys lie in one page (pages hold 32 or more, slabs start at multiples of 32)
+    // (a scalar load, through the constant address space: a vector load's wait would reach
+    // back past the copies in flight)
+    typedef const __attribute__((address_space(4))) int32_t* const_i32;
+    const const_i32 pages = (const_i32)reinterpret_cast<uintptr_t>(a.table + b * a.ld_table);
+    auto page_of = [&](int kb) -> int { return pages[kb >> a.lg_page]; };
+    // copy the slab of keys [kb, kb + 32) into a slot; returns how many of its rows exist: up to the
+    // part's last key, none where its page is not in the pool
+    auto issue = [&](int kb, int page, int slot) -> int {
+      const bool in = page >= 0 && page < a.num_pages;
+      const int64_t row = in ? ((static_cast<int64_t>(page) * a.Hkv + hkv) << a.lg_page) + (kb & ((1 << a.lg_page) - 1)) : 0;
+      const int rows = in ? min(NK, kend - kb) : 0;
+      const uint32_t dst = mine_lds + slot * SLOT;
+      wait_lds();  // earlier reads of this slot have landed
+      copy_plane(rows_desc(a.kcodes + row * KC, KC, 0, rows), dst + OFF_K, NK * KC, NKD);
+      copy_plane(rows_desc(a.ksigns + row * SC, SC, 0, rows), dst + OFF_S, NK * SC, NSD);
+      copy_plane(rows_desc(a.vcodes + row * VC, VC, 0, rows), dst + OFF_V, NK * VC, NVD);
+      if (lane < 32) {
+        dma_u16(rows_desc(a.kvn + row, 2, 0, rows), dst + OFF_N, lane * 2);
+        dma_u16(rows_desc(a.krn + row, 2, 0, rows), dst + OFF_N + NRM, lane * 2);
+        dma_u16(rows_desc(a.vvn + row, 2, 0, rows), dst + OFF_N + 2 * NRM, lane * 2);
+      }
+      return rows;
+    };
+    auto wait_slot = [&](int later) {  // until the slot issued `later` slots ago has landed
+      static_assert(R <= 4 && 3 * NDMA < 64, "ring of at most 4 slots");
+      if (R >= 4 && later >= 3) wait_vm<(R >= 4 ? 3 * NDMA : 0)>();
+      else if (R >= 3 && later >= 2) wait_vm<(R >= 3 ? 2 * NDMA : 0)>();
+      else if (later >= 1) wait_vm<NDMA>();
+      else wait_vm<0>();
+    };
+    // the first slabs fly while the queries are set up
+    const int k0w = kbeg + wave * NK;
+    int nrows[R];
 #pragma unroll
-          for (int sh = 32; sh >= 1; sh >>= 1) t = fmaxf(t, __shfl_xor(t, sh, 64));
+    for (int r = 0; r < R; ++r) nrows[r] = k0w + r * RK < kend ? issue(k0w + r * RK, page_of(k0w + r * RK), r) : 0;
+
+
+    // ---- the block's queries as B fragments, the same in every wave.  q_proj (f32) enters as f16 hi + lo
+    // parts, scaled together by a power of two that keeps both in range (qproj_split_scale)
+    // (columns behind the last repeat it; they are not stored)
+    uint64_t anc[NT];  // of the lane's column in each tile
+    half8 qr[NT][KS], qh[NT][KS], ql[LO_LDS ? 1 : NT][KS];
+    float qmax = 0.f;
+    const float* qp[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int c = min(ct0 + 16 * t + l16, a.C - 1), node = c / a.G;
+      const int64_t row = ((static_cast<int64_t>(b) * a.Hq + hkv * a.G + (c - node * a.G)) * a.T + node) * D + lg * (D / 4);
+      anc[t] = sm.anc[node];
+      qp[t] = a.q_proj + row;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        qmax = fmaxf(qmax, absmax8(qp[t] + ks * 8));
+        qr[t][ks] = *reinterpret_cast<const half8*>(a.q_rot + row + ks * 8);
+      }
+    }
+    const float qs = qproj_split_scale(wave_max(qmax));
+    const float fb = a.coeff * fa / qs;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        half8 lo;
+        split8s(qp[t] + ks * 8, qs, qh[t][ks], lo);
+        if constexpr (!LO_LDS) ql[t][ks] = lo;
+        else if (wave == 0) *reinterpret_cast<half8*>(sm.lo + ((t * KS + ks) * 64 + lane) * 16) = lo;
+      }
+    if constexpr (LO_LDS) __syncthreads();
+    auto qlo = [&](int t, int ks) -> half8 {
+      if constexpr (!LO_LDS) return ql[t][ks];
+      else return *reinterpret_cast<const half8*>(sm.lo + ((t * KS + ks) * 64 + lane) * 16);
+    };
+
+    // column state: reference mref = m - PUP (0 until the column has a maximum m), the threshold a
+    // score relative to mref must exceed to move it (-inf until then, TAU + PUP after), the sum
+    float mref[NT], thr[NT], l_run[NT];
+    // value norms enter P as vn / vcap <= 1; vcap is a power of two that only grows (O is rescaled
+    // when it does) and multiplies O back at the end
+    float vcap = 0x1p-24f, inv_vcap = 0x1p24f;
+    float4v oacc[NT][DB];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      mref[t] = 0.f;
+      thr[t] = -INFINITY;
+      l_run[t] = 0.f;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) oacc[t][db] = float4v{0.f, 0.f, 0.f, 0.f};
+    }
+
+    auto slab = [&](const uint8_t* src, int ks0, int rows) {
+      const bool edge = rows < NK || ks0 + NK > nctx;  // wave-uniform: a visibility to look up
+      // bit k: key ks0 + k is one of the slab's rows and cached, or a drafted token in `tokens`
+      auto visible = [&](uint64_t tokens) -> uint32_t {
+        const int d = nctx - ks0;  // slab bit of the first drafted token
+        const uint64_t cached = d <= 0 ? 0 : d >= 32 ? ~0ull : (1ull << d) - 1;
+        const uint64_t drafted = d <= -64 || d >= 32 ? 0 : d >= 0 ? tokens << d : tokens >> -d;
+        return static_cast<uint32_t>((cached | drafted) & ((1ull << rows) - 1));
+      };
+      // ---- per-key factors: lanes 0-31 fa vn_k, lanes 32-63 fb rn_k, then lanes 0-31 vn_v / vcap
+      {
+        const int k = lane & 31;
+        const uint8_t* nsrc = src + OFF_N + k * 4;
+        float v = h2f(static_cast<uint16_t>(*reinterpret_cast<const uint32_t*>(nsrc + (lane >> 5) * NRM)));
+        float nv = h2f(static_cast<uint16_t>(*reinterpret_cast<const uint32_t*>(nsrc + 2 * NRM)));
+        if (edge && !((visible(live) >> k) & 1)) v = nv = 0.f;  // seen by nobody, whatever its row holds
+        if (__any(nv > vcap)) {
+          float t = fminf(nv, 65504.f);
+#pragma unroll
+          for (int sh = 16; sh >= 1; sh >>= 1) t = fmaxf(t, __shfl_xor(t, sh, 64));
           int ex;
           frexpf(t, &ex);  // t < 2^ex; every lane holds the same t
           ex = __builtin_amdgcn_readfirstlane(ex);
@@ -360,199 +388,233 @@ tree_attn_kernel(TreeArgs a) {
             inv_vcap = ldexpf(1.f, -ex);
           }
         }
+        (&fw[0][0])[lane] = v * (lane < 32 ? fa : fb);
+        if (lane < 32) fw[2][k] = nv * inv_vcap;
       }
-      if (i < 3 * NK) fw[which][k] = (which == 0) ? fa * v : (which == 1 ? fb * v : v * inv_vcap);
-    }
-    // ---- the slab's key operands, shared by the column tiles
-    half8 kc[2][KS], sg[2][KS];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      uint32_t kw[KW32];
-      load_key_field<KLANE>(src + OFF_K + (16 * j + l16) * KC + lg * KLANE, kw);
-      const uint32_t sw = load_sign_field<D>(src + OFF_S + (16 * j + l16) * SC + lg * SLANE);
-      static_for<KS>([&](auto cc) {
-        constexpr int ks = decltype(cc)::value;
-        kc[j][ks] = key_operand<KB, KW32, ks>(tK, kw);
-        sg[j][ks] = nib2x4<ks>(tS, sw);
-      });
-    }
-    // ---- scores, softmax step and P of one column tile after the other
-    half8 pb[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float4v s1[2], s2[2];
+      // ---- scores S^T = K^ Q^T (term 1) and Sign Q_proj^T (term 2); a key operand feeds every tile
+      float4v s1[NT][2], s2[NT][2];
+      uint32_t kw[2][KW32], sw[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        s1[j] = float4v{0.f, 0.f, 0.f, 0.f};
-        s2[j] = float4v{0.f, 0.f, 0.f, 0.f};
-      }
+        load_key_field<KLANE>(src + OFF_K + (16 * j + l16) * KC + lg * KLANE, kw[j]);
+        sw[j] = load_sign_field<D>(src + OFF_S + (16 * j + l16) * SC + lg * SLANE);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const half8 qr = qfrag(t, ks), qh = qfrag(t, KS + ks), ql = qfrag(t, 2 * KS + ks);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          s1[j] = mfma16x16x32(kc[j][ks], qr, s1[j]);
-          s2[j] = mfma16x16x32(sg[j][ks], qh, s2[j]);
-          s2[j] = mfma16x16x32(sg[j][ks], ql, s2[j]);
+        for (int t = 0; t < NT; ++t) {
+          s1[t][j] = float4v{0.f, 0.f, 0.f, 0.f};
+          s2[t][j] = float4v{0.f, 0.f, 0.f, 0.f};
         }
       }
-      float sc[2][4];  // log2-domain scores of keys ks0 + 16j + 4lg + e for this lane's column
+      static_for<KS>([&](auto cc) {
+        constexpr int ks = decltype(cc)::value;
+        half8 sg[2], kc[2], lo[NT];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) sg[j] = nib2x4<ks>(tS, sw[j]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) kc[j] = key_operand<KB, KW32, ks>(tK, kw[j]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) lo[t] = qlo(t, ks);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) s2[t][j] = mfma16x16x32(sg[j], qh[t][ks], s2[t][j]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) s1[t][j] = mfma16x16x32(kc[j], qr[t][ks], s1[t][j]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) s2[t][j] = mfma16x16x32(sg[j], lo[t], s2[t][j]);
+        if constexpr (LO_LDS) __builtin_amdgcn_sched_barrier(0);  // one step's operands at a time
+      });
+      // ---- softmax step and P of each tile; the lane's keys are ks0 + 16j + 4lg + e
+      float4v ka[2], kb[2], nv[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float4v ka = *reinterpret_cast<const float4v*>(&fw[0][16 * j + 4 * lg]);
-        const float4v kb2 = *reinterpret_cast<const float4v*>(&fw[1][16 * j + 4 * lg]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sc[j][e] = fmaf(s2[j][e], kb2[e], s1[j][e] * ka[e]);
+        ka[j] = *reinterpret_cast<const float4v*>(&fw[0][16 * j + 4 * lg]);
+        kb[j] = *reinterpret_cast<const float4v*>(&fw[1][16 * j + 4 * lg]);
+        nv[j] = *reinterpret_cast<const float4v*>(&fw[2][16 * j + 4 * lg]);
       }
-      if (edge) {
+      half8 pb[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float sc[2][4];  // log2-domain scores relative to mref
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[j][e] = fmaf(s1[t][j][e], ka[j][e], fmaf(s2[t][j][e], kb[j][e], -mref[t]));
+        if (edge) {
+          const uint32_t see = visible(anc[t]) >> (4 * lg);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[j][e] = see & (1u << (16 * j + e)) ? sc[j][e] : -INFINITY;
+        }
+        const float lmax = max8_raw(sc[0][0], sc[0][1], sc[0][2], sc[0][3], sc[1][0], sc[1][1], sc[1][2], sc[1][3]);
+        if (__any(lmax > thr[t])) {
+          float m = lmax;
+          m = fmaxf(m, __shfl_xor(m, 16, 64));
+          m = fmaxf(m, __shfl_xor(m, 32, 64));
+          if (m > thr[t]) {
+            const float shift = m - PUP;
+            const float alpha = (thr[t] == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(-shift);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sc[j][e] -= shift;
+            mref[t] += shift;
+            thr[t] = TAU + PUP;
+            l_run[t] *= alpha;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) oacc[t][db] *= alpha;
+          }
+        }
+        float p[2][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int k = 16 * j + 4 * lg + e, d = ks0 + k - nctx;
-            const bool sees = k < rows && (d < 0 || ((anc[t] >> (d & 63)) & 1));
-            if (!sees) sc[j][e] = -INFINITY;
+            p[j][e] = __builtin_amdgcn_exp2f(sc[j][e]);
+            l_run[t] += p[j][e];
           }
-      }
-      const float lmax = max8_raw(sc[0][0], sc[0][1], sc[0][2], sc[0][3], sc[1][0], sc[1][1], sc[1][2], sc[1][3]);
-      if (__any(lmax > m_run[t] + TAU)) {
-        float x = lmax;
-        x = fmaxf(x, __shfl_xor(x, 16, 64));
-        x = fmaxf(x, __shfl_xor(x, 32, 64));
-        if (x > m_run[t] + TAU) {
-          const float alpha = (m_run[t] == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(m_run[t] - x);
-          m_run[t] = x;
-          l_run[t] *= alpha;
+        u32x4 w;
+        if (edge) {  // a masked key's norm may be anything: it takes no part in the product
 #pragma unroll
-          for (int db = 0; db < DB; ++db) oacc[t][db] *= alpha;
+          for (int i = 0; i < 4; ++i) {
+            const int j = i >> 1, e = 2 * (i & 1);
+            w[i] = mul2_f16(p[j][e], sc[j][e] == -INFINITY ? 0.f : nv[j][e], p[j][e + 1],
+                            sc[j][e + 1] == -INFINITY ? 0.f : nv[j][e + 1]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = i >> 1, e = 2 * (i & 1);
+            w[i] = mul2_f16(p[j][e], nv[j][e], p[j][e + 1], nv[j][e + 1]);
+          }
         }
+        pb[t] = __builtin_bit_cast(half8, w);
       }
-      const float m_use = (m_run[t] == -INFINITY) ? 0.f : m_run[t] - PUP;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float4v nv = *reinterpret_cast<const float4v*>(&fw[2][16 * j + 4 * lg]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p = __builtin_amdgcn_exp2f(sc[j][e] - m_use);
-          l_run[t] += p;
-          // a masked key's norm may be anything: it takes no part in the product
-          const float pv = edge && sc[j][e] == -INFINITY ? 0.f : p * nv[e];
-          pb[t][4 * j + e] = static_cast<_Float16>(pv);
-        }
-      }
-    }
-    // ---- O^T += V^T (P vn)^T over the slab's 32 keys: K slot 8lg + 4j + e is key 16j + 4lg + e;
-    // an A dword is one dim of a key pair, read from the pair table after interleaving the two
-    // keys' code fields (parity 0: even dims, 1: odd dims)
-    constexpr uint32_t M = odd_fields<VB>();
-    uint32_t w[2][4];
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        const uint32_t* vp = reinterpret_cast<const uint32_t*>(src + OFF_V + (16 * j + 4 * lg + kk) * VC + vbase);
-        if constexpr (VW32 == 2) w[j][kk] = __builtin_amdgcn_alignbit(vp[1], vp[0], vshift);
-        else w[j][kk] = vp[0] >> vshift;
-      }
-#pragma unroll
-    for (int par = 0; par < 2; ++par) {
-      uint32_t f[2][2];
+      // ---- O^T += V^T (P vn)^T over the slab's 32 keys: K slot 8lg + 4j + e is key 16j + 4lg + e;
+      // an A dword is one dim of a key pair, read from the pair table after interleaving the two
+      // keys' code fields (parity 0: even dims, 1: odd dims)
+      constexpr uint32_t M = odd_fields<VB>();
+      uint32_t w[2][4];
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint32_t wa = w[j][2 * c], wb = w[j][2 * c + 1];
-          f[j][c] = par ? bfi32(M, wb, wa >> VB) : bfi32(M, wb << VB, wa);
+        for (int kk = 0; kk < 4; ++kk) {
+          const uint32_t* vp = reinterpret_cast<const uint32_t*>(src + OFF_V + (16 * j + 4 * lg + kk) * VC + vbase);
+          if constexpr (VW32 == 2) w[j][kk] = __builtin_amdgcn_alignbit(vp[1], vp[0], vshift);
+          else w[j][kk] = vp[0] >> vshift;
         }
-      static_for<NPAIR>([&](auto ic) {
-        constexpr int i = decltype(ic)::value;
-        const half8 va = __builtin_bit_cast(half8, u32x4{value_pair<VB, i>(tV, f[0][0]), value_pair<VB, i>(tV, f[0][1]),
-                                                         value_pair<VB, i>(tV, f[1][0]), value_pair<VB, i>(tV, f[1][1])});
 #pragma unroll
-        for (int t = 0; t < NT; ++t) oacc[t][2 * i + par] = mfma16x16x32(va, pb[t], oacc[t][2 * i + par]);
-      });
-    }
-  };
-
-  __builtin_amdgcn_s_waitcnt(0);  // no load of the compiler's own reaches back past a copy
-  const int k0w = kbeg + wave * NK;
+      for (int par = 0; par < 2; ++par) {
+        uint32_t f[2][2];
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-    if (k0w + r * RK < kend) issue(k0w + r * RK, r);
-  __syncthreads();  // tables and queries in place
-  for (int k0 = k0w; k0 < kend; k0 += R * RK) {
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int ks0 = k0 + r * RK;
-      if (ks0 < kend) {
-        wait_slot(ks0 + RK < kend ? 1 : 0);
-        slab(mine + r * SLOT, ks0);
-        if (ks0 + R * RK < kend) issue(ks0 + R * RK, r);
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t wa = w[j][2 * c], wb = w[j][2 * c + 1];
+            f[j][c] = par ? bfi32(M, wb, wa >> VB) : bfi32(M, wb << VB, wa);
+          }
+        static_for<NPAIR>([&](auto ic) {
+          constexpr int i = decltype(ic)::value;
+          const half8 va = __builtin_bit_cast(half8, u32x4{value_pair<VB, i>(tV, f[0][0]), value_pair<VB, i>(tV, f[0][1]),
+                                                           value_pair<VB, i>(tV, f[1][0]), value_pair<VB, i>(tV, f[1][1])});
+#pragma unroll
+          for (int t = 0; t < NT; ++t) oacc[t][2 * i + par] = mfma16x16x32(va, pb[t], oacc[t][2 * i + par]);
+        });
       }
-    }
-  }
+    };
 
-  // ---- the waves' states joined in LDS, one column tile at a time (rings and queries are done)
-  float* const mrg = reinterpret_cast<float*>(area);  // [wave][column][D + 2]
-  const int64_t base = (static_cast<int64_t>(rec) * a.Hkv + hkv) * a.C + ct0;
+    int slot = 0;
+    for (int ks0 = k0w; ks0 < kend; ks0 += RK) {
+      // the next R - 1 slabs, as far as they exist, were issued after this one
+      const int later = (kend - 1 - ks0) / RK;
+      const bool more = later >= R;
+      const int page = more ? page_of(ks0 + R * RK) : -1;  // read ahead of the slab's work
+      wait_slot(later);
+      slab(mine + slot * SLOT, ks0, nrows[0]);
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    __syncthreads();
-    float l = l_run[t];
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    float* my = mrg + (wave * 16 + l16) * (D + 2);
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) my[(lg * 4 + e) * DB + db] = oacc[t][db][e] * vcap;
-    if (lg == 0) {
-      // a node without a place leaves an empty record; a column of NaN scores, whose maximum never
-      // moved, a NaN one
-      my[D] = !anc[t] ? -INFINITY : (m_run[t] == -INFINITY && l != l) ? 0.f : m_run[t];
-      my[D + 1] = l;
+      for (int r = 1; r < R; ++r) nrows[r - 1] = nrows[r];
+      if (more) nrows[R - 1] = issue(ks0 + R * RK, page, slot);
+      slot = slot + 1 == R ? 0 : slot + 1;
     }
-    __syncthreads();
-    const int ncol = min(16, a.C - ct0 - 16 * t);
-    for (int it = tid; it < ncol * D; it += 64 * NW) {
-      const int c = it / D, d = it % D;
-      float mx = -INFINITY;
+
+    // ---- the waves' states joined in LDS, one column tile at a time (the rings are done); thread
+    // (column tid / 16, dims DB (tid % 16) ..) joins
+    constexpr int LDM = SM::LDM;
+    float* const mrg = reinterpret_cast<float*>(area);  // [wave][column][LDM]
+    const int64_t base = (static_cast<int64_t>(rec) * a.Hkv + hkv) * a.C + ct0;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) mx = fmaxf(mx, mrg[(w * 16 + c) * (D + 2) + D]);
-      float o = 0.f, ls = 0.f;
+    for (int t = 0; t < NT; ++t) {
+      __syncthreads();
+      float l = l_run[t];
+      l += __shfl_xor(l, 16, 64);
+      l += __shfl_xor(l, 32, 64);
+      float* const my = mrg + (wave * 16 + l16) * LDM;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const float* s = mrg + (w * 16 + c) * (D + 2);
-        if (s[D] != -INFINITY) {
-          const float f = __builtin_amdgcn_exp2f(s[D] - mx);
-          o += f * s[d];
-          ls += f * s[D + 1];
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int db = 0; db < DB; db += 4)
+          *reinterpret_cast<float4v*>(my + (lg * 4 + e) * DB + db) =
+              float4v{oacc[t][db][e], oacc[t][db + 1][e], oacc[t][db + 2][e], oacc[t][db + 3][e]} * vcap;
+      if (lg == 0) {
+        // a node without a place leaves an empty record; a column of NaN scores, whose maximum never
+        // moved, a NaN one
+        my[D] = !anc[t] || (thr[t] == -INFINITY && l == l) ? -INFINITY : mref[t];
+        my[D + 1] = l;
+      }
+      __syncthreads();
+      const int c = tid >> 4, d0 = (tid & 15) * DB;
+      if (tid < 256 && ct0 + 16 * t + c < a.C) {
+        float m[NW], mx = -INFINITY, ls = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          m[w] = mrg[(w * 16 + c) * LDM + D];
+          mx = fmaxf(mx, m[w]);
         }
-      }
-      a.part_o[(base + 16 * t + c) * D + d] = o;
-      if (d == 0) {
-        a.part_ml[(base + 16 * t + c) * 2] = mx;
-        a.part_ml[(base + 16 * t + c) * 2 + 1] = ls;
+        float4v o[DB / 4];
+#pragma unroll
+        for (int i = 0; i < DB / 4; ++i) o[i] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const float* s = mrg + (w * 16 + c) * LDM;
+          const float f = m[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[w] - mx);
+          const float lw = s[D + 1];
+          ls += f == 0.f ? 0.f : f * lw;
+#pragma unroll
+          for (int i = 0; i < DB / 4; ++i) {
+            const float4v x4 = *reinterpret_cast<const float4v*>(s + d0 + 4 * i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] += f == 0.f ? 0.f : f * x4[e];
+          }
+        }
+        const int64_t at = base + 16 * t + c;
+#pragma unroll
+        for (int i = 0; i < DB / 4; ++i) *reinterpret_cast<float4v*>(a.part_o + at * D + d0 + 4 * i) = o[i];
+        if ((tid & 15) == 0) {
+          a.part_ml[at * 2] = mx;
+          a.part_ml[at * 2 + 1] = ls;
+        }
       }
     }
   }
 }
 
 // ---------------------------------------------------------------- merge
-// One block per (sequence, kv head, 16 columns): wave w joins columns w, w + 4, ... (the records'
-// maxima and weights one per lane, then D / 64 dims per lane summed over the records), then
-// out^T = Pi_v^T o^T on MFMA with both operands split into f16 hi + lo.
-template <int D, int RK>
+// One block per (sequence, kv head, 4 CW columns): wave w joins columns w, w + 4, ... (the records'
+// maxima and weights one per lane, then D / 64 dims per lane summed over the records, 16 of them in
+// flight), then out^T = Pi_v^T o^T on MFMA with both operands split into f16 hi + lo.  CW = 1 has the fewest
+// dependent round trips, CW = 4 reads Pi_v a quarter as often.
+template <int D, int RK, int CW>
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
-  constexpr int PL = D / 64, RB = D / 64;
+  constexpr int PL = D / 64, RB = D / 64, NC = 4 * CW, NB = 16;
   typedef float floatPL __attribute__((ext_vector_type(PL)));
-  __shared__ __attribute__((aligned(16))) float o_s[16][D + 4];
-  __shared__ float s_up[16];
-  const int c0 = blockIdx.x * 16, hkv = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  __shared__ __attribute__((aligned(16))) float o_s[NC][D + 4];
+  __shared__ float s_up[NC];
+  const int c0 = blockIdx.x * NC, hkv = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6, l16 = lane & 15, lg = lane >> 4;
-  const TreeSplit<RK> split(a);
-  int first = 0, n = 0;
-  split.records(a, b, first, n);
 
   const _Float16* Ph = reinterpret_cast<const _Float16*>(a.vpit);
   const _Float16* Pl = Ph + D * D;
@@ -566,37 +628,51 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
       al[rb][ks] = *reinterpret_cast<const half8*>(Pl + i * D + ks * 32 + lg * 8);
     }
   }
+  const TreeSplit<RK> split(a);
+  int first = 0, n = 0;
+  split.rounds_of(a, b, first, n);
+  if (n > 0) {  // records k + b of the blocks k that hold the sequence's rounds
+    const int k0 = split.block_of(first), k1 = split.block_of(first + n - 1);
+    first = k0 + b;
+    n = k1 - k0 + 1;
+  }
   const int64_t step = static_cast<int64_t>(a.Hkv) * a.C;  // columns between records
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < CW; ++k) {
     const int cc = wave + 4 * k, c = c0 + cc;
     floatPL o = floatPL{};
     if (c < a.C) {
       const int64_t at = (static_cast<int64_t>(first) * a.Hkv + hkv) * a.C + c;
       const float* ml = a.part_ml + at * 2;
       const float* src = a.part_o + at * D + PL * lane;
-      float mx = -INFINITY;
-      for (int r = lane; r < n; r += 64) mx = fmaxf(mx, ml[r * step * 2]);
+      floatPL v[NB];
+#pragma unroll
+      for (int q = 0; q < NB; ++q) v[q] = q < n ? *reinterpret_cast<const floatPL*>(src + q * step * D) : floatPL{};
+      const float m_first = lane < n ? ml[lane * step * 2] : -INFINITY;
+      const float l_first = lane < n ? ml[lane * step * 2 + 1] : 0.f;
+      float mx = m_first;
+      for (int r = lane + 64; r < n; r += 64) mx = fmaxf(mx, ml[r * step * 2]);
 #pragma unroll
       for (int sh = 32; sh >= 1; sh >>= 1) mx = fmaxf(mx, __shfl_xor(mx, sh, 64));
       float lsum = 0.f;
       for (int r0 = 0; r0 < n; r0 += 64) {
         float w = 0.f;
         if (r0 + lane < n) {
-          const float m = ml[(r0 + lane) * step * 2];
+          const float m = r0 == 0 ? m_first : ml[(r0 + lane) * step * 2];
           if (m != -INFINITY) {
             w = __builtin_amdgcn_exp2f(m - mx);
-            lsum += w * ml[(r0 + lane) * step * 2 + 1];
+            lsum += w * (r0 == 0 ? l_first : ml[(r0 + lane) * step * 2 + 1]);
           }
         }
         const int nb = min(64, n - r0);
-        for (int u = 0; u < nb; u += 8) {
-          floatPL v[8];
+        for (int u = 0; u < nb; u += NB) {
+          if (r0 + u > 0) {
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            v[q] = u + q < nb ? *reinterpret_cast<const floatPL*>(src + (r0 + u + q) * step * D) : floatPL{};
+            for (int q = 0; q < NB; ++q)
+              v[q] = u + q < nb ? *reinterpret_cast<const floatPL*>(src + (r0 + u + q) * step * D) : floatPL{};
+          }
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const float ww = __shfl(w, (u + q) & 63, 64);
+          for (int q = 0; q < NB; ++q) {
+            const float ww = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), u + q));
 #pragma unroll
             for (int e = 0; e < PL; ++e) o[e] = fmaf(ww, v[q][e], o[e]);
           }
@@ -623,20 +699,21 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
   }
   __syncthreads();
 
-  const float up = s_up[l16];
+  const int lc = l16 & (NC - 1);  // with fewer than 16 columns the others repeat them and are not stored
+  const float up = s_up[lc];
   half8 bh[D / 32], bl[D / 32];
 #pragma unroll
   for (int ks = 0; ks < D / 32; ++ks)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       _Float16 h, lo;
-      split_f16(o_s[l16][ks * 32 + lg * 8 + e] * up, h, lo);
+      split_f16(o_s[lc][ks * 32 + lg * 8 + e] * up, h, lo);
       bh[ks][e] = h;
       bl[ks][e] = lo;
     }
   const int c = c0 + l16;
-  if (c >= a.C) return;
-  const int qi = c / a.G, h = hkv * a.G + c % a.G;
+  const bool mine = l16 < NC && c < a.C;
+  const int qi = mine ? c / a.G : 0, h = hkv * a.G + (mine ? c % a.G : 0);
   const float down = kUnsplit2 / up * kSplit;
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
@@ -647,14 +724,16 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
       f = mfma16x16x32(al[rb][ks], bh[ks], f);
       f = mfma16x16x32(ah[rb][ks], bl[ks], f);
     }
-    const int64_t off = static_cast<int64_t>(b) * a.sob + static_cast<int64_t>(h) * a.soh +
-                        static_cast<int64_t>(qi) * a.sos + wave * (D / 4) + rb * 16 + lg * 4;
+    if (mine) {
+      const int64_t off = static_cast<int64_t>(b) * a.sob + static_cast<int64_t>(h) * a.soh +
+                          static_cast<int64_t>(qi) * a.sos + wave * (D / 4) + rb * 16 + lg * 4;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float v = f[e] * down;
-      if (a.out_dtype == TQ_BF16) store_act<TQ_BF16>(a.out, off + e, v);
-      else if (a.out_dtype == TQ_F16) store_act<TQ_F16>(a.out, off + e, v);
-      else store_act<TQ_F32>(a.out, off + e, v);
+      for (int e = 0; e < 4; ++e) {
+        const float v = f[e] * down;
+        if (a.out_dtype == TQ_BF16) store_act<TQ_BF16>(a.out, off + e, v);
+        else if (a.out_dtype == TQ_F16) store_act<TQ_F16>(a.out, off + e, v);
+        else store_act<TQ_F32>(a.out, off + e, v);
+      }
     }
   }
 }
@@ -663,7 +742,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
 struct TreePlan {
   int nt, nw;   // column tiles of a block, waves of a block
   int ncol;     // blocks along the columns
-  int slots, nrec;
+  int slots;
   int64_t bytes;
 };
 
@@ -686,13 +765,13 @@ static TreePlan plan_tree(int B, int Hq, int Hkv, int T, int64_t maxpos, int d, 
   int res;
   if (d == 64) res = bits == 2 ? tree_resident_nt<64, 2>(p.nt) : bits == 3 ? tree_resident_nt<64, 3>(p.nt) : tree_resident_nt<64, 4>(p.nt);
   else res = bits == 2 ? tree_resident_nt<128, 2>(p.nt) : bits == 3 ? tree_resident_nt<128, 3>(p.nt) : tree_resident_nt<128, 4>(p.nt);
-  const int rk = 32 * p.nw;
-  p.slots = res / (Hkv * p.ncol);
+  p.slots = res / (Hkv * p.ncol);  // one round of resident blocks
   if (p.slots < 1) p.slots = 1;
-  // sum of ceil(rounds / chunk) <= slots + B, and at most every round
+  // no more blocks than rounds
+  const int rk = 32 * p.nw;
   const int64_t most = static_cast<int64_t>(B) * ((maxpos + rk - 1) / rk);
-  const int64_t nrec = static_cast<int64_t>(p.slots) + B < most ? static_cast<int64_t>(p.slots) + B : most;
-  p.nrec = static_cast<int>(nrec);
+  if (p.slots > most) p.slots = static_cast<int>(most);
+  const int64_t nrec = static_cast<int64_t>(p.slots) + B;
   p.bytes = nrec * Hkv * C * static_cast<int64_t>(d + 2) * 4;
   return p;
 }
@@ -705,10 +784,14 @@ static bool tree_shape(int B, int Hq, int Hkv, int T, int64_t maxpos, int d, int
 
 template <int D, int BITS>
 static void launch_tree(const TreeArgs& a, const TreePlan& p, hipStream_t s) {
-  const dim3 grid(p.nrec, p.ncol, a.Hkv);
+  const dim3 grid(p.slots, p.ncol, a.Hkv);
   if (p.nt == 1) tree_attn_kernel<D, BITS, 1, 4><<<grid, 256, 0, s>>>(a);
   else tree_attn_kernel<D, BITS, 2, 4><<<grid, 256, 0, s>>>(a);
-  tree_merge_kernel<D, 128><<<dim3((a.C + 15) / 16, a.Hkv, a.B), 256, 0, s>>>(a);
+  // enough blocks of 16 columns to fill the chip, else blocks of 4
+  if (static_cast<int64_t>((a.C + 15) / 16) * a.Hkv * a.B >= 512)
+    tree_merge_kernel<D, 128, 4><<<dim3((a.C + 15) / 16, a.Hkv, a.B), 256, 0, s>>>(a);
+  else
+    tree_merge_kernel<D, 128, 1><<<dim3((a.C + 3) / 4, a.Hkv, a.B), 256, 0, s>>>(a);
 }
 
 }  // namespace tq
@@ -786,11 +869,10 @@ int tq_tree_attention(const uint16_t* q_rot, const float* q_proj, const uint8_t*
   a.G = Hq / Hkv;
   a.C = a.G * T;
   a.slots = p.slots;
-  a.nrec = p.nrec;
   a.coeff = coeff;
   a.scale = scale;
   a.part_o = static_cast<float*>(workspace);
-  a.part_ml = a.part_o + static_cast<int64_t>(p.nrec) * Hkv * a.C * d;
+  a.part_ml = a.part_o + (static_cast<int64_t>(p.slots) + B) * Hkv * a.C * d;
   a.vpit = val_pit_split;
   a.out = out;
   a.out_dtype = out_dtype;
