@@ -168,24 +168,34 @@ struct TreeSmem {
   static constexpr int OFF_K = 0, OFF_S = NK * KC, OFF_V = OFF_S + NK * SC, OFF_N = OFF_V + NK * VC;
   static constexpr int NRM = NK * 4;
   static constexpr int SLOT = OFF_N + 3 * NRM;
-  static constexpr int R = NT == 1 || BITS == 4 ? 3 : 4;  // slabs of a wave in flight: two blocks fit a compute unit
+  static constexpr int R = 3;  // slabs of a wave in flight
   static constexpr int RING = NW * R * SLOT;
   static constexpr int LDM = D + 4;  // floats of a column in the merge of the waves: O, maximum, sum
   static constexpr int MERGE = NW * 16 * LDM * 4;
-  // the lo parts of q_proj stay in LDS where the registers would not hold them next to O
-  static constexpr bool LO_LDS = D == 128;
+  static constexpr int QKIND = NT * (D / 32) * 1024;  // fragments of one kind: q_rot, q_proj hi, q_proj lo
   uint8_t luts[(L::BYTES + 15) / 16 * 16];
   __attribute__((aligned(16))) uint8_t area[RING > MERGE ? RING : MERGE];
-  __attribute__((aligned(16))) float fac[NW][3][NK];  // a slab's fa vn_k, fb rn_k, vn_v / vcap
-  __attribute__((aligned(16))) uint8_t lo[LO_LDS ? NT * (D / 32) * 1024 : 16];
+  __attribute__((aligned(16))) uint8_t q[3 * QKIND];
   uint64_t anc[64];
+  float qmax[NW];
 };
 
-// (f16(x0 y0), f16(x1 y1)), one rounding each
-__device__ __forceinline__ uint32_t mul2_f16(float x0, float y0, float x1, float y1) {
+// Products with an f16 factor in the low half of y (v_fma_mix takes it as it is):
+//   mul_f16 = x y, fma_f16 = x y + z in f32; mul2_f16 = (f16(x0 y0), f16(x1 y1)), one rounding each
+__device__ __forceinline__ float mul_f16(float x, uint32_t y) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(r) : "v"(x), "v"(y));
+  return r;
+}
+__device__ __forceinline__ float fma_f16(float x, uint32_t y, float z) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel_hi:[0,1,0]" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+  return r;
+}
+__device__ __forceinline__ uint32_t mul2_f16(float x0, uint32_t y0, float x1, uint32_t y1) {
   uint32_t r;
-  asm("v_fma_mixlo_f16 %0, %1, %2, 0" : "=&v"(r) : "v"(x0), "v"(y0));
-  asm("v_fma_mixhi_f16 %0, %1, %2, 0" : "+v"(r) : "v"(x1), "v"(y1));
+  asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=&v"(r) : "v"(x0), "v"(y0));
+  asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "+v"(r) : "v"(x1), "v"(y1));
   return r;
 }
 
@@ -205,11 +215,13 @@ tree_attn_kernel(TreeArgs a) {
   constexpr int NK = SM::NK, RK = NW * NK;
   constexpr int OFF_K = SM::OFF_K, OFF_S = SM::OFF_S, OFF_V = SM::OFF_V, OFF_N = SM::OFF_N, NRM = SM::NRM;
   constexpr int SLOT = SM::SLOT, R = SM::R;
-  constexpr bool LO_LDS = SM::LO_LDS;
+  constexpr int QKIND = SM::QKIND;
+  constexpr bool HOLD_HI = NT == 1 || D == 64;  // q_proj hi fragments in registers
+  constexpr bool AHEAD = NT == 1;  // score operands looked up a step ahead, where registers allow
   constexpr float LOG2E = 1.4426950408889634f;
   constexpr float TAU = 8.0f;  // a column's reference moves when a score exceeds it by more (log2 units)
-  // weights are 2^(s - m + PUP) <= 2^(TAU + PUP): keys down to ~2^-31 of the heaviest still reach
-  // the f16 operand P, whose subnormals end at 2^-24, and p vn / vcap stays below the f16 maximum
+  // p vn <= 2^(s - m + PUP) <= 2^(TAU + PUP): keys down to ~2^-31 of the heaviest still reach the
+  // f16 operand P, whose subnormals end at 2^-24
   constexpr float PUP = 6.0f;
 
   __shared__ __attribute__((aligned(16))) SM sm;
@@ -234,10 +246,10 @@ tree_attn_kernel(TreeArgs a) {
     build_small_luts<BITS, true>(t, luts, tid);
   }
   const float fa = a.scale * LOG2E;
+  float qs;
   const int vbit = l16 * VFB, vbase = (vbit >> 5) * 4, vshift = vbit & 31;
   uint8_t* const mine = area + wave * (R * SLOT);
   const uint32_t mine_lds = lds_offset(mine);
-  float (*fw)[NK] = sm.fac[wave];
 
   // ---- one part after the other: the rounds of this block's stretch that belong to one sequence
   while (x < x_end) {
@@ -251,7 +263,7 @@ tree_attn_kernel(TreeArgs a) {
     const uint64_t anc_lane = tree_ancestors(a, b);
     if (wave == 0) sm.anc[lane] = anc_lane;
     const uint64_t live = __ballot(anc_lane != 0);  // tokens with a place: some node sees them
-    __syncthreads();  // tables and ancestors in place; the previous part's merge is done with the area
+    __syncthreads();  // tables and ancestors in place; the previous part is done with the LDS
 
     // ---- the stream
     constexpr int NKD = (NK * KC + 1023) / 1024, NSD = (NK * SC + 1023) / 1024, NVD = (NK * VC + 1023) / 1024;
@@ -289,9 +301,8 @@ tree_attn_kernel(TreeArgs a) {
       return rows;
     };
     auto wait_slot = [&](int later) {  // until the slot issued `later` slots ago has landed
-      static_assert(R <= 4 && 3 * NDMA < 64, "ring of at most 4 slots");
-      if (R >= 4 && later >= 3) wait_vm<(R >= 4 ? 3 * NDMA : 0)>();
-      else if (R >= 3 && later >= 2) wait_vm<(R >= 3 ? 2 * NDMA : 0)>();
+      static_assert(R == 3 && 2 * NDMA < 64, "ring of 3 slots");
+      if (later >= 2) wait_vm<2 * NDMA>();
       else if (later >= 1) wait_vm<NDMA>();
       else wait_vm<0>();
     };
@@ -302,60 +313,94 @@ tree_attn_kernel(TreeArgs a) {
     for (int r = 0; r < R; ++r) nrows[r] = k0w + r * RK < kend ? issue(k0w + r * RK, page_of(k0w + r * RK), r) : 0;
 
 
-    // ---- the block's queries as B fragments, the same in every wave.  q_proj (f32) enters as f16 hi + lo
-    // parts, scaled together by a power of two that keeps both in range (qproj_split_scale)
-    // (columns behind the last repeat it; they are not stored)
+    // ---- the block's queries, laid out by all its threads as B fragments (lane (column l16, group lg)
+    // of k-step ks holds dims lg D / 4 + 8 ks ..): q_rot, and coeff q_proj (f32) as f16 hi + lo
+    // parts.  All are scaled by one power of two qs that puts the largest q_rot or coeff q_proj in
+    // [2^13, 2^14): q_rot stays exact, and the lo parts stay normal f16 down to 2^-17 of it.
+    // Columns behind the last repeat it; they are not stored.
+    {
+      constexpr int TPC = 64 * NW / (16 * NT), DPT = D / TPC;  // threads per column, dims per thread
+      static_assert(DPT == 4 || DPT == 8 || DPT == 16, "whole fragments or halves of one");
+      const int col = tid / TPC, d0 = (tid % TPC) * DPT;
+      const int c = min(ct0 + col, a.C - 1), node = c / a.G;
+      const int64_t row = ((static_cast<int64_t>(b) * a.Hq + hkv * a.G + (c - node * a.G)) * a.T + node) * D + d0;
+      float pj[DPT], rt[DPT];
+#pragma unroll
+      for (int i = 0; i < DPT; i += 4) {
+        const float4v x4 = *reinterpret_cast<const float4v*>(a.q_proj + row + i);
+        const half4 h4 = *reinterpret_cast<const half4*>(a.q_rot + row + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          pj[i + e] = x4[e] * a.coeff;
+          rt[i + e] = static_cast<float>(h4[e]);
+        }
+      }
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < DPT; ++i) m = fmaxf(m, fmaxf(fabsf(pj[i]), fabsf(rt[i])));
+      m = wave_max(m);
+      if (lane == 0) sm.qmax[wave] = m;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < NW; ++w) m = fmaxf(m, sm.qmax[w]);
+      qs = fminf(qproj_split_scale(m), 0x1p100f);
+      constexpr int PER = DPT < 8 ? DPT : 8;
+#pragma unroll
+      for (int i = 0; i < DPT; i += PER) {
+        const int d = d0 + i, lgd = d / (D / 4), ks = (d % (D / 4)) / 8;
+        _Float16* const dst =
+            reinterpret_cast<_Float16*>(sm.q + (((col / 16) * KS + ks) * 64 + lgd * 16 + col % 16) * 16) + d % 8;
+        typedef _Float16 halfP __attribute__((ext_vector_type(PER)));
+        halfP r, hi, lo;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          _Float16 h, l;
+          split_f16(pj[i + e] * qs, h, l);
+          r[e] = static_cast<_Float16>(rt[i + e] * qs);
+          hi[e] = h;
+          lo[e] = l;
+        }
+        *reinterpret_cast<halfP*>(dst) = r;
+        *reinterpret_cast<halfP*>(dst + QKIND / 2) = hi;
+        *reinterpret_cast<halfP*>(dst + QKIND) = lo;
+      }
+      __syncthreads();
+    }
+    const float fs = fa / qs;
+    auto qfrag = [&](int kind, int t, int ks) -> half8 {
+      return *reinterpret_cast<const half8*>(sm.q + kind * QKIND + ((t * KS + ks) * 64 + lane) * 16);
+    };
     uint64_t anc[NT];  // of the lane's column in each tile
-    half8 qr[NT][KS], qh[NT][KS], ql[LO_LDS ? 1 : NT][KS];
-    float qmax = 0.f;
-    const float* qp[NT];
+    half8 qr[NT][KS], qh[HOLD_HI ? NT : 1][KS];  // held; the others are read from LDS at their use
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int c = min(ct0 + 16 * t + l16, a.C - 1), node = c / a.G;
-      const int64_t row = ((static_cast<int64_t>(b) * a.Hq + hkv * a.G + (c - node * a.G)) * a.T + node) * D + lg * (D / 4);
-      anc[t] = sm.anc[node];
-      qp[t] = a.q_proj + row;
+      anc[t] = sm.anc[min(ct0 + 16 * t + l16, a.C - 1) / a.G];
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        qmax = fmaxf(qmax, absmax8(qp[t] + ks * 8));
-        qr[t][ks] = *reinterpret_cast<const half8*>(a.q_rot + row + ks * 8);
+        qr[t][ks] = qfrag(0, t, ks);
+        if constexpr (HOLD_HI) qh[t][ks] = qfrag(1, t, ks);
       }
     }
-    const float qs = qproj_split_scale(wave_max(qmax));
-    const float fb = a.coeff * fa / qs;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        half8 lo;
-        split8s(qp[t] + ks * 8, qs, qh[t][ks], lo);
-        if constexpr (!LO_LDS) ql[t][ks] = lo;
-        else if (wave == 0) *reinterpret_cast<half8*>(sm.lo + ((t * KS + ks) * 64 + lane) * 16) = lo;
-      }
-    if constexpr (LO_LDS) __syncthreads();
-    auto qlo = [&](int t, int ks) -> half8 {
-      if constexpr (!LO_LDS) return ql[t][ks];
-      else return *reinterpret_cast<const half8*>(sm.lo + ((t * KS + ks) * 64 + lane) * 16);
-    };
 
-    // column state: reference mref = m - PUP (0 until the column has a maximum m), the threshold a
-    // score relative to mref must exceed to move it (-inf until then, TAU + PUP after), the sum
-    float mref[NT], thr[NT], l_run[NT];
-    // value norms enter P as vn / vcap <= 1; vcap is a power of two that only grows (O is rescaled
-    // when it does) and multiplies O back at the end
-    float vcap = 0x1p-24f, inv_vcap = 0x1p24f;
+    // Column state: weights are p = 2^(s - mref) with mref = m - PUP + cap, where m is the column's
+    // reference maximum and 2^cap bounds the value norms met, so that p vn stays within f16; both
+    // only grow, O and l being rescaled when they do.  lim is the largest s - mref that does not
+    // move m (-inf while the column has none; mref is 0 then).
+    float mref[NT], lim[NT], l_run[NT], cap = -24.f;
+    uint32_t cap16 = 0;  // 2^cap as f16 bits, once it is one: norms are compared as integers
     float4v oacc[NT][DB];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       mref[t] = 0.f;
-      thr[t] = -INFINITY;
+      lim[t] = -INFINITY;
       l_run[t] = 0.f;
 #pragma unroll
       for (int db = 0; db < DB; ++db) oacc[t][db] = float4v{0.f, 0.f, 0.f, 0.f};
     }
 
-    auto slab = [&](const uint8_t* src, int ks0, int rows) {
-      const bool edge = rows < NK || ks0 + NK > nctx;  // wave-uniform: a visibility to look up
+    // EDGE: some of the slab's rows do not exist, or hold drafted tokens
+    auto slab = [&](auto edge_c, const uint8_t* src, int ks0, int rows) {
+      constexpr bool EDGE = decltype(edge_c)::value;
       // bit k: key ks0 + k is one of the slab's rows and cached, or a drafted token in `tokens`
       auto visible = [&](uint64_t tokens) -> uint32_t {
         const int d = nctx - ks0;  // slab bit of the first drafted token
@@ -363,183 +408,218 @@ tree_attn_kernel(TreeArgs a) {
         const uint64_t drafted = d <= -64 || d >= 32 ? 0 : d >= 0 ? tokens << d : tokens >> -d;
         return static_cast<uint32_t>((cached | drafted) & ((1ull << rows) - 1));
       };
-      // ---- per-key factors: lanes 0-31 fa vn_k, lanes 32-63 fb rn_k, then lanes 0-31 vn_v / vcap
-      {
-        const int k = lane & 31;
-        const uint8_t* nsrc = src + OFF_N + k * 4;
-        float v = h2f(static_cast<uint16_t>(*reinterpret_cast<const uint32_t*>(nsrc + (lane >> 5) * NRM)));
-        float nv = h2f(static_cast<uint16_t>(*reinterpret_cast<const uint32_t*>(nsrc + 2 * NRM)));
-        if (edge && !((visible(live) >> k) & 1)) v = nv = 0.f;  // seen by nobody, whatever its row holds
-        if (__any(nv > vcap)) {
-          float t = fminf(nv, 65504.f);
-#pragma unroll
-          for (int sh = 16; sh >= 1; sh >>= 1) t = fmaxf(t, __shfl_xor(t, sh, 64));
-          int ex;
-          frexpf(t, &ex);  // t < 2^ex; every lane holds the same t
-          ex = __builtin_amdgcn_readfirstlane(ex);
-          const float cap = ldexpf(1.f, ex);
-          if (cap > vcap) {
-            const float shrink = vcap / cap;
-#pragma unroll
-            for (int c = 0; c < NT; ++c)
-#pragma unroll
-              for (int db = 0; db < DB; ++db) oacc[c][db] *= shrink;
-            vcap = cap;
-            inv_vcap = ldexpf(1.f, -ex);
-          }
-        }
-        (&fw[0][0])[lane] = v * (lane < 32 ? fa : fb);
-        if (lane < 32) fw[2][k] = nv * inv_vcap;
-      }
-      // ---- scores S^T = K^ Q^T (term 1) and Sign Q_proj^T (term 2); a key operand feeds every tile
-      float4v s1[NT][2], s2[NT][2];
+      // ---- everything the slab needs from its raw rows; the lane's keys are ks0 + 16j + 4lg + e
       uint32_t kw[2][KW32], sw[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         load_key_field<KLANE>(src + OFF_K + (16 * j + l16) * KC + lg * KLANE, kw[j]);
         sw[j] = load_sign_field<D>(src + OFF_S + (16 * j + l16) * SC + lg * SLANE);
+      }
+      // ---- scores S^T = K^ Q^T (term 1) and Sign Q_proj^T (term 2); a key operand feeds every tile.
+      float4v s1[NT][2], s2[NT][2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
           s1[t][j] = float4v{0.f, 0.f, 0.f, 0.f};
           s2[t][j] = float4v{0.f, 0.f, 0.f, 0.f};
         }
-      }
+      constexpr int NB = AHEAD ? 2 : 1;
+      half8 sg[NB][2], kc[NB][2], hi[NB][NT], lo[NB][NT];
+      auto look = [&](auto cc) {
+        constexpr int ks = decltype(cc)::value, h = ks % NB;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) sg[h][j] = nib2x4<ks>(tS, sw[j]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) kc[h][j] = key_operand<KB, KW32, ks>(tK, kw[j]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if constexpr (HOLD_HI) hi[h][t] = qh[t][ks];
+          else hi[h][t] = qfrag(1, t, ks);
+          lo[h][t] = qfrag(2, t, ks);
+        }
+      };
+      if constexpr (AHEAD) look(std::integral_constant<int, 0>{});
       static_for<KS>([&](auto cc) {
-        constexpr int ks = decltype(cc)::value;
-        half8 sg[2], kc[2], lo[NT];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) sg[j] = nib2x4<ks>(tS, sw[j]);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) kc[j] = key_operand<KB, KW32, ks>(tK, kw[j]);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) lo[t] = qlo(t, ks);
+        constexpr int ks = decltype(cc)::value, h = ks % NB, next = ks + NB - 1;
+        if constexpr (next < KS) look(std::integral_constant<int, next>{});
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) s2[t][j] = mfma16x16x32(sg[j], qh[t][ks], s2[t][j]);
+          for (int j = 0; j < 2; ++j) s2[t][j] = mfma16x16x32(sg[h][j], hi[h][t], s2[t][j]);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) s1[t][j] = mfma16x16x32(kc[j], qr[t][ks], s1[t][j]);
+          for (int j = 0; j < 2; ++j) s1[t][j] = mfma16x16x32(kc[h][j], qr[t][ks], s1[t][j]);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) s2[t][j] = mfma16x16x32(sg[j], lo[t], s2[t][j]);
-        if constexpr (LO_LDS) __builtin_amdgcn_sched_barrier(0);  // one step's operands at a time
+          for (int j = 0; j < 2; ++j) s2[t][j] = mfma16x16x32(sg[h][j], lo[h][t], s2[t][j]);
+        if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
       });
-      // ---- softmax step and P of each tile; the lane's keys are ks0 + 16j + 4lg + e
-      float4v ka[2], kb[2], nv[2];
+      // ---- norms
+      u32x4 kn[2], rn[2], vn[2];  // norms, f16 in the low half
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        ka[j] = *reinterpret_cast<const float4v*>(&fw[0][16 * j + 4 * lg]);
-        kb[j] = *reinterpret_cast<const float4v*>(&fw[1][16 * j + 4 * lg]);
-        nv[j] = *reinterpret_cast<const float4v*>(&fw[2][16 * j + 4 * lg]);
+        const uint8_t* const n = src + OFF_N + (16 * j + 4 * lg) * 4;
+        kn[j] = *reinterpret_cast<const u32x4*>(n);
+        rn[j] = *reinterpret_cast<const u32x4*>(n + NRM);
+        vn[j] = *reinterpret_cast<const u32x4*>(n + 2 * NRM);
       }
-      half8 pb[NT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float sc[2][4];  // log2-domain scores relative to mref
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[j][e] = fmaf(s1[t][j][e], ka[j][e], fmaf(s2[t][j][e], kb[j][e], -mref[t]));
-        if (edge) {
-          const uint32_t see = visible(anc[t]) >> (4 * lg);
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[j][e] = see & (1u << (16 * j + e)) ? sc[j][e] : -INFINITY;
-        }
-        const float lmax = max8_raw(sc[0][0], sc[0][1], sc[0][2], sc[0][3], sc[1][0], sc[1][1], sc[1][2], sc[1][3]);
-        if (__any(lmax > thr[t])) {
-          float m = lmax;
-          m = fmaxf(m, __shfl_xor(m, 16, 64));
-          m = fmaxf(m, __shfl_xor(m, 32, 64));
-          if (m > thr[t]) {
-            const float shift = m - PUP;
-            const float alpha = (thr[t] == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(-shift);
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) sc[j][e] -= shift;
-            mref[t] += shift;
-            thr[t] = TAU + PUP;
-            l_run[t] *= alpha;
-#pragma unroll
-            for (int db = 0; db < DB; ++db) oacc[t][db] *= alpha;
-          }
-        }
-        float p[2][4];
+      if constexpr (EDGE) {  // keys that nobody sees weigh nothing, whatever their rows hold
+        const uint32_t any = visible(live) >> (4 * lg);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            p[j][e] = __builtin_amdgcn_exp2f(sc[j][e]);
-            l_run[t] += p[j][e];
+            const bool on = any & (1u << (16 * j + e));
+            kn[j][e] = on ? kn[j][e] : 0;
+            rn[j][e] = on ? rn[j][e] : 0;
+            vn[j][e] = on ? vn[j][e] : 0;
           }
-        u32x4 w;
-        if (edge) {  // a masked key's norm may be anything: it takes no part in the product
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = i >> 1, e = 2 * (i & 1);
-            w[i] = mul2_f16(p[j][e], sc[j][e] == -INFINITY ? 0.f : nv[j][e], p[j][e + 1],
-                            sc[j][e + 1] == -INFINITY ? 0.f : nv[j][e + 1]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = i >> 1, e = 2 * (i & 1);
-            w[i] = mul2_f16(p[j][e], nv[j][e], p[j][e + 1], nv[j][e + 1]);
-          }
-        }
-        pb[t] = __builtin_bit_cast(half8, w);
       }
-      // ---- O^T += V^T (P vn)^T over the slab's 32 keys: K slot 8lg + 4j + e is key 16j + 4lg + e;
-      // an A dword is one dim of a key pair, read from the pair table after interleaving the two
-      // keys' code fields (parity 0: even dims, 1: odd dims)
-      constexpr uint32_t M = odd_fields<VB>();
-      uint32_t w[2][4];
+      // ---- value norms stay below 2^cap
+      {
+        uint32_t top = max(max(max(vn[0][0], vn[0][1]), max(vn[0][2], vn[0][3])),
+                           max(max(vn[1][0], vn[1][1]), max(vn[1][2], vn[1][3])));
+        if (__any(top > cap16)) {
+          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, 64)));
+          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, 64)));
+          int ex;
+          frexpf(fminf(h2f(static_cast<uint16_t>(top)), 65504.f), &ex);  // < 2^ex; the same in every lane
+          ex = max(__builtin_amdgcn_readfirstlane(ex), -24);
+          const float grow = static_cast<float>(ex) - cap;
+          if (grow > 0.f) {
+            const float shrink = ldexpf(1.f, -static_cast<int>(grow));
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+            for (int t = 0; t < NT; ++t) {
+              if (lim[t] != -INFINITY) {
+                mref[t] += grow;
+                lim[t] -= grow;
+              }
+              l_run[t] *= shrink;
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          const uint32_t* vp = reinterpret_cast<const uint32_t*>(src + OFF_V + (16 * j + 4 * lg + kk) * VC + vbase);
-          if constexpr (VW32 == 2) w[j][kk] = __builtin_amdgcn_alignbit(vp[1], vp[0], vshift);
-          else w[j][kk] = vp[0] >> vshift;
+              for (int db = 0; db < DB; ++db) oacc[t][db] *= shrink;
+            }
+            cap = static_cast<float>(ex);
+          }
+          cap16 = ex > 15 ? 0xFFFFu : static_cast<uint32_t>(f2h(ldexpf(1.f, ex)));
         }
+      }
+      // ---- log2-domain scores relative to mref, and the softmax step
+      float sc[NT][2][4];
+      bool hit = false;
+      float lmax[NT];
 #pragma unroll
-      for (int par = 0; par < 2; ++par) {
-        uint32_t f[2][2];
+      for (int t = 0; t < NT; ++t) {
+        uint32_t see = 0;
+        if constexpr (EDGE) see = visible(anc[t]) >> (4 * lg);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const uint32_t wa = w[j][2 * c], wb = w[j][2 * c + 1];
-            f[j][c] = par ? bfi32(M, wb, wa >> VB) : bfi32(M, wb << VB, wa);
+          for (int e = 0; e < 4; ++e) {
+            const float x = fmaf(fma_f16(s1[t][j][e], kn[j][e], mul_f16(s2[t][j][e], rn[j][e])), fs, -mref[t]);
+            sc[t][j][e] = !EDGE || (see & (1u << (16 * j + e))) ? x : -INFINITY;
           }
+        lmax[t] = max8_raw(sc[t][0][0], sc[t][0][1], sc[t][0][2], sc[t][0][3], sc[t][1][0], sc[t][1][1], sc[t][1][2],
+                           sc[t][1][3]);
+        hit = hit || lmax[t] > lim[t];
+      }
+      if (__any(hit)) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          float m = lmax[t];
+          m = fmaxf(m, __shfl_xor(m, 16, 64));
+          m = fmaxf(m, __shfl_xor(m, 32, 64));
+          const bool move = m > lim[t];
+          const float shift = move ? m - PUP + cap : 0.f;
+          const float alpha = !move ? 1.f : lim[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-shift);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[t][j][e] -= shift;
+          mref[t] += shift;
+          lim[t] = move ? TAU + PUP - cap : lim[t];
+          l_run[t] *= alpha;
+#pragma unroll
+          for (int db = 0; db < DB; ++db) oacc[t][db] *= alpha;
+        }
+      }
+      // ---- value words: the lane's field of each of its keys, key pairs interleaved: f[par][j][c] holds
+      // the even (0) or odd (1) dims of keys 16j + 4lg + 2c, + 1
+      constexpr uint32_t M = odd_fields<VB>();
+      uint32_t f[2][2][2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t w[4];
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const uint32_t* vp = reinterpret_cast<const uint32_t*>(src + OFF_V + (16 * j + 4 * lg + kk) * VC + vbase);
+          if constexpr (VW32 == 2) w[kk] = __builtin_amdgcn_alignbit(vp[1], vp[0], vshift);
+          else w[kk] = vp[0] >> vshift;
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          f[0][j][c] = bfi32(M, w[2 * c + 1] << VB, w[2 * c]);
+          f[1][j][c] = bfi32(M, w[2 * c + 1], w[2 * c] >> VB);
+        }
+      }
+      // ---- P vn as the f16 operand
+      half8 pb[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float p[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[j][e] = __builtin_amdgcn_exp2f(sc[t][j][e]);
+        l_run[t] += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = i >> 1, e = 2 * (i & 1);
+          uint32_t v0 = vn[j][e], v1 = vn[j][e + 1];
+          if constexpr (EDGE) {  // a masked key's norm may be anything: it takes no part in the product
+            v0 = sc[t][j][e] == -INFINITY ? 0 : v0;
+            v1 = sc[t][j][e + 1] == -INFINITY ? 0 : v1;
+          }
+          w[i] = mul2_f16(p[j][e], v0, p[j][e + 1], v1);
+        }
+        pb[t] = __builtin_bit_cast(half8, w);
+      }
+      // ---- O^T += V^T (P vn)^T over the slab's 32 keys: K slot 8lg + 4j + e is key 16j + 4lg + e; an A
+      // dword is one dim of a key pair, read from the pair table
+#pragma unroll
+      for (int par = 0; par < 2; ++par)
         static_for<NPAIR>([&](auto ic) {
           constexpr int i = decltype(ic)::value;
-          const half8 va = __builtin_bit_cast(half8, u32x4{value_pair<VB, i>(tV, f[0][0]), value_pair<VB, i>(tV, f[0][1]),
-                                                           value_pair<VB, i>(tV, f[1][0]), value_pair<VB, i>(tV, f[1][1])});
+          const half8 va = __builtin_bit_cast(
+              half8, u32x4{value_pair<VB, i>(tV, f[par][0][0]), value_pair<VB, i>(tV, f[par][0][1]),
+                           value_pair<VB, i>(tV, f[par][1][0]), value_pair<VB, i>(tV, f[par][1][1])});
 #pragma unroll
           for (int t = 0; t < NT; ++t) oacc[t][2 * i + par] = mfma16x16x32(va, pb[t], oacc[t][2 * i + par]);
         });
-      }
     };
 
-    int slot = 0;
-    for (int ks0 = k0w; ks0 < kend; ks0 += RK) {
-      // the next R - 1 slabs, as far as they exist, were issued after this one
-      const int later = (kend - 1 - ks0) / RK;
-      const bool more = later >= R;
-      const int page = more ? page_of(ks0 + R * RK) : -1;  // read ahead of the slab's work
-      wait_slot(later);
-      slab(mine + slot * SLOT, ks0, nrows[0]);
+    // first the slabs of cached keys only, then those that hold drafted tokens or end the part
+    int slot = 0, ks0 = k0w;
+    auto slabs = [&](auto edge_c, int end) {
+      for (; ks0 < end; ks0 += RK) {
+        // the next R - 1 slabs, as far as they exist, were issued after this one
+        const int later = (kend - 1 - ks0) / RK;
+        const bool more = later >= R;
+        const int page = more ? page_of(ks0 + R * RK) : -1;  // read ahead of the slab's work
+        wait_slot(later);
+        if (nrows[0]) slab(edge_c, mine + slot * SLOT, ks0, nrows[0]);
 #pragma unroll
-      for (int r = 1; r < R; ++r) nrows[r - 1] = nrows[r];
-      if (more) nrows[R - 1] = issue(ks0 + R * RK, page, slot);
-      slot = slot + 1 == R ? 0 : slot + 1;
-    }
+        for (int r = 1; r < R; ++r) nrows[r - 1] = nrows[r];
+        if (more) nrows[R - 1] = issue(ks0 + R * RK, page, slot);
+        slot = slot + 1 == R ? 0 : slot + 1;
+      }
+    };
+    slabs(std::false_type{}, min(kend, nctx) - (NK - 1));
+    slabs(std::true_type{}, kend);
 
     // ---- the waves' states joined in LDS, one column tile at a time (the rings are done); thread
     // (column tid / 16, dims DB (tid % 16) ..) joins
@@ -558,11 +638,11 @@ tree_attn_kernel(TreeArgs a) {
 #pragma unroll
         for (int db = 0; db < DB; db += 4)
           *reinterpret_cast<float4v*>(my + (lg * 4 + e) * DB + db) =
-              float4v{oacc[t][db][e], oacc[t][db + 1][e], oacc[t][db + 2][e], oacc[t][db + 3][e]} * vcap;
+              float4v{oacc[t][db][e], oacc[t][db + 1][e], oacc[t][db + 2][e], oacc[t][db + 3][e]};
       if (lg == 0) {
         // a node without a place leaves an empty record; a column of NaN scores, whose maximum never
         // moved, a NaN one
-        my[D] = !anc[t] || (thr[t] == -INFINITY && l == l) ? -INFINITY : mref[t];
+        my[D] = !anc[t] || (lim[t] == -INFINITY && l == l) ? -INFINITY : mref[t];
         my[D + 1] = l;
       }
       __syncthreads();
