@@ -684,12 +684,12 @@ tree_attn_kernel(TreeArgs a) {
 
 // ---------------------------------------------------------------- merge
 // One block per (sequence, kv head, 4 CW columns): wave w joins columns w, w + 4, ... (the records'
-// maxima and weights one per lane, then D / 64 dims per lane summed over the records, 16 of them in
-// flight), then out^T = Pi_v^T o^T on MFMA with both operands split into f16 hi + lo.  CW = 1 has the fewest
+// maxima and weights one per lane, then D / 64 dims per lane summed over the records, 16 / CW of them in
+// flight per column), then out^T = Pi_v^T o^T on MFMA with both operands split into f16 hi + lo.  CW = 1 has the fewest
 // dependent round trips, CW = 4 reads Pi_v a quarter as often.
 template <int D, int RK, int CW>
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
-  constexpr int PL = D / 64, RB = D / 64, NC = 4 * CW, NB = 16;
+  constexpr int PL = D / 64, RB = D / 64, NC = 4 * CW, NB = 16 / CW;
   typedef float floatPL __attribute__((ext_vector_type(PL)));
   __shared__ __attribute__((aligned(16))) float o_s[NC][D + 4];
   __shared__ float s_up[NC];
@@ -717,6 +717,20 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
     n = k1 - k0 + 1;
   }
   const int64_t step = static_cast<int64_t>(a.Hkv) * a.C;  // columns between records
+  // one memory round trip for the first NB records of all the wave's columns: partial O, and a record's
+  // maximum and sum per lane
+  floatPL v0[CW][NB];
+  float m0[CW], l0[CW];
+#pragma unroll
+  for (int k = 0; k < CW; ++k) {
+    const int64_t at = (static_cast<int64_t>(first) * a.Hkv + hkv) * a.C + min(c0 + wave + 4 * k, a.C - 1);
+#pragma unroll
+    for (int q = 0; q < NB; ++q)
+      v0[k][q] = q < n ? *reinterpret_cast<const floatPL*>(a.part_o + (at + q * step) * D + PL * lane) : floatPL{};
+    m0[k] = lane < n ? a.part_ml[(at + lane * step) * 2] : -INFINITY;
+    l0[k] = lane < n ? a.part_ml[(at + lane * step) * 2 + 1] : 0.f;
+  }
+#pragma unroll
   for (int k = 0; k < CW; ++k) {
     const int cc = wave + 4 * k, c = c0 + cc;
     floatPL o = floatPL{};
@@ -724,12 +738,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
       const int64_t at = (static_cast<int64_t>(first) * a.Hkv + hkv) * a.C + c;
       const float* ml = a.part_ml + at * 2;
       const float* src = a.part_o + at * D + PL * lane;
-      floatPL v[NB];
-#pragma unroll
-      for (int q = 0; q < NB; ++q) v[q] = q < n ? *reinterpret_cast<const floatPL*>(src + q * step * D) : floatPL{};
-      const float m_first = lane < n ? ml[lane * step * 2] : -INFINITY;
-      const float l_first = lane < n ? ml[lane * step * 2 + 1] : 0.f;
-      float mx = m_first;
+      float mx = m0[k];
       for (int r = lane + 64; r < n; r += 64) mx = fmaxf(mx, ml[r * step * 2]);
 #pragma unroll
       for (int sh = 32; sh >= 1; sh >>= 1) mx = fmaxf(mx, __shfl_xor(mx, sh, 64));
@@ -737,25 +746,28 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
       for (int r0 = 0; r0 < n; r0 += 64) {
         float w = 0.f;
         if (r0 + lane < n) {
-          const float m = r0 == 0 ? m_first : ml[(r0 + lane) * step * 2];
+          const float m = r0 == 0 ? m0[k] : ml[(r0 + lane) * step * 2];
           if (m != -INFINITY) {
             w = __builtin_amdgcn_exp2f(m - mx);
-            lsum += w * (r0 == 0 ? l_first : ml[(r0 + lane) * step * 2 + 1]);
+            lsum += w * (r0 == 0 ? l0[k] : ml[(r0 + lane) * step * 2 + 1]);
           }
         }
-        const int nb = min(64, n - r0);
-        for (int u = 0; u < nb; u += NB) {
-          if (r0 + u > 0) {
-#pragma unroll
-            for (int q = 0; q < NB; ++q)
-              v[q] = u + q < nb ? *reinterpret_cast<const floatPL*>(src + (r0 + u + q) * step * D) : floatPL{};
-          }
+        auto add = [&](const floatPL (&v)[NB], int u) {
 #pragma unroll
           for (int q = 0; q < NB; ++q) {
             const float ww = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), u + q));
 #pragma unroll
             for (int e = 0; e < PL; ++e) o[e] = fmaf(ww, v[q][e], o[e]);
           }
+        };
+        if (r0 == 0) add(v0[k], 0);
+        const int nb = min(64, n - r0);
+        for (int u = r0 == 0 ? NB : 0; u < nb; u += NB) {
+          floatPL v[NB];
+#pragma unroll
+          for (int q = 0; q < NB; ++q)
+            v[q] = u + q < nb ? *reinterpret_cast<const floatPL*>(src + (r0 + u + q) * step * D) : floatPL{};
+          add(v, u);
         }
       }
 #pragma unroll
