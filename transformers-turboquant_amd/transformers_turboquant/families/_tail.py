@@ -12,7 +12,8 @@ the reference's own sequence runs on its unpacked format.
 
 With a ``TurboQuantCache`` as the decoder's cache only the new tokens are
 compressed (appended to the cache) and attention runs over every cached
-position; any other transformers cache keeps the uncompressed K/V (its own
+position; with a ``TurboQuantPagedCache`` they go into its pages, and the cache decides what each
+token sees; any other transformers cache keeps the uncompressed K/V (its own
 ``update``), which are compressed whole on every step.
 """
 
@@ -26,6 +27,7 @@ import torch.nn.functional as F
 from turboquant_pytorch.fused import compressed_attention
 
 from ..cache import TurboQuantCache
+from ..paged_cache import TurboQuantPagedCache
 
 
 def additive_mask(mask: torch.Tensor | None, dtype=torch.float32) -> torch.Tensor | None:
@@ -63,6 +65,16 @@ def attention_tail(module, q, k, v, attention_mask, output_attentions: bool = Fa
     kc, vc = module.key_compressor, module.val_compressor
 
     fused = q.device.type == "cuda" and not output_attentions and not drop_active
+    if isinstance(cache, TurboQuantPagedCache):
+        if not fused:
+            raise ValueError("a paged cache serves GPU attention without attention weights or dropout (model.eval())")
+        if attention_mask is not None:
+            raise ValueError("a paged cache masks by itself and takes no attention mask: run prompts unpadded, under the "
+                             "sdpa attention implementation")
+        if not causal:
+            raise ValueError('a paged cache attends causally: apply_turboquant(model, causal="auto")')
+        out = cache.append_attend(module.layer_idx, kc, vc, k, v, q, scale=1.0 / math.sqrt(D), out_dtype=q.dtype)
+        return out.reshape(B, T, Hq * D), None
     cached = None  # (compressed keys, compressed values) of every cached position
     if isinstance(cache, TurboQuantCache):
         if fused:
