@@ -180,23 +180,20 @@ struct TreeSmem {
   float qmax[NW];
 };
 
-// Products with an f16 factor in the low half of y (v_fma_mix takes it as it is):
+// Products with an f16 factor in the low half of y, which v_fma_mix takes as it is (a fused multiply-add
+// with +0, so that the compiler does not split it into a conversion and a product; and not inline asm, whose
+// operands the compiler does not keep apart from the matrix and transcendental instructions that
+// write them):
 //   mul_f16 = x y, fma_f16 = x y + z in f32; mul2_f16 = (f16(x0 y0), f16(x1 y1)), one rounding each
-__device__ __forceinline__ float mul_f16(float x, uint32_t y) {
-  float r;
-  asm("v_fma_mix_f32 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(r) : "v"(x), "v"(y));
-  return r;
+__device__ __forceinline__ float low_f16(uint32_t y) {
+  typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+  return static_cast<float>(__builtin_bit_cast(half2v, y)[0]);
 }
-__device__ __forceinline__ float fma_f16(float x, uint32_t y, float z) {
-  float r;
-  asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel_hi:[0,1,0]" : "=v"(r) : "v"(x), "v"(y), "v"(z));
-  return r;
-}
+__device__ __forceinline__ float fma_f16(float x, uint32_t y, float z) { return fmaf(x, low_f16(y), z); }
+__device__ __forceinline__ float mul_f16(float x, uint32_t y) { return fmaf(x, low_f16(y), 0.f); }
 __device__ __forceinline__ uint32_t mul2_f16(float x0, uint32_t y0, float x1, uint32_t y1) {
-  uint32_t r;
-  asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=&v"(r) : "v"(x0), "v"(y0));
-  asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "+v"(r) : "v"(x1), "v"(y1));
-  return r;
+  typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, half2v{static_cast<_Float16>(mul_f16(x0, y0)), static_cast<_Float16>(mul_f16(x1, y1))});
 }
 
 template <int D, int BITS, int NT, int NW>
