@@ -157,19 +157,136 @@ __device__ __forceinline__ uint64_t tree_ancestors(const TreeArgs& a, int b) {
   return placed ? seen : 0;
 }
 
-// ---------------------------------------------------------------- attention
+// Bit k: key ks0 + k of a slab of `rows` rows is cached, or a drafted token in `tokens`; the slab's first
+// drafted token has bit d = n_b - ks0.
+__device__ __forceinline__ uint32_t tree_visible(uint64_t tokens, int d, int rows) {
+  const uint64_t cached = d <= 0 ? 0 : d >= 32 ? ~0ull : (1ull << d) - 1;
+  const uint64_t drafted = d <= -64 || d >= 32 ? 0 : d >= 0 ? tokens << d : tokens >> -d;
+  return static_cast<uint32_t>((cached | drafted) & ((1ull << rows) - 1));
+}
+
+// ---------------------------------------------------------------- the stream of packed rows
+// A wave's ring of slabs of 32 keys, filled by direct copies to LDS.
+template <int D, int KB, int VB, int R>
+struct TreeStream {
+  static constexpr int KC = D * KB / 8, SC = D / 8, VC = D * VB / 8;
+  static constexpr int NK = 32;  // keys of a slab
+  static constexpr int OFF_K = 0, OFF_S = NK * KC, OFF_V = OFF_S + NK * SC, OFF_N = OFF_V + NK * VC;
+  static constexpr int NRM = NK * 4;
+  static constexpr int SLOT = OFF_N + 3 * NRM;
+  static constexpr int NKD = (NK * KC + 1023) / 1024, NSD = (NK * SC + 1023) / 1024, NVD = (NK * VC + 1023) / 1024;
+  static constexpr int NDMA = NKD + NSD + NVD + 3;
+  // (read by scalar loads, through the constant address space: a vector load's wait would reach
+  // back past the copies in flight)
+  typedef const __attribute__((address_space(4))) int32_t* const_i32;
+
+  const TreeArgs& a;
+  const int hkv, lane, kend;
+  const_i32 pages;
+
+  __device__ __forceinline__ TreeStream(const TreeArgs& a_, int b, int hkv_, int kend_)
+      : a(a_), hkv(hkv_), lane(threadIdx.x & 63), kend(kend_),
+        pages((const_i32)reinterpret_cast<uintptr_t>(a_.table + b * a_.ld_table)) {}
+  // A slab's 32 keys lie in one page (pages hold 32 or more, slabs start at multiples of 32)
+  __device__ __forceinline__ int page_of(int kb) const { return pages[kb >> a.lg_page]; }
+  __device__ __forceinline__ void copy_plane(const i32x4& r, uint32_t dst, int bytes, int nrounds) const {
+    const uint32_t lo = lane * 16;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      if (c >= nrounds) break;
+      if ((c + 1) * 1024 <= bytes || lane * 16 < bytes - c * 1024) dma16(r, dst + c * 1024, lo + c * 1024);
+    }
+  }
+  // copy the slab of keys [kb, kb + 32) to LDS offset dst; returns how many of its rows exist: up to
+  // the part's last key, none where its page is not in the pool
+  __device__ __forceinline__ int issue(int kb, int page, uint32_t dst) const {
+    const bool in = page >= 0 && page < a.num_pages;
+    const int64_t row = in ? ((static_cast<int64_t>(page) * a.Hkv + hkv) << a.lg_page) + (kb & ((1 << a.lg_page) - 1)) : 0;
+    const int rows = in ? min(NK, kend - kb) : 0;
+    wait_lds();  // earlier reads of this slot have landed
+    copy_plane(rows_desc(a.kcodes + row * KC, KC, 0, rows), dst + OFF_K, NK * KC, NKD);
+    copy_plane(rows_desc(a.ksigns + row * SC, SC, 0, rows), dst + OFF_S, NK * SC, NSD);
+    copy_plane(rows_desc(a.vcodes + row * VC, VC, 0, rows), dst + OFF_V, NK * VC, NVD);
+    if (lane < 32) {
+      dma_u16(rows_desc(a.kvn + row, 2, 0, rows), dst + OFF_N, lane * 2);
+      dma_u16(rows_desc(a.krn + row, 2, 0, rows), dst + OFF_N + NRM, lane * 2);
+      dma_u16(rows_desc(a.vvn + row, 2, 0, rows), dst + OFF_N + 2 * NRM, lane * 2);
+    }
+    return rows;
+  }
+  // until the slab issued `later` slabs ago has landed
+  __device__ __forceinline__ static void wait_slab(int later) {
+    static_assert((R == 2 || R == 3) && 2 * NDMA < 64, "ring of 2 or 3 slots");
+    if (R == 3 && later >= 2) wait_vm<2 * NDMA>();
+    else if (later >= 1) wait_vm<NDMA>();
+    else wait_vm<0>();
+  }
+  // the wave's slabs from ks0 on up to `end`, every RK keys, in ring slots STRIDE bytes apart; work(ring
+  // slot, first key, rows)
+  template <int RK, int STRIDE, class Work>
+  __device__ __forceinline__ void run(int& ks0, int end, int (&nrows)[R], int& slot, uint32_t ring, Work work) const {
+    for (; ks0 < end; ks0 += RK) {
+      // the next R - 1 slabs, as far as they exist, were issued after this one
+      const int later = (kend - 1 - ks0) / RK;
+      const bool more = later >= R;
+      const int page = more ? page_of(ks0 + R * RK) : -1;  // read ahead of the slab's work
+      wait_slab(later);
+      if (nrows[0]) work(slot, ks0, nrows[0]);
+#pragma unroll
+      for (int r = 1; r < R; ++r) nrows[r - 1] = nrows[r];
+      if (more) nrows[R - 1] = issue(ks0 + R * RK, page, ring + slot * STRIDE);
+      slot = slot + 1 == R ? 0 : slot + 1;
+    }
+  }
+};
+
+// The waves' states of up to TC columns joined into a record: thread (column tid / 16, dims
+// D / 16 (tid % 16) ..); mrg [wave][column][D + 4] holds O, the maximum (log2) and the sum.
+template <int D, int NW, int TC>
+__device__ __forceinline__ void tree_join(const TreeArgs& a, const float* mrg, int64_t at, int ncols, int tid) {
+  constexpr int LDM = D + 4, DB = D / 16;
+  const int c = tid >> 4, d0 = (tid & 15) * DB;
+  if (tid >= 16 * TC || c >= ncols) return;
+  float m[NW], mx = -INFINITY, ls = 0.f;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    m[w] = mrg[(w * TC + c) * LDM + D];
+    mx = fmaxf(mx, m[w]);
+  }
+  float4v o[DB / 4];
+#pragma unroll
+  for (int i = 0; i < DB / 4; ++i) o[i] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    const float* s = mrg + (w * TC + c) * LDM;
+    const float f = m[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[w] - mx);
+    const float lw = s[D + 1];
+    ls += f == 0.f ? 0.f : f * lw;
+#pragma unroll
+    for (int i = 0; i < DB / 4; ++i) {
+      const float4v x4 = *reinterpret_cast<const float4v*>(s + d0 + 4 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] += f == 0.f ? 0.f : f * x4[e];
+    }
+  }
+  at += c;
+#pragma unroll
+  for (int i = 0; i < DB / 4; ++i) *reinterpret_cast<float4v*>(a.part_o + at * D + d0 + 4 * i) = o[i];
+  if ((tid & 15) == 0) {
+    a.part_ml[at * 2] = mx;
+    a.part_ml[at * 2 + 1] = ls;
+  }
+}
+
+// ---------------------------------------------------------------- attention, operands from tables
 // One object, so that the lookup tables lie at LDS address 0: a lookup's byte offset then is its
 // address (elsewhere every lookup pays an addition, 86 of ~330 VALU instructions a slab).
 template <int D, int BITS, int NT, int NW>
 struct TreeSmem {
   using L = SmallLuts<BITS>;
-  static constexpr int KC = D * L::KB / 8, SC = D / 8, VC = D * L::VB / 8;
-  static constexpr int NK = 32;  // keys of a wave's slab
-  static constexpr int OFF_K = 0, OFF_S = NK * KC, OFF_V = OFF_S + NK * SC, OFF_N = OFF_V + NK * VC;
-  static constexpr int NRM = NK * 4;
-  static constexpr int SLOT = OFF_N + 3 * NRM;
   static constexpr int R = 3;  // slabs of a wave in flight
-  static constexpr int RING = NW * R * SLOT;
+  using ST = TreeStream<D, L::KB, L::VB, R>;
+  static constexpr int RING = NW * R * ST::SLOT;
   static constexpr int LDM = D + 4;  // floats of a column in the merge of the waves: O, maximum, sum
   static constexpr int MERGE = NW * 16 * LDM * 4;
   static constexpr int QKIND = NT * (D / 32) * 1024;  // fragments of one kind: q_rot, q_proj hi, q_proj lo
@@ -197,7 +314,7 @@ __device__ __forceinline__ uint32_t mul2_f16(float x0, uint32_t y0, float x1, ui
 }
 
 template <int D, int BITS, int NT, int NW>
-__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NT == 1 ? 3 : 2)))
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)))
 tree_attn_kernel(TreeArgs a) {
   using SM = TreeSmem<D, BITS, NT, NW>;
   using L = typename SM::L;
@@ -205,13 +322,14 @@ tree_attn_kernel(TreeArgs a) {
   constexpr int KS = D / 32;           // score k-steps
   constexpr int DB = D / 16;           // value row blocks: lane l16 holds dims DB l16 .. DB l16 + DB - 1
   constexpr int NPAIR = D / 32;        // pair-table groups per parity
-  constexpr int KC = SM::KC, SC = SM::SC, VC = SM::VC;
+  using ST = typename SM::ST;
+  constexpr int KC = ST::KC, SC = ST::SC, VC = ST::VC;
   constexpr int KLANE = KC / 4, KW32 = (KLANE + 3) / 4, SLANE = SC / 4;
   constexpr int VFB = DB * VB;
   constexpr int VW32 = (VB == 3) ? 2 : 1;
-  constexpr int NK = SM::NK, RK = NW * NK;
-  constexpr int OFF_K = SM::OFF_K, OFF_S = SM::OFF_S, OFF_V = SM::OFF_V, OFF_N = SM::OFF_N, NRM = SM::NRM;
-  constexpr int SLOT = SM::SLOT, R = SM::R;
+  constexpr int NK = ST::NK, RK = NW * NK;
+  constexpr int OFF_K = ST::OFF_K, OFF_S = ST::OFF_S, OFF_V = ST::OFF_V, OFF_N = ST::OFF_N, NRM = ST::NRM;
+  constexpr int SLOT = ST::SLOT, R = SM::R;
   constexpr int QKIND = SM::QKIND;
   constexpr bool HOLD_HI = NT == 1 || D == 64;  // q_proj hi fragments in registers
   constexpr bool AHEAD = NT == 1;  // score operands looked up a step ahead, where registers allow
@@ -262,53 +380,12 @@ tree_attn_kernel(TreeArgs a) {
     const uint64_t live = __ballot(anc_lane != 0);  // tokens with a place: some node sees them
     __syncthreads();  // tables and ancestors in place; the previous part is done with the LDS
 
-    // ---- the stream
-    constexpr int NKD = (NK * KC + 1023) / 1024, NSD = (NK * SC + 1023) / 1024, NVD = (NK * VC + 1023) / 1024;
-    constexpr int NDMA = NKD + NSD + NVD + 3;
-    auto copy_plane = [&](const i32x4& r, uint32_t dst, int bytes, int nrounds) {
-      const uint32_t lo = lane * 16;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if (c >= nrounds) break;
-        if ((c + 1) * 1024 <= bytes || lane * 16 < bytes - c * 1024) dma16(r, dst + c * 1024, lo + c * 1024);
-      }
-    };
-    // A slab's 32 keys lie in one page (pages hold 32 or more, slabs start at multiples of 32)
-    // (a scalar load, through the constant address space: a vector load's wait would reach
-    // back past the copies in flight)
-    typedef const __attribute__((address_space(4))) int32_t* const_i32;
-    const const_i32 pages = (const_i32)reinterpret_cast<uintptr_t>(a.table + b * a.ld_table);
-    auto page_of = [&](int kb) -> int { return pages[kb >> a.lg_page]; };
-    // copy the slab of keys [kb, kb + 32) into a slot; returns how many of its rows exist: up to the
-    // part's last key, none where its page is not in the pool
-    auto issue = [&](int kb, int page, int slot) -> int {
-      const bool in = page >= 0 && page < a.num_pages;
-      const int64_t row = in ? ((static_cast<int64_t>(page) * a.Hkv + hkv) << a.lg_page) + (kb & ((1 << a.lg_page) - 1)) : 0;
-      const int rows = in ? min(NK, kend - kb) : 0;
-      const uint32_t dst = mine_lds + slot * SLOT;
-      wait_lds();  // earlier reads of this slot have landed
-      copy_plane(rows_desc(a.kcodes + row * KC, KC, 0, rows), dst + OFF_K, NK * KC, NKD);
-      copy_plane(rows_desc(a.ksigns + row * SC, SC, 0, rows), dst + OFF_S, NK * SC, NSD);
-      copy_plane(rows_desc(a.vcodes + row * VC, VC, 0, rows), dst + OFF_V, NK * VC, NVD);
-      if (lane < 32) {
-        dma_u16(rows_desc(a.kvn + row, 2, 0, rows), dst + OFF_N, lane * 2);
-        dma_u16(rows_desc(a.krn + row, 2, 0, rows), dst + OFF_N + NRM, lane * 2);
-        dma_u16(rows_desc(a.vvn + row, 2, 0, rows), dst + OFF_N + 2 * NRM, lane * 2);
-      }
-      return rows;
-    };
-    auto wait_slot = [&](int later) {  // until the slot issued `later` slots ago has landed
-      static_assert(R == 3 && 2 * NDMA < 64, "ring of 3 slots");
-      if (later >= 2) wait_vm<2 * NDMA>();
-      else if (later >= 1) wait_vm<NDMA>();
-      else wait_vm<0>();
-    };
+    const ST stream(a, b, hkv, kend);
     // the first slabs fly while the queries are set up
     const int k0w = kbeg + wave * NK;
     int nrows[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) nrows[r] = k0w + r * RK < kend ? issue(k0w + r * RK, page_of(k0w + r * RK), r) : 0;
-
+    for (int r = 0; r < R; ++r) nrows[r] = k0w + r * RK < kend ? stream.issue(k0w + r * RK, stream.page_of(k0w + r * RK), mine_lds + r * SLOT) : 0;
 
     // ---- the block's queries, laid out by all its threads as B fragments (lane (column l16, group lg)
     // of k-step ks holds dims lg D / 4 + 8 ks ..): q_rot, and coeff q_proj (f32) as f16 hi + lo
@@ -398,13 +475,7 @@ tree_attn_kernel(TreeArgs a) {
     // EDGE: some of the slab's rows do not exist, or hold drafted tokens
     auto slab = [&](auto edge_c, const uint8_t* src, int ks0, int rows) {
       constexpr bool EDGE = decltype(edge_c)::value;
-      // bit k: key ks0 + k is one of the slab's rows and cached, or a drafted token in `tokens`
-      auto visible = [&](uint64_t tokens) -> uint32_t {
-        const int d = nctx - ks0;  // slab bit of the first drafted token
-        const uint64_t cached = d <= 0 ? 0 : d >= 32 ? ~0ull : (1ull << d) - 1;
-        const uint64_t drafted = d <= -64 || d >= 32 ? 0 : d >= 0 ? tokens << d : tokens >> -d;
-        return static_cast<uint32_t>((cached | drafted) & ((1ull << rows) - 1));
-      };
+      auto visible = [&](uint64_t tokens) { return tree_visible(tokens, nctx - ks0, rows); };
       // ---- everything the slab needs from its raw rows; the lane's keys are ks0 + 16j + 4lg + e
       uint32_t kw[2][KW32], sw[2];
 #pragma unroll
@@ -602,24 +673,13 @@ tree_attn_kernel(TreeArgs a) {
     // first the slabs of cached keys only, then those that hold drafted tokens or end the part
     int slot = 0, ks0 = k0w;
     auto slabs = [&](auto edge_c, int end) {
-      for (; ks0 < end; ks0 += RK) {
-        // the next R - 1 slabs, as far as they exist, were issued after this one
-        const int later = (kend - 1 - ks0) / RK;
-        const bool more = later >= R;
-        const int page = more ? page_of(ks0 + R * RK) : -1;  // read ahead of the slab's work
-        wait_slot(later);
-        if (nrows[0]) slab(edge_c, mine + slot * SLOT, ks0, nrows[0]);
-#pragma unroll
-        for (int r = 1; r < R; ++r) nrows[r - 1] = nrows[r];
-        if (more) nrows[R - 1] = issue(ks0 + R * RK, page, slot);
-        slot = slot + 1 == R ? 0 : slot + 1;
-      }
+      stream.template run<RK, SLOT>(ks0, end, nrows, slot, mine_lds,
+                              [&](int at, int k0, int rows) { slab(edge_c, mine + at * SLOT, k0, rows); });
     };
     slabs(std::false_type{}, min(kend, nctx) - (NK - 1));
     slabs(std::true_type{}, kend);
 
-    // ---- the waves' states joined in LDS, one column tile at a time (the rings are done); thread
-    // (column tid / 16, dims DB (tid % 16) ..) joins
+    // ---- the waves' states joined in LDS, one column tile at a time (the rings are done)
     constexpr int LDM = SM::LDM;
     float* const mrg = reinterpret_cast<float*>(area);  // [wave][column][LDM]
     const int64_t base = (static_cast<int64_t>(rec) * a.Hkv + hkv) * a.C + ct0;
@@ -643,39 +703,306 @@ tree_attn_kernel(TreeArgs a) {
         my[D + 1] = l;
       }
       __syncthreads();
-      const int c = tid >> 4, d0 = (tid & 15) * DB;
-      if (tid < 256 && ct0 + 16 * t + c < a.C) {
-        float m[NW], mx = -INFINITY, ls = 0.f;
+      tree_join<D, NW, 16>(a, mrg, base + 16 * t, a.C - ct0 - 16 * t, tid);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- attention, scores from bit planes
+// At most 8 columns (a decoding step, a short chain) and 1- or 2-bit key codes: both terms of a score
+// are sums of query values over the set bits of the packed row, taken exactly from the integer matrix
+// product (PlaneQuery: query values as base-256 digits in the rows, masked packed words as the
+// columns, no lookups).  Keys stand on the N side, so that a lane has its own key against columns
+// lg + 4g: one exponential per (column, key) instead of one per key and column of a 16-wide tile.
+// P reaches the operand of O^T += V^T P^T through a small LDS tile of the wave; column n of O^T
+// serves column n mod NC.
+template <int D, int KB, int NCG, int NW>
+struct TreePlaneSmem {
+  using L = SmallLuts<KB + 1>;
+  using PQ = PlaneQuery<KB, NCG, D>;
+  static constexpr int R = D == 64 ? 3 : 2;  // slabs of a wave in flight
+  using ST = TreeStream<D, KB, KB + 1, R>;
+  static constexpr int NC = PQ::NC, LDM = D + 4;
+  // slot r of the waves stands at r * STRIDE; the last NSTG slots first serve the queries' set-up
+  static constexpr int STRIDE = NW * ST::SLOT;
+  static constexpr int NSTG = (PQ::STAGE_BYTES + STRIDE - 1) / STRIDE;
+  static_assert(NSTG < R, "a slot flies during the set-up");
+  static constexpr int RING = R * STRIDE;
+  static constexpr int MERGE = NW * NC * LDM * 4;
+  static constexpr int AREA = RING > MERGE ? RING : MERGE;
+  uint8_t luts[(L::BYTES + 15) / 16 * 16];
+  __attribute__((aligned(16))) uint8_t area[AREA];
+  __attribute__((aligned(16))) _Float16 p[NW][NC][32];  // P of a slab [column][key]
+  uint64_t anc[64];
+};
+
+template <int D, int KB, int NCG, int NW>
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)))
+tree_plane_kernel(TreeArgs a) {
+  using SM = TreePlaneSmem<D, KB, NCG, NW>;
+  using L = typename SM::L;
+  using PQ = typename SM::PQ;
+  using ST = typename SM::ST;
+  constexpr int BITS = KB + 1, VB = BITS, R = SM::R, NC = SM::NC, STRIDE = SM::STRIDE;
+  constexpr int DB = D / 16, NPAIR = D / 32;
+  constexpr int KLANE = ST::KC / 4, SLANE = ST::SC / 4, VFB = DB * VB, VW32 = VB == 3 ? 2 : 1;
+  constexpr int NK = ST::NK, RK = NW * NK;
+  constexpr float LOG2E = 1.4426950408889634f;
+  constexpr float TAU = 8.0f, PUP = 6.0f;  // as in tree_attn_kernel
+
+  __shared__ __attribute__((aligned(16))) SM sm;
+  const uint8_t* const tV = sm.luts + L::VAL_OFF;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l16 = lane & 15, lg = lane >> 4;
+  const int hkv = blockIdx.z;
+  const TreeSplit<RK> split(a);
+  if (static_cast<int>(blockIdx.x) >= split.blocks) return;  // block-uniform
+  int x = split.begin(blockIdx.x);
+  const int x_end = split.begin(blockIdx.x + 1);
+
+  DecodeArgs qa{};
+  qa.q_rot = a.q_rot;
+  qa.q_proj = a.q_proj;
+  qa.kcent = a.kcent;
+  qa.vcent = a.vcent;
+  qa.Hq = a.Hq;
+  qa.Sq = a.T;
+  qa.G = a.G;
+  qa.C = a.C;
+  build_small_luts<BITS, true>(qa, sm.luts, tid);
+  const float fa = a.scale * LOG2E;
+  const int vbit = l16 * VFB, vbase = (vbit >> 5) * 4, vshift = vbit & 31;
+  uint8_t* const mine = sm.area + wave * ST::SLOT;
+  const uint32_t mine_lds = lds_offset(mine);
+  _Float16* const pt = &sm.p[wave][0][0];
+
+  while (x < x_end) {
+    int b, first, n;
+    split.sequence_at(a, x, b, first, n);
+    const int rec = static_cast<int>(blockIdx.x) + b;
+    const int nkeys = tree_keys(a, b), nctx = nkeys - a.T;
+    const int kbeg = (x - first) * RK, kend = min(nkeys, (min(x_end, first + n) - first) * RK);
+    x = min(x_end, first + n);
+
+    const uint64_t anc_lane = tree_ancestors(a, b);
+    if (wave == 0) sm.anc[lane] = anc_lane;
+    const uint64_t live = __ballot(anc_lane != 0);
+    __syncthreads();  // tables and ancestors in place; the previous part is done with the LDS
+    const ST stream(a, b, hkv, kend);
+    const int k0w = kbeg + wave * NK;
+    int nrows[R];
+    auto start = [&](int r) {
+      nrows[r] = k0w + r * RK < kend ? stream.issue(k0w + r * RK, stream.page_of(k0w + r * RK), mine_lds + r * STRIDE) : 0;
+    };
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          m[w] = mrg[(w * 16 + c) * LDM + D];
-          mx = fmaxf(mx, m[w]);
-        }
-        float4v o[DB / 4];
+    for (int r = 0; r < R - SM::NSTG; ++r) start(r);
+    PQ pq;
+    pq.setup(qa, b, hkv, sm.area + (R - SM::NSTG) * STRIDE, tid);
+    __syncthreads();  // fragments held: the staging slots join the ring
 #pragma unroll
-        for (int i = 0; i < DB / 4; ++i) o[i] = float4v{0.f, 0.f, 0.f, 0.f};
+    for (int r = R - SM::NSTG; r < R; ++r) start(r);
+    uint64_t anc[NCG];  // of columns lg + 4g
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          const float* s = mrg + (w * 16 + c) * LDM;
-          const float f = m[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[w] - mx);
-          const float lw = s[D + 1];
-          ls += f == 0.f ? 0.f : f * lw;
+    for (int g = 0; g < NCG; ++g) anc[g] = sm.anc[min(lg + 4 * g, a.C - 1) / a.G];
+
+    // column state as in tree_attn_kernel, the same in the 16 lanes of a column
+    float mref[NCG], lim[NCG], l_run[NCG], cap = -24.f;
+    uint32_t cap16 = 0;
+    float4v oacc[DB];
 #pragma unroll
-          for (int i = 0; i < DB / 4; ++i) {
-            const float4v x4 = *reinterpret_cast<const float4v*>(s + d0 + 4 * i);
+    for (int g = 0; g < NCG; ++g) {
+      mref[g] = 0.f;
+      lim[g] = -INFINITY;
+      l_run[g] = 0.f;
+    }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[i][e] += f == 0.f ? 0.f : f * x4[e];
-          }
-        }
-        const int64_t at = base + 16 * t + c;
+    for (int db = 0; db < DB; ++db) oacc[db] = float4v{0.f, 0.f, 0.f, 0.f};
+
+    auto slab = [&](auto edge_c, const uint8_t* src, int ks0, int rows) {
+      constexpr bool EDGE = decltype(edge_c)::value;
+      auto visible = [&](uint64_t tokens) { return tree_visible(tokens, nctx - ks0, rows) >> l16; };
+      // ---- scores of keys ks0 + 16j + l16 for columns lg + 4g
+      float t1[2][NCG], t2[2][NCG];
+      pq.dots2(src + ST::OFF_K + l16 * ST::KC + lg * KLANE, src + ST::OFF_S + l16 * ST::SC + lg * SLANE,
+               src + ST::OFF_K + (16 + l16) * ST::KC + lg * KLANE, src + ST::OFF_S + (16 + l16) * ST::SC + lg * SLANE, t1, t2);
+      uint32_t kn[2], rn[2], vn[2];  // norms, f16 in the low half
 #pragma unroll
-        for (int i = 0; i < DB / 4; ++i) *reinterpret_cast<float4v*>(a.part_o + at * D + d0 + 4 * i) = o[i];
-        if ((tid & 15) == 0) {
-          a.part_ml[at * 2] = mx;
-          a.part_ml[at * 2 + 1] = ls;
+      for (int j = 0; j < 2; ++j) {
+        const uint8_t* const nr = src + ST::OFF_N + (16 * j + l16) * 4;
+        kn[j] = *reinterpret_cast<const uint32_t*>(nr);
+        rn[j] = *reinterpret_cast<const uint32_t*>(nr + ST::NRM);
+        vn[j] = *reinterpret_cast<const uint32_t*>(nr + 2 * ST::NRM);
+      }
+      if constexpr (EDGE) {  // keys that nobody sees weigh nothing, whatever their rows hold
+        const uint32_t any = visible(live);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const bool on = any & (1u << (16 * j));
+          kn[j] = on ? kn[j] : 0;
+          rn[j] = on ? rn[j] : 0;
+          vn[j] = on ? vn[j] : 0;
         }
       }
+      // ---- value norms stay below 2^cap
+      uint32_t top = max(vn[0], vn[1]);
+      if (__any(top > cap16)) {
+#pragma unroll
+        for (int sh = 8; sh >= 1; sh >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), sh, 64)));
+        int ex;
+        frexpf(fminf(h2f(static_cast<uint16_t>(top)), 65504.f), &ex);  // < 2^ex; the same in every lane
+        ex = max(__builtin_amdgcn_readfirstlane(ex), -24);
+        const float grow = static_cast<float>(ex) - cap;
+        if (grow > 0.f) {
+          const float shrink = ldexpf(1.f, -static_cast<int>(grow));
+#pragma unroll
+          for (int g = 0; g < NCG; ++g) {
+            if (lim[g] != -INFINITY) {
+              mref[g] += grow;
+              lim[g] -= grow;
+            }
+            l_run[g] *= shrink;
+          }
+#pragma unroll
+          for (int db = 0; db < DB; ++db) oacc[db] *= shrink;
+          cap = static_cast<float>(ex);
+        }
+        cap16 = ex > 15 ? 0xFFFFu : static_cast<uint32_t>(f2h(ldexpf(1.f, ex)));
+      }
+      // ---- log2-domain scores relative to mref, and the softmax step
+      float sc[NCG][2], lmax[NCG];
+      bool hit = false;
+#pragma unroll
+      for (int g = 0; g < NCG; ++g) {
+        uint32_t see = 0;
+        if constexpr (EDGE) see = visible(anc[g]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float s = fmaf(fma_f16(t1[j][g], kn[j], mul_f16(t2[j][g] * a.coeff, rn[j])), fa, -mref[g]);
+          sc[g][j] = !EDGE || (see & (1u << (16 * j))) ? s : -INFINITY;
+        }
+        lmax[g] = max_raw(sc[g][0], sc[g][1]);
+        hit = hit || lmax[g] > lim[g];
+      }
+      if (__any(hit)) {
+        float alpha[NCG];
+#pragma unroll
+        for (int g = 0; g < NCG; ++g) {
+          float m = lmax[g];
+#pragma unroll
+          for (int sh = 8; sh >= 1; sh >>= 1) m = fmaxf(m, __shfl_xor(m, sh, 64));
+          const bool move = m > lim[g];
+          const float shift = move ? m - PUP + cap : 0.f;
+          alpha[g] = !move ? 1.f : lim[g] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-shift);
+          sc[g][0] -= shift;
+          sc[g][1] -= shift;
+          mref[g] += shift;
+          lim[g] = move ? TAU + PUP - cap : lim[g];
+          l_run[g] *= alpha[g];
+        }
+        // column l16 & (NC - 1) of O^T belongs to lane group l16 & 3
+        float ac = __shfl(alpha[0], 16 * (l16 & 3), 64);
+        if constexpr (NCG == 2) {
+          const float a1 = __shfl(alpha[1], 16 * (l16 & 3), 64);
+          ac = (l16 & 4) ? a1 : ac;
+        }
+#pragma unroll
+        for (int db = 0; db < DB; ++db) oacc[db] *= ac;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int g = 0; g < NCG; ++g) {
+          const float p = __builtin_amdgcn_exp2f(sc[g][j]);
+          l_run[g] += p;
+          uint32_t v = vn[j];
+          if constexpr (EDGE) v = sc[g][j] == -INFINITY ? 0 : v;  // a masked key's norm may be anything
+          pt[(lg + 4 * g) * NK + 16 * j + l16] = static_cast<_Float16>(mul_f16(p, v));
+        }
+      // ---- O^T += V^T (P vn)^T, as in tree_attn_kernel; the 8 row reads go out as one batch
+      uint32_t r0[2][4], r1[2][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const uint32_t* vp = reinterpret_cast<const uint32_t*>(src + ST::OFF_V + (16 * j + 4 * lg + kk) * ST::VC + vbase);
+          r0[j][kk] = vp[0];
+          if constexpr (VW32 == 2) r1[j][kk] = vp[1];
+        }
+      const _Float16* const pr = pt + (l16 & (NC - 1)) * NK + 4 * lg;
+      const u32x2 p0 = *reinterpret_cast<const u32x2*>(pr);
+      const u32x2 p1 = *reinterpret_cast<const u32x2*>(pr + 16);
+      const half8 pb = __builtin_bit_cast(half8, u32x4{p0[0], p0[1], p1[0], p1[1]});
+      __builtin_amdgcn_sched_barrier(0);
+      constexpr uint32_t M = odd_fields<VB>();
+      uint32_t w[2][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          if constexpr (VW32 == 2) w[j][kk] = __builtin_amdgcn_alignbit(r1[j][kk], r0[j][kk], vshift);
+          else w[j][kk] = r0[j][kk] >> vshift;
+        }
+#pragma unroll
+      for (int par = 0; par < 2; ++par) {
+        uint32_t f[2][2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t wa = w[j][2 * c], wb = w[j][2 * c + 1];
+            f[j][c] = par ? bfi32(M, wb, wa >> VB) : bfi32(M, wb << VB, wa);
+          }
+        auto look = [&](auto ic) {  // a group is looked up while the one before it is multiplied
+          constexpr int i = decltype(ic)::value;
+          return __builtin_bit_cast(half8, u32x4{value_pair<VB, i>(tV, f[0][0]), value_pair<VB, i>(tV, f[0][1]),
+                                                 value_pair<VB, i>(tV, f[1][0]), value_pair<VB, i>(tV, f[1][1])});
+        };
+        half8 va = look(std::integral_constant<int, 0>{});
+        static_for<NPAIR>([&](auto ic) {
+          constexpr int i = decltype(ic)::value;
+          half8 next = va;
+          if constexpr (i + 1 < NPAIR) next = look(std::integral_constant<int, i + 1>{});
+          __builtin_amdgcn_sched_barrier(0);
+          oacc[2 * i + par] = mfma16x16x32(va, pb, oacc[2 * i + par]);
+          va = next;
+        });
+      }
+    };
+
+    int slot = 0, ks0 = k0w;
+    auto slabs = [&](auto edge_c, int end) {
+      stream.template run<RK, STRIDE>(ks0, end, nrows, slot, mine_lds,
+                              [&](int at, int k0, int rows) { slab(edge_c, mine + at * STRIDE, k0, rows); });
+    };
+    slabs(std::false_type{}, min(kend, nctx) - (NK - 1));
+    slabs(std::true_type{}, kend);
+
+    // ---- the waves' states joined in LDS (the rings are done)
+    constexpr int LDM = SM::LDM;
+    float* const mrg = reinterpret_cast<float*>(sm.area);  // [wave][column][LDM]
+    __syncthreads();
+    if (l16 < NC) {
+      float* const my = mrg + (wave * NC + l16) * LDM;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int db = 0; db < DB; db += 4)
+          *reinterpret_cast<float4v*>(my + (lg * 4 + e) * DB + db) =
+              float4v{oacc[db][e], oacc[db + 1][e], oacc[db + 2][e], oacc[db + 3][e]};
     }
+#pragma unroll
+    for (int g = 0; g < NCG; ++g) {
+      float l = l_run[g];
+#pragma unroll
+      for (int sh = 8; sh >= 1; sh >>= 1) l += __shfl_xor(l, sh, 64);
+      if (l16 == 0) {
+        float* const my = mrg + (wave * NC + lg + 4 * g) * LDM;
+        my[D] = !anc[g] || (lim[g] == -INFINITY && l == l) ? -INFINITY : mref[g];
+        my[D + 1] = l;
+      }
+    }
+    __syncthreads();
+    tree_join<D, NW, NC>(a, mrg, (static_cast<int64_t>(rec) * a.Hkv + hkv) * a.C, a.C, tid);
   }
 }
 
@@ -829,35 +1156,42 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
 
 // ---------------------------------------------------------------- launch
 struct TreePlan {
-  int nt, nw;   // column tiles of a block, waves of a block
-  int ncol;     // blocks along the columns
+  void (*kernel)(TreeArgs);
+  int ncol;  // blocks along the columns
   int slots;
   int64_t bytes;
 };
 
-template <int D, int BITS, int NT, int NW>
-static int tree_resident() {
-  static int cache[16] = {};
-  return resident_blocks(reinterpret_cast<const void*>(&tree_attn_kernel<D, BITS, NT, NW>), 64 * NW, cache);
-}
+// The kernel of C columns: 1 and 2 scores from bit planes for up to 4 and 8 columns (2 and 3 bits), 3 and
+// 4 operands from tables for one and two tiles of 16.
+static int tree_kind(int C, int bits) { return bits <= 3 && C <= 8 ? (C <= 4 ? 1 : 2) : C <= 16 ? 3 : 4; }
+
+using TreeKernel = void (*)(TreeArgs);
 template <int D, int BITS>
-static int tree_resident_nt(int nt) {
-  return nt == 1 ? tree_resident<D, BITS, 1, 4>() : tree_resident<D, BITS, 2, 4>();
+static TreeKernel tree_kernel(int kind) {
+  if constexpr (BITS <= 3) {
+    if (kind == 1) return &tree_plane_kernel<D, BITS - 1, 1, 4>;
+    if (kind == 2) return &tree_plane_kernel<D, BITS - 1, 2, 4>;
+  }
+  return kind == 3 ? &tree_attn_kernel<D, BITS, 1, 4> : &tree_attn_kernel<D, BITS, 2, 4>;
+}
+static TreeKernel tree_kernel(int d, int bits, int kind) {
+  if (d == 64) return bits == 2 ? tree_kernel<64, 2>(kind) : bits == 3 ? tree_kernel<64, 3>(kind) : tree_kernel<64, 4>(kind);
+  return bits == 2 ? tree_kernel<128, 2>(kind) : bits == 3 ? tree_kernel<128, 3>(kind) : tree_kernel<128, 4>(kind);
 }
 
 static TreePlan plan_tree(int B, int Hq, int Hkv, int T, int64_t maxpos, int d, int bits) {
+  static int resident[2][3][5][16] = {};  // per kernel, per device
   TreePlan p{};
   const int C = Hq / Hkv * T;
-  p.nt = C <= 16 ? 1 : 2;
-  p.nw = 4;
-  p.ncol = (C + 16 * p.nt - 1) / (16 * p.nt);
-  int res;
-  if (d == 64) res = bits == 2 ? tree_resident_nt<64, 2>(p.nt) : bits == 3 ? tree_resident_nt<64, 3>(p.nt) : tree_resident_nt<64, 4>(p.nt);
-  else res = bits == 2 ? tree_resident_nt<128, 2>(p.nt) : bits == 3 ? tree_resident_nt<128, 3>(p.nt) : tree_resident_nt<128, 4>(p.nt);
+  const int kind = tree_kind(C, bits);
+  p.kernel = tree_kernel(d, bits, kind);
+  p.ncol = kind == 4 ? (C + 31) / 32 : 1;
+  const int res = resident_blocks(reinterpret_cast<const void*>(p.kernel), 256, resident[d == 128][bits - 2][kind]);
   p.slots = res / (Hkv * p.ncol);  // one round of resident blocks
   if (p.slots < 1) p.slots = 1;
   // no more blocks than rounds
-  const int rk = 32 * p.nw;
+  const int rk = 128;
   const int64_t most = static_cast<int64_t>(B) * ((maxpos + rk - 1) / rk);
   if (p.slots > most) p.slots = static_cast<int>(most);
   const int64_t nrec = static_cast<int64_t>(p.slots) + B;
@@ -871,11 +1205,9 @@ static bool tree_shape(int B, int Hq, int Hkv, int T, int64_t maxpos, int d, int
          static_cast<int64_t>(B) * ((maxpos + 127) / 128) < (int64_t(1) << 31);
 }
 
-template <int D, int BITS>
+template <int D>
 static void launch_tree(const TreeArgs& a, const TreePlan& p, hipStream_t s) {
-  const dim3 grid(p.slots, p.ncol, a.Hkv);
-  if (p.nt == 1) tree_attn_kernel<D, BITS, 1, 4><<<grid, 256, 0, s>>>(a);
-  else tree_attn_kernel<D, BITS, 2, 4><<<grid, 256, 0, s>>>(a);
+  p.kernel<<<dim3(p.slots, p.ncol, a.Hkv), 256, 0, s>>>(a);
   // enough blocks of 16 columns to fill the chip, else blocks of 4
   if (static_cast<int64_t>((a.C + 15) / 16) * a.Hkv * a.B >= 512)
     tree_merge_kernel<D, 128, 4><<<dim3((a.C + 15) / 16, a.Hkv, a.B), 256, 0, s>>>(a);
@@ -969,15 +1301,8 @@ int tq_tree_attention(const uint16_t* q_rot, const float* q_proj, const uint8_t*
   a.soh = soh;
   a.sos = sos;
   hipStream_t s = as_stream(stream);
-  if (d == 64) {
-    if (bits == 2) launch_tree<64, 2>(a, p, s);
-    else if (bits == 3) launch_tree<64, 3>(a, p, s);
-    else launch_tree<64, 4>(a, p, s);
-  } else {
-    if (bits == 2) launch_tree<128, 2>(a, p, s);
-    else if (bits == 3) launch_tree<128, 3>(a, p, s);
-    else launch_tree<128, 4>(a, p, s);
-  }
+  if (d == 64) launch_tree<64>(a, p, s);
+  else launch_tree<128>(a, p, s);
   return launch_status("tq_tree_attention");
 }
 
