@@ -44,6 +44,7 @@ struct TreeArgs {
   int lg_page, maxpos;  // maxpos: positions a table row can hold
   int B, Hq, Hkv, T, G, C;
   int slots;            // blocks along x: stretches of the rounds of all sequences
+  int lg_least;         // a stretch has 2^lg_least rounds or more, where there are as many
   float coeff, scale;
   float *part_o, *part_ml;  // records [slots + B, Hkv, C, D], [slots + B, Hkv, C, 2]
   const uint16_t* vpit;
@@ -74,7 +75,7 @@ __device__ __forceinline__ int scan64(int v) {
 }
 
 // Every wave of a block computes the same, 64 sequences per step (one per lane).  Block k of
-// n = min(slots, R) has the rounds [begin(k), begin(k + 1)) of the R in all: R / n of them, the first
+// n = min(slots, R / 2^lg_least) has the rounds [begin(k), begin(k + 1)) of the R in all: R / n of them, the first
 // R % n blocks one more.  Walking along the rounds, every step to the next part moves to the next
 // block, the next sequence or both, so k + b is a different number for every part, and the
 // parts of one sequence have consecutive ones: the record.
@@ -82,7 +83,7 @@ template <int RK>
 struct TreeSplit {
   int r0, upto0;    // of sequence `lane`: its rounds, and their sum up to it
   int total;        // rounds of all sequences
-  int blocks;       // that have any: every one of them at least a round
+  int blocks;       // that have any: every one of them at least a round, so that no record is left unwritten
   int each, extra;  // rounds of a block, blocks with one more
   __device__ __forceinline__ static int rounds(const TreeArgs& a, int b) {
     return b < a.B ? static_cast<int>(static_cast<unsigned>(tree_keys(a, b) + RK - 1) / RK) : 0;
@@ -93,7 +94,7 @@ struct TreeSplit {
     upto0 = scan64(r0);
     total = __builtin_amdgcn_readlane(upto0, 63);
     for (int b0 = 64; b0 < a.B; b0 += 64) total += __builtin_amdgcn_readlane(scan64(rounds(a, b0 + lane)), 63);
-    blocks = min(a.slots, total);
+    blocks = min(a.slots, static_cast<int>((static_cast<unsigned>(total) + (1u << a.lg_least) - 1) >> a.lg_least));
     each = blocks ? static_cast<unsigned>(total) / static_cast<unsigned>(blocks) : 0;
     extra = total - each * blocks;
   }
@@ -1158,6 +1159,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
 struct TreePlan {
   void (*kernel)(TreeArgs);
   int ncol;  // blocks along the columns
+  int lg_least;
   int slots;
   int64_t bytes;
 };
@@ -1187,6 +1189,10 @@ static TreePlan plan_tree(int B, int Hq, int Hkv, int T, int64_t maxpos, int d, 
   const int kind = tree_kind(C, bits);
   p.kernel = tree_kernel(d, bits, kind);
   p.ncol = kind == 4 ? (C + 31) / 32 : 1;
+  // One round is over soon and leaves a record for the merge.  With more than 16 columns, records
+  // are large and two rounds to a stretch pay (64 columns, 4k keys: 22.9 against 25.3 us); with
+  // fewer, more blocks do (8 columns or less, 4k keys: 15.8 and 15.8 us, 1k keys: 12.1 against 12.8).
+  p.lg_least = kind == 4 ? 1 : 0;
   const int res = resident_blocks(reinterpret_cast<const void*>(p.kernel), 256, resident[d == 128][bits - 2][kind]);
   p.slots = res / (Hkv * p.ncol);  // one round of resident blocks
   if (p.slots < 1) p.slots = 1;
@@ -1290,6 +1296,7 @@ int tq_tree_attention(const uint16_t* q_rot, const float* q_proj, const uint8_t*
   a.G = Hq / Hkv;
   a.C = a.G * T;
   a.slots = p.slots;
+  a.lg_least = p.lg_least;
   a.coeff = coeff;
   a.scale = scale;
   a.part_o = static_cast<float*>(workspace);
