@@ -36,6 +36,7 @@ class _DeviceTables:
     cent32: torch.Tensor              # f32 [2^b]
     cent16: torch.Tensor              # f16 [2^b]
     bounds32: torch.Tensor            # f32 [2^b - 1]
+    scaled: tuple | None = None       # f32 [2^b] scaled centroids, f16 [2, d, d] split of Pi^T over the scale
 
 
 def _tables(comp, device: torch.device, with_qjl: bool) -> _DeviceTables:
@@ -65,6 +66,21 @@ def _tables(comp, device: torch.device, with_qjl: bool) -> _DeviceTables:
     )
     comp._dev_tables = t
     return t
+
+
+def _scaled_tables(comp, t: _DeviceTables) -> tuple[torch.Tensor, torch.Tensor]:
+    """Centroids times a common factor from [1, 2), and the split of Pi^T divided by it: kernels that hold value
+    centroids as f16 lose less by the rounding.  Of 2^14 factors the one with the least squared error:
+    relative to the centroids 2e-6, 2e-5 and 4e-5 (rms) at 2, 3 and 4 bits, 1.5e-4 to 3e-4 unscaled."""
+    if t.scaled is None:
+        cent = comp.centroids.detach().to("cpu", torch.float64)
+        factors = 1 + torch.arange(2 ** 14, dtype=torch.float64) / 2 ** 14
+        x = cent * factors[:, None]
+        best = factors[((x - x.to(torch.float16).double()) / factors[:, None]).square().sum(1).argmin()]
+        pi = comp.Pi.detach().to("cpu", torch.float64)
+        t.scaled = ((cent * best).float().to(t.cent32.device),
+                    split_f16((pi.T / best).float().contiguous()).to(t.cent32.device))
+    return t.scaled
 
 
 class TurboQuantCompressorV2:

@@ -12,7 +12,7 @@ import math
 import torch
 
 from ._ops import ops
-from .compressors import TurboQuantCompressorMSE, TurboQuantCompressorV2, _tables
+from .compressors import TurboQuantCompressorMSE, TurboQuantCompressorV2, _scaled_tables, _tables
 from .pages import PagePool
 
 __all__ = ["tree_attention", "tree_attention_from_prepared", "verify_drafts"]
@@ -54,11 +54,11 @@ def _tree_args(D, dev, key_compressor, val_compressor, pool, layer, block_table,
         raise ValueError(f"tree attention needs keys and values of one bit width, got {key_compressor.mse_bits + 1} "
                          f"and {val_compressor.bits}")
     tk = _tables(key_compressor, dev, with_qjl=True)
-    tv = _tables(val_compressor, dev, with_qjl=False)
+    vcent, vpit = _scaled_tables(val_compressor, _tables(val_compressor, dev, with_qjl=False))
     kcodes, ksigns, krn, kvn, vcodes, vvn = pool._layer[layer]
     if out_dtype not in (torch.float32, torch.float16, torch.bfloat16):
         out_dtype = torch.float32
-    return (kcodes, ksigns, krn, kvn, tk.cent16, val_compressor.bits, vcodes, vvn, tv.cent32, tv.pit_split, block_table,
+    return (kcodes, ksigns, krn, kvn, tk.cent16, val_compressor.bits, vcodes, vvn, vcent, vpit, block_table,
             lengths, parents, math.sqrt(math.pi / 2) / key_compressor.S.shape[0],
             float(scale if scale is not None else 1.0 / math.sqrt(D)), out_dtype)
 
