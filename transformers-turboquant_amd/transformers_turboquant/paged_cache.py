@@ -61,7 +61,7 @@ class TurboQuantPagedCache(Cache):
         self._drafted = False  # the step's rows are drafted tokens that accept() may keep
         self._written: set[int] = set()  # layers of the step under way that hold its rows
         self._step = 0  # tokens of the step under way
-        self._device_state = None  # (block table, lengths) of the active sequences
+        self._device_state = None  # (block table, lengths) of the active sequences; None: to be made
 
     # ------------------------------------------------------------------ sequences
     def add(self, n: int = 1) -> list[int]:
@@ -299,9 +299,10 @@ class TurboQuantPagedCache(Cache):
         if len(self._written) == self.num_layers and self._tree is None:
             for i in self._active:
                 self._seqs[i].length += self._step
+            table, lengths = self._device_state
+            self._device_state = (table, lengths + self._step)  # stands until a page is added
             self._written.clear()
             self._step = 0
-            self._device_state = None
 
     def _check_codec(self, layer_idx, key_compressor, val_compressor) -> None:
         if val_compressor.bits != key_compressor.mse_bits + 1:
@@ -373,6 +374,8 @@ class TurboQuantPagedCache(Cache):
                 self._refs[s.pages[at]] -= 1
                 s.pages[at] = new
             s.pages.extend(self._take() for _ in range(fresh))
+        if self._device_state is not None and not need:
+            return
         dev = self.pool.device
         width = max(len(s.pages) for s in seqs)
         state = torch.tensor([s.pages + [-1] * (width - len(s.pages)) + [s.length] for s in seqs], dtype=torch.int32)
