@@ -83,19 +83,17 @@ __device__ __forceinline__ Left walk(const VerifyArgs& a, int b, int64_t* s_rej,
     if (a.draft) {
       if (inner && tok >= 0 && tok < a.V) bar = u * static_cast<double>(load_act<DT>(a.draft, b * a.db + par * a.dt + tok));
     } else {
-      // a candidate that repeats an earlier sibling has nothing left to accept
-      bool again = false;
-      for (int j = 0; j < a.T; ++j) {
+      // the earlier siblings in index order; a candidate that repeats one has nothing left to accept
+      double rem = 1.0;
+      const int T = a.parents ? a.T : 0;  // a chain has no siblings
+      for (int j = 0; j < T; ++j) {
         const int pj = lane_value(par, j);
         const int64_t tj = lane_value(tok, j);
-        again = again || (j < i && pj == par && tj == tok);
-      }
-      if (again) p = 0.0;
-      double rem = 1.0;
-      for (int j = 0; j < a.T; ++j) {
-        const int pj = lane_value(par, j);
-        const double qj = lane_value(p, j);
-        if (j < i && pj == par) rem -= qj;
+        const double qj = lane_value(p, j);  // settled: every earlier sibling of j has had its turn
+        if (j < i && pj == par) {
+          rem -= qj;
+          if (tj == tok) p = 0.0;
+        }
       }
       bar = u * rem;
     }
