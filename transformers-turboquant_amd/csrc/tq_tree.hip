@@ -283,10 +283,9 @@ __device__ __forceinline__ void tree_join(const TreeArgs& a, const float* mrg, i
 // parts, so that there are three passes of scores and one of values to a key and column.
 // P is rounded to f16 (relative 2^-11 of each weight, a hundredth of what the codes lose), sums and
 // maxima are f32.
-// 16 nodes, 16 sequences of 8k to 32k, 32/8 heads, 3 bits: 200 us for 0.17 TFLOP of matrix work, 36%
-// of the matrix rate that a large library product reaches; of 451k cycles the matrix unit is busy
-// in 164k, the VALU in 217k, the LDS in 239k, over the two waves per SIMD that the registers of two
-// tiles leave.  Measured against it and dropped: four tiles at one wave per SIMD (236 against 275 us in
+// 16 nodes, 16 sequences of 8k to 32k, 32/8 heads, 3 bits: 200 us for 0.17 TFLOP of matrix work, 0.86
+// PFLOP/s (a large library product reaches 1.16); of 451k cycles the matrix unit is busy in 164k, the
+// VALU in 217k, the LDS in 239k, over the two waves per SIMD that the registers of two tiles leave.  Measured against it and dropped: four tiles at one wave per SIMD (236 against 275 us in
 // all), three waves with spills (226 and 309), operands looked up a step ahead at two tiles (216 and 224).
 //
 // The shared memory is one object, so that the lookup tables lie at LDS address 0: a lookup's byte
