@@ -281,6 +281,27 @@ def test_many_parts_of_a_block(bits):
         _check(out[some], kc, vc, pool, table[some], lengths[some], q[some], par[some])
 
 
+@pytest.mark.parametrize("T,Hq,Hkv,wide", [(1, 4, 1, 0), (4, 6, 2, 0), (12, 6, 2, 0), (12, 6, 2, 4096)])
+def test_a_query_that_is_not_finite_spoils_itself_only(T, Hq, Hkv, wide):
+    print("case:", T, Hq, Hkv, wide, flush=True)
+    kc, vc, pool, table, lengths, q = _setup(128, 3, 2, Hq, Hkv, T, [400, 37], 32, seed=15)
+    if wide:
+        table = _widen(table, wide)
+    q_rot, q_proj = kc.prepare_queries(q)
+    clean = tree_attention_from_prepared(q_rot, q_proj, kc, vc, pool, 1, table, lengths)
+    for bad in (float("inf"), float("nan")):
+        r, p = q_rot.clone(), q_proj.clone()
+        r[0, 1, T - 1, ::2] = bad
+        r[0, 1, T - 1, 1::2] = -bad
+        p[0, 1, T - 1] = bad
+        out = tree_attention_from_prepared(r, p, kc, vc, pool, 1, table, lengths)
+        hurt = torch.zeros(out.shape[:3], dtype=torch.bool, device=DEV)
+        hurt[0, T - 1, 1] = True
+        assert torch.isnan(out[hurt]).all()
+        # the others' queries may be scaled by another power of two, which rounds their low parts only
+        assert (out[~hurt] - clean[~hurt]).norm() <= 2.0 ** -16 * clean[~hurt].norm()
+
+
 def test_agrees_with_the_cache_of_one_length():
     """A chain over pages against compressed_attention over contiguous planes of the same rows."""
     from turboquant_pytorch import compressed_attention

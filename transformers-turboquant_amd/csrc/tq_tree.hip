@@ -421,7 +421,10 @@ tree_attn_kernel(TreeArgs a) {
       }
       float m = 0.f;
 #pragma unroll
-      for (int i = 0; i < DPT; ++i) m = fmaxf(m, fmaxf(fabsf(pj[i]), fabsf(rt[i])));
+      for (int i = 0; i < DPT; ++i) {  // of the finite ones: a column with others spoils itself only
+        if (fabsf(pj[i]) < INFINITY) m = fmaxf(m, fabsf(pj[i]));
+        if (fabsf(rt[i]) < INFINITY) m = fmaxf(m, fabsf(rt[i]));
+      }
       m = wave_max(m);
       if (lane == 0) sm.qmax[wave] = m;
       __syncthreads();
