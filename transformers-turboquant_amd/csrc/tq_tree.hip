@@ -51,11 +51,10 @@ struct TreeArgs {
 };
 
 // ---------------------------------------------------------------- the split of the keys
-// keys of sequence b (cached and drafted), 0 where its length does not fit its table
-__device__ __forceinline__ int tree_keys(const TreeArgs& a, int b) {
-  const int n = a.lengths[b];
-  return n >= 0 && n <= a.maxpos - a.T ? n + a.T : 0;
-}
+// length of sequence b, -1 behind the last
+__device__ __forceinline__ int tree_length(const TreeArgs& a, int b) { return b < a.B ? a.lengths[b] : -1; }
+// keys of a sequence of length n (cached and drafted), 0 where it does not fit its table
+__device__ __forceinline__ int tree_keys(const TreeArgs& a, int n) { return n >= 0 && n <= a.maxpos - a.T ? n + a.T : 0; }
 // Inclusive sum over the wave through DPP (shifts within rows of 16 lanes, then row 0's sum into
 // row 1 and row 2's into row 3, then lane 31's into the upper half): no LDS round trips.
 template <int CTRL, int ROWS>
@@ -78,19 +77,19 @@ __device__ __forceinline__ int scan64(int v) {
 // parts of one sequence have consecutive ones: the record.
 template <int RK>
 struct TreeSplit {
-  int r0, upto0;    // of sequence `lane`: its rounds, and their sum up to it
+  int k0, upto0;    // of sequence `lane`: its keys, and the sum of rounds up to it
   int total;        // rounds of all sequences
   int blocks;       // that have any: every one of them at least a round, so that no record is left unwritten
   int each, extra;  // rounds of a block, blocks with one more
-  __device__ __forceinline__ static int rounds(const TreeArgs& a, int b) {
-    return b < a.B ? static_cast<int>(static_cast<unsigned>(tree_keys(a, b) + RK - 1) / RK) : 0;
-  }
-  __device__ __forceinline__ explicit TreeSplit(const TreeArgs& a) {
+  __device__ __forceinline__ static int rounds(int keys) { return static_cast<int>(static_cast<unsigned>(keys + RK - 1) / RK); }
+  // n0: tree_length of sequence `lane`, loaded early by the caller
+  __device__ __forceinline__ TreeSplit(const TreeArgs& a, int n0) {
     const int lane = threadIdx.x & 63;
-    r0 = rounds(a, lane);
-    upto0 = scan64(r0);
+    k0 = tree_keys(a, n0);
+    upto0 = scan64(rounds(k0));
     total = __builtin_amdgcn_readlane(upto0, 63);
-    for (int b0 = 64; b0 < a.B; b0 += 64) total += __builtin_amdgcn_readlane(scan64(rounds(a, b0 + lane)), 63);
+    for (int b0 = 64; b0 < a.B; b0 += 64)
+      total += __builtin_amdgcn_readlane(scan64(rounds(tree_keys(a, tree_length(a, b0 + lane)))), 63);
     blocks = min(a.slots, static_cast<int>((static_cast<unsigned>(total) + (1u << a.lg_least) - 1) >> a.lg_least));
     each = blocks ? static_cast<unsigned>(total) / static_cast<unsigned>(blocks) : 0;
     extra = total - each * blocks;
@@ -100,46 +99,48 @@ struct TreeSplit {
     const unsigned big = extra * (each + 1), x = round;
     return x < big ? x / static_cast<unsigned>(each + 1) : extra + (x - big) / static_cast<unsigned>(each);
   }
-  // the sequence of round x < total, its first round and its number of rounds
-  __device__ __forceinline__ void sequence_at(const TreeArgs& a, int x, int& b, int& first, int& n) const {
-    int r = r0, upto = upto0;
+  // the sequence of round x < total, its first round and its keys
+  __device__ __forceinline__ void sequence_at(const TreeArgs& a, int x, int& b, int& first, int& keys) const {
+    int k = k0, upto = upto0;
     for (int b0 = 0;; b0 += 64) {
       const uint64_t m = __ballot(x < upto);
       if (m) {
         const int l = __builtin_ctzll(m);
         b = b0 + l;
-        n = __builtin_amdgcn_readlane(r, l);
-        first = __builtin_amdgcn_readlane(upto, l) - n;
+        keys = __builtin_amdgcn_readlane(k, l);
+        first = __builtin_amdgcn_readlane(upto, l) - rounds(keys);
         return;
       }
-      const int run = __builtin_amdgcn_readlane(upto, 63);
-      r = rounds(a, b0 + 64 + static_cast<int>(threadIdx.x & 63));
-      upto = scan64(r) + run;
+      next(a, b0 + 64, k, upto);
     }
   }
   // first round and number of rounds of sequence b
   __device__ __forceinline__ void rounds_of(const TreeArgs& a, int b, int& first, int& n) const {
-    int r = r0, upto = upto0;
-    for (int b0 = 0;; b0 += 64) {
-      if (b < b0 + 64) {
-        n = __builtin_amdgcn_readlane(r, b - b0);
-        first = __builtin_amdgcn_readlane(upto, b - b0) - n;
-        return;
-      }
-      const int run = __builtin_amdgcn_readlane(upto, 63);
-      r = rounds(a, b0 + 64 + static_cast<int>(threadIdx.x & 63));
-      upto = scan64(r) + run;
-    }
+    int k = k0, upto = upto0;
+    int b0 = 0;
+    for (; b >= b0 + 64; b0 += 64) next(a, b0 + 64, k, upto);
+    n = rounds(__builtin_amdgcn_readlane(k, b - b0));
+    first = __builtin_amdgcn_readlane(upto, b - b0) - n;
+  }
+
+ private:
+  // on to the 64 sequences from b0 on
+  __device__ __forceinline__ static void next(const TreeArgs& a, int b0, int& k, int& upto) {
+    const int run = __builtin_amdgcn_readlane(upto, 63);
+    k = tree_keys(a, tree_length(a, b0 + static_cast<int>(threadIdx.x & 63)));
+    upto = scan64(rounds(k)) + run;
   }
 };
 
 // Bit t of the result: node `lane` sees drafted token t (its ancestors and itself).  A parent that
 // is neither -1 nor an earlier node leaves the node without a place: it sees nothing and nothing
 // sees it.  Pointer doubling: after k steps a lane has its next 2^k ancestors.
-__device__ __forceinline__ uint64_t tree_ancestors(const TreeArgs& a, int b) {
+__device__ __forceinline__ int tree_parent(const TreeArgs& a, int b) {
   const int i = threadIdx.x & 63;
-  int par = -2;
-  if (i < a.T) par = a.parents ? a.parents[b * a.ld_parents + i] : i - 1;
+  return i >= a.T ? -2 : a.parents ? a.parents[b * a.ld_parents + i] : i - 1;
+}
+__device__ __forceinline__ uint64_t tree_ancestors(const TreeArgs& a, int par) {
+  const int i = threadIdx.x & 63;
   const bool placed = par >= -1 && par < i;
   uint64_t seen = placed ? 1ull << i : 0;
   int up = placed ? par : -1;
@@ -162,6 +163,40 @@ __device__ __forceinline__ uint32_t tree_visible(uint64_t tokens, int d, int row
   const uint64_t drafted = d <= -64 || d >= 32 ? 0 : d >= 0 ? tokens << d : tokens >> -d;
   return static_cast<uint32_t>((cached | drafted) & ((1ull << rows) - 1));
 }
+
+// A thread's entries of the lookup tables (SmallLuts): everything that a block loads before it
+// knows its sequence is loaded at once, the tables are written when it has arrived.
+template <int BITS>
+struct TreeTables {
+  using L = SmallLuts<BITS>;
+  static constexpr int KB = L::KB, VB = L::VB, KM = (1 << KB) - 1, VM = (1 << VB) - 1;
+  uint16_t k0, k1;
+  float v0, v1;
+  __device__ __forceinline__ TreeTables(const TreeArgs& a, int tid)
+      : k0(a.kcent[KB == 1 ? 0 : tid & KM]), k1(a.kcent[KB == 1 ? 1 : (tid >> KB) & KM]), v0(a.vcent[tid & VM]),
+        v1(a.vcent[(tid >> VB) & VM]) {}
+  __device__ __forceinline__ void keys(uint8_t* t, int tid) const {
+    if (tid < 16) {
+      half4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = static_cast<_Float16>((tid >> j) & 1 ? 1.f : -1.f);
+      *reinterpret_cast<half4*>(t + L::SGN_OFF + tid * 8) = v;
+    }
+    if constexpr (KB == 1) {
+      typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+      if (tid < 16)
+        *reinterpret_cast<u16x4*>(t + L::KEY_OFF + tid * 8) =
+            u16x4{tid & 1 ? k1 : k0, tid & 2 ? k1 : k0, tid & 4 ? k1 : k0, tid & 8 ? k1 : k0};
+    } else {
+      if (tid < L::KEY_BYTES / 4) *reinterpret_cast<uint32_t*>(t + L::KEY_OFF + tid * 4) = k0 | static_cast<uint32_t>(k1) << 16;
+    }
+  }
+  __device__ __forceinline__ void values(uint8_t* t, int tid) const {
+    typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+    if (tid < L::VAL_BYTES / 4)
+      *reinterpret_cast<half2v*>(t + L::VAL_OFF + tid * 4) = half2v{static_cast<_Float16>(v0), static_cast<_Float16>(v1)};
+  }
+};
 
 // ---------------------------------------------------------------- the stream of packed rows
 // A wave's ring of slabs of 32 keys, filled by direct copies to LDS.
@@ -359,17 +394,15 @@ tree_attn_kernel(TreeArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, lg = lane >> 4;
   const int ct0 = blockIdx.y * (16 * NT), hkv = blockIdx.z;
-  const TreeSplit<RK> split(a);
+  const int n0 = tree_length(a, lane);
+  const TreeTables<BITS> tables(a, tid);
+  const TreeSplit<RK> split(a, n0);
   if (static_cast<int>(blockIdx.x) >= split.blocks) return;  // block-uniform
   int x = split.begin(blockIdx.x);
   const int x_end = split.begin(blockIdx.x + 1);
 
-  {
-    DecodeArgs t{};
-    t.kcent = a.kcent;
-    t.vcent = a.vcent;
-    build_small_luts<BITS, true>(t, luts, tid);
-  }
+  tables.keys(luts, tid);
+  tables.values(luts, tid);
   const float fa = a.scale * LOG2E;
   float qs;
   const int vbit = l16 * VFB, vbase = (vbit >> 5) * 4, vshift = vbit & 31;
@@ -378,24 +411,42 @@ tree_attn_kernel(TreeArgs a) {
 
   // ---- one part after the other: the rounds of this block's stretch that belong to one sequence
   while (x < x_end) {
-    int b, first, n;
-    split.sequence_at(a, x, b, first, n);
+    int b, first, nkeys;
+    split.sequence_at(a, x, b, first, nkeys);
     const int rec = static_cast<int>(blockIdx.x) + b;
-    const int nkeys = tree_keys(a, b), nctx = nkeys - a.T;
-    const int kbeg = (x - first) * RK, kend = min(nkeys, (min(x_end, first + n) - first) * RK);
-    x = min(x_end, first + n);
+    const int nctx = nkeys - a.T, last = min(x_end, first + split.rounds(nkeys));
+    const int kbeg = (x - first) * RK, kend = min(nkeys, (last - first) * RK);
+    x = last;
 
-    const uint64_t anc_lane = tree_ancestors(a, b);
+    // parents, the first slabs' pages and the queries come in one round trip
+    const int par = tree_parent(a, b);
+    const ST stream(a, b, hkv, kend);
+    const int k0w = kbeg + wave * NK;
+    int nrows[R], pages[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) pages[r] = k0w + r * RK < kend ? stream.page_of(k0w + r * RK) : -1;
+    constexpr int TPC = 64 * NW / (16 * NT), DPT = D / TPC;  // threads per column, dims per thread
+    static_assert(DPT == 4 || DPT == 8 || DPT == 16, "whole fragments or halves of one");
+    const int qcol = tid / TPC, d0 = (tid % TPC) * DPT;
+    float4v pj4[DPT / 4];
+    half4 rt4[DPT / 4];
+    {
+      const int c = min(ct0 + qcol, a.C - 1), node = c / a.G;
+      const int64_t row = ((static_cast<int64_t>(b) * a.Hq + hkv * a.G + (c - node * a.G)) * a.T + node) * D + d0;
+#pragma unroll
+      for (int i = 0; i < DPT / 4; ++i) {
+        pj4[i] = *reinterpret_cast<const float4v*>(a.q_proj + row + 4 * i);
+        rt4[i] = *reinterpret_cast<const half4*>(a.q_rot + row + 4 * i);
+      }
+    }
+    const uint64_t anc_lane = tree_ancestors(a, par);
     if (wave == 0) sm.anc[lane] = anc_lane;
     const uint64_t live = __ballot(anc_lane != 0);  // tokens with a place: some node sees them
     __syncthreads();  // tables and ancestors in place; the previous part is done with the LDS
 
-    const ST stream(a, b, hkv, kend);
     // the first slabs fly while the queries are set up
-    const int k0w = kbeg + wave * NK;
-    int nrows[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) nrows[r] = k0w + r * RK < kend ? stream.issue(k0w + r * RK, stream.page_of(k0w + r * RK), mine_lds + r * SLOT) : 0;
+    for (int r = 0; r < R; ++r) nrows[r] = k0w + r * RK < kend ? stream.issue(k0w + r * RK, pages[r], mine_lds + r * SLOT) : 0;
 
     // ---- the block's queries, laid out by all its threads as B fragments (lane (column l16, group lg)
     // of k-step ks holds dims lg D / 4 + 8 ks ..): q_rot, and coeff q_proj (f32) as f16 hi + lo
@@ -403,16 +454,12 @@ tree_attn_kernel(TreeArgs a) {
     // [2^13, 2^14): q_rot stays exact, and the lo parts stay normal f16 down to 2^-17 of it.
     // Columns behind the last repeat it; they are not stored.
     {
-      constexpr int TPC = 64 * NW / (16 * NT), DPT = D / TPC;  // threads per column, dims per thread
-      static_assert(DPT == 4 || DPT == 8 || DPT == 16, "whole fragments or halves of one");
-      const int col = tid / TPC, d0 = (tid % TPC) * DPT;
-      const int c = min(ct0 + col, a.C - 1), node = c / a.G;
-      const int64_t row = ((static_cast<int64_t>(b) * a.Hq + hkv * a.G + (c - node * a.G)) * a.T + node) * D + d0;
+      const int col = qcol;
       float pj[DPT], rt[DPT];
 #pragma unroll
       for (int i = 0; i < DPT; i += 4) {
-        const float4v x4 = *reinterpret_cast<const float4v*>(a.q_proj + row + i);
-        const half4 h4 = *reinterpret_cast<const half4*>(a.q_rot + row + i);
+        const float4v x4 = pj4[i / 4];
+        const half4 h4 = rt4[i / 4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           pj[i + e] = x4[e] * a.coeff;
@@ -524,7 +571,6 @@ tree_attn_kernel(TreeArgs a) {
       static_for<KS>([&](auto cc) {
         constexpr int ks = decltype(cc)::value, h = ks % NB, next = ks + NB - 1;
         if constexpr (next < KS) look(std::integral_constant<int, next>{});
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -772,7 +818,9 @@ tree_plane_kernel(TreeArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, lg = lane >> 4;
   const int hkv = blockIdx.z;
-  const TreeSplit<RK> split(a);
+  const int n0 = tree_length(a, lane);
+  const TreeTables<BITS> tables(a, tid);
+  const TreeSplit<RK> split(a, n0);
   if (static_cast<int>(blockIdx.x) >= split.blocks) return;  // block-uniform
   int x = split.begin(blockIdx.x);
   const int x_end = split.begin(blockIdx.x + 1);
@@ -781,12 +829,11 @@ tree_plane_kernel(TreeArgs a) {
   qa.q_rot = a.q_rot;
   qa.q_proj = a.q_proj;
   qa.kcent = a.kcent;
-  qa.vcent = a.vcent;
   qa.Hq = a.Hq;
   qa.Sq = a.T;
   qa.G = a.G;
   qa.C = a.C;
-  build_small_luts<BITS, true>(qa, sm.luts, tid);
+  tables.values(sm.luts, tid);
   const float fa = a.scale * LOG2E;
   const int vbit = l16 * VFB, vbase = (vbit >> 5) * 4, vshift = vbit & 31;
   uint8_t* const mine = sm.area + wave * ST::SLOT;
@@ -794,23 +841,25 @@ tree_plane_kernel(TreeArgs a) {
   _Float16* const pt = &sm.p[wave][0][0];
 
   while (x < x_end) {
-    int b, first, n;
-    split.sequence_at(a, x, b, first, n);
+    int b, first, nkeys;
+    split.sequence_at(a, x, b, first, nkeys);
     const int rec = static_cast<int>(blockIdx.x) + b;
-    const int nkeys = tree_keys(a, b), nctx = nkeys - a.T;
-    const int kbeg = (x - first) * RK, kend = min(nkeys, (min(x_end, first + n) - first) * RK);
-    x = min(x_end, first + n);
+    const int nctx = nkeys - a.T, last = min(x_end, first + split.rounds(nkeys));
+    const int kbeg = (x - first) * RK, kend = min(nkeys, (last - first) * RK);
+    x = last;
 
-    const uint64_t anc_lane = tree_ancestors(a, b);
+    // parents, the first slabs' pages and the queries come in one round trip
+    const int par = tree_parent(a, b);
+    const ST stream(a, b, hkv, kend);
+    const int k0w = kbeg + wave * NK;
+    int nrows[R], pages[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) pages[r] = k0w + r * RK < kend ? stream.page_of(k0w + r * RK) : -1;
+    const uint64_t anc_lane = tree_ancestors(a, par);
     if (wave == 0) sm.anc[lane] = anc_lane;
     const uint64_t live = __ballot(anc_lane != 0);
     __syncthreads();  // tables and ancestors in place; the previous part is done with the LDS
-    const ST stream(a, b, hkv, kend);
-    const int k0w = kbeg + wave * NK;
-    int nrows[R];
-    auto start = [&](int r) {
-      nrows[r] = k0w + r * RK < kend ? stream.issue(k0w + r * RK, stream.page_of(k0w + r * RK), mine_lds + r * STRIDE) : 0;
-    };
+    auto start = [&](int r) { nrows[r] = k0w + r * RK < kend ? stream.issue(k0w + r * RK, pages[r], mine_lds + r * STRIDE) : 0; };
 #pragma unroll
     for (int r = 0; r < R - SM::NSTG; ++r) start(r);
     PQ pq;
@@ -1009,6 +1058,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
   const int c0 = blockIdx.x * NC, hkv = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6, l16 = lane & 15, lg = lane >> 4;
 
+  const int n0 = tree_length(a, lane);  // before Pi_v: waited for first
   const _Float16* Ph = reinterpret_cast<const _Float16*>(a.vpit);
   const _Float16* Pl = Ph + D * D;
   half8 ah[RB][D / 32], al[RB][D / 32];
@@ -1021,7 +1071,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
       al[rb][ks] = *reinterpret_cast<const half8*>(Pl + i * D + ks * 32 + lg * 8);
     }
   }
-  const TreeSplit<RK> split(a);
+  const TreeSplit<RK> split(a, n0);
   int first = 0, n = 0;
   split.rounds_of(a, b, first, n);
   if (n > 0) {  // records k + b of the blocks k that hold the sequence's rounds
