@@ -1017,6 +1017,27 @@ Tensor tree_attention_meta(const Tensor& q_rot, const Tensor& q_proj, const Tens
   return check_tree(c, q_rot, pool, kcent16, bits, vcent32, vpit, table, lengths, parents, out_dtype);
 }
 
+int64_t tree_workspace(const Tensor& q, const Tensor& kvn, const Tensor& table, int64_t bits) {
+  return tq_tree_workspace_size(i32(q.size(0)), i32(q.size(1)), i32(kvn.size(1)), i32(q.size(2)), i32(table.size(1)),
+                                i32(kvn.size(2)), i32(q.size(3)), i32(bits));
+}
+// out [B, T, Hq, D]; arguments checked
+void tree_launch(const uint16_t* q_rot, const float* q_proj, const Tensor& kcodes, const Tensor& ksigns, const Tensor& krn,
+                 const Tensor& kvn, const Tensor& kcent16, int64_t bits, const Tensor& vcodes, const Tensor& vvn,
+                 const Tensor& vcent32, const Tensor& vpit, const Tensor& table, const Tensor& lengths,
+                 const c10::optional<Tensor>& parents, double coeff, double scale, const Tensor& out, void* ws, int64_t bytes) {
+  const int32_t B = i32(out.size(0)), T = i32(out.size(1)), Hq = i32(out.size(2)), D = i32(out.size(3)), W = i32(table.size(1));
+  const bool tree = parents.has_value() && parents->defined();
+  check_status(tq_tree_attention(q_rot, q_proj, ptr<uint8_t>(kcodes), ptr<uint8_t>(ksigns), ptr<uint16_t>(krn),
+                                 ptr<uint16_t>(kvn), ptr<uint16_t>(kcent16), i32(bits), ptr<uint8_t>(vcodes),
+                                 ptr<uint16_t>(vvn), ptr<float>(vcent32), ptr<uint16_t>(vpit), kvn.size(0), i32(kvn.size(2)),
+                                 ptr<int32_t>(table), W, W, ptr<int32_t>(lengths), tree ? ptr<int32_t>(*parents) : nullptr,
+                                 tree && parents->dim() == 2 ? T : 0, B, Hq, i32(kvn.size(1)), T, D, static_cast<float>(coeff),
+                                 static_cast<float>(scale), out.data_ptr(), dtype_code(out.scalar_type()), out.stride(0),
+                                 out.stride(2), out.stride(1), ws, bytes, stream_of(out)),
+               "tree_attention");
+}
+
 Tensor tree_attention(const Tensor& q_rot, const Tensor& q_proj, const Tensor& kcodes, const Tensor& ksigns,
                       const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits, const Tensor& vcodes,
                       const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit, const Tensor& table,
@@ -1025,20 +1046,10 @@ Tensor tree_attention(const Tensor& q_rot, const Tensor& q_proj, const Tensor& k
   Tensor out = tree_attention_meta(q_rot, q_proj, kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn, vcent32, vpit, table,
                                    lengths, parents, coeff, scale, out_dtype);
   const c10::DeviceGuard g(q_rot.device());
-  const int32_t B = i32(q_rot.size(0)), Hq = i32(q_rot.size(1)), T = i32(q_rot.size(2)), D = i32(q_rot.size(3));
-  const int32_t Hkv = i32(kvn.size(1)), P = i32(kvn.size(2)), W = i32(table.size(1));
-  const int64_t bytes = tq_tree_workspace_size(B, Hq, Hkv, T, W, P, D, i32(bits));
+  const int64_t bytes = tree_workspace(q_rot, kvn, table, bits);
   Tensor ws = at::empty({bytes}, q_rot.options().dtype(at::kByte));
-  const bool tree = parents.has_value() && parents->defined();
-  check_status(tq_tree_attention(ptr<uint16_t>(q_rot), ptr<float>(q_proj), ptr<uint8_t>(kcodes), ptr<uint8_t>(ksigns),
-                                 ptr<uint16_t>(krn), ptr<uint16_t>(kvn), ptr<uint16_t>(kcent16), i32(bits),
-                                 ptr<uint8_t>(vcodes), ptr<uint16_t>(vvn), ptr<float>(vcent32), ptr<uint16_t>(vpit),
-                                 kvn.size(0), P, ptr<int32_t>(table), W, W, ptr<int32_t>(lengths),
-                                 tree ? ptr<int32_t>(*parents) : nullptr, tree && parents->dim() == 2 ? T : 0, B, Hq, Hkv, T,
-                                 D, static_cast<float>(coeff), static_cast<float>(scale), out.data_ptr(),
-                                 dtype_code(out_dtype), out.stride(0), out.stride(2), out.stride(1), ws.data_ptr(), bytes,
-                                 stream_of(out)),
-               "tree_attention");
+  tree_launch(ptr<uint16_t>(q_rot), ptr<float>(q_proj), kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn, vcent32, vpit,
+              table, lengths, parents, coeff, scale, out, ws.data_ptr(), bytes);
   return out;
 }
 
@@ -1055,14 +1066,28 @@ Tensor tree_attend_meta(const Tensor& q, const Tensor& pi_split, const Tensor& s
   return out;
 }
 
-Tensor tree_attend(const Tensor& q, const Tensor& pi_split, const Tensor& s_eff16, const Tensor& kcodes,
+Tensor tree_attend(const Tensor& q_in, const Tensor& pi_split, const Tensor& s_eff16, const Tensor& kcodes,
                    const Tensor& ksigns, const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits,
                    const Tensor& vcodes, const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit, const Tensor& table,
                    const Tensor& lengths, const c10::optional<Tensor>& parents, double coeff, double scale,
                    at::ScalarType out_dtype) {
-  auto qp = query_prep(q, pi_split, s_eff16);
-  return tree_attention(std::get<0>(qp), std::get<1>(qp), kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn, vcent32, vpit,
-                        table, lengths, parents, coeff, scale, out_dtype);
+  Tensor out = tree_attend_meta(q_in, pi_split, s_eff16, kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn, vcent32, vpit,
+                                table, lengths, parents, coeff, scale, out_dtype);
+  const c10::DeviceGuard g(q_in.device());
+  Tensor q = activation(q_in);
+  // one allocation: the workspace, then the prepared queries
+  const int64_t bytes = (tree_workspace(q, kvn, table, bits) + 15) / 16 * 16, n = q.numel();
+  Tensor ws = at::empty({bytes + n * 6}, q.options().dtype(at::kByte));
+  uint8_t* const base = ptr<uint8_t>(ws);
+  float* const q_proj = reinterpret_cast<float*>(base + bytes);
+  uint16_t* const q_rot = reinterpret_cast<uint16_t*>(q_proj + n);
+  check_status(tq_query_prep(q.data_ptr(), dtype_code(q.scalar_type()), i32(q.size(0)), i32(q.size(1)), i32(q.size(2)),
+                             i32(q.size(3)), q.stride(0), q.stride(1), q.stride(2), ptr<uint16_t>(pi_split),
+                             ptr<uint16_t>(s_eff16), q_rot, q_proj, stream_of(q)),
+               "tree_attention");
+  tree_launch(q_rot, q_proj, kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn, vcent32, vpit, table, lengths, parents, coeff,
+              scale, out, base, bytes);
+  return out;
 }
 
 using Verified = std::tuple<Tensor, Tensor, Tensor>;
