@@ -358,6 +358,19 @@ int tq_page_write(void* const* pool, void* const* rows, int32_t B, int32_t H, in
                   int32_t page_size, const int32_t* block_table, int64_t ld_table,
                   int32_t table_width, const int32_t* start, void* stream);
 
+/* tq_cache_append into pages: new keys and values [B, H, S, d] (head_dim 64 or 128, 2 <= bits <= 4,
+ * key codes of bits - 1) compressed into positions start[b] + s, and, with q, the new queries
+ * prepared, in one launch.  The rows are those of tq_compress_keys / tq_compress_values. */
+int tq_page_append(const void* k, const void* v, int32_t dtype, int32_t B, int32_t H, int32_t S,
+                   int32_t d, int64_t skb, int64_t skh, int64_t sks, int64_t svb, int64_t svh,
+                   int64_t svs, const uint16_t* key_pi_split, const uint16_t* key_seff_split,
+                   const float* key_centroids, const float* key_bounds, const uint16_t* val_pi_split,
+                   const float* val_bounds, int32_t bits, void* const* pool, int64_t num_pages,
+                   int32_t page_size, const int32_t* block_table, int64_t ld_table,
+                   int32_t table_width, const int32_t* start, const void* q, int32_t Hq, int64_t sqb,
+                   int64_t sqh, int64_t sqs, const uint16_t* key_s_eff_f16, uint16_t* q_rot,
+                   float* q_proj, void* stream);
+
 /* Positions s < min(S, lengths[b]) to rows [B, H, S] of six contiguous planes; zeros behind, and
  * where a position has no page. */
 int tq_page_read(void* const* pool, void* const* rows, int32_t B, int32_t H, int32_t S, int32_t d,

@@ -222,3 +222,51 @@ def test_c_entries_refuse():
     assert b"chain" in lib.tq_last_error()
     assert lib.tq_verify_drafts(16, 16, 0, 0, 0, none, 0, 0, 16, 16, 0, 1, 2, 10, 16, 16, 16, 16, 1, none) == -1
     assert b"workspace" in lib.tq_last_error()
+
+
+def _append_args():
+    t = dict(_tree_args(True))
+    head = dict(k=_e(B, H, T, D, dtype=torch.bfloat16), v=_e(B, H, T, D, dtype=torch.bfloat16), q=t.pop("q"),
+                pi=t.pop("pi"), ks=_e(2, D, D, dtype=F16), kc=_e(4), kb=_e(3), vpi=_e(2, D, D, dtype=F16), vb=_e(7),
+                se=t.pop("se"))
+    return {**head, **t}
+
+
+@pytest.mark.parametrize("bad,match", POOL + [
+    (dict(k=_e(B, H, T + 1, D)), "k and v must be"),
+    (dict(v=_e(B, H, T, D // 2)), "k and v must be"),
+    (dict(k=_e(B, H + 1, T, D), v=_e(B, H + 1, T, D)), "k and v must be"),
+    (dict(ks=_e(D, D, dtype=F16)), "key split S_eff"),
+    (dict(kc=_e(3)), "key centroids"),
+    (dict(kb=_e(2)), "key boundaries"),
+    (dict(vpi=_e(2, D, D)), "value split Pi"),
+    (dict(vb=_e(6)), "value boundaries"),
+    (dict(se=_e(2, D, dtype=F16)), "f16 S_eff"),
+    (dict(q=_e(B, 8, 65, D)), "1 to 64"),
+    (dict(bits=4), "the pool holds"),
+    (dict(parents=_e(T + 1, dtype=I32)), "parents must be"),
+    (dict(lengths=_e(B + 1, dtype=I32)), "lengths must be"),
+    (dict(out=torch.int32), "out_dtype"),
+])
+def test_page_attend_refuses(bad, match):
+    out = ops().page_attend(*_append_args().values())
+    assert out.shape == (B, T, 8, D) and out.dtype == torch.bfloat16
+    _refuses(ops().page_attend, _append_args(), bad, match)
+
+
+def test_page_append_c_entry_refuses():
+    lib = _native.lib()
+    six = (ctypes.c_void_p * 6)(*[16 * (i + 1) for i in range(6)])
+    odd = (ctypes.c_void_p * 6)(*[16 * (i + 1) + 4 for i in range(6)])
+    none = None
+
+    def call(pool=six, dt=0, B=1, H=2, S=3, d=64, bits=3, n=5, P=64, W=2, k=16, q=16, qr=16):
+        return lib.tq_page_append(k, 16, dt, B, H, S, d, *[0] * 6, *[16] * 6, bits, pool, n, P, 16, W, W, 16, q, 4, 0, 0, 0,
+                                  16, qr, 16, none)
+
+    assert call(d=96) == -2 and call(bits=5) == -2 and call(bits=1) == -2
+    for kw, msg in ((dict(dt=7), b"dtype"), (dict(P=48), b"power of two"), (dict(P=16), b"power of two"), (dict(n=0), b"bad pool"),
+                    (dict(S=-1), b"bad shape"), (dict(H=0), b"bad shape"), (dict(k=none), b"null"), (dict(pool=odd), b"16-byte"),
+                    (dict(qr=4), b"q_rot"), (dict(B=1 << 20, H=1 << 10, S=64), b"2^31")):
+        assert call(**kw) == -1 and msg in lib.tq_last_error(), kw
+    assert call(B=0, k=none) == 0 and call(S=0, k=none) == 0

@@ -565,14 +565,30 @@ struct TileArgs {
   // norm planes (a cache of ldo positions per (batch, head), filled from position off); ldo = 0
   // writes row (b, h, s) to (b * H + h) * S + s
   int64_t ldo, off;
+  // pages: row (b, h, s) is position start[b] + s of sequence b
+  const int32_t *table, *start;
+  int64_t ld_table, num_pages;
+  int table_width, lg_page;
 };
 
-// packed / norm plane row of input row gr (< 2^31); MAP = false: the kernel ignores ldo / off
-template <bool MAP>
+// where a kernel's output rows stand: as the input's, in capacity planes (ldo, off), or in pages
+enum OutMap { kMapNone, kMapCapacity, kMapPages };
+
+// packed / norm plane row of input row gr (< 2^31); pages: -1 for a row without a page
+template <int MAP>
 __device__ __forceinline__ int64_t out_row(const TileArgs& a, int64_t gr) {
-  if (!MAP || a.ldo == 0) return gr;
+  if (MAP == kMapNone || (MAP == kMapCapacity && a.ldo == 0)) return gr;
   const uint32_t r32 = static_cast<uint32_t>(gr);
   const uint32_t bh = a.S.div(r32);
+  if constexpr (MAP == kMapPages) {
+    const uint32_t b = a.H.div(bh);
+    const int from = a.start[b];
+    const int64_t pos = static_cast<int64_t>(from) + (r32 - bh * a.S.d), slot = pos >> a.lg_page;
+    if (from < 0 || slot >= a.table_width) return -1;
+    const int64_t page = a.table[b * a.ld_table + slot];
+    if (page < 0 || page >= a.num_pages) return -1;
+    return ((page * a.H.d + (bh - b * a.H.d)) << a.lg_page) + (pos & ((int64_t(1) << a.lg_page) - 1));
+  }
   return static_cast<int64_t>(bh) * a.ldo + a.off + (r32 - bh * a.S.d);
 }
 
@@ -734,9 +750,9 @@ struct RowsSmem {
 };
 
 // One block of the row-owned kernels: block `block` of `nblocks` blocks that share the rows.
-// MAP: outputs go to the rows out_row<true> names (a cache append); the plain form keeps the
+// MAP: outputs go to the rows out_row<MAP> names (a cache append); the plain form keeps the
 // registers that mapping needs free for the tile loop.
-template <int D, int DT, int MODE, int BB, int NW_, bool MAP>
+template <int D, int DT, int MODE, int BB, int NW_, int MAP>
 __device__ __forceinline__ void rows_body(const TileArgs& a, RowsSmem<D, MODE, BB, NW_>& sm, int block,
                                           int nblocks) {
   using T = RT<D, NW_>;
@@ -900,15 +916,16 @@ __device__ __forceinline__ void rows_body(const TileArgs& a, RowsSmem<D, MODE, B
   auto store_rows = [&](const uint8_t* src, uint8_t* out, int64_t row0, int bytes) {
     const int64_t nr = a.n - row0 < 16 ? a.n - row0 : 16;
     const int nd = static_cast<int>(nr) * bytes / 4;
-    if (!MAP || a.ldo == 0) {
+    if (MAP == kMapNone || (MAP == kMapCapacity && a.ldo == 0)) {
       uint32_t* dst = reinterpret_cast<uint32_t*>(out + row0 * bytes);
       for (int i = lane; i < nd; i += 64) dst[i] = reinterpret_cast<const uint32_t*>(src)[i];
     } else {
       const int wpr = bytes / 4;  // dwords per row (rows of d * b / 8 bytes, d = 64 or 128)
       for (int i = lane; i < nd; i += 64) {
         const int r = i / wpr;
-        reinterpret_cast<uint32_t*>(out + out_row<MAP>(a, row0 + r) * bytes)[i - r * wpr] =
-            reinterpret_cast<const uint32_t*>(src)[i];
+        const int64_t orow = out_row<MAP>(a, row0 + r);
+        if (MAP == kMapPages && orow < 0) continue;
+        reinterpret_cast<uint32_t*>(out + orow * bytes)[i - r * wpr] = reinterpret_cast<const uint32_t*>(src)[i];
       }
     }
   };
@@ -1079,7 +1096,10 @@ __device__ __forceinline__ void rows_body(const TileArgs& a, RowsSmem<D, MODE, B
       float vn_p = 0.f;
       auto flush = [&]() {
         const int64_t grp = tp * 16 + l16;
-        if (g == 0 && grp < a.n) a.vn[out_row<MAP>(a, grp)] = f2h(vn_p);
+        if (g == 0 && grp < a.n) {
+          const int64_t orow = out_row<MAP>(a, grp);
+          if (MAP != kMapPages || orow >= 0) a.vn[orow] = f2h(vn_p);
+        }
         wave_sync();
         store_rows(stg, a.codes, tp * 16, KC);
         wave_sync();
@@ -1132,8 +1152,10 @@ __device__ __forceinline__ void rows_body(const TileArgs& a, RowsSmem<D, MODE, B
         const int64_t grp = tp * 16 + l16;
         if (g == 0 && grp < a.n) {
           const int64_t orow = out_row<MAP>(a, grp);
-          a.vn[orow] = f2h(vn_p);
-          a.rn[orow] = f2h(rn_p);
+          if (MAP != kMapPages || orow >= 0) {
+            a.vn[orow] = f2h(vn_p);
+            a.rn[orow] = f2h(rn_p);
+          }
         }
         wave_sync();
         store_rows(stg, a.codes, tp * 16, KC);
@@ -1224,7 +1246,7 @@ template <int D, int DT, int MODE, int BB>
 __global__ void __launch_bounds__((64 * row_waves<MODE, DT>())) rows_kernel(TileArgs a) {
   using SM = RowsSmem<D, MODE, BB, row_waves<MODE, DT>()>;
   __shared__ __attribute__((aligned(16))) uint8_t smem[sizeof(SM)];
-  rows_body<D, DT, MODE, BB, row_waves<MODE, DT>(), false>(a, *reinterpret_cast<SM*>(smem), blockIdx.x, gridDim.x);
+  rows_body<D, DT, MODE, BB, row_waves<MODE, DT>(), kMapNone>(a, *reinterpret_cast<SM*>(smem), blockIdx.x, gridDim.x);
 }
 
 // Few rows (a decode step's queries): blocks of 4 waves, one per SIMD, so that the rows'
@@ -1235,15 +1257,15 @@ template <int D, int DT, int MODE, int BB>
 __global__ void __launch_bounds__(64 * kFewWaves) rows_few_kernel(TileArgs a) {
   using SM = RowsSmem<D, MODE, BB, kFewWaves>;
   __shared__ __attribute__((aligned(16))) uint8_t smem[sizeof(SM)];
-  rows_body<D, DT, MODE, BB, kFewWaves, false>(a, *reinterpret_cast<SM*>(smem), blockIdx.x, gridDim.x);
+  rows_body<D, DT, MODE, BB, kFewWaves, kMapNone>(a, *reinterpret_cast<SM*>(smem), blockIdx.x, gridDim.x);
 }
 
 // A cache append in one launch: blocks [0, nbk) compress the new keys, [nbk, nbk + nbv) the
 // new values, the rest prepare the new queries (nbq blocks, 0 without queries).  Every block
 // has 4 waves (one per SIMD: a step's few tiles spread over compute units); the LDS holds one
-// mode's layout at a time.
+// mode's layout at a time.  MAP: capacity planes, or pages.
 constexpr int kAppendWaves = 4;
-template <int D, int DT, int KBB, int VB>
+template <int D, int DT, int KBB, int VB, int MAP>
 __global__ void __launch_bounds__(64 * kAppendWaves) append_kernel(TileArgs ka, TileArgs va, TileArgs qa, int nbk,
                                                                    int nbv, int nbq) {
   constexpr int NW = kAppendWaves;
@@ -1254,9 +1276,9 @@ __global__ void __launch_bounds__(64 * kAppendWaves) append_kernel(TileArgs ka, 
                                                    : (sizeof(SV) > sizeof(SQ) ? sizeof(SV) : sizeof(SQ));
   __shared__ __attribute__((aligned(16))) uint8_t smem[BYTES];
   const int blk = static_cast<int>(blockIdx.x);
-  if (blk < nbk) rows_body<D, DT, TM_KEYS, KBB, NW, true>(ka, *reinterpret_cast<SK*>(smem), blk, nbk);
-  else if (blk < nbk + nbv) rows_body<D, DT, TM_VALUES, VB, NW, true>(va, *reinterpret_cast<SV*>(smem), blk - nbk, nbv);
-  else rows_body<D, DT, TM_QUERY, 1, NW, false>(qa, *reinterpret_cast<SQ*>(smem), blk - nbk - nbv, nbq);
+  if (blk < nbk) rows_body<D, DT, TM_KEYS, KBB, NW, MAP>(ka, *reinterpret_cast<SK*>(smem), blk, nbk);
+  else if (blk < nbk + nbv) rows_body<D, DT, TM_VALUES, VB, NW, MAP>(va, *reinterpret_cast<SV*>(smem), blk - nbk, nbv);
+  else rows_body<D, DT, TM_QUERY, 1, NW, kMapNone>(qa, *reinterpret_cast<SQ*>(smem), blk - nbk - nbv, nbq);
 }
 
 // Blocks of `kernel` the device holds at once (occupancy x compute units), per device.
@@ -1319,11 +1341,11 @@ void dispatch_tile<TM_QUERY>(const TileArgs& a, int d, int dtype, int, hipStream
 }
 
 // ---------------------------------------------------------------- cache append (one launch)
-template <int D, int DT, int KBB, int VB>
+template <int MAP, int D, int DT, int KBB, int VB>
 static void launch_append(const TileArgs& ka, const TileArgs& va, const TileArgs& qa, hipStream_t s) {
   static int cache[16] = {};
   constexpr int NT = 64 * kAppendWaves, RROWS = 16 * kAppendWaves;
-  const int64_t res = resident_blocks(reinterpret_cast<const void*>(&append_kernel<D, DT, KBB, VB>), NT, cache);
+  const int64_t res = resident_blocks(reinterpret_cast<const void*>(&append_kernel<D, DT, KBB, VB, MAP>), NT, cache);
   // a block takes rounds of RROWS rows; when the three modes need more blocks than the device
   // holds at once, they share the resident blocks by work (a key row costs about two value or
   // query rows)
@@ -1336,27 +1358,28 @@ static void launch_append(const TileArgs& ka, const TileArgs& va, const TileArgs
     nv = std::max<int64_t>(1, std::min<int64_t>(nv, static_cast<int64_t>(res * wv / w)));
     nq = qa.n > 0 ? std::max<int64_t>(1, std::min<int64_t>(nq, res - nk - nv)) : 0;
   }
-  append_kernel<D, DT, KBB, VB><<<static_cast<unsigned>(nk + nv + nq), NT, 0, s>>>(
+  append_kernel<D, DT, KBB, VB, MAP><<<static_cast<unsigned>(nk + nv + nq), NT, 0, s>>>(
       ka, va, qa, static_cast<int>(nk), static_cast<int>(nv), static_cast<int>(nq));
 }
 
-template <int D, int KBB, int VB>
+template <int MAP, int D, int KBB, int VB>
 static void launch_append_dt(const TileArgs& ka, const TileArgs& va, const TileArgs& qa, int dtype, hipStream_t s) {
-  if (dtype == TQ_F32) launch_append<D, TQ_F32, KBB, VB>(ka, va, qa, s);
-  else if (dtype == TQ_F16) launch_append<D, TQ_F16, KBB, VB>(ka, va, qa, s);
-  else launch_append<D, TQ_BF16, KBB, VB>(ka, va, qa, s);
+  if (dtype == TQ_F32) launch_append<MAP, D, TQ_F32, KBB, VB>(ka, va, qa, s);
+  else if (dtype == TQ_F16) launch_append<MAP, D, TQ_F16, KBB, VB>(ka, va, qa, s);
+  else launch_append<MAP, D, TQ_BF16, KBB, VB>(ka, va, qa, s);
 }
 
 // head_dim 64 / 128, value bits 2-4 with key code bits one fewer (a compressor pair of one bit width)
+template <int MAP>
 static void dispatch_append(const TileArgs& ka, const TileArgs& va, const TileArgs& qa, int d, int dtype, int vb,
                             hipStream_t s) {
   switch (d * 8 + vb) {
-    case 64 * 8 + 2: launch_append_dt<64, 1, 2>(ka, va, qa, dtype, s); break;
-    case 64 * 8 + 3: launch_append_dt<64, 2, 3>(ka, va, qa, dtype, s); break;
-    case 64 * 8 + 4: launch_append_dt<64, 3, 4>(ka, va, qa, dtype, s); break;
-    case 128 * 8 + 2: launch_append_dt<128, 1, 2>(ka, va, qa, dtype, s); break;
-    case 128 * 8 + 3: launch_append_dt<128, 2, 3>(ka, va, qa, dtype, s); break;
-    default: launch_append_dt<128, 3, 4>(ka, va, qa, dtype, s); break;
+    case 64 * 8 + 2: launch_append_dt<MAP, 64, 1, 2>(ka, va, qa, dtype, s); break;
+    case 64 * 8 + 3: launch_append_dt<MAP, 64, 2, 3>(ka, va, qa, dtype, s); break;
+    case 64 * 8 + 4: launch_append_dt<MAP, 64, 3, 4>(ka, va, qa, dtype, s); break;
+    case 128 * 8 + 2: launch_append_dt<MAP, 128, 1, 2>(ka, va, qa, dtype, s); break;
+    case 128 * 8 + 3: launch_append_dt<MAP, 128, 2, 3>(ka, va, qa, dtype, s); break;
+    default: launch_append_dt<MAP, 128, 3, 4>(ka, va, qa, dtype, s); break;
   }
 }
 
@@ -1537,7 +1560,7 @@ int tq_cache_append(const void* k, const void* v, int32_t dtype, int32_t B, int3
       qa.sb = sqb; qa.sh = sqh; qa.ss = sqs; qa.vec = tile_vec(q, dtype, sqb, sqh, sqs);
       qa.w1 = key_pi_split; qa.w2 = key_s_eff_f16; qa.q_rot = q_rot; qa.q_proj = q_proj;
     }
-    dispatch_append(ka, va, qa, d, dtype, val_bits, st);
+    dispatch_append<kMapCapacity>(ka, va, qa, d, dtype, val_bits, st);
     return launch_status("tq_cache_append");
   }
   // other head dims and bit widths: the tile kernels, writing the same mapped rows
@@ -1554,6 +1577,56 @@ int tq_cache_append(const void* k, const void* v, int32_t dtype, int32_t B, int3
   if (nq > 0)
     return tq_query_prep(q, dtype, B, Hq, S, d, sqb, sqh, sqs, key_pi_split, key_s_eff_f16, q_rot, q_proj, stream);
   return TQ_OK;
+}
+
+int tq_page_append(const void* k, const void* v, int32_t dtype, int32_t B, int32_t H, int32_t S, int32_t d, int64_t skb,
+                   int64_t skh, int64_t sks, int64_t svb, int64_t svh, int64_t svs, const uint16_t* key_pi_split,
+                   const uint16_t* key_seff_split, const float* key_centroids, const float* key_bounds,
+                   const uint16_t* val_pi_split, const float* val_bounds, int32_t bits, void* const* pool,
+                   int64_t num_pages, int32_t page_size, const int32_t* block_table, int64_t ld_table, int32_t table_width,
+                   const int32_t* start, const void* q, int32_t Hq, int64_t sqb, int64_t sqh, int64_t sqs,
+                   const uint16_t* key_s_eff_f16, uint16_t* q_rot, float* q_proj, void* stream) {
+  if ((d != 64 && d != 128) || bits < 2 || bits > 4) {
+    set_error("tq_page_append: head_dim 64 or 128 and 2 to 4 bits, got %d and %d", d, bits);
+    return TQ_EUNSUPPORTED;
+  }
+  TQ_REQUIRE(dtype == TQ_F32 || dtype == TQ_F16 || dtype == TQ_BF16, "tq_page_append: unknown dtype %d", dtype);
+  TQ_REQUIRE(B >= 0 && H >= 1 && S >= 0 && (!q || Hq >= 1), "tq_page_append: bad shape");
+  TQ_REQUIRE(page_size >= 32 && page_size <= (1 << 20) && (page_size & (page_size - 1)) == 0,
+             "tq_page_append: page_size must be a power of two from 32 to 2^20, got %d", page_size);
+  TQ_REQUIRE(num_pages >= 1 && num_pages < (int64_t(1) << 31) && table_width >= 0 && ld_table >= table_width,
+             "tq_page_append: bad pool");
+  if (B == 0 || S == 0) return TQ_OK;
+  const int64_t n = static_cast<int64_t>(B) * H * S, nq = q ? static_cast<int64_t>(B) * Hq * S : 0;
+  TQ_REQUIRE(n < (int64_t(1) << 31) && nq < (int64_t(1) << 31), "tq_page_append: fewer than 2^31 rows in one call");
+  TQ_REQUIRE(k && v && key_pi_split && key_seff_split && key_centroids && key_bounds && val_pi_split && val_bounds && pool &&
+                 block_table && start,
+             "tq_page_append: null pointer");
+  for (int i = 0; i < 6; ++i)
+    TQ_REQUIRE(pool[i] && reinterpret_cast<uintptr_t>(pool[i]) % 16 == 0, "tq_page_append: pool planes must be 16-byte aligned");
+  TQ_REQUIRE(nq == 0 || (key_s_eff_f16 && q_rot && q_proj && reinterpret_cast<uintptr_t>(q_rot) % 8 == 0 &&
+                         reinterpret_cast<uintptr_t>(q_proj) % 16 == 0),
+             "tq_page_append: q_rot must be 8-byte and q_proj 16-byte aligned");
+  TileArgs ka{}, va{}, qa{};
+  ka.x = k; ka.n = n; ka.H = make_div(static_cast<uint32_t>(H)); ka.S = make_div(static_cast<uint32_t>(S));
+  ka.sb = skb; ka.sh = skh; ka.ss = sks; ka.vec = tile_vec(k, dtype, skb, skh, sks);
+  ka.w1 = key_pi_split; ka.w3 = key_seff_split; ka.cent = key_centroids; ka.bounds = key_bounds;
+  ka.codes = static_cast<uint8_t*>(pool[0]); ka.signs = static_cast<uint8_t*>(pool[1]);
+  ka.rn = static_cast<uint16_t*>(pool[2]); ka.vn = static_cast<uint16_t*>(pool[3]);
+  ka.table = block_table; ka.start = start; ka.ld_table = ld_table; ka.num_pages = num_pages;
+  ka.table_width = table_width; ka.lg_page = __builtin_ctz(static_cast<unsigned>(page_size));
+  va = ka;
+  va.x = v; va.sb = svb; va.sh = svh; va.ss = svs; va.vec = tile_vec(v, dtype, svb, svh, svs);
+  va.w1 = val_pi_split; va.w3 = nullptr; va.cent = nullptr; va.bounds = val_bounds;
+  va.codes = static_cast<uint8_t*>(pool[4]); va.signs = nullptr; va.rn = nullptr; va.vn = static_cast<uint16_t*>(pool[5]);
+  qa.n = nq;
+  if (nq > 0) {
+    qa.x = q; qa.H = make_div(static_cast<uint32_t>(Hq)); qa.S = ka.S;
+    qa.sb = sqb; qa.sh = sqh; qa.ss = sqs; qa.vec = tile_vec(q, dtype, sqb, sqh, sqs);
+    qa.w1 = key_pi_split; qa.w2 = key_s_eff_f16; qa.q_rot = q_rot; qa.q_proj = q_proj;
+  }
+  dispatch_append<kMapPages>(ka, va, qa, d, dtype, bits, as_stream(stream));
+  return launch_status("tq_page_append");
 }
 
 }  // extern "C"

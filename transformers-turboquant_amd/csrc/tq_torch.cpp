@@ -1090,6 +1090,68 @@ Tensor tree_attend(const Tensor& q_in, const Tensor& pi_split, const Tensor& s_e
   return out;
 }
 
+// A layer's decoding or speculation step in one call: the new tokens' keys and values compressed into
+// their pages (positions lengths[b] + i) and the queries prepared in one launch, then tree attention.
+Tensor page_attend_meta(const Tensor& k, const Tensor& v, const Tensor& q, const Tensor& kpi, const Tensor& kseff,
+                        const Tensor& kcent, const Tensor& kbounds, const Tensor& vpi, const Tensor& vbounds,
+                        const Tensor& kseff16, const Tensor& kcodes, const Tensor& ksigns, const Tensor& krn,
+                        const Tensor& kvn, const Tensor& kcent16, int64_t bits, const Tensor& vcodes, const Tensor& vvn,
+                        const Tensor& vcent32, const Tensor& vpit, const Tensor& table, const Tensor& lengths,
+                        const c10::optional<Tensor>& parents, double coeff, double scale, at::ScalarType out_dtype) {
+  const Checker c{"tq::page_attend", q.device()};
+  Pool pool{&kcodes, &ksigns, &krn, &kvn, &vcodes, &vvn};
+  Tensor out = check_tree(c, q, pool, kcent16, bits, vcent32, vpit, table, lengths, parents, out_dtype);
+  const int64_t D = q.size(3);
+  TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(1) == pool.H &&
+                  k.size(2) == q.size(2) && k.size(3) == D,
+              c.op, ": k and v must be [", q.size(0), ", ", pool.H, ", ", q.size(2), ", ", D, "], got ", k.sizes(), " and ",
+              v.sizes());
+  c.same_device(k, "k");
+  c.same_device(v, "v");
+  c.table(kpi, "key split Pi", at::kHalf, 2 * D * D);
+  c.table(kseff, "key split S_eff", at::kHalf, 2 * D * D);
+  c.table(kcent, "key centroids", at::kFloat, int64_t{1} << (bits - 1));
+  c.table(kbounds, "key boundaries", at::kFloat, (int64_t{1} << (bits - 1)) - 1);
+  c.table(vpi, "value split Pi", at::kHalf, 2 * D * D);
+  c.table(vbounds, "value boundaries", at::kFloat, (int64_t{1} << bits) - 1);
+  c.table(kseff16, "key f16 S_eff", at::kHalf, D * D);
+  return out;
+}
+
+Tensor page_attend(const Tensor& k_in, const Tensor& v_in, const Tensor& q_in, const Tensor& kpi, const Tensor& kseff,
+                   const Tensor& kcent, const Tensor& kbounds, const Tensor& vpi, const Tensor& vbounds,
+                   const Tensor& kseff16, const Tensor& kcodes, const Tensor& ksigns, const Tensor& krn, const Tensor& kvn,
+                   const Tensor& kcent16, int64_t bits, const Tensor& vcodes, const Tensor& vvn, const Tensor& vcent32,
+                   const Tensor& vpit, const Tensor& table, const Tensor& lengths, const c10::optional<Tensor>& parents,
+                   double coeff, double scale, at::ScalarType out_dtype) {
+  Tensor out = page_attend_meta(k_in, v_in, q_in, kpi, kseff, kcent, kbounds, vpi, vbounds, kseff16, kcodes, ksigns, krn, kvn,
+                                kcent16, bits, vcodes, vvn, vcent32, vpit, table, lengths, parents, coeff, scale, out_dtype);
+  const c10::DeviceGuard g(q_in.device());
+  Tensor k = activation(k_in);
+  auto like_k = [&](const Tensor& t) {
+    return t.scalar_type() == k.scalar_type() && t.stride(-1) == 1 ? t : t.to(k.scalar_type()).contiguous();
+  };
+  Tensor v = like_k(v_in), q = like_k(q_in);
+  // one allocation: the workspace, then the prepared queries
+  const int64_t bytes = (tree_workspace(q, kvn, table, bits) + 15) / 16 * 16, n = q.numel();
+  Tensor ws = at::empty({bytes + n * 6}, q.options().dtype(at::kByte));
+  uint8_t* const base = ptr<uint8_t>(ws);
+  float* const q_proj = reinterpret_cast<float*>(base + bytes);
+  uint16_t* const q_rot = reinterpret_cast<uint16_t*>(q_proj + n);
+  void* pool[6] = {kcodes.data_ptr(), ksigns.data_ptr(), krn.data_ptr(), kvn.data_ptr(), vcodes.data_ptr(), vvn.data_ptr()};
+  const int32_t W = i32(table.size(1));
+  check_status(tq_page_append(k.data_ptr(), v.data_ptr(), dtype_code(k.scalar_type()), i32(k.size(0)), i32(k.size(1)),
+                              i32(k.size(2)), i32(k.size(3)), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1),
+                              v.stride(2), ptr<uint16_t>(kpi), ptr<uint16_t>(kseff), ptr<float>(kcent), ptr<float>(kbounds),
+                              ptr<uint16_t>(vpi), ptr<float>(vbounds), i32(bits), pool, kvn.size(0), i32(kvn.size(2)),
+                              ptr<int32_t>(table), W, W, ptr<int32_t>(lengths), q.data_ptr(), i32(q.size(1)), q.stride(0),
+                              q.stride(1), q.stride(2), ptr<uint16_t>(kseff16), q_rot, q_proj, stream_of(k)),
+               "append_tree_attention");
+  tree_launch(q_rot, q_proj, kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn, vcent32, vpit, table, lengths, parents, coeff,
+              scale, out, base, bytes);
+  return out;
+}
+
 using Verified = std::tuple<Tensor, Tensor, Tensor>;
 
 Verified verify_drafts_meta(const Tensor& tokens, const Tensor& target, const Tensor& uniforms,
@@ -1200,6 +1262,10 @@ TORCH_LIBRARY(tq, m) {
   m.def("tree_attention(Tensor q_rot, Tensor q_proj, Tensor kcodes, Tensor ksigns, Tensor krn, Tensor kvn, "
         "Tensor kcent, int bits, Tensor vcodes, Tensor vvn, Tensor vcent, Tensor vpit, Tensor block_table, "
         "Tensor lengths, Tensor? parents, float coeff, float scale, ScalarType out_dtype) -> Tensor");
+  m.def("page_attend(Tensor k, Tensor v, Tensor q, Tensor kpi, Tensor kseff, Tensor kcent, Tensor kbounds, Tensor vpi, "
+        "Tensor vbounds, Tensor kseff16, Tensor(a!) kcodes, Tensor(b!) ksigns, Tensor(c!) krn, Tensor(d!) kvn, "
+        "Tensor kcent16, int bits, Tensor(e!) vcodes, Tensor(f!) vvn, Tensor vcent32, Tensor vpit, Tensor table, "
+        "Tensor lengths, Tensor? parents, float coeff, float scale, ScalarType out_dtype) -> Tensor");
   m.def("tree_attend(Tensor q, Tensor pi_split, Tensor s_eff, Tensor kcodes, Tensor ksigns, Tensor krn, Tensor kvn, "
         "Tensor kcent, int bits, Tensor vcodes, Tensor vvn, Tensor vcent, Tensor vpit, Tensor block_table, "
         "Tensor lengths, Tensor? parents, float coeff, float scale, ScalarType out_dtype) -> Tensor");
@@ -1229,6 +1295,7 @@ TORCH_LIBRARY_IMPL(tq, CUDA, m) {
   m.impl("page_keep", &page_keep);
   m.impl("tree_attention", &tree_attention);
   m.impl("tree_attend", &tree_attend);
+  m.impl("page_attend", &page_attend);
   m.impl("verify_drafts", &verify_drafts);
 }
 
@@ -1254,5 +1321,6 @@ TORCH_LIBRARY_IMPL(tq, Meta, m) {
   m.impl("page_keep", &page_keep_meta);
   m.impl("tree_attention", &tree_attention_meta);
   m.impl("tree_attend", &tree_attend_meta);
+  m.impl("page_attend", &page_attend_meta);
   m.impl("verify_drafts", &verify_drafts_meta);
 }

@@ -26,6 +26,7 @@ import math
 
 import torch
 from transformers.cache_utils import Cache
+from turboquant_pytorch.drafts import append_tree_attention
 
 __all__ = ["TurboQuantPagedCache"]
 
@@ -288,7 +289,9 @@ class TurboQuantPagedCache(Cache):
         self._begin(layer_idx, k, bits)
         table, lengths = self._device_state
         if fast:
-            out = self._attend_tree(layer_idx, key_compressor, val_compressor, k, v, q, table, lengths, scale, out_dtype)
+            parents = self._tree[0] if self._tree else None
+            out = append_tree_attention(k, v, q, key_compressor, val_compressor, self.pool, layer_idx, table, lengths,
+                                        parents, scale, out_dtype)
         else:
             out = self._attend_prompt(layer_idx, key_compressor, val_compressor, k, v, q, table, lengths, scale, out_dtype)
         self._finish(layer_idx)
@@ -389,30 +392,6 @@ class TurboQuantPagedCache(Cache):
         p = self._free.pop()
         self._refs[p] = 1
         return p
-
-    def _attend_tree(self, layer_idx, key_compressor, val_compressor, k, v, q, table, lengths, scale, out_dtype):
-        """Few tokens: one launch compresses them and prepares the queries, one puts the rows into pages,
-        then attention over the pages."""
-        from turboquant_pytorch._ops import ops
-        from turboquant_pytorch.compressors import _tables
-        from turboquant_pytorch.drafts import tree_attention_from_prepared
-
-        B, H, T, D = k.shape
-        tk = _tables(key_compressor, k.device, with_qjl=True)
-        tv = _tables(val_compressor, k.device, with_qjl=False)
-        pl = self.pool.planes(layer_idx)
-        rows = {n: torch.empty((B, H, T) + tuple(t.shape[3:]), dtype=t.dtype, device=t.device) for n, t in pl.items()}
-        q_rot, q_proj = ops().cache_append(
-            k, v, q, tk.pi_split, tk.seff_split, tk.cent32, tk.bounds32, key_compressor.mse_bits, tv.pi_split, tv.bounds32,
-            val_compressor.bits, tk.s_eff16, rows["kcodes"], rows["ksigns"], rows["krn"], rows["kvn"], rows["vcodes"],
-            rows["vvn"], 0)
-        ck = {"packed_key_indices": rows["kcodes"], "packed_qjl_signs": rows["ksigns"], "residual_norm": rows["krn"],
-              "vec_norms": rows["kvn"], "shape": (B, H, T, D)}
-        cv = {"packed_indices": rows["vcodes"], "vec_norms": rows["vvn"], "shape": (B, H, T, D)}
-        self.pool.write(layer_idx, ck, cv, table, lengths)
-        parents = self._tree[0] if self._tree else None
-        return tree_attention_from_prepared(q_rot, q_proj, key_compressor, val_compressor, self.pool, layer_idx, table,
-                                            lengths, parents, scale, out_dtype or q.dtype)
 
     def _attend_prompt(self, layer_idx, key_compressor, val_compressor, k, v, q, table, lengths, scale, out_dtype):
         """Many tokens, or rows that tree attention does not take: attention over contiguous rows, the

@@ -69,6 +69,8 @@ _SIGNATURES = {
     "tq_prefill_scores_workspace_size": [_i32, _i32, _i32, _i32, _i32, _i32],
     "tq_prefill_workspace_size": [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32],
     "tq_page_write": [_p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i64, _i32, _p, _i64, _i32, _p, _p],
+    "tq_page_append": [_p, _p, _i32, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _i32,
+                       _p, _i64, _i32, _p, _i64, _i32, _p, _p, _i32, _i64, _i64, _i64, _p, _p, _p, _p],
     "tq_page_read": [_p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i64, _i32, _p, _i64, _i32, _p, _p],
     "tq_page_copy": [_p, _i32, _i32, _i32, _i32, _i32, _i64, _i32, _p, _p, _i32, _p],
     "tq_page_keep": [_p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i64, _i32, _p, _i64, _i32, _p, _p, _p, _p, _p],

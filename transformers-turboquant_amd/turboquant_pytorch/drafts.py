@@ -15,7 +15,7 @@ from ._ops import ops
 from .compressors import TurboQuantCompressorMSE, TurboQuantCompressorV2, _scaled_tables, _tables
 from .pages import PagePool
 
-__all__ = ["tree_attention", "tree_attention_from_prepared", "verify_drafts"]
+__all__ = ["append_tree_attention", "tree_attention", "tree_attention_from_prepared", "verify_drafts"]
 
 
 def tree_attention(queries: torch.Tensor, key_compressor: TurboQuantCompressorV2,
@@ -45,6 +45,20 @@ def tree_attention_from_prepared(q_rot: torch.Tensor, q_proj: torch.Tensor, key_
     return ops().tree_attention(q_rot, q_proj,
                                 *_tree_args(q_rot.shape[-1], q_rot.device, key_compressor, val_compressor, pool, layer,
                                             block_table, lengths, parents, scale, out_dtype))
+
+
+def append_tree_attention(k: torch.Tensor, v: torch.Tensor, queries: torch.Tensor, key_compressor, val_compressor,
+                          pool: PagePool, layer: int, block_table: torch.Tensor, lengths: torch.Tensor,
+                          parents: torch.Tensor | None = None, scale: float | None = None,
+                          out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """One layer's decoding or speculation step: the T new tokens' keys and values k, v [B, Hkv, T, D]
+    compressed into their pages (positions ``lengths[b] + i``) and the queries prepared in one launch,
+    then tree_attention.  A new row whose page is missing is not written."""
+    tk = _tables(key_compressor, queries.device, with_qjl=True)
+    tv = _tables(val_compressor, queries.device, with_qjl=False)
+    return ops().page_attend(k, v, queries, tk.pi_split, tk.seff_split, tk.cent32, tk.bounds32, tv.pi_split, tv.bounds32,
+                             tk.s_eff16, *_tree_args(queries.shape[-1], queries.device, key_compressor, val_compressor, pool,
+                                                     layer, block_table, lengths, parents, scale, out_dtype or queries.dtype))
 
 
 def _tree_args(D, dev, key_compressor, val_compressor, pool, layer, block_table, lengths, parents, scale, out_dtype):
