@@ -565,7 +565,10 @@ struct TileArgs {
   // norm planes (a cache of ldo positions per (batch, head), filled from position off); ldo = 0
   // writes row (b, h, s) to (b * H + h) * S + s
   int64_t ldo, off;
-  // pages: row (b, h, s) is position start[b] + s of sequence b
+};
+
+// output rows in pages: row (b, h, s) is position start[b] + s of sequence b
+struct PageMap {
   const int32_t *table, *start;
   int64_t ld_table, num_pages;
   int table_width, lg_page;
@@ -576,18 +579,18 @@ enum OutMap { kMapNone, kMapCapacity, kMapPages };
 
 // packed / norm plane row of input row gr (< 2^31); pages: -1 for a row without a page
 template <int MAP>
-__device__ __forceinline__ int64_t out_row(const TileArgs& a, int64_t gr) {
+__device__ __forceinline__ int64_t out_row(const TileArgs& a, const PageMap& pm, int64_t gr) {
   if (MAP == kMapNone || (MAP == kMapCapacity && a.ldo == 0)) return gr;
   const uint32_t r32 = static_cast<uint32_t>(gr);
   const uint32_t bh = a.S.div(r32);
   if constexpr (MAP == kMapPages) {
     const uint32_t b = a.H.div(bh);
-    const int from = a.start[b];
-    const int64_t pos = static_cast<int64_t>(from) + (r32 - bh * a.S.d), slot = pos >> a.lg_page;
-    if (from < 0 || slot >= a.table_width) return -1;
-    const int64_t page = a.table[b * a.ld_table + slot];
-    if (page < 0 || page >= a.num_pages) return -1;
-    return ((page * a.H.d + (bh - b * a.H.d)) << a.lg_page) + (pos & ((int64_t(1) << a.lg_page) - 1));
+    const int from = pm.start[b];
+    const int64_t pos = static_cast<int64_t>(from) + (r32 - bh * a.S.d), slot = pos >> pm.lg_page;
+    if (from < 0 || slot >= pm.table_width) return -1;
+    const int64_t page = pm.table[b * pm.ld_table + slot];
+    if (page < 0 || page >= pm.num_pages) return -1;
+    return ((page * a.H.d + (bh - b * a.H.d)) << pm.lg_page) + (pos & ((int64_t(1) << pm.lg_page) - 1));
   }
   return static_cast<int64_t>(bh) * a.ldo + a.off + (r32 - bh * a.S.d);
 }
@@ -753,8 +756,8 @@ struct RowsSmem {
 // MAP: outputs go to the rows out_row<MAP> names (a cache append); the plain form keeps the
 // registers that mapping needs free for the tile loop.
 template <int D, int DT, int MODE, int BB, int NW_, int MAP>
-__device__ __forceinline__ void rows_body(const TileArgs& a, RowsSmem<D, MODE, BB, NW_>& sm, int block,
-                                          int nblocks) {
+__device__ __forceinline__ void rows_body(const TileArgs& a, const PageMap& pm, RowsSmem<D, MODE, BB, NW_>& sm,
+                                          int block, int nblocks) {
   using T = RT<D, NW_>;
   using SM = RowsSmem<D, MODE, BB, NW_>;
   constexpr bool DBUF = NW_ <= 8;  // weight fragments double-buffered
@@ -923,7 +926,7 @@ __device__ __forceinline__ void rows_body(const TileArgs& a, RowsSmem<D, MODE, B
       const int wpr = bytes / 4;  // dwords per row (rows of d * b / 8 bytes, d = 64 or 128)
       for (int i = lane; i < nd; i += 64) {
         const int r = i / wpr;
-        const int64_t orow = out_row<MAP>(a, row0 + r);
+        const int64_t orow = out_row<MAP>(a, pm, row0 + r);
         if (MAP == kMapPages && orow < 0) continue;
         reinterpret_cast<uint32_t*>(out + orow * bytes)[i - r * wpr] = reinterpret_cast<const uint32_t*>(src)[i];
       }
@@ -1097,7 +1100,7 @@ __device__ __forceinline__ void rows_body(const TileArgs& a, RowsSmem<D, MODE, B
       auto flush = [&]() {
         const int64_t grp = tp * 16 + l16;
         if (g == 0 && grp < a.n) {
-          const int64_t orow = out_row<MAP>(a, grp);
+          const int64_t orow = out_row<MAP>(a, pm, grp);
           if (MAP != kMapPages || orow >= 0) a.vn[orow] = f2h(vn_p);
         }
         wave_sync();
@@ -1151,7 +1154,7 @@ __device__ __forceinline__ void rows_body(const TileArgs& a, RowsSmem<D, MODE, B
       auto flush = [&]() {
         const int64_t grp = tp * 16 + l16;
         if (g == 0 && grp < a.n) {
-          const int64_t orow = out_row<MAP>(a, grp);
+          const int64_t orow = out_row<MAP>(a, pm, grp);
           if (MAP != kMapPages || orow >= 0) {
             a.vn[orow] = f2h(vn_p);
             a.rn[orow] = f2h(rn_p);
@@ -1246,7 +1249,7 @@ template <int D, int DT, int MODE, int BB>
 __global__ void __launch_bounds__((64 * row_waves<MODE, DT>())) rows_kernel(TileArgs a) {
   using SM = RowsSmem<D, MODE, BB, row_waves<MODE, DT>()>;
   __shared__ __attribute__((aligned(16))) uint8_t smem[sizeof(SM)];
-  rows_body<D, DT, MODE, BB, row_waves<MODE, DT>(), kMapNone>(a, *reinterpret_cast<SM*>(smem), blockIdx.x, gridDim.x);
+  rows_body<D, DT, MODE, BB, row_waves<MODE, DT>(), kMapNone>(a, PageMap{}, *reinterpret_cast<SM*>(smem), blockIdx.x, gridDim.x);
 }
 
 // Few rows (a decode step's queries): blocks of 4 waves, one per SIMD, so that the rows'
@@ -1257,7 +1260,7 @@ template <int D, int DT, int MODE, int BB>
 __global__ void __launch_bounds__(64 * kFewWaves) rows_few_kernel(TileArgs a) {
   using SM = RowsSmem<D, MODE, BB, kFewWaves>;
   __shared__ __attribute__((aligned(16))) uint8_t smem[sizeof(SM)];
-  rows_body<D, DT, MODE, BB, kFewWaves, kMapNone>(a, *reinterpret_cast<SM*>(smem), blockIdx.x, gridDim.x);
+  rows_body<D, DT, MODE, BB, kFewWaves, kMapNone>(a, PageMap{}, *reinterpret_cast<SM*>(smem), blockIdx.x, gridDim.x);
 }
 
 // A cache append in one launch: blocks [0, nbk) compress the new keys, [nbk, nbk + nbv) the
@@ -1266,8 +1269,8 @@ __global__ void __launch_bounds__(64 * kFewWaves) rows_few_kernel(TileArgs a) {
 // mode's layout at a time.  MAP: capacity planes, or pages.
 constexpr int kAppendWaves = 4;
 template <int D, int DT, int KBB, int VB, int MAP>
-__global__ void __launch_bounds__(64 * kAppendWaves) append_kernel(TileArgs ka, TileArgs va, TileArgs qa, int nbk,
-                                                                   int nbv, int nbq) {
+__global__ void __launch_bounds__(64 * kAppendWaves) append_kernel(TileArgs ka, TileArgs va, TileArgs qa,
+                                                                   PageMap pm, int nbk, int nbv, int nbq) {
   constexpr int NW = kAppendWaves;
   using SK = RowsSmem<D, TM_KEYS, KBB, NW>;
   using SV = RowsSmem<D, TM_VALUES, VB, NW>;
@@ -1276,9 +1279,9 @@ __global__ void __launch_bounds__(64 * kAppendWaves) append_kernel(TileArgs ka, 
                                                    : (sizeof(SV) > sizeof(SQ) ? sizeof(SV) : sizeof(SQ));
   __shared__ __attribute__((aligned(16))) uint8_t smem[BYTES];
   const int blk = static_cast<int>(blockIdx.x);
-  if (blk < nbk) rows_body<D, DT, TM_KEYS, KBB, NW, MAP>(ka, *reinterpret_cast<SK*>(smem), blk, nbk);
-  else if (blk < nbk + nbv) rows_body<D, DT, TM_VALUES, VB, NW, MAP>(va, *reinterpret_cast<SV*>(smem), blk - nbk, nbv);
-  else rows_body<D, DT, TM_QUERY, 1, NW, kMapNone>(qa, *reinterpret_cast<SQ*>(smem), blk - nbk - nbv, nbq);
+  if (blk < nbk) rows_body<D, DT, TM_KEYS, KBB, NW, MAP>(ka, pm, *reinterpret_cast<SK*>(smem), blk, nbk);
+  else if (blk < nbk + nbv) rows_body<D, DT, TM_VALUES, VB, NW, MAP>(va, pm, *reinterpret_cast<SV*>(smem), blk - nbk, nbv);
+  else rows_body<D, DT, TM_QUERY, 1, NW, kMapNone>(qa, pm, *reinterpret_cast<SQ*>(smem), blk - nbk - nbv, nbq);
 }
 
 // Blocks of `kernel` the device holds at once (occupancy x compute units), per device.
@@ -1342,7 +1345,7 @@ void dispatch_tile<TM_QUERY>(const TileArgs& a, int d, int dtype, int, hipStream
 
 // ---------------------------------------------------------------- cache append (one launch)
 template <int MAP, int D, int DT, int KBB, int VB>
-static void launch_append(const TileArgs& ka, const TileArgs& va, const TileArgs& qa, hipStream_t s) {
+static void launch_append(const TileArgs& ka, const TileArgs& va, const TileArgs& qa, const PageMap& pm, hipStream_t s) {
   static int cache[16] = {};
   constexpr int NT = 64 * kAppendWaves, RROWS = 16 * kAppendWaves;
   const int64_t res = resident_blocks(reinterpret_cast<const void*>(&append_kernel<D, DT, KBB, VB, MAP>), NT, cache);
@@ -1359,27 +1362,28 @@ static void launch_append(const TileArgs& ka, const TileArgs& va, const TileArgs
     nq = qa.n > 0 ? std::max<int64_t>(1, std::min<int64_t>(nq, res - nk - nv)) : 0;
   }
   append_kernel<D, DT, KBB, VB, MAP><<<static_cast<unsigned>(nk + nv + nq), NT, 0, s>>>(
-      ka, va, qa, static_cast<int>(nk), static_cast<int>(nv), static_cast<int>(nq));
+      ka, va, qa, pm, static_cast<int>(nk), static_cast<int>(nv), static_cast<int>(nq));
 }
 
 template <int MAP, int D, int KBB, int VB>
-static void launch_append_dt(const TileArgs& ka, const TileArgs& va, const TileArgs& qa, int dtype, hipStream_t s) {
-  if (dtype == TQ_F32) launch_append<MAP, D, TQ_F32, KBB, VB>(ka, va, qa, s);
-  else if (dtype == TQ_F16) launch_append<MAP, D, TQ_F16, KBB, VB>(ka, va, qa, s);
-  else launch_append<MAP, D, TQ_BF16, KBB, VB>(ka, va, qa, s);
+static void launch_append_dt(const TileArgs& ka, const TileArgs& va, const TileArgs& qa, const PageMap& pm, int dtype,
+                             hipStream_t s) {
+  if (dtype == TQ_F32) launch_append<MAP, D, TQ_F32, KBB, VB>(ka, va, qa, pm, s);
+  else if (dtype == TQ_F16) launch_append<MAP, D, TQ_F16, KBB, VB>(ka, va, qa, pm, s);
+  else launch_append<MAP, D, TQ_BF16, KBB, VB>(ka, va, qa, pm, s);
 }
 
 // head_dim 64 / 128, value bits 2-4 with key code bits one fewer (a compressor pair of one bit width)
 template <int MAP>
-static void dispatch_append(const TileArgs& ka, const TileArgs& va, const TileArgs& qa, int d, int dtype, int vb,
+static void dispatch_append(const TileArgs& ka, const TileArgs& va, const TileArgs& qa, const PageMap& pm, int d, int dtype, int vb,
                             hipStream_t s) {
   switch (d * 8 + vb) {
-    case 64 * 8 + 2: launch_append_dt<MAP, 64, 1, 2>(ka, va, qa, dtype, s); break;
-    case 64 * 8 + 3: launch_append_dt<MAP, 64, 2, 3>(ka, va, qa, dtype, s); break;
-    case 64 * 8 + 4: launch_append_dt<MAP, 64, 3, 4>(ka, va, qa, dtype, s); break;
-    case 128 * 8 + 2: launch_append_dt<MAP, 128, 1, 2>(ka, va, qa, dtype, s); break;
-    case 128 * 8 + 3: launch_append_dt<MAP, 128, 2, 3>(ka, va, qa, dtype, s); break;
-    default: launch_append_dt<MAP, 128, 3, 4>(ka, va, qa, dtype, s); break;
+    case 64 * 8 + 2: launch_append_dt<MAP, 64, 1, 2>(ka, va, qa, pm, dtype, s); break;
+    case 64 * 8 + 3: launch_append_dt<MAP, 64, 2, 3>(ka, va, qa, pm, dtype, s); break;
+    case 64 * 8 + 4: launch_append_dt<MAP, 64, 3, 4>(ka, va, qa, pm, dtype, s); break;
+    case 128 * 8 + 2: launch_append_dt<MAP, 128, 1, 2>(ka, va, qa, pm, dtype, s); break;
+    case 128 * 8 + 3: launch_append_dt<MAP, 128, 2, 3>(ka, va, qa, pm, dtype, s); break;
+    default: launch_append_dt<MAP, 128, 3, 4>(ka, va, qa, pm, dtype, s); break;
   }
 }
 
@@ -1560,7 +1564,7 @@ int tq_cache_append(const void* k, const void* v, int32_t dtype, int32_t B, int3
       qa.sb = sqb; qa.sh = sqh; qa.ss = sqs; qa.vec = tile_vec(q, dtype, sqb, sqh, sqs);
       qa.w1 = key_pi_split; qa.w2 = key_s_eff_f16; qa.q_rot = q_rot; qa.q_proj = q_proj;
     }
-    dispatch_append<kMapCapacity>(ka, va, qa, d, dtype, val_bits, st);
+    dispatch_append<kMapCapacity>(ka, va, qa, PageMap{}, d, dtype, val_bits, st);
     return launch_status("tq_cache_append");
   }
   // other head dims and bit widths: the tile kernels, writing the same mapped rows
@@ -1613,8 +1617,7 @@ int tq_page_append(const void* k, const void* v, int32_t dtype, int32_t B, int32
   ka.w1 = key_pi_split; ka.w3 = key_seff_split; ka.cent = key_centroids; ka.bounds = key_bounds;
   ka.codes = static_cast<uint8_t*>(pool[0]); ka.signs = static_cast<uint8_t*>(pool[1]);
   ka.rn = static_cast<uint16_t*>(pool[2]); ka.vn = static_cast<uint16_t*>(pool[3]);
-  ka.table = block_table; ka.start = start; ka.ld_table = ld_table; ka.num_pages = num_pages;
-  ka.table_width = table_width; ka.lg_page = __builtin_ctz(static_cast<unsigned>(page_size));
+  const PageMap pm{block_table, start, ld_table, num_pages, table_width, __builtin_ctz(static_cast<unsigned>(page_size))};
   va = ka;
   va.x = v; va.sb = svb; va.sh = svh; va.ss = svs; va.vec = tile_vec(v, dtype, svb, svh, svs);
   va.w1 = val_pi_split; va.w3 = nullptr; va.cent = nullptr; va.bounds = val_bounds;
@@ -1625,7 +1628,7 @@ int tq_page_append(const void* k, const void* v, int32_t dtype, int32_t B, int32
     qa.sb = sqb; qa.sh = sqh; qa.ss = sqs; qa.vec = tile_vec(q, dtype, sqb, sqh, sqs);
     qa.w1 = key_pi_split; qa.w2 = key_s_eff_f16; qa.q_rot = q_rot; qa.q_proj = q_proj;
   }
-  dispatch_append<kMapPages>(ka, va, qa, d, dtype, bits, as_stream(stream));
+  dispatch_append<kMapPages>(ka, va, qa, pm, d, dtype, bits, as_stream(stream));
   return launch_status("tq_page_append");
 }
 
