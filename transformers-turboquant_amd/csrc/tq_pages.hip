@@ -74,7 +74,7 @@ __device__ __forceinline__ int64_t page_row(const PagePlanes& a, int b, int h, i
 // run through in order.  Norm planes (2 bytes a row) move in groups of 8 rows that lie together in
 // a page; the flat side of a group starts anywhere, so it is accessed as unaligned 16 bytes.  (One piece a
 // thread and one norm at a time took 14.6 us for the read above, four pieces in flight and groups 11.7.)
-constexpr int kRowSteps = 4;  // pieces of a thread, loaded together
+constexpr int kRowSteps = 4;  // pieces of a thread, loaded together (the read above: 11.6 us; with 2 or 8 of them 12.8)
 template <bool WRITE>
 __device__ __forceinline__ void code_pieces(const PagePlanes& a, int p, int b, int h, int64_t flat_row, int from, int S) {
   const uint32_t unit = a.unit[p], per = a.width[p] / unit;
