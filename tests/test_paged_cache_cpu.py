@@ -76,7 +76,7 @@ def test_sequences_grow_and_are_freed():
     step(cache, [[7], [8]])
     assert text(cache, a) == [1, 2, 3, 8] and text(cache, c) == [*range(100, 170), 7] and text(cache, b) == [4, 5, 6]
     check(cache)
-    cache.free(c)
+    cache.free(c, c)
     assert cache.active == [a] and cache.free_pages == 10
     cache.reset()
     assert cache.free_pages == 12 and cache.active == []

@@ -84,6 +84,7 @@ class TurboQuantPagedCache(Cache):
 
     def free(self, *seqs: int) -> None:
         """Forget sequences; pages that no other sequence shares are free again."""
+        seqs = tuple(dict.fromkeys(seqs))
         for i in seqs:
             self._seq(i)
         if any(i in self._active for i in seqs):
