@@ -28,13 +28,13 @@ def tree_attention(queries: torch.Tensor, key_compressor: TurboQuantCompressorV2
     own rows stand at ``lengths[b] + i`` (``pool.write``).  Node i sees the cached positions, its
     ancestors and itself.  parents int32 [T] (one tree for all sequences) or [B, T]; a value that is
     neither -1 nor an earlier node leaves the node without a place: its output is zero and no node
-    sees it (padding of smaller trees).  A sequence with a negative length gets zeros.  head_dim 64 or
-    128, 2 to 4 bits.
+    sees it (padding of smaller trees).  A sequence with a negative length, or whose table has no room for
+    lengths[b] + T positions, gets zeros.  head_dim 64 or 128, 2 to 4 bits.
     """
-    t = _tables(key_compressor, queries.device, with_qjl=True)
-    return ops().tree_attend(queries, t.pi_split, t.s_eff16,
-                             *_tree_args(queries.shape[-1], queries.device, key_compressor, val_compressor, pool, layer,
-                                         block_table, lengths, parents, scale, out_dtype or queries.dtype))
+    tk, tv = _both_tables(key_compressor, val_compressor, queries.device)
+    return ops().tree_attend(queries, tk.pi_split, tk.s_eff16,
+                             *_tree_args(tk, tv, queries.shape[-1], key_compressor, val_compressor, pool, layer, block_table,
+                                         lengths, parents, scale, out_dtype or queries.dtype))
 
 
 def tree_attention_from_prepared(q_rot: torch.Tensor, q_proj: torch.Tensor, key_compressor, val_compressor,
@@ -42,9 +42,10 @@ def tree_attention_from_prepared(q_rot: torch.Tensor, q_proj: torch.Tensor, key_
                                  parents: torch.Tensor | None = None, scale: float | None = None,
                                  out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """tree_attention on queries already prepared by ``key_compressor.prepare_queries``."""
+    tk, tv = _both_tables(key_compressor, val_compressor, q_rot.device)
     return ops().tree_attention(q_rot, q_proj,
-                                *_tree_args(q_rot.shape[-1], q_rot.device, key_compressor, val_compressor, pool, layer,
-                                            block_table, lengths, parents, scale, out_dtype))
+                                *_tree_args(tk, tv, q_rot.shape[-1], key_compressor, val_compressor, pool, layer, block_table,
+                                            lengths, parents, scale, out_dtype))
 
 
 def append_tree_attention(k: torch.Tensor, v: torch.Tensor, queries: torch.Tensor, key_compressor, val_compressor,
@@ -54,21 +55,23 @@ def append_tree_attention(k: torch.Tensor, v: torch.Tensor, queries: torch.Tenso
     """One layer's decoding or speculation step: the T new tokens' keys and values k, v [B, Hkv, T, D]
     compressed into their pages (positions ``lengths[b] + i``) and the queries prepared in one launch,
     then tree_attention.  A new row whose page is missing is not written."""
-    tk = _tables(key_compressor, queries.device, with_qjl=True)
-    tv = _tables(val_compressor, queries.device, with_qjl=False)
+    tk, tv = _both_tables(key_compressor, val_compressor, queries.device)
     return ops().page_attend(k, v, queries, tk.pi_split, tk.seff_split, tk.cent32, tk.bounds32, tv.pi_split, tv.bounds32,
-                             tk.s_eff16, *_tree_args(queries.shape[-1], queries.device, key_compressor, val_compressor, pool,
-                                                     layer, block_table, lengths, parents, scale, out_dtype or queries.dtype))
+                             tk.s_eff16, *_tree_args(tk, tv, queries.shape[-1], key_compressor, val_compressor, pool, layer,
+                                                     block_table, lengths, parents, scale, out_dtype or queries.dtype))
 
 
-def _tree_args(D, dev, key_compressor, val_compressor, pool, layer, block_table, lengths, parents, scale, out_dtype):
+def _both_tables(key_compressor, val_compressor, dev):
+    return _tables(key_compressor, dev, with_qjl=True), _tables(val_compressor, dev, with_qjl=False)
+
+
+def _tree_args(tk, tv, D, key_compressor, val_compressor, pool, layer, block_table, lengths, parents, scale, out_dtype):
     if key_compressor.S.shape[0] != D:
         raise ValueError("tree attention needs a square QJL matrix")
     if val_compressor.bits != key_compressor.mse_bits + 1:
         raise ValueError(f"tree attention needs keys and values of one bit width, got {key_compressor.mse_bits + 1} "
                          f"and {val_compressor.bits}")
-    tk = _tables(key_compressor, dev, with_qjl=True)
-    vcent, vpit = _scaled_tables(val_compressor, _tables(val_compressor, dev, with_qjl=False))
+    vcent, vpit = _scaled_tables(val_compressor, tv)
     kcodes, ksigns, krn, kvn, vcodes, vvn = pool._layer[layer]
     if out_dtype not in (torch.float32, torch.float16, torch.bfloat16):
         out_dtype = torch.float32
