@@ -117,3 +117,35 @@ def test_captured_steps():
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(lengths, length2), i
     _same(one, two)
+
+
+@pytest.mark.parametrize("bits,pages", [(3, 96000), (4, 70000)])
+def test_pages_past_4_gib(bits, pages):
+    """The last pages of a pool whose planes pass 2^32 bytes: the same outputs as in a small pool."""
+    print("case:", bits, pages, flush=True)
+    kc = TurboQuantCompressorV2(128, bits, seed=42, device=DEV)
+    vc = TurboQuantCompressorMSE(128, bits, seed=10042, device=DEV)
+    page, Hkv = 128, 8
+    big, small = PagePool(pages, page, Hkv, 128, bits, device=DEV), PagePool(8, page, Hkv, 128, bits, device=DEV)
+    assert big.planes(0)["vcodes"].numel() > 2 ** 32
+    table = torch.tensor([[3, 0, 5, -1], [1, 7, 2, 6]], dtype=torch.int32, device=DEV)
+    far = torch.where(table < 0, table, table + (pages - 8))
+    g = torch.Generator(device=DEV).manual_seed(8)
+    lengths = torch.tensor([250, 300], dtype=torch.int32, device=DEV)
+    ck, cv = (c.compress(torch.randn(2, Hkv, 300, 128, device=DEV, generator=g)) for c in (kc, vc))
+    for pool, t in ((big, far), (small, table)):
+        pool.write(0, ck, cv, t, torch.zeros_like(lengths))
+    for Hq, T in ((8, 1), (32, 1), (16, 5), (64, 40)):  # every form
+        k, v, q = (torch.randn(2, h, T, 128, device=DEV, generator=g) for h in (Hkv, Hkv, Hq))
+        wide = torch.full((2, 4096), -1, dtype=torch.int32, device=DEV)
+        for pad in (False, True):
+            out = []
+            for pool, t in ((big, far), (small, table)):
+                if pad:
+                    w = wide.clone()
+                    w[:, :4] = t
+                    t = w
+                out.append(append_tree_attention(k, v, q, kc, vc, pool, 0, t, lengths))
+            assert torch.equal(*out) and torch.isfinite(out[0]).all()
+    for name, t in big.planes(0).items():
+        assert torch.equal(t[pages - 8:].view(torch.uint8), small.planes(0)[name].view(torch.uint8)), name
