@@ -354,3 +354,61 @@ def test_another_stream():
     torch.cuda.synchronize()
     for o in got:
         assert torch.equal(o, want)
+
+
+# planes, one column tile, two column tiles
+FORMS = [(1, 4, 2, 0), (4, 2, 2, 0), (5, 4, 2, 0), (16, 4, 2, 4096)]
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,Hq,Hkv,wide", FORMS)
+def test_large_norms_of_keys_that_weigh_nothing(D, T, Hq, Hkv, wide):
+    """Every slab of 32 keys holds a key of weight 1 and value norm 2^-6, one of weight e^-100 and norm 6e4,
+    and 30 of weight 2^-15.2 and norm 1, whose values point one way: 5% of the row's weighted norms.  Each of those
+    contributions is 2^-9 of the largest one, far above the 2^-30 that the bound leaves out."""
+    print("case:", D, T, Hq, Hkv, wide, flush=True)
+    n = 4096
+    kc, vc, pool, table, lengths, q = _setup(D, 3, 1, Hq, Hkv, T, [n], 32, seed=40)
+    if wide:
+        table = _widen(table, wide)
+    G = Hq // Hkv
+    q = q[:, ::G, :1].repeat_interleave(G, 1).expand(1, Hq, T, D).contiguous()  # a kv head's columns are alike
+    q_rot = kc.prepare_queries(q)[0][0, ::G, 0].double()  # [Hkv, D]
+    top = float(kc.centroids.half().max())
+    codes = torch.where(q_rot < 0, 3, 0).to(torch.uint8)  # <q_rot, C[codes]> = -top sum |q_rot| (symmetric codebook)
+    unit = top * q_rot.abs().sum(-1) / math.sqrt(D)  # minus a score, per unit of key norm
+    pl = pool.planes(1)
+    pl["krn"].zero_()
+    pl["kvn"].copy_((15.2 * math.log(2) / unit)[None, :, None].expand(pl["kvn"].shape))
+    pl["kvn"][:, :, 3] = 0
+    pl["kvn"][:, :, 7] = (100 / unit)[None].half()
+    pl["vvn"].fill_(1)
+    pl["vvn"][:, :, 3] = 2.0 ** -6
+    pl["vvn"][:, :, 7] = 6e4
+    packed = torch.from_numpy(O.pack_bits(codes.cpu().numpy(), 2)).to(DEV)
+    pl["kcodes"].copy_(packed[None, :, None].expand(pl["kcodes"].shape))
+    pl["vcodes"].fill_(255)
+    pl["vcodes"][:, :, 3] = 0
+    par = _tree(T, 1, 3, pads=False)
+    out = tree_attention(q, kc, vc, pool, 1, table, lengths, par, out_dtype=torch.float32)
+    _check(out, kc, vc, pool, table, lengths, q, par)
+
+
+@pytest.mark.parametrize("T,Hq,Hkv,wide", [(4, 2, 2, 0), (6, 4, 2, 0), (16, 4, 2, 4096)])
+def test_norms_of_a_row_do_not_reach_the_nodes_that_do_not_see_it(T, Hq, Hkv, wide):
+    """Bit for bit: a sibling's value norm, however large, changes nothing for the other branches."""
+    print("case:", T, Hq, Hkv, wide, flush=True)
+    kc, vc, pool, table, lengths, q = _setup(128, 3, 1, Hq, Hkv, T, [45], 32, seed=41)
+    if wide:
+        table = _widen(table, wide)
+    par = torch.tensor([[-1, 0, 0, 1] + [2] * (T - 4)], dtype=torch.int32, device=DEV)
+    clean = tree_attention(q, kc, vc, pool, 1, table, lengths, par, out_dtype=torch.float32)
+    rest = [i for i in range(T) if i not in (1, 3)]
+    pos = 45 + 1  # node 1: seen by 1 and 3
+    row = pool.planes(1)["vvn"][int(table[0, pos // 32]), :, pos % 32]
+    for val in (6e4, 100.0, float("inf"), float("nan"), 0.0):
+        row.fill_(val)
+        out = tree_attention(q, kc, vc, pool, 1, table, lengths, par, out_dtype=torch.float32)
+        assert torch.equal(out[:, rest], clean[:, rest]), val
+        if math.isfinite(val):
+            _check(out, kc, vc, pool, table, lengths, q, par)

@@ -358,6 +358,16 @@ __device__ __forceinline__ uint32_t mul2_f16(float x0, uint32_t y0, float x1, ui
   return __builtin_bit_cast(uint32_t, half2v{static_cast<_Float16>(mul_f16(x0, y0)), static_cast<_Float16>(mul_f16(x1, y1))});
 }
 
+// The f16 operand is P vn, so a column's reference is that of s + E (log2 units), E being a key's
+// f16 exponent field: vn < 2^(E - 14).  Weights are p = 2^(s - mref) with mref = max(s + E) - PUP at the
+// last move, the maximum over the keys that the column sees, and the reference moves when s + E exceeds
+// it by more than TAU: p vn < 2^(PUP + TAU - 14) = 2^14 within f16's range, and the largest was 2^5 or
+// more when the reference moved.  A contribution p vn that is 2^-30 of the column's largest still
+// reaches the operand, whose subnormals end at 2^-24, whatever norms the other keys have.  (A norm below
+// 2^-14 counts as 2^-14.)  p itself stays below 2^28, in f32.
+constexpr float kTau = 8.0f, kPup = 20.0f;
+__device__ __forceinline__ float norm_exponent(uint32_t vn) { return static_cast<float>(vn >> 10); }
+
 template <int D, int BITS, int NT, int NW>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)))
 tree_attn_kernel(TreeArgs a) {
@@ -379,10 +389,7 @@ tree_attn_kernel(TreeArgs a) {
   constexpr bool HOLD_HI = NT == 1 || D == 64;  // q_proj hi fragments in registers
   constexpr bool AHEAD = NT == 1;  // score operands looked up a step ahead, where registers allow
   constexpr float LOG2E = 1.4426950408889634f;
-  constexpr float TAU = 8.0f;  // a column's reference moves when a score exceeds it by more (log2 units)
-  // p vn <= 2^(s - m + PUP) <= 2^(TAU + PUP): keys down to ~2^-31 of the heaviest still reach the
-  // f16 operand P, whose subnormals end at 2^-24
-  constexpr float PUP = 6.0f;
+  constexpr float TAU = kTau, PUP = kPup;
 
   __shared__ __attribute__((aligned(16))) SM sm;
   uint8_t* const luts = sm.luts;
@@ -516,12 +523,9 @@ tree_attn_kernel(TreeArgs a) {
       }
     }
 
-    // Column state: weights are p = 2^(s - mref) with mref = m - PUP + cap, where m is the column's
-    // reference maximum and 2^cap bounds the value norms met, so that p vn stays within f16; both
-    // only grow, O and l being rescaled when they do.  lim is the largest s - mref that does not
-    // move m (-inf while the column has none; mref is 0 then).
-    float mref[NT], lim[NT], l_run[NT], cap = -24.f;
-    uint32_t cap16 = 0;  // 2^cap as f16 bits, once it is one: norms are compared as integers
+    // Column state: the reference mref, O and l relative to it, and lim, the largest s + E - mref that
+    // does not move it (-inf while the column has none; mref is 0 then).
+    float mref[NT], lim[NT], l_run[NT];
     float4v oacc[NT][DB];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -606,38 +610,12 @@ tree_attn_kernel(TreeArgs a) {
             vn[j][e] = on ? vn[j][e] : 0;
           }
       }
-      // ---- value norms stay below 2^cap
-      {
-        uint32_t top = max(max(max(vn[0][0], vn[0][1]), max(vn[0][2], vn[0][3])),
-                           max(max(vn[1][0], vn[1][1]), max(vn[1][2], vn[1][3])));
-        if (__any(top > cap16)) {
-          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, 64)));
-          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, 64)));
-          int ex;
-          frexpf(fminf(h2f(static_cast<uint16_t>(top)), 65504.f), &ex);  // < 2^ex; the same in every lane
-          ex = max(__builtin_amdgcn_readfirstlane(ex), -24);
-          const float grow = static_cast<float>(ex) - cap;
-          if (grow > 0.f) {
-            const float shrink = ldexpf(1.f, -static_cast<int>(grow));
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              if (lim[t] != -INFINITY) {
-                mref[t] += grow;
-                lim[t] -= grow;
-              }
-              l_run[t] *= shrink;
-#pragma unroll
-              for (int db = 0; db < DB; ++db) oacc[t][db] *= shrink;
-            }
-            cap = static_cast<float>(ex);
-          }
-          cap16 = ex > 15 ? 0xFFFFu : static_cast<uint32_t>(f2h(ldexpf(1.f, ex)));
-        }
-      }
       // ---- log2-domain scores relative to mref, and the softmax step
       float sc[NT][2][4];
       bool hit = false;
-      float lmax[NT];
+      // the lane's largest score and largest exponent bound its s + E
+      const float top = norm_exponent(max(max(max(vn[0][0], vn[0][1]), max(vn[0][2], vn[0][3])),
+                                          max(max(vn[1][0], vn[1][1]), max(vn[1][2], vn[1][3]))));
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         uint32_t see = 0;
@@ -649,25 +627,29 @@ tree_attn_kernel(TreeArgs a) {
             const float x = fmaf(fma_f16(s1[t][j][e], kn[j][e], mul_f16(s2[t][j][e], rn[j][e])), fs, -mref[t]);
             sc[t][j][e] = !EDGE || (see & (1u << (16 * j + e))) ? x : -INFINITY;
           }
-        lmax[t] = max8_raw(sc[t][0][0], sc[t][0][1], sc[t][0][2], sc[t][0][3], sc[t][1][0], sc[t][1][1], sc[t][1][2],
-                           sc[t][1][3]);
-        hit = hit || lmax[t] > lim[t];
+        const float lmax = max8_raw(sc[t][0][0], sc[t][0][1], sc[t][0][2], sc[t][0][3], sc[t][1][0], sc[t][1][1],
+                                    sc[t][1][2], sc[t][1][3]);
+        hit = hit || lmax + top > lim[t];
       }
       if (__any(hit)) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          float m = lmax[t];
+          float m = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m = fmaxf(m, sc[t][j][e] + norm_exponent(vn[j][e]));
           m = fmaxf(m, __shfl_xor(m, 16, 64));
           m = fmaxf(m, __shfl_xor(m, 32, 64));
           const bool move = m > lim[t];
-          const float shift = move ? m - PUP + cap : 0.f;
+          const float shift = move ? m - PUP : 0.f;
           const float alpha = !move ? 1.f : lim[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-shift);
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) sc[t][j][e] -= shift;
           mref[t] += shift;
-          lim[t] = move ? TAU + PUP - cap : lim[t];
+          lim[t] = move ? TAU + PUP : lim[t];
           l_run[t] *= alpha;
 #pragma unroll
           for (int db = 0; db < DB; ++db) oacc[t][db] *= alpha;
@@ -811,7 +793,7 @@ tree_plane_kernel(TreeArgs a) {
   constexpr int KLANE = ST::KC / 4, SLANE = ST::SC / 4, VFB = DB * VB, VW32 = VB == 3 ? 2 : 1;
   constexpr int NK = ST::NK, RK = NW * NK;
   constexpr float LOG2E = 1.4426950408889634f;
-  constexpr float TAU = 8.0f, PUP = 6.0f;  // as in tree_attn_kernel
+  constexpr float TAU = kTau, PUP = kPup;
 
   __shared__ __attribute__((aligned(16))) SM sm;
   const uint8_t* const tV = sm.luts + L::VAL_OFF;
@@ -870,8 +852,7 @@ tree_plane_kernel(TreeArgs a) {
     const uint64_t anc = sm.anc[min(lg, a.C - 1) / a.G];  // of column lg
 
     // column state as in tree_attn_kernel, the same in the 16 lanes of a column
-    float mref = 0.f, lim = -INFINITY, l_run = 0.f, cap = -24.f;
-    uint32_t cap16 = 0;
+    float mref = 0.f, lim = -INFINITY, l_run = 0.f;
     float4v oacc[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db) oacc[db] = float4v{0.f, 0.f, 0.f, 0.f};
@@ -901,28 +882,6 @@ tree_plane_kernel(TreeArgs a) {
           vn[j] = on ? vn[j] : 0;
         }
       }
-      // ---- value norms stay below 2^cap
-      uint32_t top = max(vn[0], vn[1]);
-      if (__any(top > cap16)) {
-#pragma unroll
-        for (int sh = 8; sh >= 1; sh >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), sh, 64)));
-        int ex;
-        frexpf(fminf(h2f(static_cast<uint16_t>(top)), 65504.f), &ex);  // < 2^ex; the same in every lane
-        ex = max(__builtin_amdgcn_readfirstlane(ex), -24);
-        const float grow = static_cast<float>(ex) - cap;
-        if (grow > 0.f) {
-          const float shrink = ldexpf(1.f, -static_cast<int>(grow));
-          if (lim != -INFINITY) {
-            mref += grow;
-            lim -= grow;
-          }
-          l_run *= shrink;
-#pragma unroll
-          for (int db = 0; db < DB; ++db) oacc[db] *= shrink;
-          cap = static_cast<float>(ex);
-        }
-        cap16 = ex > 15 ? 0xFFFFu : static_cast<uint32_t>(f2h(ldexpf(1.f, ex)));
-      }
       // ---- log2-domain scores relative to mref, and the softmax step
       float sc[2];
       uint32_t see = 0;
@@ -932,18 +891,18 @@ tree_plane_kernel(TreeArgs a) {
         const float s = fmaf(fma_f16(t1[j][0], kn[j], mul_f16(t2[j][0] * a.coeff, rn[j])), fa, -mref);
         sc[j] = !EDGE || (see & (1u << (16 * j))) ? s : -INFINITY;
       }
-      const float lmax = max_raw(sc[0], sc[1]);
+      const float lmax = max_raw(sc[0] + norm_exponent(vn[0]), sc[1] + norm_exponent(vn[1]));
       if (__any(lmax > lim)) {
         float m = lmax;
 #pragma unroll
         for (int sh = 8; sh >= 1; sh >>= 1) m = fmaxf(m, __shfl_xor(m, sh, 64));
         const bool move = m > lim;
-        const float shift = move ? m - PUP + cap : 0.f;
+        const float shift = move ? m - PUP : 0.f;
         const float alpha = !move ? 1.f : lim == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-shift);
         sc[0] -= shift;
         sc[1] -= shift;
         mref += shift;
-        lim = move ? TAU + PUP - cap : lim;
+        lim = move ? TAU + PUP : lim;
         l_run *= alpha;
         const float ac = __shfl(alpha, 16 * (l16 & 3), 64);  // column l16 & 3 of O^T belongs to that lane group
 #pragma unroll
