@@ -201,3 +201,23 @@ def test_graph_replays():
         graph.replay()
         torch.cuda.synchronize()
         _equal(got, _walk(tokens, target, u, par, None))
+
+
+def test_nodes_without_a_place_spoil_no_sibling():
+    """A node whose parent is no earlier node is nobody's earlier sibling, whatever its token is."""
+    V = 40
+    ones = torch.ones(1, 4, V, device=DEV)
+    tok, u = torch.tensor([[0, 7, 5, 7]], device=DEV), torch.zeros(1, 4, device=DEV)
+    for first in (2, -2, 1, 99, -1):
+        par = torch.tensor([[-1, first, 0, 2]], dtype=torch.int32, device=DEV)
+        path, count, nxt = verify_drafts(tok, ones, u, parents=par)
+        assert path.tolist() == [[0, 2, 3, -1]] and count.tolist() == [3], first
+        _equal((path, count, nxt), _walk(tok, ones, u, par))
+    # many such nodes in random trees, few distinct tokens
+    for seed in range(20):
+        tokens, target, uni, par, _ = _inputs(16, 24, 6, torch.float32, 100 + seed, True)
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        i = torch.arange(24, device=DEV)
+        far = torch.randint(0, 24, (16, 24), device=DEV, generator=g).maximum(i).to(torch.int32)
+        par = torch.where((torch.rand(16, 24, device=DEV, generator=g) < 0.4) & (i > 0), far, par)
+        _equal(verify_drafts(tokens, target, uni, parents=par), _walk(tokens, target, uni, par))

@@ -87,11 +87,13 @@ __device__ __forceinline__ Left walk(const VerifyArgs& a, int b, int64_t* s_rej,
     if (a.draft) {
       if (inner && tok >= 0 && tok < a.V) bar = u * static_cast<double>(load_act<DT>(a.draft, b * a.db + par * a.dt + tok));
     } else {
-      // the earlier siblings in index order; a candidate that repeats one has nothing left to accept
+      // the earlier siblings in index order; a candidate that repeats one has nothing left to accept.
+      // A node whose parent is not an earlier node has no place in the tree and is nobody's sibling.
       double rem = 1.0;
       const int T = a.parents ? a.T : 0;  // a chain has no siblings
+      const int placed = inner ? par : -1;
       for (int j = 0; j < T; ++j) {
-        const int pj = lane_value(par, j);
+        const int pj = lane_value(placed, j);
         const int64_t tj = lane_value(tok, j);
         const double qj = lane_value(p, j);  // settled: every earlier sibling of j has had its turn
         if (j < i && pj == par) {
