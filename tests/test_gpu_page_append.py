@@ -149,3 +149,22 @@ def test_pages_past_4_gib(bits, pages):
             assert torch.equal(*out) and torch.isfinite(out[0]).all()
     for name, t in big.planes(0).items():
         assert torch.equal(t[pages - 8:].view(torch.uint8), small.planes(0)[name].view(torch.uint8)), name
+
+
+@pytest.mark.parametrize("kt,vt,qt", [(torch.bfloat16, torch.bfloat16, torch.float32), (torch.float16, torch.float16, torch.float32),
+                                      (torch.float16, torch.float16, torch.bfloat16), (torch.bfloat16, torch.float32, torch.bfloat16),
+                                      (torch.float16, torch.bfloat16, torch.float32), (torch.float32, torch.float16, torch.bfloat16)])
+@pytest.mark.parametrize("D,T", [(64, 1), (128, 9)])
+def test_mixed_types_lose_nothing(kt, vt, qt, D, T):
+    """Rows and outputs bit for bit those of the separate operators, each on its own type."""
+    print("case:", kt, vt, qt, D, T, flush=True)
+    kc, vc, (one, two), table, lengths, g = _setup(D, 3, 3, 2, T, [0, 31, 200], 32, 5)
+    k, v, q = (torch.randn(3, T, h, D, device=DEV, generator=g).to(t).transpose(1, 2) for h, t in ((2, kt), (2, vt), (4, qt)))
+    two.write(1, kc.compress(k), vc.compress(v), table, lengths)
+    want = tree_attention(q, kc, vc, two, 1, table, lengths)
+    out = append_tree_attention(k, v, q, kc, vc, one, 1, table, lengths)
+    assert out.dtype == qt and torch.isfinite(out[0]).all()
+    assert torch.equal(out.nan_to_num(7.0), want.nan_to_num(7.0))  # positions behind a prefix hold random rows
+    _same(one, two)
+    empty = append_tree_attention(k[:0], v[:0], q[:0], kc, vc, one, 1, table[:0], lengths[:0])
+    assert empty.shape == (0, T, 4, D) and empty.dtype == qt

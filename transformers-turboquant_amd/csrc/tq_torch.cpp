@@ -1127,11 +1127,16 @@ Tensor page_attend(const Tensor& k_in, const Tensor& v_in, const Tensor& q_in, c
   Tensor out = page_attend_meta(k_in, v_in, q_in, kpi, kseff, kcent, kbounds, vpi, vbounds, kseff16, kcodes, ksigns, krn, kvn,
                                 kcent16, bits, vcodes, vvn, vcent32, vpit, table, lengths, parents, coeff, scale, out_dtype);
   const c10::DeviceGuard g(q_in.device());
-  Tensor k = activation(k_in);
-  auto like_k = [&](const Tensor& t) {
-    return t.scalar_type() == k.scalar_type() && t.stride(-1) == 1 ? t : t.to(k.scalar_type()).contiguous();
-  };
-  Tensor v = like_k(v_in), q = like_k(q_in);
+  Tensor k = activation(k_in), v = activation(v_in), q = activation(q_in);
+  if (v.scalar_type() != k.scalar_type() || q.scalar_type() != k.scalar_type()) {
+    // the fused launch takes one type: the separate operators take each tensor in its own, and lose nothing
+    const auto ck = compress_keys(k, kpi, kseff, kcent, kbounds, bits - 1, c10::nullopt, c10::nullopt);
+    const auto cv = compress_values(v, vpi, vbounds, bits, c10::nullopt);
+    page_write(std::get<0>(ck), std::get<1>(ck), std::get<2>(ck), std::get<3>(ck), std::get<0>(cv), std::get<1>(cv), kcodes,
+               ksigns, krn, kvn, vcodes, vvn, table, lengths, k.size(2));
+    return tree_attend(q, kpi, kseff16, kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn, vcent32, vpit, table, lengths,
+                       parents, coeff, scale, out_dtype);
+  }
   // one allocation: the workspace, then the prepared queries
   const int64_t bytes = (tree_workspace(q, kvn, table, bits) + 15) / 16 * 16, n = q.numel();
   Tensor ws = at::empty({bytes + n * 6}, q.options().dtype(at::kByte));

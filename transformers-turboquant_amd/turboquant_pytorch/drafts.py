@@ -54,7 +54,8 @@ def append_tree_attention(k: torch.Tensor, v: torch.Tensor, queries: torch.Tenso
                           out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """One layer's decoding or speculation step: the T new tokens' keys and values k, v [B, Hkv, T, D]
     compressed into their pages (positions ``lengths[b] + i``) and the queries prepared in one launch,
-    then tree_attention.  A new row whose page is missing is not written."""
+    then tree_attention.  A new row whose page is missing is not written.  k, v and queries of different
+    types run as the separate operators (compress, ``pool.write``, tree_attention), each in its own type."""
     tk, tv = _both_tables(key_compressor, val_compressor, queries.device)
     return ops().page_attend(k, v, queries, tk.pi_split, tk.seff_split, tk.cent32, tk.bounds32, tv.pi_split, tv.bounds32,
                              tk.s_eff16, *_tree_args(tk, tv, queries.shape[-1], key_compressor, val_compressor, pool, layer,
