@@ -356,6 +356,19 @@ def test_another_stream():
         assert torch.equal(o, want)
 
 
+@pytest.mark.parametrize("bits", [2, 3])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,Hq,Hkv", [(2, 4, 2), (2, 2, 2), (3, 2, 2), (4, 3, 3)])
+def test_few_drafted_tokens_per_head(D, bits, T, Hq, Hkv):
+    """Up to 4 columns per kv head from several nodes: speculation with few query heads per kv head."""
+    print("case:", D, bits, T, Hq, Hkv, flush=True)
+    lens = [0, 31, 500, 1, 64]
+    kc, vc, pool, table, lengths, q = _setup(D, bits, len(lens), Hq, Hkv, T, lens, 32, seed=30 + T)
+    for par in (None, _tree(T, len(lens), T), torch.tensor([-1] + [0] * (T - 1), dtype=torch.int32, device=DEV)):
+        out = tree_attention(q, kc, vc, pool, 1, table, lengths, par, out_dtype=torch.float32)
+        _check(out, kc, vc, pool, table, lengths, q, par)
+
+
 # planes, one column tile, two column tiles
 FORMS = [(1, 4, 2, 0), (4, 2, 2, 0), (5, 4, 2, 0), (16, 4, 2, 4096)]
 
