@@ -270,3 +270,11 @@ def test_page_append_c_entry_refuses():
                     (dict(qr=4), b"q_rot"), (dict(B=1 << 20, H=1 << 10, S=64), b"2^31")):
         assert call(**kw) == -1 and msg in lib.tq_last_error(), kw
     assert call(B=0, k=none) == 0 and call(S=0, k=none) == 0
+
+
+def test_more_sequences_than_a_grid_takes_are_refused_before_a_row_is_written():
+    n = 65536
+    big = dict(table=_e(n, W, dtype=I32), lengths=_e(n, dtype=I32))
+    for args, fn in ((_append_args(), ops().page_attend), (_tree_args(True), ops().tree_attend)):
+        new = {k: _e(n, *args[k].shape[1:], dtype=args[k].dtype) for k in ("k", "v", "q") if k in args}
+        _refuses(fn, args, {**new, **big}, "at most 65535 sequences")

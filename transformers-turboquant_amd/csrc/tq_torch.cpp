@@ -988,6 +988,7 @@ Tensor check_tree(const Checker& c, const Tensor& q, Pool& pool, const Tensor& k
               " value bits; expected head_dim ", D, " with ", bits - 1, " and ", bits, " (2 to 4 bits)");
   TORCH_CHECK(Hq >= pool.H && Hq % pool.H == 0, c.op, ": ", Hq, " query heads are not a multiple of ", pool.H, " kv heads");
   TORCH_CHECK(T >= 1 && T <= 64, c.op, ": 1 to 64 drafted tokens, got ", T);
+  TORCH_CHECK(B <= 65535 && pool.H <= 65535, c.op, ": at most 65535 sequences and kv heads, got ", B, " and ", pool.H);
   check_table(c, table);
   TORCH_CHECK(table.size(0) == B, c.op, ": block_table has ", table.size(0), " rows for ", B, " sequences");
   TORCH_CHECK(table.size(1) * pool.P >= T && table.size(1) * pool.P <= (int64_t{1} << 24), c.op, ": a row of ", table.size(1),
