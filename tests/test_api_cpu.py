@@ -245,3 +245,44 @@ def test_default_is_reference_noncausal_under_sdpa():
         assert torch.equal(none, zero)
         assert not torch.allclose(model(input_ids=ids).logits, _small_gpt2("eager")(input_ids=ids).logits,
                                   atol=1e-3)
+
+
+def test_kernel_operands_follow_the_compressors_tensors():
+    """Tensors assigned or written in place are what the kernels get, whichever tensors those replaced."""
+    from turboquant_pytorch.codebook import random_rotation, split_f16
+    from turboquant_pytorch.compressors import _scaled_tables, _tables
+
+    cpu = torch.device("cpu")
+
+    def check(c, keys):
+        t = _tables(c, cpu, keys)
+        assert torch.equal(t.pi_split, split_f16(c.Pi)) and torch.equal(t.pit_split, split_f16(c.Pi.T.contiguous()))
+        assert torch.equal(t.cent32, c.centroids) and torch.equal(t.cent16, c.centroids.half())
+        assert torch.equal(t.bounds32, c.boundaries)
+        if keys:
+            assert torch.equal(t.s_eff16, (c.S @ c.Pi.T).half())
+        else:
+            cent, pit = _scaled_tables(c, t)
+            f = round(float(cent[0] / c.centroids[0]) * 2 ** 14) / 2 ** 14  # the common factor, a multiple of 2^-14
+            assert torch.allclose(cent, c.centroids * f, rtol=1e-6, atol=0)
+            assert torch.equal(pit, split_f16((c.Pi.T.double() / f).float().contiguous()))
+        assert _tables(c, cpu, keys) is t
+
+    for c, keys in ((TurboQuantCompressorV2(64, 3, 1), True), (TurboQuantCompressorMSE(64, 3, 2), False)):
+        check(c, keys)
+        c.Pi.copy_(random_rotation(64, 77))  # in place
+        check(c, keys)
+        c.centroids.mul_(1.25)
+        check(c, keys)
+        c.boundaries.add_(0.01)
+        check(c, keys)
+        if keys:
+            c.S.neg_()
+            check(c, keys)
+        for i in range(30):  # twice between calls: the freed tensor's address may serve the second
+            c.Pi = random_rotation(64, 100 + 2 * i)
+            c.Pi = random_rotation(64, 101 + 2 * i)
+            check(c, keys)
+        with torch.inference_mode():
+            c.Pi = random_rotation(64, 5)
+        check(c, keys)

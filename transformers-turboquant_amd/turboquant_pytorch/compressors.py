@@ -28,7 +28,9 @@ __all__ = ["TurboQuantCompressorV2", "TurboQuantCompressorMSE"]
 @dataclass
 class _DeviceTables:
     """Per-device operands of the HIP kernels, derived from the compressor's tensors."""
-    key: tuple
+    device: torch.device
+    sources: tuple                    # the tensors they were made from, held so that `is` means something
+    versions: tuple                   # and how often those had been written in place
     pi_split: torch.Tensor            # f16 [2, d, d]  split of Pi
     pit_split: torch.Tensor           # f16 [2, d, d]  split of Pi^T
     seff_split: torch.Tensor | None   # f16 [2, d, d]  split of the f32 S_eff = S Pi^T (keys)
@@ -39,12 +41,21 @@ class _DeviceTables:
     scaled: tuple | None = None       # f32 [2^b] scaled centroids, f16 [2, d, d] split of Pi^T over the scale
 
 
+def _version(t: torch.Tensor | None) -> int | None:
+    # tensors made under torch.inference_mode() count no writes: assign new ones there
+    return None if t is None or t.is_inference() else t._version
+
+
 def _tables(comp, device: torch.device, with_qjl: bool) -> _DeviceTables:
+    device = torch.device(device)
     s = getattr(comp, "S", None) if with_qjl else None
-    key = (str(device), id(comp.Pi), id(s), id(comp.centroids), id(comp.boundaries))
-    cached = getattr(comp, "_dev_tables", None)
-    if cached is not None and cached.key == key:
-        return cached
+    pi_, cent_, bounds_ = comp.Pi, comp.centroids, comp.boundaries
+    versions = (_version(pi_), _version(s), _version(cent_), _version(bounds_))
+    t = getattr(comp, "_dev_tables", None)
+    if t is not None and t.device == device and t.versions == versions:
+        h = t.sources
+        if h[0] is pi_ and h[1] is s and h[2] is cent_ and h[3] is bounds_:
+            return t
     pi = comp.Pi.detach().to("cpu", torch.float32)
     cent = comp.centroids.detach().to("cpu", torch.float32)
     bounds = comp.boundaries.detach().to("cpu", torch.float32)
@@ -55,7 +66,9 @@ def _tables(comp, device: torch.device, with_qjl: bool) -> _DeviceTables:
         seff_split = split_f16(s_eff32).to(device)
         s_eff = s_eff32.to(torch.float16).contiguous().to(device)
     t = _DeviceTables(
-        key=key,
+        device=device,
+        sources=(pi_, s, cent_, bounds_),
+        versions=versions,
         pi_split=split_f16(pi).to(device),
         pit_split=split_f16(pi.T.contiguous()).to(device),
         seff_split=seff_split,
