@@ -14,6 +14,7 @@ to callers; the methods dispatch on its keys (compressors.py:178, :301).
 
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 
@@ -41,21 +42,24 @@ class _DeviceTables:
     scaled: tuple | None = None       # f32 [2^b] scaled centroids, f16 [2, d, d] split of Pi^T over the scale
 
 
-def _version(t: torch.Tensor | None) -> int | None:
+def _writes(*tensors) -> tuple:
     # tensors made under torch.inference_mode() count no writes: assign new ones there
-    return None if t is None or t.is_inference() else t._version
+    return tuple(None if t is None or t.is_inference() else t._version for t in tensors)
 
 
 def _tables(comp, device: torch.device, with_qjl: bool) -> _DeviceTables:
-    device = torch.device(device)
     s = getattr(comp, "S", None) if with_qjl else None
     pi_, cent_, bounds_ = comp.Pi, comp.centroids, comp.boundaries
-    versions = (_version(pi_), _version(s), _version(cent_), _version(bounds_))
+    try:
+        versions = (pi_._version, cent_._version, bounds_._version, None if s is None else s._version)
+    except RuntimeError:
+        versions = _writes(pi_, cent_, bounds_, s)
     t = getattr(comp, "_dev_tables", None)
-    if t is not None and t.device == device and t.versions == versions:
+    if t is not None and t.versions == versions and t.device == device:
         h = t.sources
-        if h[0] is pi_ and h[1] is s and h[2] is cent_ and h[3] is bounds_:
+        if h[0] is pi_ and h[1] is cent_ and h[2] is bounds_ and h[3] is s:
             return t
+    device = torch.device(device)
     pi = comp.Pi.detach().to("cpu", torch.float32)
     cent = comp.centroids.detach().to("cpu", torch.float32)
     bounds = comp.boundaries.detach().to("cpu", torch.float32)
@@ -67,7 +71,7 @@ def _tables(comp, device: torch.device, with_qjl: bool) -> _DeviceTables:
         s_eff = s_eff32.to(torch.float16).contiguous().to(device)
     t = _DeviceTables(
         device=device,
-        sources=(pi_, s, cent_, bounds_),
+        sources=(pi_, cent_, bounds_, s),
         versions=versions,
         pi_split=split_f16(pi).to(device),
         pit_split=split_f16(pi.T.contiguous()).to(device),
@@ -81,15 +85,22 @@ def _tables(comp, device: torch.device, with_qjl: bool) -> _DeviceTables:
     return t
 
 
+@functools.lru_cache(maxsize=64)
+def _f16_factor(centroids: tuple) -> float:
+    """The factor of 1 + i / 2^14 under which centroids lose least by rounding to f16 (least squared error): relative
+    to them 2e-6, 2e-5 and 4e-5 (rms) at 2, 3 and 4 bits, 1.5e-4 to 3e-4 unscaled.  Searched once per codebook
+    (0.3 ms), which a model's layers share."""
+    factors = 1 + torch.arange(2 ** 14, dtype=torch.float64) / 2 ** 14
+    x = torch.tensor(centroids, dtype=torch.float64) * factors[:, None]
+    return float(factors[((x - x.to(torch.float16).double()) / factors[:, None]).square().sum(1).argmin()])
+
+
 def _scaled_tables(comp, t: _DeviceTables) -> tuple[torch.Tensor, torch.Tensor]:
     """Centroids times a common factor from [1, 2), and the split of Pi^T divided by it: kernels that hold value
-    centroids as f16 lose less by the rounding.  Of 2^14 factors the one with the least squared error:
-    relative to the centroids 2e-6, 2e-5 and 4e-5 (rms) at 2, 3 and 4 bits, 1.5e-4 to 3e-4 unscaled."""
+    centroids as f16 lose less by the rounding."""
     if t.scaled is None:
         cent = comp.centroids.detach().to("cpu", torch.float64)
-        factors = 1 + torch.arange(2 ** 14, dtype=torch.float64) / 2 ** 14
-        x = cent * factors[:, None]
-        best = factors[((x - x.to(torch.float16).double()) / factors[:, None]).square().sum(1).argmin()]
+        best = _f16_factor(tuple(cent.tolist()))
         pi = comp.Pi.detach().to("cpu", torch.float64)
         t.scaled = ((cent * best).float().to(t.cent32.device),
                     split_f16((pi.T / best).float().contiguous()).to(t.cent32.device))
