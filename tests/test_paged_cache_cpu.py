@@ -344,3 +344,50 @@ def test_tree_depths_and_their_refusals():
                        (torch.zeros(1, 2, dtype=torch.long), {"parents": [-1, 0], "draft_probs": torch.ones(1, 1, 4)})):
         with pytest.raises(ValueError):
             speculative_step(None, cache, tokens, **kw)
+
+
+def _tiny(kind, **kw):
+    import transformers as tr
+
+    cfg = getattr(tr, kind + "Config")(vocab_size=128, hidden_size=128, intermediate_size=128, num_hidden_layers=2,
+                                       num_attention_heads=2, num_key_value_heads=2, **kw)
+    cfg._attn_implementation = "sdpa"
+    return apply_turboquant(getattr(tr, kind + "ForCausalLM")(cfg).eval(), bits=3, causal="auto")
+
+
+def _ids(B, T):
+    return torch.zeros(B, T, dtype=torch.long)
+
+
+@pytest.mark.parametrize("kind,kw", [("Mistral", dict(sliding_window=24)),
+                                     ("Qwen2", dict(use_sliding_window=True, sliding_window=24, max_window_layers=1)),
+                                     ("Qwen2", dict(use_sliding_window=True, sliding_window=24, max_window_layers=0))])
+def test_sliding_windows_are_refused_once_a_token_is_past_them(kind, kw):
+    model = _tiny(kind, **kw)
+    for n, T, past in ((0, 24, False), (20, 4, False), (23, 1, False), (0, 25, True), (20, 5, True), (24, 1, True), (300, 1, True)):
+        for call in (model, model.model):  # the decoder may be called by itself
+            cache = make(pages=40)
+            if n:
+                step(cache, [[1] * n])
+            free = cache.free_pages
+            with pytest.raises(ValueError, match="sliding window of 24" if past else "GPU"):
+                call(input_ids=_ids(1, T), past_key_values=cache, use_cache=True)
+            assert cache.free_pages == free and cache.get_seq_length() == n
+            with pytest.raises(ValueError, match="sliding window of 24" if past else "GPU"):
+                call(_ids(1, T), None, None, cache)
+    # other caches keep their masks
+    from transformers_turboquant import TurboQuantCache
+
+    assert model(input_ids=_ids(1, 30), past_key_values=TurboQuantCache(), use_cache=True).logits.shape == (1, 30, 128)
+
+
+def test_windows_of_attention_modules():
+    for kind, kw, want in (("Llama", {}, [None, None]), ("Qwen2", dict(sliding_window=8), [None, None]),
+                           ("Mistral", dict(sliding_window=None), [None, None]), ("Mistral", dict(sliding_window=8), [8, 8]),
+                           ("Qwen2", dict(use_sliding_window=True, sliding_window=8, max_window_layers=1), [None, 8])):
+        model = _tiny(kind, **kw)
+        assert [layer.self_attn.sliding_window for layer in model.model.layers] == want
+        with pytest.raises(ValueError, match="GPU" if want[1] is None else "window"):
+            model(input_ids=_ids(1, 100), past_key_values=make(), use_cache=True)
+    # patched a second time: still one check
+    assert len(apply_turboquant(model, bits=3).model._forward_pre_hooks) == 1

@@ -28,6 +28,7 @@ from turboquant_pytorch.fused import compressed_attention
 
 from ..cache import TurboQuantCache
 from ..paged_cache import TurboQuantPagedCache
+from ..paged_call import check_window
 
 
 def additive_mask(mask: torch.Tensor | None, dtype=torch.float32) -> torch.Tensor | None:
@@ -68,6 +69,7 @@ def attention_tail(module, q, k, v, attention_mask, output_attentions: bool = Fa
     if isinstance(cache, TurboQuantPagedCache):
         if not fused:
             raise ValueError("a paged cache serves GPU attention without attention weights or dropout (model.eval())")
+        check_window(getattr(module, "sliding_window", None), cache.get_seq_length(), T)
         if attention_mask is not None:
             raise ValueError("a paged cache masks by itself and takes no attention mask: run prompts unpadded, under the "
                              "sdpa attention implementation")

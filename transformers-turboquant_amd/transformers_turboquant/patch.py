@@ -4,6 +4,7 @@ from __future__ import annotations
 
 from turboquant_pytorch.compressors import TurboQuantCompressorMSE, TurboQuantCompressorV2
 
+from .paged_call import PagedCall, attention_window
 from .registry import get_attention_class
 
 
@@ -42,7 +43,9 @@ def apply_turboquant(model, bits: int = 3, seed: int = 42, use_triton: bool = Tr
             vc = TurboQuantCompressorMSE(d, bits, seed=seed + i + 10000, device=device, use_triton=use_triton)
             new = family.from_original(child, kc, vc)
             new.causal_mode = causal
+            new.sliding_window = attention_window(child)
             setattr(parent, name, new)
             i += 1
+    PagedCall.install(model)
     model.config.use_cache = False
     return model
