@@ -391,3 +391,29 @@ def test_windows_of_attention_modules():
             model(input_ids=_ids(1, 100), past_key_values=make(), use_cache=True)
     # patched a second time: still one check
     assert len(apply_turboquant(model, bits=3).model._forward_pre_hooks) == 1
+
+
+@pytest.mark.parametrize("kind", ["Llama", "GPT2"])
+def test_padding_over_a_cache_is_refused(kind):
+    """A zero anywhere in the 2-D mask, over cached positions or new ones."""
+    if kind == "GPT2":
+        from transformers import GPT2Config, GPT2LMHeadModel
+
+        model = apply_turboquant(GPT2LMHeadModel(GPT2Config(n_layer=2, n_embd=128, n_head=2, vocab_size=128)).eval(), bits=3,
+                                 causal="auto")
+    else:
+        model = _tiny(kind)
+    cache = make()
+    step(cache, [[1] * 20, [2] * 20])
+    for T in (1, 10):
+        for where in (None, 0, 7, 19, 20 + T // 2, 19 + T):
+            for dtype in (torch.long, torch.bool, torch.float32):
+                mask = torch.ones(2, 20 + T, dtype=dtype)
+                if where is not None:
+                    mask[1, where] = 0
+                for call in (model, model.base_model):
+                    with pytest.raises(ValueError, match="GPU" if where is None else "padding"):
+                        call(input_ids=_ids(2, T), attention_mask=mask, past_key_values=cache, use_cache=True)
+    assert cache.lengths() == [20, 20] and cache.free_pages == 10
+    with pytest.raises(ValueError, match="padding"):
+        model(input_ids=_ids(2, 3), attention_mask=torch.tensor([[1, 1, 1], [0, 1, 1]]), past_key_values=make(), use_cache=True)

@@ -9,6 +9,8 @@ from __future__ import annotations
 
 import inspect
 
+import torch
+
 from .paged_cache import TurboQuantPagedCache
 
 __all__ = ["PagedCall", "attention_window"]
@@ -65,4 +67,9 @@ class PagedCall:
         if tokens is None:
             return None
         check_window(self.window, cache.get_seq_length(), tokens.shape[1])
+        mask = given.get("attention_mask")
+        # over a cache that masks by itself the decoder reduces a 2-D mask to its first columns, and to None
+        # where those are ones: padding is only seen here (masks of other forms reach the layers, which refuse them)
+        if isinstance(mask, torch.Tensor) and mask.dim() == 2 and not bool(mask.all()):
+            raise ValueError("a paged cache masks by itself and takes no padding: run prompts unpadded, in batches of one length")
         return None
