@@ -262,3 +262,28 @@ def test_refusals_under_a_model():
     run(model, short, ids(1, 4))
     with pytest.raises(RuntimeError, match="wrote 2 of the cache's 3 layers"):
         run(model, short, ids(1, 4))
+
+
+def test_positions_of_unequal_sequences_and_trees():
+    """Without position_ids: sequences of unequal length, and a drafted tree, against recomputation."""
+    print("case: paged positions", flush=True)
+    model, cache = llama(), TurboQuantPagedCache(40, 2, 32)
+    text = ids(2, 120)
+    a, b = cache.add(2)
+    for i, n in ((a, 90), (b, 33)):
+        cache.use([i])
+        with torch.no_grad():
+            model(input_ids=text[[a, b].index(i)][None, :n], past_key_values=cache, use_cache=True)
+    cache.use([a, b])
+    with torch.no_grad():
+        got = model(input_ids=torch.stack([text[0, 90:95], text[1, 33:38]]), past_key_values=cache, use_cache=True).logits.float()
+    close(got[0], recompute(model, text[:1, :95])[0, 90:])
+    close(got[1], recompute(model, text[1:, :38])[0, 33:])
+    tree = torch.tensor([-1, 0, 0, 1], dtype=torch.int32, device="cuda")
+    drafted = torch.stack([text[0, [95, 96, 7, 97]], text[1, [38, 39, 7, 40]]])
+    with cache.draft(tree), torch.no_grad():
+        got = model(input_ids=drafted, past_key_values=cache, use_cache=True).logits.float()
+    for row, (n, t) in enumerate(((95, text[0]), (38, text[1]))):
+        close(got[row, [0, 1, 3]], recompute(model, t[None, :n + 3])[0, n:])
+        close(got[row, 2], recompute(model, torch.cat([t[:n + 1], t[7:8]])[None])[0, -1])
+    assert cache.lengths() == [95, 38]

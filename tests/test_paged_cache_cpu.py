@@ -417,3 +417,67 @@ def test_padding_over_a_cache_is_refused(kind):
     assert cache.lengths() == [20, 20] and cache.free_pages == 10
     with pytest.raises(ValueError, match="padding"):
         model(input_ids=_ids(2, 3), attention_mask=torch.tensor([[1, 1, 1], [0, 1, 1]]), past_key_values=make(), use_cache=True)
+
+
+def _positions(call, layer, **kw):
+    """The position_ids that the decoder's layers get (the CPU is refused behind them)."""
+    seen = []
+    hook = layer.register_forward_pre_hook(lambda m, a, k: seen.append(k.get("position_ids")), with_kwargs=True)
+    with pytest.raises(ValueError, match="GPU"):
+        call(**kw, use_cache=True)
+    hook.remove()
+    return seen[0].tolist()
+
+
+def test_tokens_stand_behind_their_own_sequence():
+    model = _tiny("Llama")
+    layer = model.model.layers[0]
+    cache = make()
+    a, b = cache.add(2)
+    for i, n in ((a, 20), (b, 33)):
+        cache.use([i])
+        step(cache, [[1] * n])
+    cache.use([b])
+    assert _positions(model, layer, input_ids=_ids(1, 2), past_key_values=cache) == [[33, 34]]
+    cache.use([a, b])
+    for call in (model, model.model):
+        got = _positions(call, layer, input_ids=_ids(2, 3), past_key_values=cache)
+        assert got == [[20, 21, 22], [33, 34, 35]]
+        given = torch.tensor([[5, 6], [7, 8]])
+        assert _positions(call, layer, input_ids=_ids(2, 2), past_key_values=cache, position_ids=given) == given.tolist()
+        ones = torch.ones(2, 2, dtype=torch.long)
+        assert _positions(call, layer, input_ids=_ids(2, 2), past_key_values=cache, attention_mask=ones) == [[20, 21], [33, 34]]
+        with pytest.raises(ValueError, match="position_ids"):
+            call(input_ids=_ids(2, 2), past_key_values=cache, position_ids=torch.tensor([[33, 34]]), use_cache=True)
+        with pytest.raises(ValueError, match="a mask of 35 positions"):
+            call(input_ids=_ids(2, 2), past_key_values=cache, attention_mask=torch.ones(2, 35, dtype=torch.long), use_cache=True)
+    seen = []
+    hook = layer.register_forward_pre_hook(lambda m, a, k: seen.append(k["position_ids"]), with_kwargs=True)
+    with pytest.raises(ValueError, match="GPU"):  # None in its place
+        model.model(_ids(2, 1), None, None, cache)
+    hook.remove()
+    assert seen[0].tolist() == [[20], [33]]
+    # generate() counts every row from the longest sequence
+    with pytest.raises(ValueError, match="a mask of 34 positions"):
+        model.generate(_ids(2, 34), past_key_values=cache, use_cache=True, max_new_tokens=2, pad_token_id=5)
+    assert cache.lengths() == [20, 33]
+
+
+def test_drafted_nodes_stand_at_their_depth():
+    model = _tiny("Llama")
+    layer = model.model.layers[0]
+    cache = make()
+    step(cache, [[1] * 20] * 2)
+    tree = torch.tensor([-1, 0, 0, 1, 3, -2, 5, -1, 7], dtype=torch.int32)
+    want = [0, 1, 1, 2, 3, 0, 1, 0, 1]
+    with cache.draft(tree):
+        assert _positions(model, layer, input_ids=_ids(2, 9), past_key_values=cache) == [[20 + d for d in want]] * 2
+    both = torch.stack([tree, torch.arange(-1, 8, dtype=torch.int32)])
+    with cache.draft(both):
+        assert _positions(model, layer, input_ids=_ids(2, 9), past_key_values=cache) == [
+            [20 + d for d in want], list(range(20, 29))]
+    with cache.draft():
+        assert _positions(model, layer, input_ids=_ids(2, 3), past_key_values=cache)[0] == [20, 21, 22]
+    fresh = TurboQuantPagedCache(8, 2, 32)
+    with fresh.draft(tree):
+        assert _positions(model, layer, input_ids=_ids(1, 9), past_key_values=fresh) == [want]

@@ -240,6 +240,11 @@ class TurboQuantPagedCache(Cache):
             if not self._drafted:
                 self._abandon()
 
+    @property
+    def draft_parents(self) -> torch.Tensor | None:
+        """The tree of the draft under way (None: no draft, or a chain)."""
+        return self._tree[0] if self._tree else None
+
     def accept(self, path: torch.Tensor, count: torch.Tensor) -> list[int]:
         """Keep the first count[b] nodes of path[b] (`verify_drafts`) of the drafted tokens, in every
         layer; the others are dropped and their pages freed.  Returns the new lengths."""
@@ -290,7 +295,7 @@ class TurboQuantPagedCache(Cache):
         self._begin(layer_idx, k, bits)
         table, lengths = self._device_state
         if fast:
-            parents = self._tree[0] if self._tree else None
+            parents = self.draft_parents
             out = append_tree_attention(k, v, q, key_compressor, val_compressor, self.pool, layer_idx, table, lengths,
                                         parents, scale, out_dtype)
         else:
@@ -344,7 +349,7 @@ class TurboQuantPagedCache(Cache):
             if T != self._step:
                 raise ValueError(f"layer {layer_idx} appends {T} tokens in a step of {self._step}")
             return
-        parents = self._tree[0] if self._tree else None
+        parents = self.draft_parents
         if parents is not None and tuple(parents.shape) not in ((T,), (B, T)):
             raise ValueError(f"parents {tuple(parents.shape)} for {B} sequences of {T} drafted tokens")
         self._reserve(T)

@@ -72,4 +72,40 @@ class PagedCall:
         # where those are ones: padding is only seen here (masks of other forms reach the layers, which refuse them)
         if isinstance(mask, torch.Tensor) and mask.dim() == 2 and not bool(mask.all()):
             raise ValueError("a paged cache masks by itself and takes no padding: run prompts unpadded, in batches of one length")
-        return None
+        return self._place(cache, tokens, mask, given.get("position_ids"), args, kwargs)
+
+    def _place(self, cache, tokens, mask, positions, args, kwargs):
+        """The arguments with the tokens' positions where the decoder would make wrong ones: from the longest
+        sequence, one after another."""
+        B, T = tokens.shape[:2]
+        lengths, tree = cache.lengths(), cache.draft_parents
+        unequal = len(set(lengths)) > 1
+        if len(lengths) not in (0, B) or (tree is not None and tuple(tree.shape) not in ((T,), (B, T))):
+            return None  # the cache refuses the step
+        if unequal and isinstance(mask, torch.Tensor) and mask.dim() == 2 and mask.shape[1] > T:
+            # generate() counts positions along such a mask
+            raise ValueError(f"a mask of {mask.shape[1]} positions for sequences of {sorted(set(lengths))} cached ones and {T} new "
+                             "tokens: pass none, and position_ids or none")
+        if positions is not None:
+            if unequal and positions.shape[0] != B:
+                raise ValueError(f"position_ids {tuple(positions.shape)} for {B} sequences of unequal length")
+            return None
+        if not unequal and tree is None or "position_ids" not in self.names:
+            return None
+        behind = torch.arange(T)[None] if tree is None else tree_depths(tree)
+        positions = (torch.tensor(lengths or [0] * B)[:, None] + behind).to(tokens.device)
+        at = self.names.index("position_ids")
+        if at < len(args):
+            return (*args[:at], positions, *args[at + 1:]), kwargs
+        return args, {**kwargs, "position_ids": positions}
+
+
+def tree_depths(parents: torch.Tensor) -> torch.Tensor:
+    """How far behind the cached text each node of the trees [T] or [B, T] stands: [1 or B, T] (0 without a place)."""
+    rows = []
+    for row in parents.reshape(-1, parents.shape[-1]).tolist():
+        depth = []
+        for i, p in enumerate(row):
+            depth.append(depth[p] + 1 if 0 <= p < i else 0)
+        rows.append(depth)
+    return torch.tensor(rows)
