@@ -184,3 +184,24 @@ def test_a_pool_past_4_gib():
     pl = pool.planes(0)
     for n in NAMES:
         assert torch.equal(pl[n][0], pl[n][N - 2]) and pl[n][0].any(), n
+
+
+def test_tables_of_no_pages():
+    """Sequences without a page yet: reads are zeros, writes go nowhere, lengths still advance."""
+    print("case: no pages", flush=True)
+    pool = PagePool(4, 32, 2, 64, 3, layers=2, device=DEV)
+    for t in pool._planes:
+        t.view(torch.uint8).fill_(0x55)
+    keep = [t.clone() for t in pool._planes]
+    table = torch.empty(3, 0, dtype=torch.int32, device=DEV)
+    at = torch.tensor([0, 7, -1], dtype=torch.int32, device=DEV)
+    ck, cv = pool.read(1, table, at, 9)
+    for t in (ck["packed_key_indices"], ck["packed_qjl_signs"], ck["residual_norm"], ck["vec_norms"], cv["packed_indices"],
+              cv["vec_norms"]):
+        assert not t.any()
+    pool.write(1, ck, cv, table, at)
+    path = torch.tensor([[0, 1], [0, -1], [0, 1]], dtype=torch.int32, device=DEV)
+    assert pool.keep(table, at, path, torch.tensor([2, 1, 2], dtype=torch.int32, device=DEV)).tolist() == [2, 8, -1]
+    torch.cuda.synchronize()
+    for t, k in zip(pool._planes, keep):
+        assert torch.equal(t.view(torch.uint8), k.view(torch.uint8))

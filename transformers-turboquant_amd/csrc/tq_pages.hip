@@ -281,7 +281,7 @@ static int rows_call(const char* what, void* const* pool, void* const* rows, int
                      const int32_t* table, int64_t ld_table, int32_t table_width, const int32_t* at, hipStream_t s) {
   TQ_REQUIRE(B >= 0 && S >= 0 && H >= 1, "%s: bad shape", what);
   if (B == 0 || S == 0) return TQ_OK;
-  TQ_REQUIRE(pool && rows && table && at, "%s: null pointer", what);
+  TQ_REQUIRE(pool && rows && (table || table_width == 0) && at, "%s: null pointer", what);
   PagePlanes a{};
   const int st = fill(what, a, pool, rows, H, num_pages, page_size, d, key_code_bits, val_bits, table, ld_table, table_width);
   if (st != TQ_OK) return st;
@@ -345,7 +345,7 @@ int tq_page_keep(void* const* pool, int32_t layers, int32_t B, int32_t H, int32_
   TQ_REQUIRE(layers >= 1 && B >= 0 && T >= 1, "tq_page_keep: bad shape");
   TQ_REQUIRE(T <= 64, "tq_page_keep: at most 64 drafted tokens, got %d", T);
   if (B == 0) return TQ_OK;
-  TQ_REQUIRE(pool && block_table && lengths && path && count && new_lengths, "tq_page_keep: null pointer");
+  TQ_REQUIRE(pool && (block_table || table_width == 0) && lengths && path && count && new_lengths, "tq_page_keep: null pointer");
   TQ_REQUIRE(layers <= 65535 && B <= 65535, "tq_page_keep: at most 65535 layers and sequences, got %d and %d", layers, B);
   PagePlanes a{};
   const int st = fill("tq_page_keep", a, pool, nullptr, H, num_pages, page_size, d, key_code_bits, val_bits, block_table,
