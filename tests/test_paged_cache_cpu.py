@@ -481,3 +481,35 @@ def test_drafted_nodes_stand_at_their_depth():
     fresh = TurboQuantPagedCache(8, 2, 32)
     with fresh.draft(tree):
         assert _positions(model, layer, input_ids=_ids(1, 9), past_key_values=fresh) == [want]
+
+
+def test_a_speculative_step_that_fails_keeps_nothing(monkeypatch):
+    import turboquant_pytorch
+
+    cache = make()
+    step(cache, [[1] * 9, [2] * 9])
+    cache.use(cache.active[:1])
+    step(cache, [[1] * 21])
+    cache.use([0, 1])
+    free, tokens = cache.free_pages, torch.tensor([[5, 6, 7, 8], [9, 10, 11, 12]])
+
+    def model(input_ids, position_ids, past_key_values, use_cache):
+        step(past_key_values, input_ids.tolist())
+        return types.SimpleNamespace(logits=torch.zeros(2, 4, 16))
+
+    path = torch.tensor([[0, 1, 2, -1], [0, 3, -1, -1]], dtype=torch.int32)
+    count = torch.tensor([3, 2], dtype=torch.int32)
+    kept = []
+    cache.pool.keep = lambda table, lengths, path, count: kept.append(1) or lengths + count
+    for bad in ([3, -1], [-1, 4]):
+        monkeypatch.setattr(turboquant_pytorch, "verify_drafts", lambda *a, **k: (path, count, torch.tensor(bad)))
+        with pytest.raises(RuntimeError, match="no positive probability"):
+            speculative_step(model, cache, tokens)
+        assert cache.lengths() == [30, 9] and cache.free_pages == free and not kept
+        with pytest.raises(RuntimeError, match="accept"):
+            cache.accept(path, count)
+        check(cache)
+    monkeypatch.setattr(turboquant_pytorch, "verify_drafts", lambda *a, **k: (path, count, torch.tensor([3, 4])))
+    assert speculative_step(model, cache, tokens) == [[6, 7, 3], [12, 4]]
+    assert cache.lengths() == [33, 11] and kept == [1]
+    check(cache)

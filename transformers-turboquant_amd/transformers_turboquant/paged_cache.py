@@ -259,6 +259,11 @@ class TurboQuantPagedCache(Cache):
         self._abandon()
         return new
 
+    def drop_draft(self) -> None:
+        """Forget drafted tokens that are not accepted, and give their pages back."""
+        if self._drafted:
+            self._abandon()
+
     def _abandon(self) -> None:
         """Drop a step under way (drafted tokens, a forward that did not finish): its rows are behind
         the lengths and get overwritten; its pages are given back."""

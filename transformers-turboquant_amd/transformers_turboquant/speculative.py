@@ -55,11 +55,14 @@ def speculative_step(model, cache: TurboQuantPagedCache, tokens: torch.Tensor, p
     if draft_probs is not None:
         draft_probs = draft_probs.to(probs.dtype)
     path, count, nxt = verify_drafts(tokens, probs, uniforms, parents=tree, draft_probs=draft_probs)
-    cache.accept(path, count)
-    paths, counts, nexts, drafted = path.tolist(), count.tolist(), nxt.tolist(), tokens.tolist()
-    if min(nexts) < 0:
+    # one transfer, and before anything is kept: a step that cannot be finished leaves the cache as it was
+    got = torch.cat([path, count[:, None], nxt[:, None]], 1).tolist()
+    if any(row[-1] < 0 for row in got):
+        cache.drop_draft()
         raise RuntimeError("the model's distribution after the accepted tokens has no positive probability")
-    return [[drafted[b][i] for i in paths[b][1:counts[b]]] + [nexts[b]] for b in range(B)]
+    cache.accept(path, count)
+    drafted = tokens.tolist()
+    return [[drafted[b][i] for i in row[1:row[T]]] + [row[T + 1]] for b, row in enumerate(got)]
 
 
 def _depths(parents, B: int, T: int):
