@@ -287,3 +287,33 @@ def test_positions_of_unequal_sequences_and_trees():
         close(got[row, [0, 1, 3]], recompute(model, t[None, :n + 3])[0, n:])
         close(got[row, 2], recompute(model, torch.cat([t[:n + 1], t[7:8]])[None])[0, -1])
     assert cache.lengths() == [95, 38]
+
+
+def test_a_step_that_fails_leaves_the_cache_as_it_was(monkeypatch):
+    print("case: paged failures", flush=True)
+    from transformers_turboquant import paged_cache
+
+    model, cache = llama(), TurboQuantPagedCache(6, 2, 32)
+    with pytest.raises(RuntimeError, match="full"):
+        run(model, cache, ids(4, 70))
+    assert cache.active == [] and cache.free_pages == 6 and cache.pool is None
+    real = paged_cache.append_tree_attention
+
+    def fail(*a, **k):
+        raise ValueError("refused by the operator")
+
+    monkeypatch.setattr(paged_cache, "append_tree_attention", fail)
+    with pytest.raises(ValueError, match="refused by the operator"):
+        run(model, cache, ids(3, 40))
+    assert cache.active == [] and cache.free_pages == 6
+    monkeypatch.setattr(paged_cache, "append_tree_attention", real)
+    plain = TurboQuantPagedCache(6, 2, 32)  # where nothing failed
+    # another batch; bit for bit
+    assert torch.equal(run(model, cache, ids(2, 40)), run(model, plain, ids(2, 40)))
+    monkeypatch.setattr(paged_cache, "append_tree_attention", fail)
+    with pytest.raises(ValueError, match="refused by the operator"):
+        run(model, cache, ids(2, 30, 6))
+    assert cache.lengths() == [40, 40] and cache.free_pages == 2
+    monkeypatch.setattr(paged_cache, "append_tree_attention", real)
+    assert torch.equal(run(model, cache, ids(2, 3, 4)), run(model, plain, ids(2, 3, 4)))
+    assert cache.lengths() == plain.lengths() and cache.free_pages == plain.free_pages

@@ -513,3 +513,36 @@ def test_a_speculative_step_that_fails_keeps_nothing(monkeypatch):
     assert speculative_step(model, cache, tokens) == [[6, 7, 3], [12, 4]]
     assert cache.lengths() == [33, 11] and kept == [1]
     check(cache)
+
+
+def test_a_refused_first_forward_leaves_an_empty_cache():
+    cache = TurboQuantPagedCache(3, 2, 32)
+
+    def empty():
+        assert (cache.active, cache.free_pages, cache.pool, cache._seqs) == ([], 3, None, {}) and not cache.is_initialized
+        check(cache)
+
+    with pytest.raises(RuntimeError, match="full: 4 more pages"):
+        cache._begin(0, torch.zeros(1, 2, 100, 64), 3)
+    empty()
+    with pytest.raises(RuntimeError, match="full: 4 more pages"):  # another batch, another geometry
+        cache._begin(0, torch.zeros(4, 3, 10, 128), 4)
+    empty()
+    with pytest.raises(ValueError, match="parents"):
+        with cache.draft(torch.zeros(3, dtype=torch.int32)):
+            cache._begin(0, torch.zeros(2, 2, 4, 64), 3)
+    empty()
+    # a forward that ends between its layers
+    cache._begin(0, torch.zeros(1, 2, 5, 64), 3)
+    cache._finish(0)
+    with pytest.raises(RuntimeError, match="wrote 1 of the cache's 2 layers"):
+        cache._begin(0, torch.zeros(1, 2, 5, 64), 3)
+    empty()
+    cache.pool = FakePool(3, 32)
+    step(cache, [[1], [2]])
+    assert cache.lengths() == [1, 1] and cache.free_pages == 1
+    # sequences that were there stay, whatever fails on them
+    with pytest.raises(RuntimeError, match="full"):
+        step(cache, [[1] * 40, [2] * 40])
+    assert cache.lengths() == [1, 1] and cache.free_pages == 1 and cache.pool is not None
+    check(cache)

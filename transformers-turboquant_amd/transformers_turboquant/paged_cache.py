@@ -63,6 +63,8 @@ class TurboQuantPagedCache(Cache):
         self._written: set[int] = set()  # layers of the step under way that hold its rows
         self._step = 0  # tokens of the step under way
         self._device_state = None  # (block table, lengths) of the active sequences; None: to be made
+        self._made: list[int] = []  # sequences that the step under way made
+        self._made_pool = False  # it made the pool, too
 
     # ------------------------------------------------------------------ sequences
     def add(self, n: int = 1) -> list[int]:
@@ -274,6 +276,17 @@ class TurboQuantPagedCache(Cache):
         self._step = 0
         self._drafted = False
         self._device_state = None
+        self._made, self._made_pool = [], False
+
+    def _undo(self) -> None:
+        """Drop a step that failed, with the sequences and the pool that it made."""
+        made, made_pool = self._made, self._made_pool
+        self._abandon()
+        for i in made:
+            self._drop(self._seqs.pop(i), 0)
+        self._active = [i for i in self._active if i not in made]
+        if made_pool:
+            self.pool = None
 
     # ------------------------------------------------------------------ compressed storage
     def append_attend(self, layer_idx: int, key_compressor, val_compressor, k: torch.Tensor, v: torch.Tensor,
@@ -299,12 +312,16 @@ class TurboQuantPagedCache(Cache):
         self._check_codec(layer_idx, key_compressor, val_compressor)
         self._begin(layer_idx, k, bits)
         table, lengths = self._device_state
-        if fast:
-            parents = self.draft_parents
-            out = append_tree_attention(k, v, q, key_compressor, val_compressor, self.pool, layer_idx, table, lengths,
-                                        parents, scale, out_dtype)
-        else:
-            out = self._attend_prompt(layer_idx, key_compressor, val_compressor, k, v, q, table, lengths, scale, out_dtype)
+        try:
+            if fast:
+                out = append_tree_attention(k, v, q, key_compressor, val_compressor, self.pool, layer_idx, table, lengths,
+                                            self.draft_parents, scale, out_dtype)
+            else:
+                out = self._attend_prompt(layer_idx, key_compressor, val_compressor, k, v, q, table, lengths, scale, out_dtype)
+        except BaseException:
+            if not self._written:  # else the next forward finds a step that is not finished
+                self._undo()
+            raise
         self._finish(layer_idx)
         return out
 
@@ -317,6 +334,7 @@ class TurboQuantPagedCache(Cache):
             self._device_state = (table, lengths + self._step)  # stands until a page is added
             self._written.clear()
             self._step = 0
+            self._made, self._made_pool = [], False
 
     def _check_codec(self, layer_idx, key_compressor, val_compressor) -> None:
         if val_compressor.bits != key_compressor.mse_bits + 1:
@@ -338,26 +356,32 @@ class TurboQuantPagedCache(Cache):
                 raise ValueError(f"a batch of {B} for {len(self._active)} active sequences (cache.use)")
         if self.pool is None:
             self.pool = PagePool(self.num_pages, self.page_size, H, D, bits, self.num_layers, k.device)
+            self._made_pool = True
         pool = self.pool
         if (H, D, bits) != (pool.num_kv_heads, pool.head_dim, pool.bits) or k.device != pool.device:
             raise ValueError(f"the cache's pages hold {pool.num_kv_heads} heads of {pool.head_dim} at {pool.bits} bits on "
                              f"{pool.device}, got {H} of {D} at {bits} bits on {k.device}")
-        if not self._active and not self._seqs:
-            self._active = self.add(B)
         if layer_idx in self._written:
             done = len(self._written)
-            self._abandon()
             if done < self.num_layers:
+                self._undo()
                 raise RuntimeError(f"the forward before this one wrote {done} of the cache's {self.num_layers} layers; its "
                                    "tokens were dropped")
+            self._abandon()
         if self._written:
             if T != self._step:
                 raise ValueError(f"layer {layer_idx} appends {T} tokens in a step of {self._step}")
             return
-        parents = self.draft_parents
-        if parents is not None and tuple(parents.shape) not in ((T,), (B, T)):
-            raise ValueError(f"parents {tuple(parents.shape)} for {B} sequences of {T} drafted tokens")
-        self._reserve(T)
+        try:
+            if not self._active and not self._seqs:
+                self._active = self._made = self.add(B)
+            parents = self.draft_parents
+            if parents is not None and tuple(parents.shape) not in ((T,), (B, T)):
+                raise ValueError(f"parents {tuple(parents.shape)} for {B} sequences of {T} drafted tokens")
+            self._reserve(T)
+        except BaseException:
+            self._undo()
+            raise
         self._step = T
 
     def _reserve(self, T: int) -> None:
