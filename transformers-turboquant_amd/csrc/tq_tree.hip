@@ -318,10 +318,13 @@ __device__ __forceinline__ void tree_join(const TreeArgs& a, const float* mrg, i
 // parts, so that there are three passes of scores and one of values to a key and column.
 // P is rounded to f16 (relative 2^-11 of each weight, a hundredth of what the codes lose), sums and
 // maxima are f32.
-// 16 nodes, 16 sequences of 8k to 32k, 32/8 heads, 3 bits: 200 us for 0.17 TFLOP of matrix work, 0.86
-// PFLOP/s (a large library product reaches 1.16); of 451k cycles the matrix unit is busy in 164k, the
-// VALU in 217k, the LDS in 239k, over the two waves per SIMD that the registers of two tiles leave.  Measured against it and dropped: four tiles at one wave per SIMD (236 against 275 us in
-// all), three waves with spills (226 and 309), operands looked up a step ahead at two tiles (216 and 224).
+// 16 nodes, 16 sequences of 8k to 32k, 32/8 heads, 3 bits, 0.17 TFLOP of matrix work: 224 us for a call in a row of
+// calls, preparation and merge included (11 and 13 us in their trace), so at most 200 us and 0.86 PFLOP/s (a large
+// library product reaches 1.16); under a kernel trace, where the clock is lower, 237 us at least and 270 in the
+// median.  Of 462k cycles the matrix unit is busy in 164k, the VALU in 231k, the LDS in 239k, over the two waves
+// per SIMD that the registers of two tiles leave.  Measured against it and dropped: four tiles at one wave per
+// SIMD (236 against 275 us in all), three waves with spills (226 and 309), operands looked up a step ahead at
+// two tiles (216 and 224).
 //
 // The shared memory is one object, so that the lookup tables lie at LDS address 0: a lookup's byte
 // offset then is its address (elsewhere every lookup pays an addition, 86 of ~330 VALU instructions
@@ -757,9 +760,10 @@ tree_attn_kernel(TreeArgs a) {
 // against column lg: one exponential per (column, key) instead of one per key and column of a
 // 16-wide tile.  P reaches the operand of O^T += V^T P^T through a small LDS tile of the wave; column n
 // of O^T serves column n mod 4.
-// 16 sequences of 8k to 32k, 32/8 heads, 3 bits: 67 us for 267 MB, 4.0 TB/s (a copy reaches 4.9); of
-// 155k cycles the VALU issues in 75k and the LDS in 71k, 27k of them conflicts of the 64-entry value
-// table.  Two waves per SIMD: at three or four, registers spill in the set-up (77 against 75 and 84 us in
+// 16 sequences of 8k to 32k, 32/8 heads, 3 bits, 267 MB: 75 us under a kernel trace, 3.5 TB/s (a copy reaches
+// 4.9); a call in a row of calls takes 80 us with preparation and merge (6 us each in their trace), which leaves it
+// 68 us, 3.9 TB/s.  Of 151k cycles the VALU issues in 76k and the LDS in 71k, 27k of them conflicts of the 64-entry
+// value table.  Two waves per SIMD: at three or four, registers spill in the set-up (77 against 75 and 84 us in
 // all, one sequence of 32k 24 against 29 and 41).
 template <int D, int KB, int NW>
 struct TreePlaneSmem {
@@ -1185,6 +1189,7 @@ static TreePlan plan_tree(int B, int Hq, int Hkv, int T, int64_t maxpos, int d, 
   TreePlan p{};
   const int C = Hq / Hkv * T;
   const int64_t most = static_cast<int64_t>(B) * ((maxpos + 127) / 128);  // rounds, at most
+  // (Times below: attention and merge over prepared queries, calls in a row.)
   // Bit planes up to 4 columns: 16 x 32k, 32/8 heads 75.5 against 90 us with tables (2 bits 57 and 81, one
   // sequence of 4k 15.6 and 14.7); with two groups of 4 they lose (16/2 heads 41.8 and 37.2).
   // Two tiles share a slab's operands: 16 nodes of 16 x 32k 218 against 298 us.  While there are

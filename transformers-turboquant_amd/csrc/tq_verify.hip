@@ -20,7 +20,9 @@
 //
 // Measured: a chain of 5, V = 50257, one sequence 11.5 us (two launches of 4 us, each a few
 // dependent round trips); chains of 8, V = 128256, 64 sequences 19.1 us (66 MB, 14.0 us for the sums: 4.7
-// TB/s); trees of 32, V = 151936, 16 sequences in bf16 13.0 us (the walk over 32 nodes).
+// TB/s); trees of 32, V = 151936, 16 sequences in bf16 13.0 us (sums 8.6: 1.8 for the siblings' loop and 0.8 for
+// striking the rejected tokens from the row, by timing copies without them; 6.1 for three dependent round
+// trips, the walk and the row).
 #include "tq_common.h"
 
 namespace tq {
