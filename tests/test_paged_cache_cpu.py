@@ -538,6 +538,11 @@ def test_a_refused_first_forward_leaves_an_empty_cache():
     with pytest.raises(RuntimeError, match="wrote 1 of the cache's 2 layers"):
         cache._begin(0, torch.zeros(1, 2, 5, 64), 3)
     empty()
+    cache._begin(0, torch.zeros(1, 2, 5, 64), 3)
+    cache._finish(0)
+    with pytest.raises(RuntimeError, match="wrote 1 of the cache's 2 layers"):  # found by another batch
+        cache._begin(0, torch.zeros(2, 2, 5, 64), 3)
+    empty()
     cache.pool = FakePool(3, 32)
     step(cache, [[1], [2]])
     assert cache.lengths() == [1, 1] and cache.free_pages == 1

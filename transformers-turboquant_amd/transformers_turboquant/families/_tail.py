@@ -69,7 +69,8 @@ def attention_tail(module, q, k, v, attention_mask, output_attentions: bool = Fa
     if isinstance(cache, TurboQuantPagedCache):
         if not fused:
             raise ValueError("a paged cache serves GPU attention without attention weights or dropout (model.eval())")
-        check_window(getattr(module, "sliding_window", None), cache.get_seq_length(), T)
+        if getattr(module, "sliding_window", None) is not None:
+            check_window(module.sliding_window, cache.get_seq_length(), T)
         if attention_mask is not None:
             raise ValueError("a paged cache masks by itself and takes no attention mask: run prompts unpadded, under the "
                              "sdpa attention implementation")

@@ -351,6 +351,11 @@ class TurboQuantPagedCache(Cache):
         from turboquant_pytorch.pages import PagePool
 
         B, H, T, D = k.shape
+        done = len(self._written)
+        if layer_idx in self._written and done < self.num_layers:
+            self._undo()
+            raise RuntimeError(f"the forward before this one wrote {done} of the cache's {self.num_layers} layers; its "
+                               "tokens were dropped")
         if self._active or self._seqs:
             if B != len(self._active):
                 raise ValueError(f"a batch of {B} for {len(self._active)} active sequences (cache.use)")
@@ -361,12 +366,7 @@ class TurboQuantPagedCache(Cache):
         if (H, D, bits) != (pool.num_kv_heads, pool.head_dim, pool.bits) or k.device != pool.device:
             raise ValueError(f"the cache's pages hold {pool.num_kv_heads} heads of {pool.head_dim} at {pool.bits} bits on "
                              f"{pool.device}, got {H} of {D} at {bits} bits on {k.device}")
-        if layer_idx in self._written:
-            done = len(self._written)
-            if done < self.num_layers:
-                self._undo()
-                raise RuntimeError(f"the forward before this one wrote {done} of the cache's {self.num_layers} layers; its "
-                                   "tokens were dropped")
+        if layer_idx in self._written:  # a draft that was not accepted
             self._abandon()
         if self._written:
             if T != self._step:
