@@ -420,6 +420,29 @@ int tq_tree_attention(const uint16_t* q_rot, const float* q_proj, const uint8_t*
 int64_t tq_tree_workspace_size(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t table_width,
                                int32_t page_size, int32_t d, int32_t bits);
 
+/* tq_tree_attention of sequences that share their first positions.  groups [B, 2] (int32, on the
+ * device): sequences that follow one another with the same groups[b][0] >= 0 and the same
+ * groups[b][1] have positions [0, groups[b][1]) in common, the same rows; they are read through the
+ * table row of one of these sequences, once for all of them (up to the last multiple of 32 positions;
+ * a batch is cut at every 64th sequence).  A sequence with a negative groups[b][0] or without shared
+ * positions is attended alone; one that is shorter than its shared positions gets zeros.  Otherwise as
+ * tq_tree_attention, with a workspace of tq_prefix_workspace_size bytes. */
+int tq_prefix_attention(const uint16_t* q_rot, const float* q_proj, const uint8_t* key_codes,
+                        const uint8_t* key_signs, const uint16_t* key_rn, const uint16_t* key_vn,
+                        const uint16_t* key_centroids_f16, int32_t bits, const uint8_t* val_codes,
+                        const uint16_t* val_vn, const float* val_centroids,
+                        const uint16_t* val_pit_split, int64_t num_pages, int32_t page_size,
+                        const int32_t* block_table, int64_t ld_table, int32_t table_width,
+                        const int32_t* lengths, const int32_t* groups, const int32_t* parents,
+                        int64_t ld_parents, int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t d,
+                        float coeff, float scale, void* out, int32_t out_dtype, int64_t sob,
+                        int64_t soh, int64_t sos, void* workspace, int64_t workspace_bytes,
+                        void* stream);
+
+/* Workspace bytes of tq_prefix_attention on the current device (0: shape not taken). */
+int64_t tq_prefix_workspace_size(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t table_width,
+                                 int32_t page_size, int32_t d, int32_t bits);
+
 /* Verification of drafted tokens.  Node 0 of a sequence is the last emitted token, node i > 0 a
  * drafted child of parents[b * ld_parents + i] < i (NULL: i - 1); target_probs[b, c, :] (element
  * strides stb, stt, 1) is the target's distribution p_c after node c.

@@ -1,0 +1,426 @@
+// Attention of sequences that share a long prefix, over a paged compressed cache.
+//
+// As tree attention (tq_tree.hip), of B sequences with T drafted tokens each; but consecutive sequences may
+// have the same rows at their first positions: groups[b] = (id, shared), and sequences in a row with the same id and
+// the same shared have positions [0, shared) in common.  The softmax over a sequence's keys is that over its parts,
+// joined by their maxima and sums:
+//   m = max(m1, m2), l = l1 2^(m1 - m) + l2 2^(m2 - m), O = O1 2^(m1 - m) + O2 2^(m2 - m),
+// so the shared rows are read and decoded once for all queries of the group (rows x T x G columns of a kv
+// head), and each sequence's own rows for its T x G.
+//
+// The work is a list of segments: a group's shared keys against a tile of 16 NTP of its columns, a
+// sequence's own keys against a tile of 16 NTO of its own.  As in tree attention their rounds (32 keys per wave of
+// a block) are dealt in equal stretches to as many blocks per kv head as the device holds at
+// once, from the lengths and groups that stand on the device; each (block, segment) part leaves a
+// record, and the merge joins those of the sequence's own segment and of the group's.
+#include "tq_tree.h"
+
+namespace tq {
+
+struct PrefixArgs : TreeArgs {
+  const int32_t* groups;  // [B, 2]
+};
+
+// A group ends with a lane's step of 64 sequences (behind it the same group begins anew): every sequence is in one
+// group, whatever the entries are, and what a lane has to know of a group stands in its own wave.
+// The shared positions that are read together: whole slabs.  The rest of them is read with the own ones,
+// through each sequence's own table row.
+constexpr int kSlab = 32;
+
+// Segments and rounds, dealt to the blocks as by TreeSplit: one sequence per lane, 64 per step.
+// A sequence's segments are those of the group it is the first of (pt tiles of pr rounds), then its
+// own (ot tiles of rounds(keys - start)).  The parts of block k in segment s have record k + s: walking
+// along the rounds, every step to the next part moves to the next block, to a later segment or both.
+template <int RK, int WP, int WO>
+struct PrefixSplit {
+  struct Row {
+    int start, keys;   // own positions [start, keys), keys = 0: none
+    int pr, pt, cols;  // of the group it is the first of: rounds of a tile, tiles, columns
+    int first;         // of the sequence's group, -1 without one
+  };
+  Row r0;           // sequence `lane`
+  int upto0, seg0;  // sums of rounds and segments up to it
+  int ot;           // tiles of a sequence's own columns
+  int total, blocks, each, extra;
+
+  __device__ __forceinline__ static int rounds(int keys) { return static_cast<int>(static_cast<unsigned>(keys + RK - 1) / RK); }
+  __device__ __forceinline__ int own_rounds(const Row& r) const { return r.keys ? rounds(r.keys - r.start) : 0; }
+  __device__ __forceinline__ int row_rounds(const Row& r) const { return r.pr * r.pt + own_rounds(r) * ot; }
+  __device__ __forceinline__ int row_segments(const Row& r) const { return r.pt + ot; }
+
+  // sequence b0 + lane, by all lanes of a wave
+  __device__ __forceinline__ static Row load(const PrefixArgs& a, int b0) {
+    const int lane = threadIdx.x & 63, b = b0 + lane;
+    int n = -1, id = -1, shared = 0;
+    if (b < a.B) {
+      n = a.lengths[b];
+      id = a.groups[static_cast<int64_t>(b) * 2];
+      shared = a.groups[static_cast<int64_t>(b) * 2 + 1];
+    }
+    const bool grouped = id >= 0 && shared >= kSlab && shared <= a.maxpos;
+    const int id1 = __shfl_up(id, 1, 64), shared1 = __shfl_up(shared, 1, 64);
+    const bool on = grouped && lane > 0 && id1 == id && shared1 == shared;  // goes on with the group before it
+    const uint64_t heads = __ballot(grouped && !on), ons = __ballot(on);
+    Row r{0, 0, 0, 0, 0, -1};
+    if (grouped) {
+      r.first = b0 + 63 - __builtin_clzll(heads & (~0ull >> (63 - lane)));
+      r.start = shared & ~(kSlab - 1);
+      if (!on) {
+        const uint64_t behind = lane < 63 ? ons >> (lane + 1) : 0;
+        r.cols = (1 + __builtin_ctzll(~behind)) * a.C;
+        r.pt = (r.cols + WP - 1) / WP;
+        r.pr = rounds(r.start);
+      }
+    }
+    const int least = id >= 0 && shared > 0 ? shared : 0;
+    r.keys = n >= least && n <= a.maxpos - a.T ? n + a.T : 0;
+    return r;
+  }
+  __device__ __forceinline__ PrefixSplit(const PrefixArgs& a, const Row& r) : r0(r) {
+    ot = (a.C + WO - 1) / WO;
+    upto0 = scan64(row_rounds(r0));
+    seg0 = scan64(row_segments(r0));
+    total = __builtin_amdgcn_readlane(upto0, 63);
+    for (int b0 = 64; b0 < a.B; b0 += 64)
+      total += __builtin_amdgcn_readlane(scan64(row_rounds(load(a, b0))), 63);
+    blocks = min(a.slots, static_cast<int>((static_cast<unsigned>(total) + (1u << a.lg_least) - 1) >> a.lg_least));
+    each = blocks ? static_cast<unsigned>(total) / static_cast<unsigned>(blocks) : 0;
+    extra = total - each * blocks;
+  }
+  __device__ __forceinline__ int begin(int k) const { return k * each + min(k, extra); }
+  __device__ __forceinline__ int block_of(int round) const {
+    const unsigned big = extra * (each + 1), x = round;
+    return x < big ? x / static_cast<unsigned>(each + 1) : extra + (x - big) / static_cast<unsigned>(each);
+  }
+  // a sequence as all lanes see it: its first round and segment, and its row
+  struct At {
+    int first, segment;
+    Row r;
+  };
+  __device__ __forceinline__ At pick(const Row& r, int upto, int seg, int l) const {
+    At at;
+    at.r.start = __builtin_amdgcn_readlane(r.start, l);
+    at.r.keys = __builtin_amdgcn_readlane(r.keys, l);
+    at.r.pr = __builtin_amdgcn_readlane(r.pr, l);
+    at.r.pt = __builtin_amdgcn_readlane(r.pt, l);
+    at.r.cols = __builtin_amdgcn_readlane(r.cols, l);
+    at.r.first = __builtin_amdgcn_readlane(r.first, l);
+    at.first = __builtin_amdgcn_readlane(upto, l) - row_rounds(at.r);
+    at.segment = __builtin_amdgcn_readlane(seg, l) - row_segments(at.r);
+    return at;
+  }
+  // the sequence of round x < total
+  __device__ __forceinline__ At sequence_at(const PrefixArgs& a, int x, int& b) const {
+    Row r = r0;
+    int upto = upto0, seg = seg0;
+    for (int b0 = 0;; b0 += 64) {
+      const uint64_t m = __ballot(x < upto);
+      if (m) {
+        const int l = __builtin_ctzll(m);
+        b = b0 + l;
+        return pick(r, upto, seg, l);
+      }
+      next(a, b0 + 64, r, upto, seg);
+    }
+  }
+  __device__ __forceinline__ At sequence(const PrefixArgs& a, int b) const {
+    Row r = r0;
+    int upto = upto0, seg = seg0, b0 = 0;
+    for (; b >= b0 + 64; b0 += 64) next(a, b0 + 64, r, upto, seg);
+    return pick(r, upto, seg, b - b0);
+  }
+
+ private:
+  __device__ __forceinline__ void next(const PrefixArgs& a, int b0, Row& r, int& upto, int& seg) const {
+    const int run = __builtin_amdgcn_readlane(upto, 63), runs = __builtin_amdgcn_readlane(seg, 63);
+    r = load(a, b0);
+    upto = scan64(row_rounds(r)) + run;
+    seg = scan64(row_segments(r)) + runs;
+  }
+};
+
+// ---------------------------------------------------------------- attention
+// NTP and NTO tiles of 16 columns to a segment of shared and of own keys (NTO <= NTP).  Records have 16 NTP columns.
+template <int D, int BITS, int NTP, int NW>
+struct PrefixSmem : TreeSmem<D, BITS, NTP, NW> {
+  float fs[16 * NTP];
+};
+
+template <int D, int BITS, int NTP, int NTO, int NW>
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)))
+prefix_attn_kernel(PrefixArgs a) {
+  constexpr int RK = 32 * NW, WP = 16 * NTP, WO = 16 * NTO;
+  using Split = PrefixSplit<RK, WP, WO>;
+  __shared__ __attribute__((aligned(16))) PrefixSmem<D, BITS, NTP, NW> sm;
+  const int tid = threadIdx.x, hkv = blockIdx.y;
+  const TreeTables<BITS> tables(a, tid);
+  const Split split(a, Split::load(a, 0));
+  if (static_cast<int>(blockIdx.x) >= split.blocks) return;  // block-uniform
+  int x = split.begin(blockIdx.x);
+  const int x_end = split.begin(blockIdx.x + 1);
+  tables.keys(sm.luts, tid);
+  tables.values(sm.luts, tid);
+  while (x < x_end) {
+    int b;
+    const typename Split::At at = split.sequence_at(a, x, b);
+    const int before = at.r.pr * at.r.pt;  // rounds of the shared keys' tiles, in front of the own ones'
+    const bool own = x - at.first >= before;
+    const int each = own ? split.own_rounds(at.r) : at.r.pr, from = at.first + (own ? before : 0);
+    const int tile = static_cast<int>(static_cast<unsigned>(x - from) / static_cast<unsigned>(each));
+    const int r0 = x - from - tile * each, r1 = min(r0 + x_end - x, each);
+    const int64_t rec = ((static_cast<int64_t>(blockIdx.x) + at.segment + tile + (own ? at.r.pt : 0)) * a.Hkv + hkv) * WP;
+    x += r1 - r0;
+    if (own) {
+      const TreePart part{b, a.C, tile * WO, at.r.keys - a.T, at.r.start + r0 * RK, min(at.r.keys, at.r.start + r1 * RK), rec};
+      tree_part<D, BITS, NTO, NW, false>(a, part, hkv, sm);
+    } else {
+      const int end = min(at.r.start, r1 * RK);
+      const TreePart part{b, at.r.cols, tile * WP, end, r0 * RK, end, rec};
+      tree_part<D, BITS, NTP, NW, true>(a, part, hkv, sm);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- merge
+// One block per (sequence, kv head, 4 CW columns), as tree_merge_kernel: a column's records are those of its
+// tile of the group's shared keys, then those of its tile of the own ones.
+template <int D, int RK, int WP, int WO, int CW>
+__global__ void __launch_bounds__(256) prefix_merge_kernel(PrefixArgs a) {
+  using Split = PrefixSplit<RK, WP, WO>;
+  using Finish = TreeFinish<D, CW>;
+  using floatPL = typename Finish::floatPL;
+  constexpr int PL = Finish::PL, NC = Finish::NC, NB = 16 / CW;
+  __shared__ typename Finish::Smem sm;
+  const int c0 = blockIdx.x * NC, hkv = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const int lane = tid & 63, wave = tid >> 6;
+
+  const typename Split::Row r0 = Split::load(a, 0);  // before Pi_v: waited for first
+  const Finish finish(a);
+  const Split split(a, r0);
+  const typename Split::At own = split.sequence(a, b);
+  const typename Split::At head = own.r.first >= 0 && own.r.first != b ? split.sequence(a, own.r.first) : own;
+  const int64_t step = static_cast<int64_t>(a.Hkv) * WP;  // columns between records
+#pragma unroll
+  for (int k = 0; k < CW; ++k) {
+    const int cc = wave + 4 * k, c = c0 + cc;
+    floatPL o = floatPL{};
+    if (c < a.C && own.r.keys) {
+      // columns of the first record of both lists, and how many records they have
+      int64_t at1 = 0, at2;
+      int n1 = 0, n2;
+      const auto records = [&](int first, int rounds, int segment, int col, int64_t& at) {
+        const int k0 = split.block_of(first), k1 = split.block_of(first + rounds - 1);
+        at = ((static_cast<int64_t>(k0) + segment) * a.Hkv + hkv) * WP + col;
+        return k1 - k0 + 1;
+      };
+      if (own.r.first >= 0) {
+        const int pc = (b - own.r.first) * a.C + c, tile = pc / WP;
+        n1 = records(head.first + tile * head.r.pr, head.r.pr, head.segment + tile, pc - tile * WP, at1);
+      }
+      {
+        const int tile = c / WO, rounds = split.own_rounds(own.r);
+        n2 = records(own.first + own.r.pr * own.r.pt + tile * rounds, rounds, own.segment + own.r.pt + tile, c - tile * WO, at2);
+      }
+      const int n = n1 + n2;
+      const auto column = [&](int q) { return q < n1 ? at1 + q * step : at2 + (q - n1) * step; };
+      float mx = -INFINITY;
+      for (int r = lane; r < n; r += 64) mx = fmaxf(mx, a.part_ml[column(r) * 2]);
+#pragma unroll
+      for (int sh = 32; sh >= 1; sh >>= 1) mx = fmaxf(mx, __shfl_xor(mx, sh, 64));
+      float lsum = 0.f;
+      for (int q0 = 0; q0 < n; q0 += 64) {
+        float w = 0.f;
+        if (q0 + lane < n) {
+          const float* const ml = a.part_ml + column(q0 + lane) * 2;
+          const float m = ml[0];
+          if (m != -INFINITY) {
+            w = __builtin_amdgcn_exp2f(m - mx);
+            lsum += w * ml[1];
+          }
+        }
+        const int nb = min(64, n - q0);
+        for (int u = 0; u < nb; u += NB) {
+          floatPL v[NB];
+#pragma unroll
+          for (int q = 0; q < NB; ++q)
+            v[q] = u + q < nb ? *reinterpret_cast<const floatPL*>(a.part_o + column(q0 + u + q) * D + PL * lane) : floatPL{};
+#pragma unroll
+          for (int q = 0; q < NB; ++q) {
+            const float ww = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), (u + q) & 63));
+#pragma unroll
+            for (int e = 0; e < PL; ++e) o[e] = fmaf(ww, v[q][e], o[e]);
+          }
+        }
+      }
+#pragma unroll
+      for (int sh = 32; sh >= 1; sh >>= 1) lsum += __shfl_xor(lsum, sh, 64);
+      o *= lsum == 0.f ? 0.f : 1.f / lsum;
+    }
+    Finish::put(sm, cc, o);
+  }
+  __syncthreads();
+  finish.store(a, sm, b, hkv, c0);
+}
+
+// ---------------------------------------------------------------- launch
+using PrefixKernel = void (*)(PrefixArgs);
+
+struct PrefixPlan {
+  PrefixKernel attend;
+  int tiles, own_tiles;  // NTP, NTO
+  int slots, lg_least;
+  int64_t records, bytes;
+};
+
+template <int D, int BITS>
+static PrefixKernel prefix_kernel(int tiles, int own_tiles) {
+  if (tiles == 1) return &prefix_attn_kernel<D, BITS, 1, 1, 4>;
+  return own_tiles == 1 ? &prefix_attn_kernel<D, BITS, 2, 1, 4> : &prefix_attn_kernel<D, BITS, 2, 2, 4>;
+}
+static PrefixKernel prefix_kernel(int d, int bits, int tiles, int own_tiles) {
+  if (d == 64)
+    return bits == 2 ? prefix_kernel<64, 2>(tiles, own_tiles) : bits == 3 ? prefix_kernel<64, 3>(tiles, own_tiles)
+                                                                          : prefix_kernel<64, 4>(tiles, own_tiles);
+  return bits == 2 ? prefix_kernel<128, 2>(tiles, own_tiles) : bits == 3 ? prefix_kernel<128, 3>(tiles, own_tiles)
+                                                                         : prefix_kernel<128, 4>(tiles, own_tiles);
+}
+
+static PrefixPlan plan_prefix(int B, int Hq, int Hkv, int T, int64_t maxpos, int d, int bits) {
+  static int resident[2][3][3][16] = {};  // per kernel, per device
+  PrefixPlan p{};
+  const int C = Hq / Hkv * T;
+  p.tiles = static_cast<int64_t>(B) * C > 16 ? 2 : 1;
+  p.own_tiles = C > 16 ? 2 : 1;
+  p.attend = prefix_kernel(d, bits, p.tiles, p.own_tiles);
+  const int res = resident_blocks(reinterpret_cast<const void*>(p.attend), 256,
+                                  resident[d == 128][bits - 2][p.tiles + p.own_tiles - 2]);
+  p.slots = res / Hkv > 1 ? res / Hkv : 1;
+  p.lg_least = p.tiles == 2 ? 1 : 0;
+  // a sequence's own tiles, and as many of its group's at most
+  const int own = (C + 16 * p.own_tiles - 1) / (16 * p.own_tiles);
+  const int64_t segments = 2 * static_cast<int64_t>(B) * own;
+  const int64_t most = segments * ((maxpos + 127) / 128);  // rounds
+  if (p.slots > most) p.slots = static_cast<int>(most);
+  p.records = p.slots + segments;
+  p.bytes = p.records * Hkv * (16 * p.tiles) * static_cast<int64_t>(d + 2) * 4;
+  return p;
+}
+
+static bool prefix_shape(int B, int Hq, int Hkv, int T, int64_t maxpos, int d, int bits) {
+  return B >= 1 && B <= 65535 && Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 && Hkv <= 65535 && T >= 1 && T <= 64 && maxpos >= T &&
+         maxpos <= (int64_t(1) << 24) && (d == 64 || d == 128) && bits >= 2 && bits <= 4 &&
+         2 * static_cast<int64_t>(B) * ((static_cast<int64_t>(Hq / Hkv) * T + 15) / 16) * ((maxpos + 127) / 128) < (int64_t(1) << 31);
+}
+
+template <int D, int WP, int WO>
+static void launch_prefix_merge(const PrefixArgs& a, hipStream_t s) {
+  // as tree attention's merge: the widest blocks that still are two to a compute unit (16 columns) or one (8)
+  const auto blocks = [&](int columns) { return static_cast<int64_t>((a.C + columns - 1) / columns) * a.Hkv * a.B; };
+  const auto grid = [&](int columns) { return dim3((a.C + columns - 1) / columns, a.Hkv, a.B); };
+  if (blocks(16) >= 512) prefix_merge_kernel<D, 128, WP, WO, 4><<<grid(16), 256, 0, s>>>(a);
+  else if (blocks(8) >= 256) prefix_merge_kernel<D, 128, WP, WO, 2><<<grid(8), 256, 0, s>>>(a);
+  else prefix_merge_kernel<D, 128, WP, WO, 1><<<grid(4), 256, 0, s>>>(a);
+}
+
+template <int D>
+static void launch_prefix(const PrefixArgs& a, const PrefixPlan& p, hipStream_t s) {
+  p.attend<<<dim3(p.slots, a.Hkv), 256, 0, s>>>(a);
+  if (p.tiles == 1) launch_prefix_merge<D, 16, 16>(a, s);
+  else if (p.own_tiles == 1) launch_prefix_merge<D, 32, 16>(a, s);
+  else launch_prefix_merge<D, 32, 32>(a, s);
+}
+
+}  // namespace tq
+
+using namespace tq;
+
+extern "C" {
+
+int64_t tq_prefix_workspace_size(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t table_width, int32_t page_size,
+                                 int32_t d, int32_t bits) {
+  const int64_t maxpos = static_cast<int64_t>(table_width) * page_size;
+  return prefix_shape(B, Hq, Hkv, T, maxpos, d, bits) ? plan_prefix(B, Hq, Hkv, T, maxpos, d, bits).bytes : 0;
+}
+
+int tq_prefix_attention(const uint16_t* q_rot, const float* q_proj, const uint8_t* key_codes, const uint8_t* key_signs,
+                        const uint16_t* key_rn, const uint16_t* key_vn, const uint16_t* key_centroids_f16, int32_t bits,
+                        const uint8_t* val_codes, const uint16_t* val_vn, const float* val_centroids,
+                        const uint16_t* val_pit_split, int64_t num_pages, int32_t page_size, const int32_t* block_table,
+                        int64_t ld_table, int32_t table_width, const int32_t* lengths, const int32_t* groups,
+                        const int32_t* parents, int64_t ld_parents, int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t d,
+                        float coeff, float scale, void* out, int32_t out_dtype, int64_t sob, int64_t soh, int64_t sos,
+                        void* workspace, int64_t workspace_bytes, void* stream) {
+  if (d != 64 && d != 128) {
+    set_error("tq_prefix_attention: head_dim %d not supported (64 or 128)", d);
+    return TQ_EUNSUPPORTED;
+  }
+  if (bits < 2 || bits > 4) {
+    set_error("tq_prefix_attention: bits %d not supported (2 to 4)", bits);
+    return TQ_EUNSUPPORTED;
+  }
+  TQ_REQUIRE(B >= 0 && Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 && T >= 1, "tq_prefix_attention: bad shape");
+  TQ_REQUIRE(T <= 64, "tq_prefix_attention: at most 64 drafted tokens, got %d", T);
+  TQ_REQUIRE(page_size >= 32 && page_size <= (1 << 20) && (page_size & (page_size - 1)) == 0,
+             "tq_prefix_attention: page_size must be a power of two from 32 to 2^20, got %d", page_size);
+  TQ_REQUIRE(num_pages >= 1 && num_pages < (int64_t(1) << 31) && ld_table >= table_width, "tq_prefix_attention: bad pool");
+  const int64_t maxpos = static_cast<int64_t>(table_width) * page_size;
+  TQ_REQUIRE(maxpos >= T, "tq_prefix_attention: a table of %d pages of %d does not hold %d drafted tokens", table_width, page_size, T);
+  TQ_REQUIRE(out_dtype == TQ_F32 || out_dtype == TQ_F16 || out_dtype == TQ_BF16, "tq_prefix_attention: unknown dtype %d", out_dtype);
+  if (B == 0) return TQ_OK;
+  TQ_REQUIRE(prefix_shape(B, Hq, Hkv, T, maxpos, d, bits),
+             "tq_prefix_attention: at most 65535 sequences and kv heads, 2^24 positions a sequence and 2^31 (128 keys, 16 "
+             "columns) blocks of work, got %d, %d and %lld", B, Hkv, (long long)maxpos);
+  TQ_REQUIRE(q_rot && q_proj && key_codes && key_signs && key_rn && key_vn && key_centroids_f16 && val_codes && val_vn &&
+                 val_centroids && val_pit_split && block_table && lengths && groups && out,
+             "tq_prefix_attention: null pointer");
+  for (const void* p : {static_cast<const void*>(q_rot), static_cast<const void*>(q_proj), static_cast<const void*>(key_codes),
+                        static_cast<const void*>(key_signs), static_cast<const void*>(val_codes), static_cast<const void*>(val_pit_split)})
+    TQ_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, "tq_prefix_attention: queries, code planes and Pi_v must be 16-byte aligned");
+  const PrefixPlan p = plan_prefix(B, Hq, Hkv, T, maxpos, d, bits);
+  TQ_REQUIRE(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= p.bytes,
+             "tq_prefix_attention: the workspace must be 16-byte aligned and hold %lld bytes", (long long)p.bytes);
+  PrefixArgs a{};
+  a.q_rot = q_rot;
+  a.q_proj = q_proj;
+  a.kcodes = key_codes;
+  a.ksigns = key_signs;
+  a.krn = key_rn;
+  a.kvn = key_vn;
+  a.kcent = key_centroids_f16;
+  a.vcodes = val_codes;
+  a.vvn = val_vn;
+  a.vcent = val_centroids;
+  a.table = block_table;
+  a.ld_table = ld_table;
+  a.lengths = lengths;
+  a.groups = groups;
+  a.parents = parents;
+  a.ld_parents = ld_parents;
+  a.num_pages = num_pages;
+  a.lg_page = __builtin_ctz(static_cast<unsigned>(page_size));
+  a.maxpos = static_cast<int>(maxpos);
+  a.B = B;
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.T = T;
+  a.G = Hq / Hkv;
+  a.C = a.G * T;
+  a.slots = p.slots;
+  a.lg_least = p.lg_least;
+  a.coeff = coeff;
+  a.scale = scale;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.part_o + p.records * Hkv * (16 * p.tiles) * d;
+  a.vpit = val_pit_split;
+  a.out = out;
+  a.out_dtype = out_dtype;
+  a.sob = sob;
+  a.soh = soh;
+  a.sos = sos;
+  hipStream_t s = as_stream(stream);
+  if (d == 64) launch_prefix<64>(a, p, s);
+  else launch_prefix<128>(a, p, s);
+  return launch_status("tq_prefix_attention");
+}
+
+}  // extern "C"

@@ -1018,17 +1018,38 @@ Tensor tree_attention_meta(const Tensor& q_rot, const Tensor& q_proj, const Tens
   return check_tree(c, q_rot, pool, kcent16, bits, vcent32, vpit, table, lengths, parents, out_dtype);
 }
 
-int64_t tree_workspace(const Tensor& q, const Tensor& kvn, const Tensor& table, int64_t bits) {
-  return tq_tree_workspace_size(i32(q.size(0)), i32(q.size(1)), i32(kvn.size(1)), i32(q.size(2)), i32(table.size(1)),
-                                i32(kvn.size(2)), i32(q.size(3)), i32(bits));
+// groups: of sequences that share their first positions (null: tree attention of each sequence alone)
+int64_t tree_workspace(const Tensor& q, const Tensor& kvn, const Tensor& table, int64_t bits, const Tensor* groups = nullptr) {
+  return (groups ? tq_prefix_workspace_size : tq_tree_workspace_size)(i32(q.size(0)), i32(q.size(1)), i32(kvn.size(1)),
+                                                                      i32(q.size(2)), i32(table.size(1)), i32(kvn.size(2)),
+                                                                      i32(q.size(3)), i32(bits));
+}
+// columns: of a kv head and sequence; positions: that a table row holds
+void check_groups(const Checker& c, const Tensor* groups, int64_t B, int64_t columns, int64_t positions) {
+  if (!groups) return;
+  check_index(c, *groups, "groups", {B, 2});
+  TORCH_CHECK(2 * B * ((columns + 15) / 16) * ((positions + 127) / 128) < (int64_t{1} << 31), c.op, ": ", B, " sequences of ",
+              columns, " query columns per kv head over tables of ", positions, " positions are more than 2^31 blocks of work");
 }
 // out [B, T, Hq, D]; arguments checked
 void tree_launch(const uint16_t* q_rot, const float* q_proj, const Tensor& kcodes, const Tensor& ksigns, const Tensor& krn,
                  const Tensor& kvn, const Tensor& kcent16, int64_t bits, const Tensor& vcodes, const Tensor& vvn,
                  const Tensor& vcent32, const Tensor& vpit, const Tensor& table, const Tensor& lengths,
-                 const c10::optional<Tensor>& parents, double coeff, double scale, const Tensor& out, void* ws, int64_t bytes) {
+                 const c10::optional<Tensor>& parents, double coeff, double scale, const Tensor& out, void* ws, int64_t bytes,
+                 const Tensor* groups = nullptr) {
   const int32_t B = i32(out.size(0)), T = i32(out.size(1)), Hq = i32(out.size(2)), D = i32(out.size(3)), W = i32(table.size(1));
   const bool tree = parents.has_value() && parents->defined();
+  if (groups) {
+    check_status(tq_prefix_attention(
+                     q_rot, q_proj, ptr<uint8_t>(kcodes), ptr<uint8_t>(ksigns), ptr<uint16_t>(krn), ptr<uint16_t>(kvn),
+                     ptr<uint16_t>(kcent16), i32(bits), ptr<uint8_t>(vcodes), ptr<uint16_t>(vvn), ptr<float>(vcent32),
+                     ptr<uint16_t>(vpit), kvn.size(0), i32(kvn.size(2)), ptr<int32_t>(table), W, W, ptr<int32_t>(lengths),
+                     ptr<int32_t>(*groups), tree ? ptr<int32_t>(*parents) : nullptr, tree && parents->dim() == 2 ? T : 0, B, Hq,
+                     i32(kvn.size(1)), T, D, static_cast<float>(coeff), static_cast<float>(scale), out.data_ptr(),
+                     dtype_code(out.scalar_type()), out.stride(0), out.stride(2), out.stride(1), ws, bytes, stream_of(out)),
+                 "prefix_attention");
+    return;
+  }
   check_status(tq_tree_attention(q_rot, q_proj, ptr<uint8_t>(kcodes), ptr<uint8_t>(ksigns), ptr<uint16_t>(krn),
                                  ptr<uint16_t>(kvn), ptr<uint16_t>(kcent16), i32(bits), ptr<uint8_t>(vcodes),
                                  ptr<uint16_t>(vvn), ptr<float>(vcent32), ptr<uint16_t>(vpit), kvn.size(0), i32(kvn.size(2)),
@@ -1054,30 +1075,32 @@ Tensor tree_attention(const Tensor& q_rot, const Tensor& q_proj, const Tensor& k
   return out;
 }
 
-Tensor tree_attend_meta(const Tensor& q, const Tensor& pi_split, const Tensor& s_eff16, const Tensor& kcodes,
-                        const Tensor& ksigns, const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits,
-                        const Tensor& vcodes, const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit,
-                        const Tensor& table, const Tensor& lengths, const c10::optional<Tensor>& parents, double coeff,
-                        double scale, at::ScalarType out_dtype) {
-  const Checker c{"tq::tree_attend", q.device()};
+// Raw queries, over sequences alone or (groups) with what they share.
+Tensor attend_pages_meta(const char* op, const Tensor& q, const Tensor& pi_split, const Tensor& s_eff16, const Tensor& kcodes,
+                         const Tensor& ksigns, const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits,
+                         const Tensor& vcodes, const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit,
+                         const Tensor& table, const Tensor& lengths, const Tensor* groups,
+                         const c10::optional<Tensor>& parents, at::ScalarType out_dtype) {
+  const Checker c{op, q.device()};
   Pool pool{&kcodes, &ksigns, &krn, &kvn, &vcodes, &vvn};
   Tensor out = check_tree(c, q, pool, kcent16, bits, vcent32, vpit, table, lengths, parents, out_dtype);
+  check_groups(c, groups, q.size(0), q.size(1) / pool.H * q.size(2), table.size(1) * pool.P);
   c.table(pi_split, "split Pi", at::kHalf, 2 * q.size(3) * q.size(3));
   c.table(s_eff16, "f16 S_eff", at::kHalf, q.size(3) * q.size(3));
   return out;
 }
 
-Tensor tree_attend(const Tensor& q_in, const Tensor& pi_split, const Tensor& s_eff16, const Tensor& kcodes,
-                   const Tensor& ksigns, const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits,
-                   const Tensor& vcodes, const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit, const Tensor& table,
-                   const Tensor& lengths, const c10::optional<Tensor>& parents, double coeff, double scale,
-                   at::ScalarType out_dtype) {
-  Tensor out = tree_attend_meta(q_in, pi_split, s_eff16, kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn, vcent32, vpit,
-                                table, lengths, parents, coeff, scale, out_dtype);
+Tensor attend_pages(const char* op, const Tensor& q_in, const Tensor& pi_split, const Tensor& s_eff16, const Tensor& kcodes,
+                    const Tensor& ksigns, const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits,
+                    const Tensor& vcodes, const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit, const Tensor& table,
+                    const Tensor& lengths, const Tensor* groups, const c10::optional<Tensor>& parents, double coeff,
+                    double scale, at::ScalarType out_dtype) {
+  Tensor out = attend_pages_meta(op, q_in, pi_split, s_eff16, kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn, vcent32,
+                                 vpit, table, lengths, groups, parents, out_dtype);
   const c10::DeviceGuard g(q_in.device());
   Tensor q = activation(q_in);
   // one allocation: the workspace, then the prepared queries
-  const int64_t bytes = (tree_workspace(q, kvn, table, bits) + 15) / 16 * 16, n = q.numel();
+  const int64_t bytes = (tree_workspace(q, kvn, table, bits, groups) + 15) / 16 * 16, n = q.numel();
   Tensor ws = at::empty({bytes + n * 6}, q.options().dtype(at::kByte));
   uint8_t* const base = ptr<uint8_t>(ws);
   float* const q_proj = reinterpret_cast<float*>(base + bytes);
@@ -1085,23 +1108,60 @@ Tensor tree_attend(const Tensor& q_in, const Tensor& pi_split, const Tensor& s_e
   check_status(tq_query_prep(q.data_ptr(), dtype_code(q.scalar_type()), i32(q.size(0)), i32(q.size(1)), i32(q.size(2)),
                              i32(q.size(3)), q.stride(0), q.stride(1), q.stride(2), ptr<uint16_t>(pi_split),
                              ptr<uint16_t>(s_eff16), q_rot, q_proj, stream_of(q)),
-               "tree_attention");
+               groups ? "prefix_attention" : "tree_attention");
   tree_launch(q_rot, q_proj, kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn, vcent32, vpit, table, lengths, parents, coeff,
-              scale, out, base, bytes);
+              scale, out, base, bytes, groups);
   return out;
+}
+
+Tensor tree_attend_meta(const Tensor& q, const Tensor& pi_split, const Tensor& s_eff16, const Tensor& kcodes,
+                        const Tensor& ksigns, const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits,
+                        const Tensor& vcodes, const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit,
+                        const Tensor& table, const Tensor& lengths, const c10::optional<Tensor>& parents, double coeff,
+                        double scale, at::ScalarType out_dtype) {
+  return attend_pages_meta("tq::tree_attend", q, pi_split, s_eff16, kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn,
+                           vcent32, vpit, table, lengths, nullptr, parents, out_dtype);
+}
+
+Tensor tree_attend(const Tensor& q, const Tensor& pi_split, const Tensor& s_eff16, const Tensor& kcodes,
+                   const Tensor& ksigns, const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits,
+                   const Tensor& vcodes, const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit, const Tensor& table,
+                   const Tensor& lengths, const c10::optional<Tensor>& parents, double coeff, double scale,
+                   at::ScalarType out_dtype) {
+  return attend_pages("tq::tree_attend", q, pi_split, s_eff16, kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn, vcent32,
+                      vpit, table, lengths, nullptr, parents, coeff, scale, out_dtype);
+}
+
+Tensor prefix_attend_meta(const Tensor& q, const Tensor& pi_split, const Tensor& s_eff16, const Tensor& kcodes,
+                          const Tensor& ksigns, const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits,
+                          const Tensor& vcodes, const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit,
+                          const Tensor& table, const Tensor& lengths, const Tensor& groups,
+                          const c10::optional<Tensor>& parents, double coeff, double scale, at::ScalarType out_dtype) {
+  return attend_pages_meta("tq::prefix_attend", q, pi_split, s_eff16, kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn,
+                           vcent32, vpit, table, lengths, &groups, parents, out_dtype);
+}
+
+Tensor prefix_attend(const Tensor& q, const Tensor& pi_split, const Tensor& s_eff16, const Tensor& kcodes,
+                     const Tensor& ksigns, const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits,
+                     const Tensor& vcodes, const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit, const Tensor& table,
+                     const Tensor& lengths, const Tensor& groups, const c10::optional<Tensor>& parents, double coeff,
+                     double scale, at::ScalarType out_dtype) {
+  return attend_pages("tq::prefix_attend", q, pi_split, s_eff16, kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn, vcent32,
+                      vpit, table, lengths, &groups, parents, coeff, scale, out_dtype);
 }
 
 // A layer's decoding or speculation step in one call: the new tokens' keys and values compressed into
 // their pages (positions lengths[b] + i) and the queries prepared in one launch, then tree attention.
-Tensor page_attend_meta(const Tensor& k, const Tensor& v, const Tensor& q, const Tensor& kpi, const Tensor& kseff,
+Tensor append_attend_meta(const char* op, const Tensor& k, const Tensor& v, const Tensor& q, const Tensor& kpi, const Tensor& kseff,
                         const Tensor& kcent, const Tensor& kbounds, const Tensor& vpi, const Tensor& vbounds,
                         const Tensor& kseff16, const Tensor& kcodes, const Tensor& ksigns, const Tensor& krn,
                         const Tensor& kvn, const Tensor& kcent16, int64_t bits, const Tensor& vcodes, const Tensor& vvn,
                         const Tensor& vcent32, const Tensor& vpit, const Tensor& table, const Tensor& lengths,
-                        const c10::optional<Tensor>& parents, double coeff, double scale, at::ScalarType out_dtype) {
-  const Checker c{"tq::page_attend", q.device()};
+                          const Tensor* groups, const c10::optional<Tensor>& parents, at::ScalarType out_dtype) {
+  const Checker c{op, q.device()};
   Pool pool{&kcodes, &ksigns, &krn, &kvn, &vcodes, &vvn};
   Tensor out = check_tree(c, q, pool, kcent16, bits, vcent32, vpit, table, lengths, parents, out_dtype);
+  check_groups(c, groups, q.size(0), q.size(1) / pool.H * q.size(2), table.size(1) * pool.P);
   const int64_t D = q.size(3);
   TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(1) == pool.H &&
                   k.size(2) == q.size(2) && k.size(3) == D,
@@ -1119,14 +1179,14 @@ Tensor page_attend_meta(const Tensor& k, const Tensor& v, const Tensor& q, const
   return out;
 }
 
-Tensor page_attend(const Tensor& k_in, const Tensor& v_in, const Tensor& q_in, const Tensor& kpi, const Tensor& kseff,
+Tensor append_attend(const char* op, const Tensor& k_in, const Tensor& v_in, const Tensor& q_in, const Tensor& kpi, const Tensor& kseff,
                    const Tensor& kcent, const Tensor& kbounds, const Tensor& vpi, const Tensor& vbounds,
                    const Tensor& kseff16, const Tensor& kcodes, const Tensor& ksigns, const Tensor& krn, const Tensor& kvn,
                    const Tensor& kcent16, int64_t bits, const Tensor& vcodes, const Tensor& vvn, const Tensor& vcent32,
-                   const Tensor& vpit, const Tensor& table, const Tensor& lengths, const c10::optional<Tensor>& parents,
-                   double coeff, double scale, at::ScalarType out_dtype) {
-  Tensor out = page_attend_meta(k_in, v_in, q_in, kpi, kseff, kcent, kbounds, vpi, vbounds, kseff16, kcodes, ksigns, krn, kvn,
-                                kcent16, bits, vcodes, vvn, vcent32, vpit, table, lengths, parents, coeff, scale, out_dtype);
+                   const Tensor& vpit, const Tensor& table, const Tensor& lengths, const Tensor* groups,
+                     const c10::optional<Tensor>& parents, double coeff, double scale, at::ScalarType out_dtype) {
+  Tensor out = append_attend_meta(op, k_in, v_in, q_in, kpi, kseff, kcent, kbounds, vpi, vbounds, kseff16, kcodes, ksigns, krn, kvn,
+                                kcent16, bits, vcodes, vvn, vcent32, vpit, table, lengths, groups, parents, out_dtype);
   const c10::DeviceGuard g(q_in.device());
   Tensor k = activation(k_in), v = activation(v_in), q = activation(q_in);
   if (v.scalar_type() != k.scalar_type() || q.scalar_type() != k.scalar_type()) {
@@ -1135,11 +1195,11 @@ Tensor page_attend(const Tensor& k_in, const Tensor& v_in, const Tensor& q_in, c
     const auto cv = compress_values(v, vpi, vbounds, bits, c10::nullopt);
     page_write(std::get<0>(ck), std::get<1>(ck), std::get<2>(ck), std::get<3>(ck), std::get<0>(cv), std::get<1>(cv), kcodes,
                ksigns, krn, kvn, vcodes, vvn, table, lengths, k.size(2));
-    return tree_attend(q, kpi, kseff16, kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn, vcent32, vpit, table, lengths,
-                       parents, coeff, scale, out_dtype);
+    return attend_pages(op, q, kpi, kseff16, kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn, vcent32, vpit, table,
+                        lengths, groups, parents, coeff, scale, out_dtype);
   }
   // one allocation: the workspace, then the prepared queries
-  const int64_t bytes = (tree_workspace(q, kvn, table, bits) + 15) / 16 * 16, n = q.numel();
+  const int64_t bytes = (tree_workspace(q, kvn, table, bits, groups) + 15) / 16 * 16, n = q.numel();
   Tensor ws = at::empty({bytes + n * 6}, q.options().dtype(at::kByte));
   uint8_t* const base = ptr<uint8_t>(ws);
   float* const q_proj = reinterpret_cast<float*>(base + bytes);
@@ -1152,10 +1212,48 @@ Tensor page_attend(const Tensor& k_in, const Tensor& v_in, const Tensor& q_in, c
                               ptr<uint16_t>(vpi), ptr<float>(vbounds), i32(bits), pool, kvn.size(0), i32(kvn.size(2)),
                               ptr<int32_t>(table), W, W, ptr<int32_t>(lengths), q.data_ptr(), i32(q.size(1)), q.stride(0),
                               q.stride(1), q.stride(2), ptr<uint16_t>(kseff16), q_rot, q_proj, stream_of(k)),
-               "append_tree_attention");
+               groups ? "append_prefix_attention" : "append_tree_attention");
   tree_launch(q_rot, q_proj, kcodes, ksigns, krn, kvn, kcent16, bits, vcodes, vvn, vcent32, vpit, table, lengths, parents, coeff,
-              scale, out, base, bytes);
+              scale, out, base, bytes, groups);
   return out;
+}
+
+Tensor page_attend_meta(const Tensor& k, const Tensor& v, const Tensor& q, const Tensor& kpi, const Tensor& kseff,
+    const Tensor& kcent, const Tensor& kbounds, const Tensor& vpi, const Tensor& vbounds, const Tensor& kseff16,
+    const Tensor& kcodes, const Tensor& ksigns, const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits,
+    const Tensor& vcodes, const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit, const Tensor& table,
+    const Tensor& lengths, const c10::optional<Tensor>& parents, double coeff, double scale,
+    at::ScalarType out_dtype) {
+  return append_attend_meta("tq::page_attend", k, v, q, kpi, kseff, kcent, kbounds, vpi, vbounds, kseff16, kcodes, ksigns, krn, kvn,
+                            kcent16, bits, vcodes, vvn, vcent32, vpit, table, lengths, nullptr, parents, out_dtype);
+}
+Tensor page_attend(const Tensor& k, const Tensor& v, const Tensor& q, const Tensor& kpi, const Tensor& kseff,
+    const Tensor& kcent, const Tensor& kbounds, const Tensor& vpi, const Tensor& vbounds, const Tensor& kseff16,
+    const Tensor& kcodes, const Tensor& ksigns, const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits,
+    const Tensor& vcodes, const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit, const Tensor& table,
+    const Tensor& lengths, const c10::optional<Tensor>& parents, double coeff, double scale,
+    at::ScalarType out_dtype) {
+  return append_attend("tq::page_attend", k, v, q, kpi, kseff, kcent, kbounds, vpi, vbounds, kseff16, kcodes, ksigns, krn, kvn,
+                       kcent16, bits, vcodes, vvn, vcent32, vpit, table, lengths, nullptr, parents, coeff, scale, out_dtype);
+}
+
+Tensor prefix_page_attend_meta(const Tensor& k, const Tensor& v, const Tensor& q, const Tensor& kpi, const Tensor& kseff,
+    const Tensor& kcent, const Tensor& kbounds, const Tensor& vpi, const Tensor& vbounds, const Tensor& kseff16,
+    const Tensor& kcodes, const Tensor& ksigns, const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits,
+    const Tensor& vcodes, const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit, const Tensor& table,
+    const Tensor& lengths, const Tensor& groups, const c10::optional<Tensor>& parents, double coeff, double scale,
+    at::ScalarType out_dtype) {
+  return append_attend_meta("tq::prefix_page_attend", k, v, q, kpi, kseff, kcent, kbounds, vpi, vbounds, kseff16, kcodes, ksigns, krn, kvn,
+                            kcent16, bits, vcodes, vvn, vcent32, vpit, table, lengths, &groups, parents, out_dtype);
+}
+Tensor prefix_page_attend(const Tensor& k, const Tensor& v, const Tensor& q, const Tensor& kpi, const Tensor& kseff,
+    const Tensor& kcent, const Tensor& kbounds, const Tensor& vpi, const Tensor& vbounds, const Tensor& kseff16,
+    const Tensor& kcodes, const Tensor& ksigns, const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits,
+    const Tensor& vcodes, const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit, const Tensor& table,
+    const Tensor& lengths, const Tensor& groups, const c10::optional<Tensor>& parents, double coeff, double scale,
+    at::ScalarType out_dtype) {
+  return append_attend("tq::prefix_page_attend", k, v, q, kpi, kseff, kcent, kbounds, vpi, vbounds, kseff16, kcodes, ksigns, krn, kvn,
+                       kcent16, bits, vcodes, vvn, vcent32, vpit, table, lengths, &groups, parents, coeff, scale, out_dtype);
 }
 
 using Verified = std::tuple<Tensor, Tensor, Tensor>;
@@ -1275,6 +1373,13 @@ TORCH_LIBRARY(tq, m) {
   m.def("tree_attend(Tensor q, Tensor pi_split, Tensor s_eff, Tensor kcodes, Tensor ksigns, Tensor krn, Tensor kvn, "
         "Tensor kcent, int bits, Tensor vcodes, Tensor vvn, Tensor vcent, Tensor vpit, Tensor block_table, "
         "Tensor lengths, Tensor? parents, float coeff, float scale, ScalarType out_dtype) -> Tensor");
+  m.def("prefix_attend(Tensor q, Tensor pi_split, Tensor s_eff, Tensor kcodes, Tensor ksigns, Tensor krn, Tensor kvn, "
+        "Tensor kcent, int bits, Tensor vcodes, Tensor vvn, Tensor vcent, Tensor vpit, Tensor block_table, "
+        "Tensor lengths, Tensor groups, Tensor? parents, float coeff, float scale, ScalarType out_dtype) -> Tensor");
+  m.def("prefix_page_attend(Tensor k, Tensor v, Tensor q, Tensor kpi, Tensor kseff, Tensor kcent, Tensor kbounds, Tensor vpi, "
+        "Tensor vbounds, Tensor kseff16, Tensor(a!) kcodes, Tensor(b!) ksigns, Tensor(c!) krn, Tensor(d!) kvn, "
+        "Tensor kcent16, int bits, Tensor(e!) vcodes, Tensor(f!) vvn, Tensor vcent32, Tensor vpit, Tensor table, "
+        "Tensor lengths, Tensor groups, Tensor? parents, float coeff, float scale, ScalarType out_dtype) -> Tensor");
   m.def("verify_drafts(Tensor tokens, Tensor target_probs, Tensor uniforms, Tensor? parents, Tensor? draft_probs) "
         "-> (Tensor, Tensor, Tensor)");
   m.def("workspace_size(int B, int Hq, int Hkv, int Sq, int Sk, int d, int bits) -> int", &workspace_size);
@@ -1302,6 +1407,8 @@ TORCH_LIBRARY_IMPL(tq, CUDA, m) {
   m.impl("tree_attention", &tree_attention);
   m.impl("tree_attend", &tree_attend);
   m.impl("page_attend", &page_attend);
+  m.impl("prefix_attend", &prefix_attend);
+  m.impl("prefix_page_attend", &prefix_page_attend);
   m.impl("verify_drafts", &verify_drafts);
 }
 
@@ -1328,5 +1435,7 @@ TORCH_LIBRARY_IMPL(tq, Meta, m) {
   m.impl("tree_attention", &tree_attention_meta);
   m.impl("tree_attend", &tree_attend_meta);
   m.impl("page_attend", &page_attend_meta);
+  m.impl("prefix_attend", &prefix_attend_meta);
+  m.impl("prefix_page_attend", &prefix_page_attend_meta);
   m.impl("verify_drafts", &verify_drafts_meta);
 }
