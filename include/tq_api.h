@@ -466,6 +466,34 @@ int tq_verify_drafts(const int64_t* tokens, const void* target_probs, int32_t dt
 /* Workspace bytes of tq_verify_drafts. */
 int64_t tq_verify_workspace_size(int32_t B, int32_t V);
 
+/* Tokens drawn from N rows of V logits (row stride ld elements) by temperature, top-k, top-p and
+ * min-p.  With m the row's largest logit (NaN counts as -inf) and tokens ranked by falling logit, equal
+ * ones by index: w_x = exp((l_x - m) / temperature); of the first top_k in rank (0: all; temperature
+ * 0: the first alone) those whose predecessors weigh less than top_p of them all, and the first one;
+ * of these the ones with w_x >= min_p.  tokens[r]: the first x with w_0 + ... + w_x > uniforms[r]
+ * times the sum over what is kept (-1 for a row without a finite or infinite logit); under an infinite m
+ * the tokens at it are equally likely.  A setting's array (one value per row, on the device) stands in
+ * place of the number where it is not NULL; there temperatures <= 0 or NaN count as 0, top_k <= 0
+ * as 0, top_p NaN as 1, min_p outside [0, 1] as its nearer end.  Weights and sums are float64 or 64-bit
+ * integers: the same call gives the same tokens.  V <= 2^24; a 16-byte aligned workspace of
+ * tq_sample_workspace_size bytes. */
+int tq_sample_tokens(const void* logits, int32_t dtype, int64_t ld, int32_t N, int32_t V,
+                     const float* uniforms, const float* temperatures, double temperature,
+                     const int32_t* top_ks, int32_t top_k, const float* top_ps, double top_p,
+                     const float* min_ps, double min_p, int64_t* tokens, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
+/* The distributions that tq_sample_tokens draws from: probs [N, V] float32, contiguous; zeros where a
+ * token is not kept. */
+int tq_filter_probs(const void* logits, int32_t dtype, int64_t ld, int32_t N, int32_t V,
+                    const float* temperatures, double temperature, const int32_t* top_ks,
+                    int32_t top_k, const float* top_ps, double top_p, const float* min_ps,
+                    double min_p, float* probs, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+
+/* Workspace bytes of both (0: shape not taken). */
+int64_t tq_sample_workspace_size(int32_t N, int32_t V);
+
 /* TQ_NOALLOC_SCRATCH_BYTES as built into the library.  Utility; no reference counterpart. */
 int64_t tq_noalloc_scratch_bytes(void);
 

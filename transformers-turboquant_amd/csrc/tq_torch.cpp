@@ -1313,6 +1313,83 @@ Verified verify_drafts(const Tensor& tokens, const Tensor& target, const Tensor&
   return out;
 }
 
+// ---------------------------------------------------------------- sampling
+using OptTensor = c10::optional<Tensor>;
+
+// A setting: one number, or float32 (top_k: int32) values of the rows
+void check_setting(const Checker& c, const OptTensor& t, const char* name, at::ScalarType dt, int64_t N) {
+  if (!t.has_value() || !t->defined()) return;
+  c.same_device(*t, name);
+  TORCH_CHECK(t->scalar_type() == dt && t->dim() == 1 && t->size(0) == N && t->is_contiguous(), c.op, ": ", name,
+              " must be one number or contiguous ", dt, " [", N, "], got ", t->scalar_type(), " ", t->sizes());
+}
+void check_logits(const Checker& c, const Tensor& logits, const OptTensor& temperatures, double temperature, const OptTensor& top_ks,
+                  int64_t top_k, const OptTensor& top_ps, double top_p, const OptTensor& min_ps, double min_p) {
+  TORCH_CHECK(logits.dim() == 2 && is_act(logits.scalar_type()), c.op, ": logits must be float32, float16 or bfloat16 [N, V], got ",
+              logits.scalar_type(), " ", logits.sizes());
+  const int64_t N = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(V >= 1 && V <= (int64_t{1} << 24) && N < (int64_t{1} << 31) && N * ((V + 2047) / 2048) < (int64_t{1} << 31), c.op,
+              ": 1 to 2^24 tokens and fewer than 2^31 tiles of 2048, got ", logits.sizes());
+  TORCH_CHECK(V == 1 || logits.stride(1) == 1, c.op, ": logits must be contiguous along the vocabulary");
+  check_setting(c, temperatures, "temperature", at::kFloat, N);
+  check_setting(c, top_ks, "top_k", at::kInt, N);
+  check_setting(c, top_ps, "top_p", at::kFloat, N);
+  check_setting(c, min_ps, "min_p", at::kFloat, N);
+  TORCH_CHECK(temperature >= 0 && top_k >= 0 && top_k < (int64_t{1} << 31) && top_p >= 0 && top_p <= 1 && min_p >= 0 && min_p <= 1,
+              c.op, ": temperature and top_k must not be negative, top_p and min_p lie in [0, 1]; got ", temperature, ", ", top_k, ", ",
+              top_p, ", ", min_p);
+}
+
+Tensor sample_tokens_meta(const Tensor& logits, const Tensor& uniforms, const OptTensor& temperatures, double temperature,
+                          const OptTensor& top_ks, int64_t top_k, const OptTensor& top_ps, double top_p,
+                          const OptTensor& min_ps, double min_p) {
+  const Checker c{"tq::sample_tokens", logits.device()};
+  check_logits(c, logits, temperatures, temperature, top_ks, top_k, top_ps, top_p, min_ps, min_p);
+  c.same_device(uniforms, "uniforms");
+  TORCH_CHECK(uniforms.scalar_type() == at::kFloat && uniforms.dim() == 1 && uniforms.size(0) == logits.size(0) &&
+                  uniforms.is_contiguous(),
+              c.op, ": uniforms must be contiguous float32 [", logits.size(0), "], got ", uniforms.scalar_type(), " ",
+              uniforms.sizes());
+  return at::empty({logits.size(0)}, logits.options().dtype(at::kLong));
+}
+
+Tensor sample_tokens(const Tensor& logits, const Tensor& uniforms, const OptTensor& temperatures, double temperature,
+                     const OptTensor& top_ks, int64_t top_k, const OptTensor& top_ps, double top_p, const OptTensor& min_ps,
+                     double min_p) {
+  Tensor out = sample_tokens_meta(logits, uniforms, temperatures, temperature, top_ks, top_k, top_ps, top_p, min_ps, min_p);
+  const c10::DeviceGuard g(logits.device());
+  const int32_t N = i32(logits.size(0)), V = i32(logits.size(1));
+  const int64_t bytes = tq_sample_workspace_size(N, V);
+  Tensor ws = at::empty({bytes}, logits.options().dtype(at::kByte));
+  check_status(tq_sample_tokens(logits.data_ptr(), dtype_code(logits.scalar_type()), logits.stride(0), N, V,
+                                ptr<float>(uniforms), optr<float>(temperatures), temperature, optr<int32_t>(top_ks), i32(top_k),
+                                optr<float>(top_ps), top_p, optr<float>(min_ps), min_p, ptr<int64_t>(out), ws.data_ptr(), bytes,
+                                stream_of(logits)),
+               "sample_tokens");
+  return out;
+}
+
+Tensor filter_probs_meta(const Tensor& logits, const OptTensor& temperatures, double temperature, const OptTensor& top_ks,
+                         int64_t top_k, const OptTensor& top_ps, double top_p, const OptTensor& min_ps, double min_p) {
+  const Checker c{"tq::filter_probs", logits.device()};
+  check_logits(c, logits, temperatures, temperature, top_ks, top_k, top_ps, top_p, min_ps, min_p);
+  return at::empty(logits.sizes(), logits.options().dtype(at::kFloat));
+}
+
+Tensor filter_probs(const Tensor& logits, const OptTensor& temperatures, double temperature, const OptTensor& top_ks,
+                    int64_t top_k, const OptTensor& top_ps, double top_p, const OptTensor& min_ps, double min_p) {
+  Tensor out = filter_probs_meta(logits, temperatures, temperature, top_ks, top_k, top_ps, top_p, min_ps, min_p);
+  const c10::DeviceGuard g(logits.device());
+  const int32_t N = i32(logits.size(0)), V = i32(logits.size(1));
+  const int64_t bytes = tq_sample_workspace_size(N, V);
+  Tensor ws = at::empty({bytes}, logits.options().dtype(at::kByte));
+  check_status(tq_filter_probs(logits.data_ptr(), dtype_code(logits.scalar_type()), logits.stride(0), N, V,
+                               optr<float>(temperatures), temperature, optr<int32_t>(top_ks), i32(top_k), optr<float>(top_ps),
+                               top_p, optr<float>(min_ps), min_p, ptr<float>(out), ws.data_ptr(), bytes, stream_of(logits)),
+               "filter_probs");
+  return out;
+}
+
 int64_t workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t d, int64_t bits) {
   return tq_attention_workspace_size(static_cast<int32_t>(B), static_cast<int32_t>(Hq), static_cast<int32_t>(Hkv),
                                      static_cast<int32_t>(Sq), static_cast<int32_t>(Sk), static_cast<int32_t>(d),
@@ -1382,6 +1459,10 @@ TORCH_LIBRARY(tq, m) {
         "Tensor lengths, Tensor groups, Tensor? parents, float coeff, float scale, ScalarType out_dtype) -> Tensor");
   m.def("verify_drafts(Tensor tokens, Tensor target_probs, Tensor uniforms, Tensor? parents, Tensor? draft_probs) "
         "-> (Tensor, Tensor, Tensor)");
+  m.def("sample_tokens(Tensor logits, Tensor uniforms, Tensor? temperatures, float temperature, Tensor? top_ks, int top_k, "
+        "Tensor? top_ps, float top_p, Tensor? min_ps, float min_p) -> Tensor");
+  m.def("filter_probs(Tensor logits, Tensor? temperatures, float temperature, Tensor? top_ks, int top_k, Tensor? top_ps, "
+        "float top_p, Tensor? min_ps, float min_p) -> Tensor");
   m.def("workspace_size(int B, int Hq, int Hkv, int Sq, int Sk, int d, int bits) -> int", &workspace_size);
 }
 
@@ -1410,6 +1491,8 @@ TORCH_LIBRARY_IMPL(tq, CUDA, m) {
   m.impl("prefix_attend", &prefix_attend);
   m.impl("prefix_page_attend", &prefix_page_attend);
   m.impl("verify_drafts", &verify_drafts);
+  m.impl("sample_tokens", &sample_tokens);
+  m.impl("filter_probs", &filter_probs);
 }
 
 // the same checks on tensor metadata, returning empty outputs of the right shapes
@@ -1438,4 +1521,6 @@ TORCH_LIBRARY_IMPL(tq, Meta, m) {
   m.impl("prefix_attend", &prefix_attend_meta);
   m.impl("prefix_page_attend", &prefix_page_attend_meta);
   m.impl("verify_drafts", &verify_drafts_meta);
+  m.impl("sample_tokens", &sample_tokens_meta);
+  m.impl("filter_probs", &filter_probs_meta);
 }

@@ -27,6 +27,7 @@ _p = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 # name -> argument types (return type is int status unless listed in _RESTYPE)
 _SIGNATURES = {
@@ -83,11 +84,14 @@ _SIGNATURES = {
     "tq_verify_drafts": [_p, _p, _i32, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i32, _i32, _i32, _p, _p, _p, _p,
                          _i64, _p],
     "tq_verify_workspace_size": [_i32, _i32],
+    "tq_sample_tokens": [_p, _i32, _i64, _i32, _i32, _p, _p, _f64, _p, _i32, _p, _f64, _p, _f64, _p, _p, _i64, _p],
+    "tq_filter_probs": [_p, _i32, _i64, _i32, _i32, _p, _f64, _p, _i32, _p, _f64, _p, _f64, _p, _p, _i64, _p],
+    "tq_sample_workspace_size": [_i32, _i32],
 }
 _RESTYPE = {"tq_last_error": ctypes.c_char_p, "tq_out_cols": _i64, "tq_attention_workspace_size": _i64,
             "tq_noalloc_scratch_bytes": _i64, "tq_prefill_workspace_size": _i64,
             "tq_prefill_scores_workspace_size": _i64, "tq_tree_workspace_size": _i64, "tq_prefix_workspace_size": _i64,
-            "tq_verify_workspace_size": _i64}
+            "tq_verify_workspace_size": _i64, "tq_sample_workspace_size": _i64}
 
 EXPORTED = tuple(_SIGNATURES)
 
