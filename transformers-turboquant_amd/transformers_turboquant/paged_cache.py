@@ -6,7 +6,8 @@ Where :class:`TurboQuantCache` holds capacity planes of one length for a whole b
 * sequences come and go (``add``, ``free``), and ``use`` picks which of them the next forward's batch
   rows are;
 * a fork (``fork``, beam search's ``reorder_cache``) shares its pages with the sequence it came from; a
-  shared page is copied before a position in it is written;
+  shared page is copied before a position in it is written; with ``shared_prefix=True`` attention reads the pages
+  that active sequences next to one another share once for all of them;
 * drafted tokens (``draft``) are appended as a tree that is not part of the text yet; after verification
   ``accept`` keeps one path of it, moved down behind the cached positions, and frees the rest.
 
@@ -27,10 +28,37 @@ import math
 import torch
 from transformers.cache_utils import Cache
 from turboquant_pytorch.drafts import append_tree_attention
+from turboquant_pytorch.prefix import append_prefix_attention
 
 __all__ = ["TurboQuantPagedCache"]
 
 MAX_DRAFT = 64  # nodes of a tree; longer appends are prompts
+
+
+def _best_runs(common: list[int]) -> list[tuple[int, int]]:
+    """len(common) + 1 sequences cut into runs (size, pages that all of it share) that save the most pages of
+    reading, (size - 1) * shared each; common[i]: pages that i and i + 1 share.  Where these are not all the same, runs
+    are of 64 at most, as the operator reads them."""
+    n = len(common) + 1
+    if len(set(common)) <= 1:
+        return [(n, common[0])] if common and common[0] else [(1, 0)] * n
+    best = [(0, 0, 0)]  # of the first j sequences: pages saved, the last run's begin and what it shares
+    for j in range(1, n + 1):
+        top, least = (best[j - 1][0], j - 1, 0), None
+        for i in range(j - 2, max(-1, j - 65), -1):
+            least = common[i] if least is None else min(least, common[i])
+            if not least:
+                break
+            saved = best[i][0] + (j - i - 1) * least
+            if saved > top[0]:
+                top = (saved, i, least)
+        best.append(top)
+    runs, j = [], n
+    while j:
+        _, i, shared = best[j]
+        runs.append((j - i, shared))
+        j = i
+    return runs[::-1]
 
 
 class _Sequence:
@@ -44,13 +72,14 @@ class _Sequence:
 class TurboQuantPagedCache(Cache):
     """A transformers ``Cache`` over pages, for models patched by ``apply_turboquant`` on the GPU."""
 
-    def __init__(self, num_pages: int, num_layers: int, page_size: int = 64):
+    def __init__(self, num_pages: int, num_layers: int, page_size: int = 64, shared_prefix: bool = False):
         super().__init__(layers=[])
         if num_pages < 1 or num_layers < 1:
             raise ValueError("a paged cache needs at least one page and one layer")
         if page_size < 32 or page_size & (page_size - 1):
             raise ValueError(f"page_size must be a power of two from 32 on, got {page_size}")
         self.num_pages, self.num_layers, self.page_size = num_pages, num_layers, page_size
+        self.shared_prefix = shared_prefix
         self.pool = None  # made by the first append, which knows heads, head_dim and bits
         self._free = list(range(num_pages - 1, -1, -1))
         self._refs = [0] * num_pages
@@ -63,6 +92,7 @@ class TurboQuantPagedCache(Cache):
         self._written: set[int] = set()  # layers of the step under way that hold its rows
         self._step = 0  # tokens of the step under way
         self._device_state = None  # (block table, lengths) of the active sequences; None: to be made
+        self._groups = None  # of the active sequences that share pages, on the device (None: attended alone)
         self._made: list[int] = []  # sequences that the step under way made
         self._made_pool = False  # it made the pool, too
 
@@ -275,7 +305,7 @@ class TurboQuantPagedCache(Cache):
         self._written.clear()
         self._step = 0
         self._drafted = False
-        self._device_state = None
+        self._device_state = self._groups = None
         self._made, self._made_pool = [], False
 
     def _undo(self) -> None:
@@ -313,7 +343,10 @@ class TurboQuantPagedCache(Cache):
         self._begin(layer_idx, k, bits)
         table, lengths = self._device_state
         try:
-            if fast:
+            if fast and self._groups is not None:
+                out = append_prefix_attention(k, v, q, key_compressor, val_compressor, self.pool, layer_idx, table, lengths,
+                                              self._groups, self.draft_parents, scale, out_dtype)
+            elif fast:
                 out = append_tree_attention(k, v, q, key_compressor, val_compressor, self.pool, layer_idx, table, lengths,
                                             self.draft_parents, scale, out_dtype)
             else:
@@ -416,12 +449,26 @@ class TurboQuantPagedCache(Cache):
             return
         dev = self.pool.device
         width = max(len(s.pages) for s in seqs)
-        state = torch.tensor([s.pages + [-1] * (width - len(s.pages)) + [s.length] for s in seqs], dtype=torch.int32)
-        state = state.to(dev)  # one copy for both
-        self._device_state = (state[:, :-1].contiguous(), state[:, -1].contiguous())
+        groups = self._shared(seqs) if self.shared_prefix else [(-1, 0)] * len(seqs)
+        state = torch.tensor([s.pages + [-1] * (width - len(s.pages)) + [s.length, *g] for s, g in zip(seqs, groups)],
+                             dtype=torch.int32)
+        state = state.to(dev)  # one copy for all
+        self._device_state = (state[:, :-3].contiguous(), state[:, -3].contiguous())
+        self._groups = state[:, -2:].contiguous() if any(n for _, n in groups) else None
         if src:
             pairs = torch.tensor([src, dst], dtype=torch.int32).to(dev)
             self.pool.copy(pairs[0], pairs[1])
+
+    def _shared(self, seqs) -> list[tuple[int, int]]:
+        """(id, shared positions) of each sequence, as `prefix_attention` takes them."""
+        common = []  # leading pages that a sequence and the next one have in common
+        for a, b in zip(seqs, seqs[1:]):
+            lo, hi = 0, min(len(a.pages), len(b.pages))
+            while lo < hi:  # behind the first page that differs, all do
+                mid = (lo + hi) // 2
+                lo, hi = (mid + 1, hi) if a.pages[mid] == b.pages[mid] else (lo, mid)
+            common.append(lo)
+        return [(i, n * self.page_size) for i, (size, n) in enumerate(_best_runs(common)) for _ in range(size)]
 
     def _take(self) -> int:
         p = self._free.pop()

@@ -16,7 +16,7 @@ __all__ = ["speculative_step"]
 @torch.no_grad()
 def speculative_step(model, cache: TurboQuantPagedCache, tokens: torch.Tensor, parents=None,
                      draft_probs: torch.Tensor | None = None, uniforms: torch.Tensor | None = None,
-                     temperature: float = 1.0) -> list[list[int]]:
+                     temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0) -> list[list[int]]:
     """Run a patched model over drafted tokens of the cache's active sequences, verify them, keep the
     accepted path in the cache, and return each sequence's emitted tokens: the accepted drafted
     ones and one more, which is the next step's root.
@@ -26,13 +26,16 @@ def speculative_step(model, cache: TurboQuantPagedCache, tokens: torch.Tensor, p
     their tree in index order: node 0 is -1, another node's parent an earlier node, -2 pads a smaller
     tree; None is a chain.  draft_probs [B, T - 1, V]: a chain's tokens were drawn from these
     distributions (`turboquant_pytorch.verify_drafts`).  temperature 0 takes the likeliest token
-    instead of drawing.  uniforms float32 [B, T] default to torch.rand."""
-    from turboquant_pytorch import verify_drafts
+    instead of drawing; top_k, top_p and min_p filter the model's distributions
+    (`turboquant_pytorch.filter_probs`).  uniforms float32 [B, T] default to torch.rand."""
+    from turboquant_pytorch import filter_probs, verify_drafts
 
     if tokens.dim() != 2 or not 1 <= tokens.shape[1] <= MAX_DRAFT:
         raise ValueError(f"tokens must be [B, 1 to {MAX_DRAFT}], got {tuple(tokens.shape)}")
     if temperature < 0:
         raise ValueError(f"temperature must not be negative, got {temperature}")
+    if top_k < 0 or not 0 <= top_p <= 1 or not 0 <= min_p <= 1:
+        raise ValueError(f"top_k must not be negative, top_p and min_p lie in [0, 1]; got {top_k}, {top_p} and {min_p}")
     B, T = tokens.shape
     dev = tokens.device
     tree, depth = _depths(parents, B, T)
@@ -48,6 +51,8 @@ def speculative_step(model, cache: TurboQuantPagedCache, tokens: torch.Tensor, p
         logits = model(input_ids=tokens, position_ids=positions, past_key_values=cache, use_cache=True).logits.float()
     if temperature == 0:
         probs = F.one_hot(logits.argmax(-1), logits.shape[-1]).float()
+    elif top_k or top_p < 1 or min_p:
+        probs = filter_probs(logits, temperature, top_k, top_p, min_p)
     else:
         probs = torch.softmax(logits / temperature, -1)
     if uniforms is None:
