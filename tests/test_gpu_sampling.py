@@ -121,7 +121,8 @@ def test_many_rows_and_large_vocabularies():
                 logits, u, *(kw.get(n, d) for n, d in zip("tkpm", (1.0, 0, 1.0, 0.0))))
             some = sorted({0, 1 % N, N // 2, N - 1})
             p2, t2 = _check(logits[some], u[some], **kw)
-            assert torch.equal(probs[some], p2) and torch.equal(tokens[some], t2)
+            # another batch is cut into other chunks: each side is within 2^-24 + 2^-40 of the exact value
+            assert ((probs[some] - p2).abs() <= p2 * (2.0 ** -23 + 2.0 ** -38)).all() and torch.equal(tokens[some], t2)
 
 
 def test_equal_logits():

@@ -13,81 +13,104 @@
 // in a few thousand tokens if sums are off by 10^-7; so weights are float64 (2^f by its Taylor series, 2 10^-13), and
 // sums are float64 in a fixed order or integers, which have none.
 //
-// Nothing is sorted.  A row is cut into chunks, one per block:
-//   scan     the chunk's maximum, and what the row's filters need: with top-k a histogram of how many logits
-//            lie in each bin of 1/16 below the maximum, with top-p of their mass, without both the mass alone
-//   select   finds in the row's joined histograms the bins that hold the borders; of the chunk, lists the few tokens in
-//            those bins, and adds up the mass of what is kept for certain (min-p alone: what is kept)
-//   draw     one block per row: decides the border by a radix selection among the listed tokens (by rank, by
-//            mass, by index among equal ones), draws the chunk by the chunks' masses, and the token in it
-//   write    the probabilities, in place of the draw
+// A row is never sorted.  It is cut into chunks, one per block, and then finished by one block:
+//   scan     the chunk's maximum; without filters its mass; for top-p its mass, and a histogram of it over bins of
+//            1/16 below the maximum, as far down as tokens can be kept (all those of weight below (1 - p) / V of the
+//            largest together weigh less than (1 - p) of the total, so p of it stands before them); for
+//            top-k a list of the tokens down to the bin that k threads' own maxima reach
+//   select   (top-p, min-p) finds the bins that hold the row's border in the joined histograms, and lists what is
+//            kept (min-p), the tokens down to the border if they are few, or else those of its bins alone, with the
+//            mass of what is kept for certain above them
+//   finish   up to 64 listed tokens are ranked by one wave, up to 2048 sorted by the block, more are selected digit
+//            by digit; then cut, and drawn from the list if it holds all that is kept, or else by the chunks' masses
+//   write    the probabilities of rows that keep many; the others' are few, in a row that the scan has cleared
 #include "tq_common.h"
 
 namespace tq {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kTileTokens = kThreads * 8;  // a thread takes 8 tokens in a row
+constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of the finish
+constexpr int kScan = 512, kScanWaves = kScan / 64;     // of scan and select: a thread takes runs of 8 tokens
 constexpr int kBins = 512, kTail = kBins - 1;  // the last bin has everything below the others
-constexpr int kMaxChunks = 512;
-constexpr int kShort = 2048;  // listed tokens that fit the draw's shared memory
-constexpr double kUnit = 0x1p48;  // of a chunk's masses: at most 2^15 tokens of weight <= 1 in 63 bits
+constexpr int kMaxChunks = 1024;
+constexpr int kShort = 2048;  // tokens that are sorted
+constexpr int kFew = 1024;    // tokens down to the border that are listed with it
+constexpr double kUnit = 0x1p48;  // of a chunk's mass: at most 2^15 tokens of weight <= 1
+constexpr int kTiny = 49;         // a weight below 2^-49 is no unit
+
+enum Mode { kAll, kMinP, kTopP, kTopK };
+
+// A row's settings as the kernels use them
+struct Settings {
+  int mode, k;
+  double c;     // log2(e) / t
+  double p, m;
+  float far;    // kept tokens' logits are down to this far from the maximum (top-p, min-p)
+  float tiny;   // weights are units down to this far
+
+  // t: NaN and what is not positive count as 0
+  __host__ __device__ Settings(int V, double t, int k_, double p_, double m_) : k(k_), p(p_), m(m_) {
+    const bool greedy = !(t > 0.0);
+    if (greedy) k = 1;
+    c = 1.4426950408889634 / (greedy ? 1.0 : t);
+    if (!(c < 1e300)) c = 1e300;
+    m = m > 0.0 ? (m < 1.0 ? m : 1.0) : 0.0;
+    const bool by_rank = k > 0 && k < V, by_mass = p < 1.0;
+    if (!by_mass) p = 1.0;
+    mode = by_rank ? kTopK : by_mass ? kTopP : m > 0.0 ? kMinP : kAll;
+    // log2 of the least weight, with room for its rounding
+    double y = m > 0.0 ? log2(m) : -1100.0;
+    if (mode == kTopP) y = fmax(y, log2((1.0 - p) / V) - 1.0);
+    const double d = (0.001 - y) / c;
+    far = d < 3e38 ? static_cast<float>(d * 1.000001) : INFINITY;
+    const double z = (kTiny + 0.01) / c;
+    tiny = z < 3e38 ? static_cast<float>(z * 1.000001) : INFINITY;
+  }
+};
+
+// Top-p: the row's mass and the bins that are listed
+struct RowCut {
+  double total;
+  int lo, hi;
+};
+
+// A row's border, and whether its probabilities are written already
+struct RowState {
+  uint32_t key;  // kept: larger keys, and this key up to index `last`
+  int last;
+  float top;
+  int done;
+  double inverse;  // 1 / kept mass
+};
 
 struct SampleArgs {
   const void* logits;
   int64_t ld;  // elements between rows
   int N, V;
-  // one setting for all rows, or one per row
+  // one setting for all rows, or (an array) one per row
   const float* t_rows;
   const int32_t* k_rows;
   const float* p_rows;
   const float* m_rows;
   double t, p, m;
   int k;
-  const float* uniforms;  // [N], or null: probabilities
-  int64_t* tokens;        // [N]
-  float* probs;           // [N, V]
-  int C, lg_chunk;        // chunks of a row, tokens of a chunk
+  Settings all;            // where no setting is the rows' own
+  const float* uniforms;   // [N], or null: probabilities
+  int64_t* tokens;         // [N]
+  float* probs;            // [N, V]
+  int C, lg_chunk, lg_room;  // chunks of a row, tokens of a chunk, places in its list
   // workspace
-  struct RowState* state;  // [N]
-  float* top;              // [N, C] chunk's maximum
-  double* mass;            // [N, C] certain mass, relative to the chunk's (scan) or the row's maximum (select)
-  uint64_t* total;         // [N, C] of the histogram
-  int32_t* listed;         // [N, C]
-  uint64_t* hist;          // [N, C, kBins]
-  uint16_t* list;          // [N, C << lg_chunk] places in the chunk
-};
+  Settings* rows;   // [N], or null: `all`
+  RowState* state;  // [N]
+  RowCut* cut;      // [N]
+  float* top;       // [N, C] chunk's maximum
+  double* mass;     // [N, C] of the chunk, relative to its maximum
+  double* kept;     // [N, C] of what is kept for certain, relative to the row's
+  int32_t* listed;  // [N, C] tokens in the list; more than fit: it is not used
+  int32_t* depth;   // [N, C] bins of the histogram
+  uint64_t* hist;   // [N, C, kBins] in units of 2^-48
+  uint2* list;      // [N, C, 2^lg_room] logit, index
 
-// What a row's borders are: written by select (goal, cut) and draw (the rest)
-struct RowState {
-  double goal;       // top-p: mass at which tokens are no longer kept
-  int cut;           // 0: top-p's border is not needed (min-p is stricter)
-  uint32_t key;      // kept: larger keys, and this key up to index `last`
-  int last;
-  float top;
-  double inverse;    // 1 / kept mass
-};
-
-enum Mode { kAll, kMinP, kTopP, kTopK };
-
-// A row's settings as the kernels use them
-struct Settings {
-  Mode mode;
-  int k;
-  double c;      // log2(e) / t
-  double p, m;
-  __device__ __forceinline__ Settings(const SampleArgs& a, int row) {
-    const double t = a.t_rows ? static_cast<double>(a.t_rows[row]) : a.t;
-    k = a.k_rows ? a.k_rows[row] : a.k;
-    p = a.p_rows ? static_cast<double>(a.p_rows[row]) : a.p;
-    m = a.m_rows ? static_cast<double>(a.m_rows[row]) : a.m;
-    const bool greedy = !(t > 0.0);
-    if (greedy) k = 1;
-    c = fmin(1.4426950408889634 / (greedy ? 1.0 : t), 1e300);
-    m = m > 0.0 ? fmin(m, 1.0) : 0.0;
-    const bool by_rank = k > 0 && k < a.V, by_mass = p < 1.0;
-    if (!by_mass) p = 1.0;
-    mode = by_rank ? kTopK : by_mass ? kTopP : m > 0.0 ? kMinP : kAll;
-  }
+  __device__ __forceinline__ const Settings& of(int row) const { return rows ? rows[row] : all; }
 };
 
 // 2^y, y <= 0: 2^n by the exponent, 2^f for |f| <= 1/2 by the series of exp(f ln 2) up to the 10th power
@@ -135,7 +158,7 @@ __device__ __forceinline__ void load_logits(const void* row, int x, int V, float
     for (int j = 0; j < 8; ++j) v[j] = x + j < V ? load_act<DT>(row, x + j) : -INFINITY;
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = v[j] == v[j] ? v[j] : -INFINITY;
+  for (int j = 0; j < 8; ++j) v[j] = fmaxf(v[j], -INFINITY);  // NaN: the other operand
 }
 template <int DT>
 __device__ __forceinline__ const void* row_of(const SampleArgs& a, int row) {
@@ -144,6 +167,8 @@ __device__ __forceinline__ const void* row_of(const SampleArgs& a, int row) {
 // Under an infinite maximum only infinite logits have a weight: as 0 against -inf, maximum 0.
 __device__ __forceinline__ float tame(float v, float m) { return m == INFINITY ? (v == INFINITY ? 0.f : -INFINITY) : v; }
 __device__ __forceinline__ float tame(float m) { return m == INFINITY ? 0.f : m; }
+// a chunk's or listed logit, tamed by its own chunk's maximum already, under the row's
+__device__ __forceinline__ bool counts(float chunk_top, float m) { return m != INFINITY || chunk_top == INFINITY; }
 
 // ---------------------------------------------------------------- over a wave, over a block
 template <class T, class Op>
@@ -162,15 +187,30 @@ __device__ __forceinline__ T wave_scan(T v) {  // inclusive
   }
   return v;
 }
-// of all threads, in a fixed order; s: kWaves values, free again behind the next barrier
-template <class T, class Op>
+// Inclusive sum of 32-bit values through DPP (shifts within rows of 16 lanes, then row 0's sum into row 1 and
+// row 2's into row 3, then lane 31's into the upper half)
+template <int CTRL, int ROWS, class T>
+__device__ __forceinline__ T dpp_add(T v) {
+  return v + __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, false));
+}
+template <class T>
+__device__ __forceinline__ T wave_scan32(T v) {
+  v = dpp_add<0x111, 0xF>(v);
+  v = dpp_add<0x112, 0xF>(v);
+  v = dpp_add<0x114, 0xF>(v);
+  v = dpp_add<0x118, 0xF>(v);
+  v = dpp_add<0x142, 0xA>(v);
+  return dpp_add<0x143, 0xC>(v);
+}
+// of all threads, in a fixed order; s: a value per wave, free again behind the next barrier
+template <int W, class T, class Op>
 __device__ __forceinline__ T block_all(T v, T* s, Op op) {
   v = wave_all(v, op);
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
   __syncthreads();
   T r = s[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) r = op(r, s[w]);
+  for (int w = 1; w < W; ++w) r = op(r, s[w]);
   return r;
 }
 struct Sum {
@@ -185,294 +225,487 @@ struct Max {
     return a > b ? a : b;
   }
 };
-
-__device__ __forceinline__ float row_top(const SampleArgs& a, int row) {
-  const int lane = threadIdx.x & 63;
-  float m = -INFINITY;
-  for (int c = lane; c < a.C; c += 64) m = fmaxf(m, a.top[static_cast<int64_t>(row) * a.C + c]);
-  return wave_all(m, Max{});
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int l) {
+  return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), l))) << 32 |
+         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), l));
+}
+__device__ __forceinline__ void add_lds(uint64_t* p, uint64_t v) {
+  atomicAdd(reinterpret_cast<unsigned long long*>(p), static_cast<unsigned long long>(v));
 }
 
 // ---------------------------------------------------------------- scan
-template <int DT, int NV>
-__global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs a) {
-  __shared__ uint64_t s_hist[kBins];
-  __shared__ float s_max[kWaves];
-  __shared__ double s_sum[kWaves];
-  __shared__ uint64_t s_total[kWaves];
-  const int row = blockIdx.x / a.C, c = blockIdx.x - row * a.C, tid = threadIdx.x;
+// A thread's tokens of a chunk: runs of 8 in a row, kScan * 8 apart, at most 64.  They are read anew in every pass
+// (from the caches behind the first): held in registers, 64 of them leave one wave per SIMD.
+template <int DT, class Fn>
+__device__ __forceinline__ void each_run(const SampleArgs& a, int row, int chunk, float m, Fn fn) {
   const void* const src = row_of<DT>(a, row);
-  float v[NV / 8][8];
+  const int x0 = (chunk << a.lg_chunk) + static_cast<int>(threadIdx.x) * 8, runs = 1 << (a.lg_chunk - 12);
+  static_assert(kScan * 8 == 1 << 12, "tokens of a block's run");
+#pragma unroll 1
+  for (int r = 0; r < runs; ++r) {
+    const int x = x0 + r * (kScan * 8);
+    float v[8];
+    load_logits<DT>(src, x, a.V, v);
+    if (m == INFINITY) {
 #pragma unroll
-  for (int j = 0; j < NV / 8; ++j) load_logits<DT>(src, (c << a.lg_chunk) + j * kTileTokens + tid * 8, a.V, v[j]);
-  const Settings set(a, row);
-  if (tid < kBins) s_hist[tid] = 0;
-  float m = -INFINITY;
+      for (int e = 0; e < 8; ++e) v[e] = tame(v[e], m);
+    }
+    fn(v, r, x);
+  }
+}
+
+// units of a weight: 16 + w has 2^-48 in its last place
+__device__ __forceinline__ uint64_t units_of(double w) { return __double_as_longlong(w + 16.0) & 0xFFFFFFFFFFFFFull; }
+
+// The block's listed tokens, bit 8 r + e of `on` for token e of the thread's run r: to the chunk's list, in any order
+template <int DT>
+__device__ __forceinline__ void list_tokens(const SampleArgs& a, int row, int chunk, float m, uint64_t on, int* s_listed) {
+  const int mine = __popcll(on);
+  int to = wave_scan32(mine);
+  const int all = __builtin_amdgcn_readlane(to, 63);
+  if (!all) return;
+  int base = 0;
+  if ((threadIdx.x & 63) == 0) base = atomicAdd(s_listed, all);
+  to += __builtin_amdgcn_readfirstlane(base) - mine;
+  const int room = 1 << a.lg_room, x0 = (chunk << a.lg_chunk) + static_cast<int>(threadIdx.x) * 8;
+  uint2* const list = a.list + ((static_cast<int64_t>(row) * a.C + chunk) << a.lg_room);
+  const void* const src = row_of<DT>(a, row);
+#pragma unroll 1
+  for (; on && to < room; on &= on - 1, ++to) {
+    const int i = __builtin_ctzll(on), x = x0 + (i >> 3) * (kScan * 8) + (i & 7);
+    list[to] = uint2{__float_as_uint(tame(load_act<DT>(src, x), m)), static_cast<uint32_t>(x)};
+  }
+}
+
+// The bin up to which the sum over 512 bins (8 to each lane of a wave) reaches `goal`: kTail if none does
+template <class T>
+__device__ __forceinline__ int reach_bin(const T (&h)[8], T goal) {
+  const int lane = threadIdx.x & 63;
+  T sum = 0;
 #pragma unroll
-  for (int j = 0; j < NV / 8; ++j)
+  for (int i = 0; i < 8; ++i) sum += h[i];
+  const T upto = wave_scan32(sum);
+  const uint64_t over = __ballot(upto >= goal);
+  if (!over) return kTail;
+  T run = upto - sum;
+  int bin = 8 * lane;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m = fmaxf(m, v[j][e]);
-  m = block_all(m, s_max, Max{});
+  for (int i = 0; i < 7; ++i) {
+    run += h[i];
+    bin += run < goal;
+  }
+  return min(__builtin_amdgcn_readlane(bin, __builtin_ctzll(over)), kTail);
+}
+
+struct ScanSmem {
+  uint64_t hist[kBins];
+  uint64_t part[kScanWaves];
+  double sum[kScanWaves];
+  float top[kScanWaves];
+  int depth[kScanWaves];
+  int listed, bin;
+  Settings set;
+  __device__ ScanSmem() = delete;
+};
+
+// Settings of a row, in shared memory where they are the row's own: made by one thread
+__device__ __forceinline__ void make_settings(const SampleArgs& a, int row, Settings* to) {
+  *to = Settings(a.V, a.t_rows ? a.t_rows[row] : a.t, a.k_rows ? a.k_rows[row] : a.k, a.p_rows ? a.p_rows[row] : a.p,
+                 a.m_rows ? a.m_rows[row] : a.m);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kScan) sample_scan_kernel(SampleArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t s_raw[sizeof(ScanSmem)];
+  ScanSmem& s = *reinterpret_cast<ScanSmem*>(s_raw);
+  const int row = blockIdx.x / a.C, c = blockIdx.x - row * a.C, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  float most = -INFINITY;
+  each_run<DT>(a, row, c, 0.f, [&](const float (&v)[8], int, int) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, v[e]);
+  });
+  static_assert(kScan == kBins, "a bin per thread");
+  s.hist[tid] = 0;
+  if (tid == 0) {
+    s.listed = 0;
+    if (a.rows) {
+      make_settings(a, row, &s.set);
+      if (c == 0) a.rows[row] = s.set;
+    }
+  }
+  const float m = block_all<kScanWaves>(most, s.top, Max{});
+  const Settings& set = a.rows ? s.set : a.all;
+  const int mode = set.mode;
   const int64_t at = static_cast<int64_t>(row) * a.C + c;
   if (tid == 0) a.top[at] = m;
-  if (set.mode == kMinP) return;
+  if (a.probs && mode != kAll) {  // kept tokens are filled in later
+    float* const to = a.probs + static_cast<int64_t>(row) * a.V;
+    const int end = min(a.V, (c + 1) << a.lg_chunk);
+#pragma unroll 1
+    for (int x = (c << a.lg_chunk) + tid * 8; x < end; x += kScan * 8) {
+      const float zero[8] = {};
+      if (x + 8 <= a.V) {
+        __builtin_memcpy(to + x, zero, 32);
+      } else {
+        for (int e = 0; x + e < a.V; ++e) to[x + e] = 0.f;
+      }
+    }
+  }
+  if (mode == kMinP) return;
   if (m == -INFINITY) {
     if (tid == 0) {
       a.mass[at] = 0.0;
-      a.total[at] = 0;
+      a.listed[at] = 0;
+      a.depth[at] = 0;
     }
-    if (set.mode != kAll && tid < kBins) a.hist[at * kBins + tid] = 0;
     return;
   }
   const float mt = tame(m);
-  if (set.mode == kAll) {
-    double sum = 0.0;
-#pragma unroll
-    for (int j = 0; j < NV / 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum += weight(tame(v[j][e], m), mt, set.c);
-    sum = block_all(sum, s_sum, Sum{});
-    if (tid == 0) a.mass[at] = sum;
-    return;
-  }
+  const double c2 = set.c;
   const int top = grid_of(mt);
-  uint64_t sum = 0;
+  if (mode == kAll) {
+    double sum = 0.0;
+    each_run<DT>(a, row, c, m, [&](const float (&v)[8], int, int) {
 #pragma unroll
-  for (int j = 0; j < NV / 8; ++j)
+      for (int e = 0; e < 8; ++e) sum += weight(v[e], mt, c2);
+    });
+    sum = block_all<kScanWaves>(sum, s.sum, Sum{});
+    if (tid == 0) a.mass[at] = sum;
+  } else if (mode == kTopK) {
+    // k threads have a token in the bins down to this one: k tokens stand before all that is below
+    most = tame(most, m);
+    if (most != -INFINITY) add_lds(s.hist + bin_of(most, top), 1);
+    __syncthreads();
+    if (wave == 0) {
+      int h[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float x = tame(v[j][e], m);
-      if (x == -INFINITY) continue;
-      uint64_t n = 1;
-      // 16 + w has units of 2^-48 in its last place
-      if (set.mode == kTopP) n = __double_as_longlong(weight(x, mt, set.c) + 16.0) & 0xFFFFFFFFFFFFFull;
-      sum += n;
-      atomicAdd(reinterpret_cast<unsigned long long*>(s_hist + bin_of(x, top)), static_cast<unsigned long long>(n));
+      for (int i = 0; i < 8; ++i) h[i] = 8 * lane + i < kTail ? static_cast<int>(s.hist[8 * lane + i]) : 0;
+      const int bin = reach_bin(h, set.k);
+      if (lane == 0) s.bin = bin;
     }
-  sum = block_all(sum, s_total, Sum{});  // its barrier is behind the histogram, too
-  if (tid == 0) a.total[at] = sum;
-  if (tid < kBins) a.hist[at * kBins + tid] = s_hist[tid];
+    __syncthreads();
+    // the bin's lower end (the grid's last value has everything below it)
+    float least = -3.4028235e38f;
+    if (s.bin < kTail && top - s.bin > -(1 << 27)) least = __double2float_rd((top - s.bin) * 0.0625);
+    uint64_t on = 0;
+    if (most >= least)
+      each_run<DT>(a, row, c, m, [&](const float (&v)[8], int r, int) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) on |= static_cast<uint64_t>(v[e] >= least) << (8 * r + e);
+      });
+    list_tokens<DT>(a, row, c, m, on, &s.listed);
+    __syncthreads();
+    if (tid == 0) a.listed[at] = s.listed;
+  } else {
+    const auto below = [&](float d) {  // a logit d below the maximum, rounded down
+      const float x = mt - d;
+      return x - 2e-7f * (fabsf(mt) + fabsf(x));
+    };
+    const float least = fmaxf(-3.4028235e38f, below(set.far)), tiny = below(set.tiny);
+    uint64_t sum = 0;
+    int deep = 0;
+    each_run<DT>(a, row, c, m, [&](const float (&v)[8], int, int) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = v[e];
+        if (__any(!(x < tiny))) {
+          const uint64_t n = units_of(weight(x, mt, c2));
+          sum += n;
+          if (x >= least) {
+            const int b = bin_of(x, top);
+            deep = max(deep, b + 1);
+            add_lds(s.hist + b, n);
+          }
+        }
+      }
+    });
+    deep = wave_all(deep, Max{});
+    if (lane == 0) s.depth[wave] = deep;
+    sum = block_all<kScanWaves>(sum, s.part, Sum{});  // its barrier is behind the histogram, too
+#pragma unroll
+    for (int w = 0; w < kScanWaves; ++w) deep = max(deep, s.depth[w]);
+    if (tid == 0) {
+      a.mass[at] = static_cast<double>(sum);
+      a.depth[at] = deep;
+    }
+    if (tid < deep) a.hist[at * kBins + tid] = s.hist[tid];
+  }
 }
 
 // ---------------------------------------------------------------- select
-template <int DT, int NV>
-__global__ void __launch_bounds__(kThreads) sample_select_kernel(SampleArgs a) {
-  __shared__ double s_sum[kWaves];
-  __shared__ uint64_t s_own[kWaves];
-  __shared__ double s_factor[kMaxChunks];  // units of a chunk's masses
-  __shared__ int s_off[kMaxChunks];        // its first bin among the row's
-  __shared__ int s_lo, s_hi, s_listed;
+struct SelectSmem {
+  float bins[kBins];
+  float factor[kMaxChunks];  // of a chunk's units: shares of the row's mass
+  int off[kMaxChunks];       // its first bin among the row's
+  int depth[kMaxChunks];
+  double total[kScanWaves];
+  uint64_t part[kScanWaves];
+  int listed, lo, hi;
+};
+
+template <int DT>
+__global__ void __launch_bounds__(kScan) sample_select_kernel(SampleArgs a) {
+  __shared__ SelectSmem s;
   const int row = blockIdx.x / a.C, c = blockIdx.x - row * a.C, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const Settings set(a, row);
-  if (set.mode == kAll) return;  // block-uniform
-  const void* const src = row_of<DT>(a, row);
-  float v[NV / 8][8];
-#pragma unroll
-  for (int j = 0; j < NV / 8; ++j) load_logits<DT>(src, (c << a.lg_chunk) + j * kTileTokens + tid * 8, a.V, v[j]);
+  const Settings& set = a.of(row);
+  const int mode = set.mode;
+  if (mode != kTopP && mode != kMinP) return;  // block-uniform
   const int64_t at0 = static_cast<int64_t>(row) * a.C, at = at0 + c;
-  const float m = row_top(a, row), mt = tame(m);
-  if (m == -INFINITY) {  // nothing to keep
+  float m = -INFINITY;
+  for (int i = lane; i < a.C; i += 64) m = fmaxf(m, a.top[at0 + i]);
+  m = wave_all(m, Max{});
+  if (tid == 0) s.listed = 0;
+  if (m == -INFINITY) {
     if (tid == 0) {
-      a.mass[at] = 0.0;
+      a.kept[at] = 0.0;
       a.listed[at] = 0;
-      if (c == 0) a.state[row] = RowState{0.0, 0, 0, 0, m, 0.0};
     }
     return;
   }
-  if (set.mode == kMinP) {
-    double sum = 0.0;
-    // a logit this far below the maximum weighs less than min_p, by a margin for the rounding of both sides
-    const float far = static_cast<float>((log2(set.m) - 0.001) / set.c * (1 + 1e-6) + static_cast<double>(mt) - 1e-6 * fabs(static_cast<double>(mt)));
-#pragma unroll
-    for (int j = 0; j < NV / 8; ++j)
+  const float mt = tame(m);
+  const double c2 = set.c, least = set.m;
+  const int top = grid_of(mt);
+  uint64_t sum = 0, on = 0;
+  if (mode == kMinP) {
+    __syncthreads();
+    const float x1 = mt - set.far, far = fmaxf(-3.4028235e38f, x1 - 2e-7f * (fabsf(mt) + fabsf(x1)));
+    each_run<DT>(a, row, c, m, [&](const float (&v)[8], int r, int) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float x = tame(v[j][e], m);
-        if (x >= far) {
-          const double w = weight(x, mt, set.c);
-          sum += w >= set.m ? w : 0.0;
+        bool take = v[e] >= far;
+        if (__any(take)) {
+          const double w = weight(v[e], mt, c2);
+          take = take && w >= least;
+          const uint64_t n = units_of(w);
+          sum += !take ? 0 : n ? n : 1;
+          on |= static_cast<uint64_t>(take) << (8 * r + e);
         }
       }
-    sum = block_all(sum, s_sum, Sum{});
-    if (tid == 0) {
-      a.mass[at] = sum;
-      a.listed[at] = 0;
-      if (c == 0) a.state[row] = RowState{0.0, 0, 0, 0, m, 0.0};
+    });
+  } else {
+    // ---- the row's histogram, as shares of its mass: bin `tid`
+    double mine = 0.0;
+    for (int i = tid; i < a.C; i += kScan) {
+      const float ct = a.top[at0 + i];
+      const bool in = ct != -INFINITY && counts(ct, m);
+      const double f = in ? weight(tame(ct), mt, c2) / kUnit : 0.0;
+      mine += in ? f * a.mass[at0 + i] : 0.0;
+      s.factor[i] = static_cast<float>(f * kUnit);
+      s.off[i] = in ? top - grid_of(tame(ct)) : kBins;
+      s.depth[i] = in ? a.depth[at0 + i] : 0;
     }
-    return;
-  }
-  // ---- the row's histogram: bin `tid`
-  const int top = grid_of(mt);
-  for (int i = tid; i < a.C; i += kThreads) {
-    const float ct = a.top[at0 + i];
-    s_off[i] = ct == -INFINITY ? kBins : top - grid_of(tame(ct, m));
-    s_factor[i] = ct == -INFINITY ? 0.0 : weight(tame(ct, m), mt, set.c) / (set.mode == kTopP ? kUnit : 1.0);
-    if (set.mode == kTopK && ct != -INFINITY) s_factor[i] = 1.0;
-  }
-  if (tid == 0) {
-    s_lo = kTail;
-    s_hi = kTail;
-    s_listed = 0;
-  }
-  __syncthreads();
-  double mine = 0.0, all = 0.0;
-  uint64_t own = 0;
-  if (tid < kTail) {
-    for (int i = 0; i < a.C; ++i) {
-      const int b = tid - s_off[i];
-      if (b >= 0) {
-        const uint64_t h = a.hist[(at0 + i) * kBins + b];
-        mine += static_cast<double>(h) * s_factor[i];
-        if (i == c) own = h;
+    const double total = block_all<kScanWaves>(mine, s.total, Sum{});  // in a fixed order
+    float share = 0.f;
+    for (int i0 = 0; i0 < a.C; i0 += 8) {
+      uint64_t h[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int k = i0 + i, b = k < a.C ? tid - s.off[k] : -1;
+        h[i] = b >= 0 && b < s.depth[min(k, a.C - 1)] && b < kTail ? a.hist[(at0 + k) * kBins + b] : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i0 + i < a.C) share += static_cast<float>(h[i]) * 0x1p-48f * s.factor[i0 + i];
+    }
+    s.bins[tid] = tid < kTail ? share * static_cast<float>(1.0 / total) : 0.f;
+    __syncthreads();
+    if (wave == 0) {
+      float h[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = s.bins[8 * lane + i];
+      // sums of shares in float, off by less than 2^-18
+      const float p = static_cast<float>(set.p);
+      int lo = reach_bin(h, p - 0x1p-17f);
+      const int hi = reach_bin(h, p + 0x1p-17f);
+      // at most so many tokens down to there: a bin's mass over the least weight in it
+      float few = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int b = 8 * lane + i;
+        const float edge = static_cast<float>((top - b) * 0.0625 - mt) * static_cast<float>(c2);
+        if (b <= hi && h[i] > 0.f) few += h[i] * static_cast<float>(total) / fmaxf(__builtin_amdgcn_exp2f(fmaxf(edge, -120.f)), 1e-30f);
+      }
+      few = wave_all(few, Sum{});
+      if (hi < kTail && few < kFew) {
+        lo = 0;
+      } else if (least > 0.0) {  // what is certain is above min-p's border, too
+        const double edge = log2(least) / c2, slack = 1e-5 * (1.0 + fabs(edge) + fabs(static_cast<double>(mt)));
+        lo = min(lo, max(0, bin_of(static_cast<float>(fmin(mt + edge + slack, 3e38)), top)));
+      }
+      if (lane == 0) {
+        s.lo = lo;
+        s.hi = hi;
+        if (c == 0) a.cut[row] = RowCut{total, lo, hi};
       }
     }
-  }
-  for (int i = 0; i < a.C; ++i) all += static_cast<double>(a.total[at0 + i]) * s_factor[i];
-  double upto = wave_scan(mine);
-  if (lane == 63) s_sum[wave] = upto;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) upto += s_sum[w];
-  // the bins' masses are off by less than 2^-24 of the total
-  const double margin = set.mode == kTopP ? all * 0x1p-20 : 0.5;
-  const double goal = set.mode == kTopP ? set.p * all : static_cast<double>(set.k);
-  if (tid < kTail) {
-    if (upto >= goal - margin) atomicMin(&s_lo, tid);
-    if (upto >= goal + (set.mode == kTopP ? margin : -margin)) atomicMin(&s_hi, tid);
-  }
-  __syncthreads();
-  int lo = set.mode == kTopK ? 0 : s_lo;
-  int hi = s_hi;
-  bool cut = true;
-  if (set.mode == kTopP && set.m > 0.0) {  // bins in which min-p's border can lie
-    const double edge = log2(set.m) / set.c, slack = 1e-5 * (1.0 + fabs(edge) + fabs(static_cast<double>(mt)));
-    const int near = bin_of(static_cast<float>(mt + edge + slack), top), far = bin_of(static_cast<float>(mt + edge - slack), top);
-    if (far < lo) {  // stricter than top-p
-      lo = near < 0 ? 0 : near;
-      hi = far;
-      cut = false;
-    } else if (near < lo) {
-      lo = near < 0 ? 0 : near;
-    }
-  }
-  // ---- certain mass and listed tokens of this chunk
-  own = tid < lo ? own : 0;
-  own = block_all(own, s_own, Sum{});
+    __syncthreads();
+    const int lo = s.lo, hi = s.hi;
+    if (a.top[at] != -INFINITY && bin_of(tame(a.top[at], m), top) <= hi)  // else the chunk has nothing to list
+      each_run<DT>(a, row, c, m, [&](const float (&v)[8], int r, int) {
 #pragma unroll
-  for (int j = 0; j < NV / 8; ++j)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float x = tame(v[j][e], m);
-      const int b = bin_of(x, top);
-      const bool on = x != -INFINITY && b >= lo && b <= hi;
-      const uint64_t some = __ballot(on);
-      if (!some) continue;
-      int to = 0;
-      if (lane == 0) to = atomicAdd(&s_listed, __popcll(some));
-      to = __shfl(to, 0, 64) + __popcll(some & ((1ull << lane) - 1));
-      if (on) a.list[(at << a.lg_chunk) + to] = static_cast<uint16_t>(j * kTileTokens + tid * 8 + e);
-    }
-  __syncthreads();
+        for (int e = 0; e < 8; ++e) {
+          const int b = bin_of(v[e], top);
+          const bool certain = b < lo;
+          if (__any(certain)) {
+            const uint64_t n = units_of(weight(v[e], mt, c2));
+            sum += certain ? n : 0;
+          }
+          on |= static_cast<uint64_t>(!certain && b <= hi && v[e] != -INFINITY) << (8 * r + e);
+        }
+      });
+  }
+  list_tokens<DT>(a, row, c, m, on, &s.listed);
+  sum = block_all<kScanWaves>(sum, s.part, Sum{});
   if (tid == 0) {
-    a.mass[at] = static_cast<double>(own) * s_factor[c];
-    a.listed[at] = s_listed;
-    if (c == 0) a.state[row] = RowState{goal, cut, 0, 0, m, 0.0};
+    a.kept[at] = static_cast<double>(sum) * (1.0 / kUnit);
+    a.listed[at] = s.listed;
   }
 }
 
-// ---------------------------------------------------------------- draw
-struct DrawSmem {
-  uint64_t hist[256];
+// ---------------------------------------------------------------- finish
+constexpr int kSegments = 2048;  // runs of 64 listed tokens that the table holds
+
+struct FinishSmem {
+  uint64_t token[kShort];  // key, then the complement of the index: larger ones rank first
+  uint64_t value[kShort];
+  uint32_t segment[kSegments];  // chunk, run of 64
+  union {
+    uint64_t digits[256];
+    uint32_t bins[kBins];
+  };
   uint64_t part[kWaves];
   double sum[kWaves];
-  float top[kWaves];
-  uint32_t keys[kWaves];
-  double mass[kMaxChunks];
-  uint64_t extra[kMaxChunks];  // kept among the listed tokens
-  int off[kMaxChunks];         // a chunk's first listed token
-  float v[kShort];
-  int x[kShort];
-  uint64_t rest, tie;
+  double mass[kMaxChunks];     // of a row without filters, relative to its maximum
+  uint64_t extra[kMaxChunks];  // kept tokens' mass as integers
+  int listed[kMaxChunks];      // -1: its tokens are read from the row
+  float top[kMaxChunks];
+  uint64_t rest;
   uint32_t digit;
-  int chunk, pick;
+  int segments, raw, lo, hi, n, chunk, pick;
   double bar;
 };
 
-// The listed tokens of a row: fn(logit, index), every thread some of them
+// The tokens of a row that may be kept, fn(logit, index): the chunks' lists, 64 to a wave, and the chunks whose list
+// does not hold them, by the whole block.
 template <int DT>
-struct Listed {
+struct Candidates {
   const SampleArgs& a;
-  DrawSmem& s;
-  const void* src;
-  int row, n;
+  const FinishSmem& s;
+  int row;
   float m;
-  __device__ __forceinline__ Listed(const SampleArgs& a_, DrawSmem& s_, int row_, float m_) : a(a_), s(s_), src(row_of<DT>(a_, row_)), row(row_), m(m_) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (wave == 0) {
-      int run = 0;
-      for (int c0 = 0; c0 < a.C; c0 += 64) {
-        const int k = c0 + lane < a.C ? a.listed[static_cast<int64_t>(row) * a.C + c0 + lane] : 0;
-        const int upto = wave_scan(k);
-        if (c0 + lane < a.C) s.off[c0 + lane] = run + upto - k;
-        run += __shfl(upto, 63, 64);
-      }
-      if (lane == 0) s.pick = run;
-    }
-    __syncthreads();
-    n = s.pick;
-    if (n <= kShort) {
-      far([&](float v, int x, int at) {
-        s.v[at] = v;
-        s.x[at] = x;
-      });
-      __syncthreads();
-    }
-  }
-  template <class Fn>
-  __device__ __forceinline__ void far(Fn fn) const {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int c = wave; c < a.C; c += kWaves) {
-      const int64_t at = static_cast<int64_t>(row) * a.C + c;
-      const int k = (c + 1 < a.C ? s.off[c + 1] : n) - s.off[c];
-      for (int i = lane; i < k; i += 64) {
-        const int x = (c << a.lg_chunk) + a.list[(at << a.lg_chunk) + i];
-        fn(tame(load_act<DT>(src, x), m), x, s.off[c] + i);
-      }
-    }
-  }
   template <class Fn>
   __device__ __forceinline__ void each(Fn fn) const {
-    if (n <= kShort) {
-      for (int i = threadIdx.x; i < n; i += kThreads) fn(s.v[i], s.x[i]);
-    } else {
-      far([&](float v, int x, int) { fn(v, x); });
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const auto load = [&](int g, uint2& t) {
+      if (g >= s.segments) return false;
+      const uint32_t seg = s.segment[g];
+      const int c = seg >> 16, i = (seg & 0xFFFF) * 64 + lane;
+      const bool on = i < s.listed[c];
+      if (on) t = a.list[((static_cast<int64_t>(row) * a.C + c) << a.lg_room) + i];
+      return on;
+    };
+    uint2 next{};
+    bool more = load(wave, next);
+#pragma unroll 1
+    for (int g = wave; g < s.segments; g += kWaves) {
+      const uint2 t = next;
+      const bool on = more;
+      more = load(g + kWaves, next);  // flies meanwhile
+      if (on) fn(__uint_as_float(t.x), static_cast<int>(t.y));
+    }
+    if (!s.raw) return;
+#pragma unroll 1
+    for (int c = 0; c < a.C; ++c) {
+      if (s.listed[c] >= 0) continue;
+      const int end = min(a.V, (c + 1) << a.lg_chunk);
+#pragma unroll 1
+      for (int x = (c << a.lg_chunk) + tid * 8; x < end; x += kThreads * 8) {
+        float v[8];
+        load_logits<DT>(row_of<DT>(a, row), x, a.V, v);
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {
+          const float y = tame(v[0], m);
+          if (y != -INFINITY) fn(y, x + e);
+#pragma unroll
+          for (int i = 0; i < 7; ++i) v[i] = v[i + 1];
+        }
+      }
     }
   }
 };
 
-// Among listed tokens: the digit in which the running sum of their values, from the largest digit down (FALL) or
-// from the smallest up, reaches goal; goal becomes what is left of it in front of that digit, and `in` the digit's sum.
-// Where the sum never reaches it: the last digit that holds any.
-template <bool FALL, class Each>
-__device__ __forceinline__ uint32_t pick_digit(DrawSmem& s, uint64_t& goal, uint64_t& in, Each each) {
+__device__ __forceinline__ uint64_t token_of(float v, int x) { return static_cast<uint64_t>(key_of(v)) << 32 | static_cast<uint32_t>(~x); }
+__device__ __forceinline__ float logit_of(uint64_t token) {
+  const uint32_t k = static_cast<uint32_t>(token >> 32);
+  return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+__device__ __forceinline__ int index_of(uint64_t token) { return static_cast<int>(~static_cast<uint32_t>(token)); }
+
+// Sorted by the block, larger ones first (FALL) or last; n <= kShort
+template <bool FALL>
+__device__ __forceinline__ void sort_tokens(uint64_t* t, int n) {
   const int tid = threadIdx.x;
-  if (tid < 256) s.hist[tid] = 0;
+  int lg = 1;
+  while ((1 << lg) < n) ++lg;
+  for (int i = n + tid; i < 1 << lg; i += kThreads) t[i] = FALL ? 0 : ~0ull;
   __syncthreads();
-  each([&](uint32_t digit, uint64_t value) {
-    atomicAdd(reinterpret_cast<unsigned long long*>(s.hist + digit), static_cast<unsigned long long>(value));
-  });
+#pragma unroll 1
+  for (int size = 1; size <= lg; ++size)
+#pragma unroll 1
+    for (int stride = size - 1; stride >= 0; --stride) {
+      if (tid < 1 << (lg - 1)) {
+        const int i = (tid >> stride << (stride + 1)) + (tid & ((1 << stride) - 1)), j = i + (1 << stride);
+        const uint64_t x = t[i], y = t[j];
+        if ((x < y) == ((((i >> size) & 1) == 0) == FALL) && x != y) {
+          t[i] = y;
+          t[j] = x;
+        }
+      }
+      __syncthreads();
+    }
+}
+static_assert(kShort <= 2 * kThreads, "a pair per thread");
+
+// inclusive sums of two values per thread, and the total
+__device__ __forceinline__ uint64_t block_scan2(uint64_t v0, uint64_t v1, uint64_t* s_part, uint64_t& upto0, uint64_t& upto1) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint64_t upto = wave_scan(v0 + v1);
+  if (lane == 63) s_part[wave] = upto;
+  __syncthreads();
+  uint64_t all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) upto += s_part[w];
+    all += s_part[w];
+  }
+  __syncthreads();
+  upto1 = upto;
+  upto0 = upto - v1;
+  return all;
+}
+
+// Among some tokens: the digit in which the running sum of their values, from the largest digit down (FALL) or
+// from the smallest up, reaches goal; goal becomes what is left of it in front of that digit.  Where the sum never
+// reaches it: the last digit that holds any.
+template <bool FALL, class Each>
+__device__ __forceinline__ uint32_t pick_digit(FinishSmem& s, uint64_t& goal, Each each) {
+  const int tid = threadIdx.x;
+  if (tid < 256) s.digits[tid] = 0;
+  __syncthreads();
+  each([&](uint32_t digit, uint64_t value) { add_lds(s.digits + digit, value); });
   __syncthreads();
   if (tid < 64) {
     uint64_t h[4], sum = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      h[i] = s.hist[FALL ? 255 - (4 * tid + i) : 4 * tid + i];
+      h[i] = s.digits[FALL ? 255 - (4 * tid + i) : 4 * tid + i];
       sum += h[i];
     }
     const uint64_t upto = wave_scan(sum);
     const uint64_t over = __ballot(sum != 0 && upto >= goal), some = __ballot(sum != 0);
     const int l = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : 0;
     if (tid == l) {
-      uint64_t before = upto - sum, at = before, held = 0;
+      uint64_t before = upto - sum, at = before;
       int d = 0;
       bool done = false;
 #pragma unroll
@@ -480,7 +713,6 @@ __device__ __forceinline__ uint32_t pick_digit(DrawSmem& s, uint64_t& goal, uint
         if (!done && h[i] != 0) {
           d = i;
           before = at;
-          held = h[i];
           done = at + h[i] >= goal;
         }
         at += h[i];
@@ -488,24 +720,22 @@ __device__ __forceinline__ uint32_t pick_digit(DrawSmem& s, uint64_t& goal, uint
       const int pos = 4 * l + d;
       s.digit = FALL ? 255 - pos : pos;
       s.rest = goal > before ? goal - before : 0;
-      s.tie = held;
     }
   }
   __syncthreads();
   goal = s.rest;
-  in = s.tie;
   return s.digit;
 }
 
-// The border in rank: of the listed tokens with key(...) below or at it.  value: 1 (by rank) or the token's mass; kept are
-// the tokens whose predecessors' values sum to less than goal (>= 1).
+// The border in rank among tokens that are too many to be sorted.  value: 1 (by rank) or the token's mass, 0: not one
+// of them; kept are the tokens whose predecessors' values sum to less than goal (>= 1).
 template <int DT, class Value>
-__device__ __forceinline__ void pick_border(const Listed<DT>& list, DrawSmem& s, uint64_t goal, Value value, uint32_t& key, int& last) {
+__device__ __forceinline__ void pick_border(const Candidates<DT>& all, FinishSmem& s, uint64_t goal, Value value, uint32_t& key, int& last) {
   uint32_t prefix = 0, mask = 0;
-  uint64_t in = 0;
+#pragma unroll 1
   for (int shift = 24; shift >= 0; shift -= 8) {
-    const uint32_t d = pick_digit<true>(s, goal, in, [&](auto add) {
-      list.each([&](float v, int x) {
+    const uint32_t d = pick_digit<true>(s, goal, [&](auto add) {
+      all.each([&](float v, int x) {
         const uint32_t k = key_of(v);
         if ((k & mask) == prefix) {
           const uint64_t n = value(v, x);
@@ -519,16 +749,16 @@ __device__ __forceinline__ void pick_border(const Listed<DT>& list, DrawSmem& s,
   key = prefix;
   // equal logits have equal values: how many of them are kept, the first in index order
   uint64_t one = 0, ties = 0;
-  list.each([&](float v, int x) {
+  all.each([&](float v, int x) {
     if (key_of(v) == key) {
       const uint64_t n = value(v, x);
       one = n > one ? n : one;
       ties += n != 0;
     }
   });
-  one = block_all(one, s.part, Max{});
+  one = block_all<kWaves>(one, s.part, Max{});
   __syncthreads();
-  ties = block_all(ties, s.part, Sum{});
+  ties = block_all<kWaves>(ties, s.part, Sum{});
   __syncthreads();
   uint64_t keep = one ? (goal + one - 1) / one : 1;
   if (keep < 1) keep = 1;
@@ -536,9 +766,10 @@ __device__ __forceinline__ void pick_border(const Listed<DT>& list, DrawSmem& s,
   if (keep >= ties) return;
   uint32_t at = 0;
   mask = 0;
+#pragma unroll 1
   for (int shift = 16; shift >= 0; shift -= 8) {
-    const uint32_t d = pick_digit<false>(s, keep, in, [&](auto add) {
-      list.each([&](float v, int x) {
+    const uint32_t d = pick_digit<false>(s, keep, [&](auto add) {
+      all.each([&](float v, int x) {
         if (key_of(v) == key && (static_cast<uint32_t>(x) & mask) == at && value(v, x)) add((x >> shift) & 255, 1);
       });
     });
@@ -549,100 +780,318 @@ __device__ __forceinline__ void pick_border(const Listed<DT>& list, DrawSmem& s,
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a) {
-  __shared__ DrawSmem s;
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const Settings set(a, row);
+__global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
+  __shared__ FinishSmem s;
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Settings& set = a.of(row);
+  const int mode = set.mode;
   const int64_t at0 = static_cast<int64_t>(row) * a.C;
-  const float m = row_top(a, row), mt = tame(m);
+  const RowCut cut = mode == kTopP ? a.cut[row] : RowCut{0.0, 0, kTail};
+  const int room = 1 << a.lg_room;
+  for (int c = tid; c < a.C; c += kThreads) {
+    s.top[c] = a.top[at0 + c];
+    const int n = mode == kAll ? 0 : a.listed[at0 + c];
+    s.listed[c] = n <= room ? n : -1;
+    s.mass[c] = mode == kTopK ? 0.0 : mode == kAll ? a.mass[at0 + c] : a.kept[at0 + c];
+    s.extra[c] = 0;
+  }
+  if (tid < kBins) s.bins[tid] = 0;
+  if (tid == 0) {
+    s.n = 0;
+    s.raw = 0;
+  }
+  __syncthreads();
+  float m = -INFINITY;
+  for (int c = lane; c < a.C; c += 64) m = fmaxf(m, s.top[c]);
+  m = wave_all(m, Max{});
+  const float mt = tame(m);
   if (m == -INFINITY) {  // no token has a weight
     if (tid == 0) {
       if (a.tokens) a.tokens[row] = -1;
-      else a.state[row] = RowState{0.0, 0, 0xFFFFFFFFu, -1, m, 0.0};
+      else a.state[row] = RowState{0xFFFFFFFFu, -1, m, mode != kAll, 0.0};
     }
     return;
   }
-  for (int c = tid; c < a.C; c += kThreads) {
-    double f = a.mass[at0 + c];
-    if (set.mode == kAll) {
-      const float ct = a.top[at0 + c];
-      f = ct == -INFINITY ? 0.0 : f * weight(tame(ct, m), mt, set.c);
-    }
-    s.mass[c] = set.mode == kTopK ? 0.0 : f;
-    s.extra[c] = 0;
-  }
-  __syncthreads();
-
-  // ---- the border
-  uint32_t key = 0;
+  const int top = grid_of(mt);
+  const double c2 = set.c, least = set.m;
+  const Candidates<DT> all{a, s, row, m};
+  uint32_t key = 0;  // the border
   int last = 0x7FFFFFFF;
-  double unit = 1.0;
-  if (set.mode >= kTopP) {
-    const RowState st = a.state[row];
-    const Listed<DT> list(a, s, row, m);
-    float peak = -INFINITY;
-    list.each([&](float v, int) { peak = fmaxf(peak, v); });
-    peak = block_all(peak, s.top, Max{});
-    // masses of listed tokens as integers: the heaviest is 2^(61 - bits of their number)
-    const double big = peak == -INFINITY ? 1.0 : weight(peak, mt, set.c);
-    unit = big > 0.0 ? ldexp(1.0, 30 + __builtin_clz(list.n | 1)) / big : 0.0;
-    if (!(unit < INFINITY)) unit = 0.0;
-    const auto integer = [&](float v) -> uint64_t {
-      const double w = weight(v, mt, set.c);
-      if (!(w > 0.0)) return 0;
-      const uint64_t n = static_cast<uint64_t>(w * unit + 0.5);
-      return n ? n : 1;
-    };
-    if (set.mode == kTopK) {
-      pick_border(list, s, static_cast<uint64_t>(set.k), [](float, int) -> uint64_t { return 1; }, key, last);
-      if (set.p < 1.0) {
-        const uint32_t key_k = key;
-        const int last_k = last;
-        const auto value = [&](float v, int x) -> uint64_t {
-          const uint32_t k = key_of(v);
-          return k > key_k || (k == key_k && x <= last_k) ? integer(v) : 0;
-        };
-        uint64_t sum = 0;
-        list.each([&](float v, int x) { sum += value(v, x); });
-        __syncthreads();
-        sum = block_all(sum, s.part, Sum{});
-        __syncthreads();
-        const double goal = ceil(set.p * static_cast<double>(sum));
-        pick_border(list, s, goal >= 1.0 ? static_cast<uint64_t>(goal) : 1, value, key, last);
+  double unit = 1.0;  // listed tokens' masses as integers
+  if (mode == kAll) {
+    for (int c = tid; c < a.C; c += kThreads)
+      s.mass[c] = s.top[c] == -INFINITY || !counts(s.top[c], m) ? 0.0 : s.mass[c] * weight(tame(s.top[c]), mt, c2);
+    __syncthreads();
+  } else {
+    // ---- a table of the lists' runs of 64, by the first wave
+    if (wave == 0) {
+      int run = 0, bad = 0, last_n = 0;
+      for (int c0 = 0; c0 < a.C; c0 += 64) {
+        const int c = c0 + lane;
+        int n = c < a.C && counts(s.top[c], m) ? s.listed[c] : 0;
+        if (c < a.C && !counts(s.top[c], m)) s.listed[c] = 0;
+        int segs = n > 0 ? (n + 63) / 64 : 0;
+        const int upto = wave_scan32(segs), from = run + upto - segs;
+        if (from + segs > kSegments) {  // no place in the table
+          n = -1;
+          s.listed[c] = -1;
+          segs = 0;
+        }
+        for (int i = 0; i < segs; ++i) s.segment[from + i] = static_cast<uint32_t>(c) << 16 | static_cast<uint32_t>(i);
+        bad |= n < 0;
+        const uint64_t in = __ballot(segs > 0);
+        if (in) last_n = __builtin_amdgcn_readlane(from + segs, 63 - __builtin_clzll(in));
+        run += __builtin_amdgcn_readlane(upto, 63);
       }
-    } else if (st.cut) {
-      double certain = 0.0;
-      for (int c = 0; c < a.C; ++c) certain += s.mass[c];
-      const double goal = ceil((st.goal - certain) * unit);
-      if (goal >= 1.0 || !(certain > 0.0)) {
-        pick_border(list, s, goal >= 1.0 ? static_cast<uint64_t>(goal) : 1, [&](float v, int) { return integer(v); }, key, last);
-      } else {  // what is certain reaches the goal
-        key = key_of(peak);
-        last = -1;
-      }
+      if (lane == 0) s.segments = min(last_n, kSegments);
+      if (__any(bad) && lane == 0) s.raw = 1;
     }
-    list.each([&](float v, int x) {
-      const uint32_t k = key_of(v);
-      if ((k > key || (k == key && x <= last)) && weight(v, mt, set.c) >= set.m)
-        atomicAdd(reinterpret_cast<unsigned long long*>(s.extra + (x >> a.lg_chunk)), static_cast<unsigned long long>(integer(v)));
+    __syncthreads();
+    int hi = cut.hi;
+    const int lo = cut.lo;
+
+    // ---- the listed tokens, as far as they can be sorted
+    float peak = -INFINITY;
+    all.each([&](float v, int x) {
+      const int b = bin_of(v, top);
+      const bool on = b >= lo && b <= hi && (mode != kMinP || weight(v, mt, c2) >= least);
+      const uint64_t some = __ballot(on);
+      if (!some) return;
+      int to = 0;
+      const int first = __builtin_ctzll(some);
+      if (lane == first) to = atomicAdd(&s.n, __popcll(some));
+      to = __builtin_amdgcn_readlane(to, first) + __popcll(some & ((1ull << lane) - 1));
+      if (on) {
+        peak = fmaxf(peak, v);
+        if (to < kShort) s.token[to] = token_of(v, x);
+      }
     });
     __syncthreads();
+    int n = s.n;
+    if (mode == kTopK && n > 64 && n <= kShort) {
+      // every chunk listed its own first k: of them all, those down to the bin that k reach
+      uint64_t t[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        t[i] = tid + i * kThreads < n ? s.token[tid + i * kThreads] : 0;
+        if (tid + i * kThreads < n) atomicAdd(s.bins + bin_of(logit_of(t[i]), top), 1u);
+      }
+      __syncthreads();
+      if (wave == 0) {
+        int h[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = 8 * lane + i < kTail ? static_cast<int>(s.bins[8 * lane + i]) : 0;
+        const int bin = reach_bin(h, set.k);
+        if (lane == 0) {
+          s.hi = bin;
+          s.n = 0;
+        }
+      }
+      __syncthreads();
+      hi = s.hi;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bool on = tid + i * kThreads < n && bin_of(logit_of(t[i]), top) <= hi;
+        const uint64_t some = __ballot(on);
+        int to = 0;
+        if (some && lane == 0) to = atomicAdd(&s.n, __popcll(some));
+        to = __builtin_amdgcn_readfirstlane(to) + __popcll(some & ((1ull << lane) - 1));
+        if (on) s.token[to] = t[i];
+      }
+      __syncthreads();
+      n = s.n;
+    }
+    const bool alone = n <= kShort && lo == 0;  // the tokens in s.token are all that can be kept
+    const double goal = set.p * cut.total;
+    const auto ceiling = [](double g) -> uint64_t { return g >= 0x1p63 ? ~0ull : g >= 1.0 ? static_cast<uint64_t>(ceil(g)) : 1; };
+    const auto integer = [&](double w) -> uint64_t {
+      if (!(w > 0.0)) return 0;
+      const uint64_t x = static_cast<uint64_t>(w * unit + 0.5);
+      return x ? x : 1;
+    };
+
+    if (n <= 64 && alone) {
+      // ---- ranked by one wave: lane i has token i, and meets every other
+      if (wave != 0) return;
+      const uint64_t t = lane < n ? s.token[lane] : 0;
+      const double w = lane < n ? weight(logit_of(t), mt, c2) : 0.0;
+      unit = 0x1p55;  // the maximum is among them
+      const uint64_t val = integer(w);
+      const int x = index_of(t);
+      s.token[lane] = t;
+      s.value[lane] = val;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      int rank = 0;
+      uint64_t before = 0;
+#pragma unroll 8
+      for (int j = 0; j < ((n + 7) & ~7); ++j) {
+        const bool ahead = s.token[j] > t;
+        rank += ahead;
+        before += ahead ? s.value[j] : 0;
+      }
+      const bool in = lane < n && (mode != kTopK || rank < set.k);
+      uint64_t bar = ~0ull;
+      if (mode == kTopP) bar = ceiling(goal * unit);
+      else if (mode == kTopK && set.p < 1.0) bar = ceiling(set.p * static_cast<double>(wave_all(in ? val : 0, Sum{})));
+      const bool on = in && before < bar && w >= least;
+      const uint64_t sum = wave_all(on ? val : 0, Sum{});
+      if (a.probs) {
+        if (on) a.probs[static_cast<int64_t>(row) * a.V + x] = static_cast<float>(w * (unit / static_cast<double>(sum)));
+        if (lane == 0) a.state[row] = RowState{0, 0, m, 1, 0.0};
+        return;
+      }
+      const double pass = static_cast<double>(a.uniforms[row]) * static_cast<double>(sum);
+      s.value[lane] = on ? val : 0;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      uint64_t upto = 0;  // of the kept tokens at or before it
+#pragma unroll 8
+      for (int j = 0; j < ((n + 7) & ~7); ++j) upto += index_of(s.token[j]) <= x ? s.value[j] : 0;
+      // the first index that passes; the last one, should u be 1 or more
+      const bool over = on && static_cast<double>(upto) > pass;
+      const int first = -wave_all(over ? -x : -0x7FFFFFFF, Max{}), end = wave_all(on ? x : -1, Max{});
+      if (lane == 0) a.tokens[row] = first < 0x7FFFFFFF ? first : end;
+      return;
+    }
+
+    double certain = 0.0;  // stands above the listed tokens
+    if (mode == kTopP && lo > 0)
+      for (int c = 0; c < a.C; ++c) certain += s.mass[c];
+    peak = block_all<kWaves>(peak, reinterpret_cast<float*>(s.part), Max{});
+    __syncthreads();
+    // the heaviest is 2^(61 - bits of their number)
+    const double big = peak == -INFINITY ? 1.0 : weight(peak, mt, c2);
+    unit = big > 0.0 ? ldexp(1.0, 30 + __builtin_clz(n | 1)) / big : 0.0;
+    if (!(unit < INFINITY)) unit = 0.0;
+    const double g = (goal - certain) * unit;
+    const bool none = mode == kTopP && certain > 0.0 && !(g > 0.0);  // what is certain reaches the goal
+    int kept = 0;
+    if (n <= kShort) {
+      // ---- sorted: kept are the first of them
+      sort_tokens<true>(s.token, n);
+      uint64_t val[2], upto[2];
+      double w[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = 2 * tid + i;
+        w[i] = at < n ? weight(logit_of(s.token[at]), mt, c2) : 0.0;
+        val[i] = at < n && !(mode == kTopK && at >= set.k) ? integer(w[i]) : 0;
+        s.value[at] = val[i];
+      }
+      const uint64_t sum = block_scan2(val[0], val[1], s.part, upto[0], upto[1]);
+      uint64_t bar = ~0ull;  // predecessors of a kept token sum to less
+      if (mode == kTopP) bar = ceiling(g);
+      else if (mode == kTopK && set.p < 1.0) bar = ceiling(set.p * static_cast<double>(sum));
+      int on = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = 2 * tid + i;
+        on += at < n && !(mode == kTopK && at >= set.k) && upto[i] - val[i] < bar && w[i] >= least && !none;
+      }
+      kept = block_all<kWaves>(on, reinterpret_cast<int*>(s.part), Sum{});
+      __syncthreads();
+      key = kept ? static_cast<uint32_t>(s.token[kept - 1] >> 32) : key_of(peak);
+      last = kept ? index_of(s.token[kept - 1]) : -1;
+      if (alone && a.probs) {
+        uint64_t mass = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) mass += 2 * tid + i < kept ? val[i] : 0;
+        mass = block_all<kWaves>(mass, s.part, Sum{});
+        const double inverse = unit / static_cast<double>(mass);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (2 * tid + i < kept)
+            a.probs[static_cast<int64_t>(row) * a.V + index_of(s.token[2 * tid + i])] = static_cast<float>(w[i] * inverse);
+        if (tid == 0) a.state[row] = RowState{0, 0, m, 1, 0.0};
+        return;
+      }
+    } else if (none) {
+      key = key_of(peak);
+      last = -1;
+    } else {
+      // ---- selected by digits
+      const auto in = [&](float v) {
+        const int b = bin_of(v, top);
+        return b >= lo && b <= hi;
+      };
+      if (mode == kTopK) {
+        pick_border(all, s, static_cast<uint64_t>(set.k), [&](float, int) -> uint64_t { return 1; }, key, last);
+        if (set.p < 1.0) {
+          const uint32_t key_k = key;
+          const int last_k = last;
+          const auto value = [&](float v, int x) -> uint64_t {
+            const uint32_t k = key_of(v);
+            return k > key_k || (k == key_k && x <= last_k) ? integer(weight(v, mt, c2)) : 0;
+          };
+          uint64_t sum = 0;
+          all.each([&](float v, int x) { sum += value(v, x); });
+          sum = block_all<kWaves>(sum, s.part, Sum{});
+          __syncthreads();
+          pick_border(all, s, ceiling(set.p * static_cast<double>(sum)), value, key, last);
+        }
+      } else if (mode == kTopP) {
+        pick_border(all, s, ceiling(g), [&](float v, int) -> uint64_t { return in(v) ? integer(weight(v, mt, c2)) : 0; }, key, last);
+      }
+    }
+    if (alone) {
+      // ---- all that is kept stands in s.token: drawn from it, in index order
+      uint64_t t[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = 2 * tid + i;
+        t[i] = at < kept ? static_cast<uint64_t>(index_of(s.token[at])) << 32 | static_cast<uint32_t>(at) : 0;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (2 * tid + i < kept) s.token[2 * tid + i] = t[i];
+      __syncthreads();
+      sort_tokens<false>(s.token, kept);
+      uint64_t val[2], upto[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = 2 * tid + i;
+        val[i] = at < kept ? s.value[static_cast<uint32_t>(s.token[at])] : 0;
+      }
+      const uint64_t sum = block_scan2(val[0], val[1], s.part, upto[0], upto[1]);
+      const double pass = static_cast<double>(a.uniforms[row]) * static_cast<double>(sum);
+      int below = 0;  // that do not pass; the last one, should u be 1 or more
+#pragma unroll
+      for (int i = 0; i < 2; ++i) below += 2 * tid + i < kept && !(static_cast<double>(upto[i]) > pass);
+      below = block_all<kWaves>(below, reinterpret_cast<int*>(s.part), Sum{});
+      if (tid == 0) a.tokens[row] = static_cast<int64_t>(s.token[min(below, kept - 1)] >> 32);
+      return;
+    }
+    // ---- the chunks' kept masses: what is certain, and the listed tokens up to the border
+    if (mode != kMinP) {
+      const double fine = ldexp(1.0, 30 + __builtin_clz(a.V | 1)) / big;
+      const double units = fine < INFINITY ? fine : 0.0;
+      all.each([&](float v, int x) {
+        const uint32_t k = key_of(v);
+        const int b = bin_of(v, top);
+        if (b >= lo && b <= hi && (k > key || (k == key && x <= last))) {
+          const double w = weight(v, mt, c2);
+          if (w >= least) add_lds(s.extra + (x >> a.lg_chunk), max(static_cast<uint64_t>(w * units + 0.5), static_cast<uint64_t>(w > 0.0)));
+        }
+      });
+      __syncthreads();
+      for (int c = tid; c < a.C; c += kThreads) s.mass[c] += units > 0.0 ? static_cast<double>(s.extra[c]) / units : 0.0;
+      __syncthreads();
+    }
   }
 
   // ---- the chunk: the first whose running sum passes u times the total
-  const auto of_chunk = [&](int c) { return s.mass[c] + (unit > 0.0 ? static_cast<double>(s.extra[c]) / unit : 0.0); };
   if (wave == 0) {
     double sum = 0.0;
-    for (int c = lane; c < a.C; c += 64) sum += of_chunk(c);
+    for (int c = lane; c < a.C; c += 64) sum += s.mass[c];
     const double total = wave_all(sum, Sum{});
     if (!a.tokens) {
-      if (lane == 0) a.state[row] = RowState{0.0, 0, key, last, m, 1.0 / total};
+      if (lane == 0) a.state[row] = RowState{key, last, m, 0, 1.0 / total};
     } else {
       const double goal = static_cast<double>(a.uniforms[row]) * total;
       double run = 0.0, bar = 0.0;
       int chunk = -1;
       for (int c0 = 0; c0 < a.C; c0 += 64) {
-        const double v = c0 + lane < a.C ? of_chunk(c0 + lane) : 0.0;
+        const double v = c0 + lane < a.C ? s.mass[c0 + lane] : 0.0;
         const double upto = wave_scan(v) + run;
         const uint64_t some = __ballot(v > 0.0), over = __ballot(v > 0.0 && upto > goal);
         if (some) {
@@ -671,7 +1120,8 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a) {
   double run = s.bar;  // what is left to pass
   const int end = min(a.V, (chunk + 1) << a.lg_chunk);
   int fallback = -1;   // the last kept token, should rounding leave the bar beyond all of them
-  for (int x0 = chunk << a.lg_chunk; x0 < end; x0 += kTileTokens) {
+#pragma unroll 1
+  for (int x0 = chunk << a.lg_chunk; x0 < end; x0 += kThreads * 8) {
     float v[8];
     const int x = x0 + tid * 8;
     load_logits<DT>(row_of<DT>(a, row), x < end ? x : a.V, a.V, v);
@@ -682,19 +1132,19 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a) {
       const uint32_t k = key_of(y);
       w[e] = 0.0;
       if (y != -INFINITY && (k > key || (k == key && x + e <= last))) {
-        const double ww = weight(y, mt, set.c);
-        w[e] = ww >= set.m ? ww : 0.0;
+        const double ww = weight(y, mt, c2);
+        w[e] = ww >= least ? ww : 0.0;
       }
       sum += w[e];
     }
     double upto = wave_scan(sum);
     if (lane == 63) s.sum[wave] = upto;
     __syncthreads();
-    double before = upto - sum, all = 0.0;
+    double before = upto - sum, tile = 0.0;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
       if (i < wave) before += s.sum[i];
-      all += s.sum[i];
+      tile += s.sum[i];
     }
     double at = before;
     int found = -1;
@@ -710,58 +1160,63 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a) {
     if (found >= 0) atomicMax(&s.pick, 0x7FFFFFFF - found);
     __syncthreads();
     if (s.pick >= 0) break;
-    run -= all;
+    run -= tile;
   }
   if (s.pick < 0) {  // block-uniform
-    const uint32_t most = block_all(static_cast<uint32_t>(fallback + 1), s.keys, Max{});
-    if (tid == 0) a.tokens[row] = static_cast<int64_t>(most) - 1;
+    const int most = block_all<kWaves>(fallback, reinterpret_cast<int*>(s.part), Max{});
+    if (tid == 0) a.tokens[row] = most;
   } else if (tid == 0) {
     a.tokens[row] = 0x7FFFFFFF - s.pick;
   }
 }
 
 // ---------------------------------------------------------------- write
+// `parts` blocks to a row
 template <int DT>
-__global__ void __launch_bounds__(256) sample_write_kernel(SampleArgs a, int tiles) {
-  const int row = blockIdx.x / tiles, x = ((blockIdx.x - row * tiles) * 256 + threadIdx.x) * 8;
-  if (x >= a.V) return;
-  const Settings set(a, row);
+__global__ void __launch_bounds__(256) sample_write_kernel(SampleArgs a, int parts) {
+  const int row = blockIdx.x / parts, part = blockIdx.x - row * parts;
   const RowState st = a.state[row];
-  float v[8], out[8];
-  load_logits<DT>(row_of<DT>(a, row), x, a.V, v);
+  if (st.done) return;
+  const Settings& set = a.of(row);
   const float mt = tame(st.top);
+  const void* const src = row_of<DT>(a, row);
+  for (int x = (part * 256 + static_cast<int>(threadIdx.x)) * 8; x < a.V; x += parts * 2048) {
+    float v[8], out[8];
+    load_logits<DT>(src, x, a.V, v);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float y = tame(v[e], st.top);
-    const uint32_t k = key_of(y);
-    out[e] = 0.f;
-    if (y != -INFINITY && (k > st.key || (k == st.key && x + e <= st.last))) {
-      const double w = weight(y, mt, set.c);
-      out[e] = w >= set.m ? static_cast<float>(w * st.inverse) : 0.f;
+    for (int e = 0; e < 8; ++e) {
+      const float y = tame(v[e], st.top);
+      const uint32_t k = key_of(y);
+      out[e] = 0.f;
+      if (y != -INFINITY && (k > st.key || (k == st.key && x + e <= st.last))) {
+        const double w = weight(y, mt, set.c);
+        out[e] = w >= set.m ? static_cast<float>(w * st.inverse) : 0.f;
+      }
     }
-  }
-  float* const to = a.probs + static_cast<int64_t>(row) * a.V + x;
-  if (x + 8 <= a.V) {
-    __builtin_memcpy(to, out, 32);
-  } else {
-    for (int e = 0; x + e < a.V; ++e) to[e] = out[e];
+    float* const to = a.probs + static_cast<int64_t>(row) * a.V + x;
+    if (x + 8 <= a.V) {
+      __builtin_memcpy(to, out, 32);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (x + e < a.V) to[e] = out[e];
+    }
   }
 }
 
 // ---------------------------------------------------------------- launch
 struct SamplePlan {
-  int nv, C, lg_chunk;
-  int64_t state, top, mass, total, listed, hist, list, bytes;  // offsets
+  int C, lg_chunk;
+  int64_t rows, state, cut, top, mass, kept, listed, depth, hist, list, bytes;  // offsets
 };
 
-// Values a thread takes: as many as leave 512 blocks, two to a compute unit.
+// Tokens of a chunk: as many as leave 1024 blocks, four to a compute unit.
 static SamplePlan plan_sample(int64_t N, int64_t V) {
   SamplePlan p{};
-  p.nv = 32;
-  const auto chunks = [&](int nv) { return (V + kThreads * nv - 1) / (kThreads * nv); };
-  while (p.nv > 8 && N * chunks(p.nv) < 512 && chunks(p.nv / 2) <= kMaxChunks) p.nv /= 2;
-  p.C = static_cast<int>(chunks(p.nv));
-  p.lg_chunk = __builtin_ctz(kThreads * p.nv);
+  p.lg_chunk = 15;
+  const auto chunks = [&](int lg) { return (V + (int64_t(1) << lg) - 1) >> lg; };
+  while (p.lg_chunk > 12 && N * chunks(p.lg_chunk) < 1024 && chunks(p.lg_chunk - 1) <= kMaxChunks) --p.lg_chunk;
+  p.C = static_cast<int>(chunks(p.lg_chunk));
   const int64_t n = N * p.C;
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
@@ -769,13 +1224,16 @@ static SamplePlan plan_sample(int64_t N, int64_t V) {
     at += (bytes + 15) / 16 * 16;
     return here;
   };
+  p.rows = take(N * static_cast<int64_t>(sizeof(Settings)));
   p.state = take(N * static_cast<int64_t>(sizeof(RowState)));
+  p.cut = take(N * static_cast<int64_t>(sizeof(RowCut)));
   p.top = take(n * 4);
   p.mass = take(n * 8);
-  p.total = take(n * 8);
+  p.kept = take(n * 8);
   p.listed = take(n * 4);
+  p.depth = take(n * 4);
   p.hist = take(n * kBins * 8);
-  p.list = take((n << p.lg_chunk) * 2);
+  p.list = take((n << (p.lg_chunk - 2)) * 8);  // a quarter of the tokens
   p.bytes = at;
   return p;
 }
@@ -784,20 +1242,17 @@ static bool sample_shape(int64_t N, int64_t V) {
 }
 
 template <int DT>
-static void launch_sample(const SampleArgs& a, const SamplePlan& p, bool select, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(a.N * p.C));
-  if (p.nv == 32) sample_scan_kernel<DT, 32><<<grid, kThreads, 0, s>>>(a);
-  else if (p.nv == 16) sample_scan_kernel<DT, 16><<<grid, kThreads, 0, s>>>(a);
-  else sample_scan_kernel<DT, 8><<<grid, kThreads, 0, s>>>(a);
-  if (select) {
-    if (p.nv == 32) sample_select_kernel<DT, 32><<<grid, kThreads, 0, s>>>(a);
-    else if (p.nv == 16) sample_select_kernel<DT, 16><<<grid, kThreads, 0, s>>>(a);
-    else sample_select_kernel<DT, 8><<<grid, kThreads, 0, s>>>(a);
-  }
-  sample_draw_kernel<DT><<<dim3(a.N), kThreads, 0, s>>>(a);
+static void launch_sample(const SampleArgs& a, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(a.N * a.C));
+  sample_scan_kernel<DT><<<grid, kScan, 0, s>>>(a);
+  // rows' own settings may be any
+  if (a.rows || a.all.mode == kTopP || a.all.mode == kMinP) sample_select_kernel<DT><<<grid, kScan, 0, s>>>(a);
+  sample_finish_kernel<DT><<<dim3(a.N), kThreads, 0, s>>>(a);
   if (!a.tokens) {
     const int tiles = (a.V + 2047) / 2048;
-    sample_write_kernel<DT><<<dim3(static_cast<unsigned>(a.N) * tiles), 256, 0, s>>>(a, tiles);
+    int parts = (4096 + a.N - 1) / a.N;
+    if (parts > tiles) parts = tiles;
+    sample_write_kernel<DT><<<dim3(static_cast<unsigned>(a.N) * parts), 256, 0, s>>>(a, parts);
   }
 }
 
@@ -819,21 +1274,23 @@ static int run_sample(const char* what, SampleArgs& a, int32_t dtype, double tem
   a.m = min_p;
   a.C = p.C;
   a.lg_chunk = p.lg_chunk;
+  a.lg_room = p.lg_chunk - 2;
+  a.all = Settings(a.V, temperature, top_k, top_p, min_p);
   uint8_t* const w = static_cast<uint8_t*>(workspace);
+  a.rows = a.t_rows || a.k_rows || a.p_rows || a.m_rows ? reinterpret_cast<Settings*>(w + p.rows) : nullptr;
   a.state = reinterpret_cast<RowState*>(w + p.state);
   a.top = reinterpret_cast<float*>(w + p.top);
   a.mass = reinterpret_cast<double*>(w + p.mass);
-  a.total = reinterpret_cast<uint64_t*>(w + p.total);
+  a.kept = reinterpret_cast<double*>(w + p.kept);
+  a.cut = reinterpret_cast<RowCut*>(w + p.cut);
   a.listed = reinterpret_cast<int32_t*>(w + p.listed);
+  a.depth = reinterpret_cast<int32_t*>(w + p.depth);
   a.hist = reinterpret_cast<uint64_t*>(w + p.hist);
-  a.list = reinterpret_cast<uint16_t*>(w + p.list);
-  // without filters the masses of the first pass are all there is to know
-  const bool select = a.t_rows || a.k_rows || a.p_rows || a.m_rows || !(temperature > 0.0) || (top_k > 0 && top_k < a.V) ||
-                      top_p < 1.0 || min_p > 0.0;
+  a.list = reinterpret_cast<uint2*>(w + p.list);
   hipStream_t s = as_stream(stream);
-  if (dtype == TQ_F32) launch_sample<TQ_F32>(a, p, select, s);
-  else if (dtype == TQ_F16) launch_sample<TQ_F16>(a, p, select, s);
-  else launch_sample<TQ_BF16>(a, p, select, s);
+  if (dtype == TQ_F32) launch_sample<TQ_F32>(a, s);
+  else if (dtype == TQ_F16) launch_sample<TQ_F16>(a, s);
+  else launch_sample<TQ_BF16>(a, s);
   return launch_status(what);
 }
 
@@ -849,7 +1306,7 @@ int tq_sample_tokens(const void* logits, int32_t dtype, int64_t ld, int32_t N, i
                      const float* temperatures, double temperature, const int32_t* top_ks, int32_t top_k,
                      const float* top_ps, double top_p, const float* min_ps, double min_p, int64_t* tokens,
                      void* workspace, int64_t workspace_bytes, void* stream) {
-  SampleArgs a{};
+  SampleArgs a{.all = Settings(1, 1.0, 0, 1.0, 0.0)};
   a.logits = logits;
   a.ld = ld;
   a.N = N;
@@ -867,7 +1324,7 @@ int tq_filter_probs(const void* logits, int32_t dtype, int64_t ld, int32_t N, in
                     double temperature, const int32_t* top_ks, int32_t top_k, const float* top_ps, double top_p,
                     const float* min_ps, double min_p, float* probs, void* workspace, int64_t workspace_bytes,
                     void* stream) {
-  SampleArgs a{};
+  SampleArgs a{.all = Settings(1, 1.0, 0, 1.0, 0.0)};
   a.logits = logits;
   a.ld = ld;
   a.N = N;
