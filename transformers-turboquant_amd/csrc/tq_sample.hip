@@ -21,8 +21,8 @@
 //   select   (top-p, min-p) finds the bins that hold the row's border in the joined histograms, and lists what is
 //            kept (min-p), the tokens down to the border if they are few, or else those of its bins alone, with the
 //            mass of what is kept for certain above them
-//   finish   up to 64 listed tokens are ranked by one wave, up to 2048 sorted by the block, more are selected digit
-//            by digit; then cut, and drawn from the list if it holds all that is kept, or else by the chunks' masses
+//   finish   up to 64 listed tokens are ranked by one wave, among more (2048 of them in shared memory) the border
+//            is selected digit by digit; drawn from the list if it holds all that is kept, else by the chunks' masses
 //   write    the probabilities of rows that keep many; the others' are few, in a row that the scan has cleared
 #include "tq_common.h"
 
@@ -32,7 +32,7 @@ constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of the finish
 constexpr int kScan = 512, kScanWaves = kScan / 64;     // of scan and select: a thread takes runs of 8 tokens
 constexpr int kBins = 512, kTail = kBins - 1;  // the last bin has everything below the others
 constexpr int kMaxChunks = 1024;
-constexpr int kShort = 2048;  // tokens that are sorted
+constexpr int kShort = 2048;  // tokens that are taken into shared memory
 constexpr int kFew = 1024;    // tokens down to the border that are listed with it
 constexpr double kUnit = 0x1p48;  // of a chunk's mass: at most 2^15 tokens of weight <= 1
 constexpr int kTiny = 49;         // a weight below 2^-49 is no unit
@@ -43,6 +43,7 @@ enum Mode { kAll, kMinP, kTopP, kTopK };
 struct Settings {
   int mode, k;
   double c;     // log2(e) / t
+  double low;   // a logit this far below the maximum weighs nothing (2^-1200)
   double p, m;
   float far;    // kept tokens' logits are down to this far from the maximum (top-p, min-p)
   float tiny;   // weights are units down to this far
@@ -52,7 +53,8 @@ struct Settings {
     const bool greedy = !(t > 0.0);
     if (greedy) k = 1;
     c = 1.4426950408889634 / (greedy ? 1.0 : t);
-    if (!(c < 1e300)) c = 1e300;
+    c = !(c < 1e290) ? 1e290 : c < 1e-290 ? 1e-290 : c;
+    low = -1200.0 / c;
     m = m > 0.0 ? (m < 1.0 ? m : 1.0) : 0.0;
     const bool by_rank = k > 0 && k < V, by_mass = p < 1.0;
     if (!by_mass) p = 1.0;
@@ -113,27 +115,42 @@ struct SampleArgs {
   __device__ __forceinline__ const Settings& of(int row) const { return rows ? rows[row] : all; }
 };
 
-// 2^y, y <= 0: 2^n by the exponent, 2^f for |f| <= 1/2 by the series of exp(f ln 2) up to the 10th power
-__device__ __forceinline__ double exp2_f64(double y) {
-  constexpr double L = 0.6931471805599453;
-  constexpr double A[11] = {1.0, L, L * L / 2, L * L * L / 6, L * L * L * L / 24, L * L * L * L * L / 120,
-                            L * L * L * L * L * L / 720, L * L * L * L * L * L * L / 5040, L * L * L * L * L * L * L * L / 40320,
-                            L * L * L * L * L * L * L * L * L / 362880, L * L * L * L * L * L * L * L * L * L / 3628800};
-  y = fmax(y, -1200.0);
-  const double r = rint(y), f = y - r;
-  double s = A[10];
-#pragma unroll
-  for (int i = 9; i >= 0; --i) s = fma(s, f, A[i]);
-  return ldexp(s, static_cast<int>(r));
-}
-// a logit's weight under maximum m (finite, or v = m)
-__device__ __forceinline__ double weight(float v, float m, double c) {
-  return exp2_f64((static_cast<double>(v) - static_cast<double>(m)) * c);
-}
+// Weights under a maximum: exp((v - top) / t) = 2^y as 2^n 2^f, n = rint(y): 2^f, |f| <= 1/2, by the series of
+// exp(f ln 2) up to the 10th power (2 10^-13).  Adding 1.5 2^52 leaves n in the low word.  -inf weighs 0.
+struct Weigh {
+  double top, c, low;  // top: of finite logits, or one that v is not above
+  __device__ __forceinline__ Weigh(const Settings& set, float m) : top(m), c(set.c), low(set.low) {}
+  __device__ __forceinline__ double operator()(float v) const {
+    constexpr double L = 0.6931471805599453, M = 0x1.8p52;
+    constexpr double A[11] = {1.0, L, L * L / 2, L * L * L / 6, L * L * L * L / 24, L * L * L * L * L / 120,
+                              L * L * L * L * L * L / 720, L * L * L * L * L * L * L / 5040, L * L * L * L * L * L * L * L / 40320,
+                              L * L * L * L * L * L * L * L * L / 362880, L * L * L * L * L * L * L * L * L * L / 3628800};
+    double d = static_cast<double>(v) - top, s;
+    asm("v_max_f64 %0, %1, %2" : "=v"(d) : "v"(d), "v"(low));  // fmax would quiet `low` first
+    const double t = fma(d, c, M), f = fma(d, c, -(t - M));
+    // the series with its constants as scalar operands; the compiler's own form copies each to vector registers
+    // (9 of ~45 instructions a token)
+    asm("v_fma_f64 %0, %1, %2, %3\n\t"
+        "v_fma_f64 %0, %0, %2, %4\n\t"
+        "v_fma_f64 %0, %0, %2, %5\n\t"
+        "v_fma_f64 %0, %0, %2, %6\n\t"
+        "v_fma_f64 %0, %0, %2, %7\n\t"
+        "v_fma_f64 %0, %0, %2, %8\n\t"
+        "v_fma_f64 %0, %0, %2, %9\n\t"
+        "v_fma_f64 %0, %0, %2, %10\n\t"
+        "v_fma_f64 %0, %0, %2, %11\n\t"
+        "v_fma_f64 %0, %0, %2, 1.0"
+        : "=&v"(s)
+        : "v"(A[10]), "v"(f), "s"(A[9]), "s"(A[8]), "s"(A[7]), "s"(A[6]), "s"(A[5]), "s"(A[4]), "s"(A[3]), "s"(A[2]), "s"(A[1]));
+    return ldexp(s, static_cast<int>(__double_as_longlong(t)));
+  }
+};
 
 // Falling bins of 1/16 on an absolute grid, so that chunks with other maxima have the same ones.  Monotone
 // in v; logits beyond 2^27 / 16 share their bins.
 __device__ __forceinline__ int grid_of(float v) { return static_cast<int>(floorf(fminf(fmaxf(v * 16.f, -0x1p27f), 0x1p27f))); }
+// the least float on the grid from g on (the last value has everything below it)
+__device__ __forceinline__ float edge_of(int g) { return g > -(1 << 27) ? __double2float_ru(g * 0.0625) : -3.4028235e38f; }
 __device__ __forceinline__ int bin_of(float v, int grid_top) { return min(grid_top - grid_of(v), kTail); }
 // larger for larger floats
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -141,8 +158,9 @@ __device__ __forceinline__ uint32_t key_of(float v) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Eight logits from x on; what is not there is -inf, and so is a NaN.
-template <int DT>
+// Eight logits from x on; what is not there is -inf.  NaN: as -inf (FIX), or as it is where every comparison leaves
+// it out.
+template <int DT, bool FIX = true>
 __device__ __forceinline__ void load_logits(const void* row, int x, int V, float (&v)[8]) {
   if (x + 8 <= V) {
     if constexpr (DT == TQ_F32) {
@@ -157,8 +175,10 @@ __device__ __forceinline__ void load_logits(const void* row, int x, int V, float
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = x + j < V ? load_act<DT>(row, x + j) : -INFINITY;
   }
+  if constexpr (FIX) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = fmaxf(v[j], -INFINITY);  // NaN: the other operand
+    for (int j = 0; j < 8; ++j) v[j] = fmaxf(v[j], -INFINITY);  // NaN: the other operand
+  }
 }
 template <int DT>
 __device__ __forceinline__ const void* row_of(const SampleArgs& a, int row) {
@@ -171,36 +191,64 @@ __device__ __forceinline__ float tame(float m) { return m == INFINITY ? 0.f : m;
 __device__ __forceinline__ bool counts(float chunk_top, float m) { return m != INFINITY || chunk_top == INFINITY; }
 
 // ---------------------------------------------------------------- over a wave, over a block
+// Lane to lane through DPP (shifts within rows of 16 lanes, then lane 15 of row 0 into row 1 and of row 2 into
+// row 3, then lane 31 into the upper half), no LDS round trips.  A lane without a source gets `none`.
+template <int CTRL, int ROWS, class T>
+__device__ __forceinline__ T dpp_from(T none, T v) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, false));
+  } else {
+    const uint64_t x = __builtin_bit_cast(uint64_t, v), o = __builtin_bit_cast(uint64_t, none);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(static_cast<int>(o), static_cast<int>(x), CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(static_cast<int>(o >> 32), static_cast<int>(x >> 32), CTRL, ROWS, 0xF, false);
+    return __builtin_bit_cast(T, static_cast<uint64_t>(hi) << 32 | lo);
+  }
+}
+struct Sum {
+  template <class T>
+  static __device__ __forceinline__ T none() {
+    return T(0);
+  }
+  template <class T>
+  __device__ __forceinline__ T operator()(T a, T b) const {
+    return a + b;
+  }
+};
+struct Max {
+  template <class T>
+  static __device__ __forceinline__ T none() {
+    if constexpr (__is_floating_point(T)) return -INFINITY;
+    else return T(-1) < T(0) ? T(T(1) << (8 * sizeof(T) - 1)) : T(0);
+  }
+  template <class T>
+  __device__ __forceinline__ T operator()(T a, T b) const {
+    return a > b ? a : b;
+  }
+};
+template <class T>
+__device__ __forceinline__ T lane_value(T v, int l) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+  } else {
+    const uint64_t x = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(x), l), hi = __builtin_amdgcn_readlane(static_cast<int>(x >> 32), l);
+    return __builtin_bit_cast(T, static_cast<uint64_t>(hi) << 32 | lo);
+  }
+}
+// inclusive, over all lanes of a wave
+template <class T, class Op = Sum>
+__device__ __forceinline__ T wave_scan(T v, Op op = Op()) {
+  const T none = Op::template none<T>();
+  v = op(dpp_from<0x111, 0xF>(none, v), v);
+  v = op(dpp_from<0x112, 0xF>(none, v), v);
+  v = op(dpp_from<0x114, 0xF>(none, v), v);
+  v = op(dpp_from<0x118, 0xF>(none, v), v);
+  v = op(dpp_from<0x142, 0xA>(none, v), v);
+  return op(dpp_from<0x143, 0xC>(none, v), v);
+}
 template <class T, class Op>
 __device__ __forceinline__ T wave_all(T v, Op op) {
-#pragma unroll
-  for (int sh = 32; sh >= 1; sh >>= 1) v = op(v, static_cast<T>(__shfl_xor(v, sh, 64)));
-  return v;
-}
-template <class T>
-__device__ __forceinline__ T wave_scan(T v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int sh = 1; sh < 64; sh <<= 1) {
-    const T t = __shfl_up(v, sh, 64);
-    if (lane >= sh) v += t;
-  }
-  return v;
-}
-// Inclusive sum of 32-bit values through DPP (shifts within rows of 16 lanes, then row 0's sum into row 1 and
-// row 2's into row 3, then lane 31's into the upper half)
-template <int CTRL, int ROWS, class T>
-__device__ __forceinline__ T dpp_add(T v) {
-  return v + __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, false));
-}
-template <class T>
-__device__ __forceinline__ T wave_scan32(T v) {
-  v = dpp_add<0x111, 0xF>(v);
-  v = dpp_add<0x112, 0xF>(v);
-  v = dpp_add<0x114, 0xF>(v);
-  v = dpp_add<0x118, 0xF>(v);
-  v = dpp_add<0x142, 0xA>(v);
-  return dpp_add<0x143, 0xC>(v);
+  return lane_value(wave_scan(v, op), 63);
 }
 // of all threads, in a fixed order; s: a value per wave, free again behind the next barrier
 template <int W, class T, class Op>
@@ -213,29 +261,13 @@ __device__ __forceinline__ T block_all(T v, T* s, Op op) {
   for (int w = 1; w < W; ++w) r = op(r, s[w]);
   return r;
 }
-struct Sum {
-  template <class T>
-  __device__ __forceinline__ T operator()(T a, T b) const {
-    return a + b;
-  }
-};
-struct Max {
-  template <class T>
-  __device__ __forceinline__ T operator()(T a, T b) const {
-    return a > b ? a : b;
-  }
-};
-__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int l) {
-  return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), l))) << 32 |
-         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), l));
-}
 __device__ __forceinline__ void add_lds(uint64_t* p, uint64_t v) {
   atomicAdd(reinterpret_cast<unsigned long long*>(p), static_cast<unsigned long long>(v));
 }
 
 // ---------------------------------------------------------------- scan
 // A thread's tokens of a chunk: runs of 8 in a row, kScan * 8 apart, at most 64.  They are read anew in every pass
-// (from the caches behind the first): held in registers, 64 of them leave one wave per SIMD.
+// (from the caches behind the first): held in registers, 64 of them leave one wave per SIMD.  NaN are NaN.
 template <int DT, class Fn>
 __device__ __forceinline__ void each_run(const SampleArgs& a, int row, int chunk, float m, Fn fn) {
   const void* const src = row_of<DT>(a, row);
@@ -245,7 +277,7 @@ __device__ __forceinline__ void each_run(const SampleArgs& a, int row, int chunk
   for (int r = 0; r < runs; ++r) {
     const int x = x0 + r * (kScan * 8);
     float v[8];
-    load_logits<DT>(src, x, a.V, v);
+    load_logits<DT, false>(src, x, a.V, v);
     if (m == INFINITY) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = tame(v[e], m);
@@ -261,7 +293,7 @@ __device__ __forceinline__ uint64_t units_of(double w) { return __double_as_long
 template <int DT>
 __device__ __forceinline__ void list_tokens(const SampleArgs& a, int row, int chunk, float m, uint64_t on, int* s_listed) {
   const int mine = __popcll(on);
-  int to = wave_scan32(mine);
+  int to = wave_scan(mine);
   const int all = __builtin_amdgcn_readlane(to, 63);
   if (!all) return;
   int base = 0;
@@ -284,7 +316,7 @@ __device__ __forceinline__ int reach_bin(const T (&h)[8], T goal) {
   T sum = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum += h[i];
-  const T upto = wave_scan32(sum);
+  const T upto = wave_scan(sum);
   const uint64_t over = __ballot(upto >= goal);
   if (!over) return kTail;
   T run = upto - sum;
@@ -361,13 +393,13 @@ __global__ void __launch_bounds__(kScan) sample_scan_kernel(SampleArgs a) {
     return;
   }
   const float mt = tame(m);
-  const double c2 = set.c;
+  const Weigh weigh(set, mt);
   const int top = grid_of(mt);
   if (mode == kAll) {
     double sum = 0.0;
     each_run<DT>(a, row, c, m, [&](const float (&v)[8], int, int) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += weight(v[e], mt, c2);
+      for (int e = 0; e < 8; ++e) sum += weigh(v[e]);
     });
     sum = block_all<kScanWaves>(sum, s.sum, Sum{});
     if (tid == 0) a.mass[at] = sum;
@@ -384,9 +416,7 @@ __global__ void __launch_bounds__(kScan) sample_scan_kernel(SampleArgs a) {
       if (lane == 0) s.bin = bin;
     }
     __syncthreads();
-    // the bin's lower end (the grid's last value has everything below it)
-    float least = -3.4028235e38f;
-    if (s.bin < kTail && top - s.bin > -(1 << 27)) least = __double2float_rd((top - s.bin) * 0.0625);
+    const float least = s.bin < kTail ? edge_of(top - s.bin) : -3.4028235e38f;
     uint64_t on = 0;
     if (most >= least)
       each_run<DT>(a, row, c, m, [&](const float (&v)[8], int r, int) {
@@ -402,33 +432,30 @@ __global__ void __launch_bounds__(kScan) sample_scan_kernel(SampleArgs a) {
       return x - 2e-7f * (fabsf(mt) + fabsf(x));
     };
     const float least = fmaxf(-3.4028235e38f, below(set.far)), tiny = below(set.tiny);
-    uint64_t sum = 0;
-    int deep = 0;
+    double sum = 0.0;
     each_run<DT>(a, row, c, m, [&](const float (&v)[8], int, int) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float x = v[e];
-        if (__any(!(x < tiny))) {
-          const uint64_t n = units_of(weight(x, mt, c2));
-          sum += n;
-          if (x >= least) {
-            const int b = bin_of(x, top);
-            deep = max(deep, b + 1);
-            add_lds(s.hist + b, n);
-          }
+        if (__any(x >= tiny)) {
+          const double w = weigh(x);  // 0 of a NaN
+          sum += w;
+          if (x >= least) add_lds(s.hist + bin_of(x, top), units_of(w));
         }
       }
     });
-    deep = wave_all(deep, Max{});
-    if (lane == 0) s.depth[wave] = deep;
-    sum = block_all<kScanWaves>(sum, s.part, Sum{});  // its barrier is behind the histogram, too
+    sum = block_all<kScanWaves>(sum, s.sum, Sum{});  // its barrier is behind the histogram, too
+    const uint64_t h = s.hist[tid], some = __ballot(h != 0);
+    if (lane == 0) s.depth[wave] = some ? 64 * wave + 64 - __builtin_clzll(some) : 0;
+    __syncthreads();
+    int deep = 0;
 #pragma unroll
     for (int w = 0; w < kScanWaves; ++w) deep = max(deep, s.depth[w]);
     if (tid == 0) {
-      a.mass[at] = static_cast<double>(sum);
+      a.mass[at] = sum;
       a.depth[at] = deep;
     }
-    if (tid < deep) a.hist[at * kBins + tid] = s.hist[tid];
+    if (tid < deep) a.hist[at * kBins + tid] = h;
   }
 }
 
@@ -463,6 +490,7 @@ __global__ void __launch_bounds__(kScan) sample_select_kernel(SampleArgs a) {
     return;
   }
   const float mt = tame(m);
+  const Weigh weigh(set, mt);
   const double c2 = set.c, least = set.m;
   const int top = grid_of(mt);
   uint64_t sum = 0, on = 0;
@@ -474,7 +502,7 @@ __global__ void __launch_bounds__(kScan) sample_select_kernel(SampleArgs a) {
       for (int e = 0; e < 8; ++e) {
         bool take = v[e] >= far;
         if (__any(take)) {
-          const double w = weight(v[e], mt, c2);
+          const double w = weigh(v[e]);
           take = take && w >= least;
           const uint64_t n = units_of(w);
           sum += !take ? 0 : n ? n : 1;
@@ -488,9 +516,9 @@ __global__ void __launch_bounds__(kScan) sample_select_kernel(SampleArgs a) {
     for (int i = tid; i < a.C; i += kScan) {
       const float ct = a.top[at0 + i];
       const bool in = ct != -INFINITY && counts(ct, m);
-      const double f = in ? weight(tame(ct), mt, c2) / kUnit : 0.0;
+      const double f = in ? weigh(tame(ct)) : 0.0;
       mine += in ? f * a.mass[at0 + i] : 0.0;
-      s.factor[i] = static_cast<float>(f * kUnit);
+      s.factor[i] = static_cast<float>(f);
       s.off[i] = in ? top - grid_of(tame(ct)) : kBins;
       s.depth[i] = in ? a.depth[at0 + i] : 0;
     }
@@ -539,18 +567,18 @@ __global__ void __launch_bounds__(kScan) sample_select_kernel(SampleArgs a) {
       }
     }
     __syncthreads();
-    const int lo = s.lo, hi = s.hi;
-    if (a.top[at] != -INFINITY && bin_of(tame(a.top[at], m), top) <= hi)  // else the chunk has nothing to list
+    // as logits: certain from `sure` on, listed from `edge` on
+    const float sure = s.lo > 0 ? edge_of(top - s.lo + 1) : INFINITY, edge = s.hi < kTail ? edge_of(top - s.hi) : -3.4028235e38f;
+    if (a.top[at] >= edge)  // else the chunk has nothing to list
       each_run<DT>(a, row, c, m, [&](const float (&v)[8], int r, int) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int b = bin_of(v[e], top);
-          const bool certain = b < lo;
+          const bool certain = v[e] >= sure;
           if (__any(certain)) {
-            const uint64_t n = units_of(weight(v[e], mt, c2));
+            const uint64_t n = units_of(weigh(v[e]));
             sum += certain ? n : 0;
           }
-          on |= static_cast<uint64_t>(!certain && b <= hi && v[e] != -INFINITY) << (8 * r + e);
+          on |= static_cast<uint64_t>(v[e] >= edge && !certain) << (8 * r + e);
         }
       });
   }
@@ -567,7 +595,7 @@ constexpr int kSegments = 2048;  // runs of 64 listed tokens that the table hold
 
 struct FinishSmem {
   uint64_t token[kShort];  // key, then the complement of the index: larger ones rank first
-  uint64_t value[kShort];
+  uint64_t value[64];
   uint32_t segment[kSegments];  // chunk, run of 64
   union {
     uint64_t digits[256];
@@ -579,8 +607,8 @@ struct FinishSmem {
   uint64_t extra[kMaxChunks];  // kept tokens' mass as integers
   int listed[kMaxChunks];      // -1: its tokens are read from the row
   float top[kMaxChunks];
-  uint64_t rest;
-  uint32_t digit;
+  uint64_t rest, one;
+  uint32_t digit, ties;
   int segments, raw, lo, hi, n, chunk, pick;
   double bar;
 };
@@ -641,48 +669,16 @@ __device__ __forceinline__ float logit_of(uint64_t token) {
 }
 __device__ __forceinline__ int index_of(uint64_t token) { return static_cast<int>(~static_cast<uint32_t>(token)); }
 
-// Sorted by the block, larger ones first (FALL) or last; n <= kShort
-template <bool FALL>
-__device__ __forceinline__ void sort_tokens(uint64_t* t, int n) {
-  const int tid = threadIdx.x;
-  int lg = 1;
-  while ((1 << lg) < n) ++lg;
-  for (int i = n + tid; i < 1 << lg; i += kThreads) t[i] = FALL ? 0 : ~0ull;
-  __syncthreads();
+// The same for tokens in shared memory
+struct Taken {
+  const FinishSmem& s;
+  int n;
+  template <class Fn>
+  __device__ __forceinline__ void each(Fn fn) const {
 #pragma unroll 1
-  for (int size = 1; size <= lg; ++size)
-#pragma unroll 1
-    for (int stride = size - 1; stride >= 0; --stride) {
-      if (tid < 1 << (lg - 1)) {
-        const int i = (tid >> stride << (stride + 1)) + (tid & ((1 << stride) - 1)), j = i + (1 << stride);
-        const uint64_t x = t[i], y = t[j];
-        if ((x < y) == ((((i >> size) & 1) == 0) == FALL) && x != y) {
-          t[i] = y;
-          t[j] = x;
-        }
-      }
-      __syncthreads();
-    }
-}
-static_assert(kShort <= 2 * kThreads, "a pair per thread");
-
-// inclusive sums of two values per thread, and the total
-__device__ __forceinline__ uint64_t block_scan2(uint64_t v0, uint64_t v1, uint64_t* s_part, uint64_t& upto0, uint64_t& upto1) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint64_t upto = wave_scan(v0 + v1);
-  if (lane == 63) s_part[wave] = upto;
-  __syncthreads();
-  uint64_t all = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) upto += s_part[w];
-    all += s_part[w];
+    for (int i = threadIdx.x; i < n; i += kThreads) fn(logit_of(s.token[i]), index_of(s.token[i]));
   }
-  __syncthreads();
-  upto1 = upto;
-  upto0 = upto - v1;
-  return all;
-}
+};
 
 // Among some tokens: the digit in which the running sum of their values, from the largest digit down (FALL) or
 // from the smallest up, reaches goal; goal becomes what is left of it in front of that digit.  Where the sum never
@@ -727,10 +723,10 @@ __device__ __forceinline__ uint32_t pick_digit(FinishSmem& s, uint64_t& goal, Ea
   return s.digit;
 }
 
-// The border in rank among tokens that are too many to be sorted.  value: 1 (by rank) or the token's mass, 0: not one
-// of them; kept are the tokens whose predecessors' values sum to less than goal (>= 1).
-template <int DT, class Value>
-__device__ __forceinline__ void pick_border(const Candidates<DT>& all, FinishSmem& s, uint64_t goal, Value value, uint32_t& key, int& last) {
+// The border in rank among some tokens.  value: 1 (by rank) or the token's mass, 0: not one of them; kept are the
+// tokens whose predecessors' values sum to less than goal (>= 1).
+template <class Tokens, class Value>
+__device__ __forceinline__ void pick_border(const Tokens& all, FinishSmem& s, uint64_t goal, Value value, uint32_t& key, int& last) {
   uint32_t prefix = 0, mask = 0;
 #pragma unroll 1
   for (int shift = 24; shift >= 0; shift -= 8) {
@@ -748,22 +744,26 @@ __device__ __forceinline__ void pick_border(const Candidates<DT>& all, FinishSme
   }
   key = prefix;
   // equal logits have equal values: how many of them are kept, the first in index order
-  uint64_t one = 0, ties = 0;
+  if (threadIdx.x == 0) {
+    s.one = 0;
+    s.ties = 0;
+  }
+  __syncthreads();
   all.each([&](float v, int x) {
     if (key_of(v) == key) {
       const uint64_t n = value(v, x);
-      one = n > one ? n : one;
-      ties += n != 0;
+      if (n) {
+        s.one = n;
+        atomicAdd(&s.ties, 1u);
+      }
     }
   });
-  one = block_all<kWaves>(one, s.part, Max{});
   __syncthreads();
-  ties = block_all<kWaves>(ties, s.part, Sum{});
-  __syncthreads();
+  const uint64_t one = s.one;
   uint64_t keep = one ? (goal + one - 1) / one : 1;
   if (keep < 1) keep = 1;
   last = 0x7FFFFFFF;
-  if (keep >= ties) return;
+  if (keep >= s.ties) return;
   uint32_t at = 0;
   mask = 0;
 #pragma unroll 1
@@ -777,6 +777,28 @@ __device__ __forceinline__ void pick_border(const Candidates<DT>& all, FinishSme
     mask |= 255u << shift;
   }
   last = static_cast<int>(at);
+}
+
+// The border of a row: by rank, then by mass
+template <class Tokens, class In, class Integer>
+__device__ __forceinline__ void cut_row(const Tokens& all, FinishSmem& s, const Settings& set, uint64_t mass_goal, In in, Integer integer, uint32_t& key, int& last) {
+  if (set.mode == kTopK) pick_border(all, s, static_cast<uint64_t>(set.k), [&](float, int) -> uint64_t { return 1; }, key, last);
+  if (set.p >= 1.0) return;
+  const uint32_t key_k = key;
+  const int last_k = last;
+  const auto value = [&](float v, int x) -> uint64_t {
+    const uint32_t k = key_of(v);
+    return in(v) && (k > key_k || (k == key_k && x <= last_k)) ? integer(v) : 0;
+  };
+  if (set.mode == kTopK) {
+    uint64_t sum = 0;
+    all.each([&](float v, int x) { sum += value(v, x); });
+    sum = block_all<kWaves>(sum, s.part, Sum{});
+    __syncthreads();
+    const double goal = ceil(set.p * static_cast<double>(sum));
+    mass_goal = goal >= 1.0 ? static_cast<uint64_t>(goal) : 1;
+  }
+  pick_border(all, s, mass_goal, value, key, last);
 }
 
 template <int DT>
@@ -813,14 +835,15 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
     return;
   }
   const int top = grid_of(mt);
-  const double c2 = set.c, least = set.m;
+  const Weigh weigh(set, mt);
+  const double least = set.m;
   const Candidates<DT> all{a, s, row, m};
   uint32_t key = 0;  // the border
   int last = 0x7FFFFFFF;
   double unit = 1.0;  // listed tokens' masses as integers
   if (mode == kAll) {
     for (int c = tid; c < a.C; c += kThreads)
-      s.mass[c] = s.top[c] == -INFINITY || !counts(s.top[c], m) ? 0.0 : s.mass[c] * weight(tame(s.top[c]), mt, c2);
+      s.mass[c] = s.top[c] == -INFINITY || !counts(s.top[c], m) ? 0.0 : s.mass[c] * weigh(tame(s.top[c]));
     __syncthreads();
   } else {
     // ---- a table of the lists' runs of 64, by the first wave
@@ -831,7 +854,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
         int n = c < a.C && counts(s.top[c], m) ? s.listed[c] : 0;
         if (c < a.C && !counts(s.top[c], m)) s.listed[c] = 0;
         int segs = n > 0 ? (n + 63) / 64 : 0;
-        const int upto = wave_scan32(segs), from = run + upto - segs;
+        const int upto = wave_scan(segs), from = run + upto - segs;
         if (from + segs > kSegments) {  // no place in the table
           n = -1;
           s.listed[c] = -1;
@@ -852,9 +875,30 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
 
     // ---- the listed tokens, as far as they can be sorted
     float peak = -INFINITY;
+    const auto reach_rank = [&]() {  // the bin that k tokens in s.bins reach
+      __syncthreads();
+      if (wave == 0) {
+        int h[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = 8 * lane + i < kTail ? static_cast<int>(s.bins[8 * lane + i]) : 0;
+        const int bin = reach_bin(h, set.k);
+        if (lane == 0) {
+          s.hi = bin;
+          s.n = 0;
+        }
+      }
+      __syncthreads();
+      return s.hi;
+    };
+    // every chunk listed its own first k: of them all, those down to the bin that k reach
+    const bool many = mode == kTopK && (s.raw || s.segments > kShort / 64);
+    if (many) {
+      all.each([&](float v, int) { atomicAdd(s.bins + bin_of(v, top), 1u); });
+      hi = reach_rank();
+    }
     all.each([&](float v, int x) {
       const int b = bin_of(v, top);
-      const bool on = b >= lo && b <= hi && (mode != kMinP || weight(v, mt, c2) >= least);
+      const bool on = b >= lo && b <= hi && (mode != kMinP || weigh(v) >= least);
       const uint64_t some = __ballot(on);
       if (!some) return;
       int to = 0;
@@ -868,27 +912,14 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
     });
     __syncthreads();
     int n = s.n;
-    if (mode == kTopK && n > 64 && n <= kShort) {
-      // every chunk listed its own first k: of them all, those down to the bin that k reach
+    if (mode == kTopK && !many && n > 64) {
       uint64_t t[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         t[i] = tid + i * kThreads < n ? s.token[tid + i * kThreads] : 0;
         if (tid + i * kThreads < n) atomicAdd(s.bins + bin_of(logit_of(t[i]), top), 1u);
       }
-      __syncthreads();
-      if (wave == 0) {
-        int h[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] = 8 * lane + i < kTail ? static_cast<int>(s.bins[8 * lane + i]) : 0;
-        const int bin = reach_bin(h, set.k);
-        if (lane == 0) {
-          s.hi = bin;
-          s.n = 0;
-        }
-      }
-      __syncthreads();
-      hi = s.hi;
+      hi = reach_rank();
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const bool on = tid + i * kThreads < n && bin_of(logit_of(t[i]), top) <= hi;
@@ -904,7 +935,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
     const bool alone = n <= kShort && lo == 0;  // the tokens in s.token are all that can be kept
     const double goal = set.p * cut.total;
     const auto ceiling = [](double g) -> uint64_t { return g >= 0x1p63 ? ~0ull : g >= 1.0 ? static_cast<uint64_t>(ceil(g)) : 1; };
-    const auto integer = [&](double w) -> uint64_t {
+    const auto integer = [&](double w) -> uint64_t {  // of listed tokens
       if (!(w > 0.0)) return 0;
       const uint64_t x = static_cast<uint64_t>(w * unit + 0.5);
       return x ? x : 1;
@@ -914,7 +945,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
       // ---- ranked by one wave: lane i has token i, and meets every other
       if (wave != 0) return;
       const uint64_t t = lane < n ? s.token[lane] : 0;
-      const double w = lane < n ? weight(logit_of(t), mt, c2) : 0.0;
+      const double w = lane < n ? weigh(logit_of(t)) : 0.0;
       unit = 0x1p55;  // the maximum is among them
       const uint64_t val = integer(w);
       const int x = index_of(t);
@@ -925,9 +956,10 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
       uint64_t before = 0;
 #pragma unroll 8
       for (int j = 0; j < ((n + 7) & ~7); ++j) {
+        const uint64_t v = s.value[j];
         const bool ahead = s.token[j] > t;
         rank += ahead;
-        before += ahead ? s.value[j] : 0;
+        before += ahead ? v : 0;
       }
       const bool in = lane < n && (mode != kTopK || rank < set.k);
       uint64_t bar = ~0ull;
@@ -945,7 +977,10 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       uint64_t upto = 0;  // of the kept tokens at or before it
 #pragma unroll 8
-      for (int j = 0; j < ((n + 7) & ~7); ++j) upto += index_of(s.token[j]) <= x ? s.value[j] : 0;
+      for (int j = 0; j < ((n + 7) & ~7); ++j) {
+        const uint64_t v = s.value[j];
+        upto += index_of(s.token[j]) <= x ? v : 0;
+      }
       // the first index that passes; the last one, should u be 1 or more
       const bool over = on && static_cast<double>(upto) > pass;
       const int first = -wave_all(over ? -x : -0x7FFFFFFF, Max{}), end = wave_all(on ? x : -1, Max{});
@@ -959,106 +994,59 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
     peak = block_all<kWaves>(peak, reinterpret_cast<float*>(s.part), Max{});
     __syncthreads();
     // the heaviest is 2^(61 - bits of their number)
-    const double big = peak == -INFINITY ? 1.0 : weight(peak, mt, c2);
+    const double big = peak == -INFINITY ? 1.0 : weigh(peak);
     unit = big > 0.0 ? ldexp(1.0, 30 + __builtin_clz(n | 1)) / big : 0.0;
     if (!(unit < INFINITY)) unit = 0.0;
     const double g = (goal - certain) * unit;
-    const bool none = mode == kTopP && certain > 0.0 && !(g > 0.0);  // what is certain reaches the goal
-    int kept = 0;
-    if (n <= kShort) {
-      // ---- sorted: kept are the first of them
-      sort_tokens<true>(s.token, n);
-      uint64_t val[2], upto[2];
-      double w[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int at = 2 * tid + i;
-        w[i] = at < n ? weight(logit_of(s.token[at]), mt, c2) : 0.0;
-        val[i] = at < n && !(mode == kTopK && at >= set.k) ? integer(w[i]) : 0;
-        s.value[at] = val[i];
-      }
-      const uint64_t sum = block_scan2(val[0], val[1], s.part, upto[0], upto[1]);
-      uint64_t bar = ~0ull;  // predecessors of a kept token sum to less
-      if (mode == kTopP) bar = ceiling(g);
-      else if (mode == kTopK && set.p < 1.0) bar = ceiling(set.p * static_cast<double>(sum));
-      int on = 0;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int at = 2 * tid + i;
-        on += at < n && !(mode == kTopK && at >= set.k) && upto[i] - val[i] < bar && w[i] >= least && !none;
-      }
-      kept = block_all<kWaves>(on, reinterpret_cast<int*>(s.part), Sum{});
-      __syncthreads();
-      key = kept ? static_cast<uint32_t>(s.token[kept - 1] >> 32) : key_of(peak);
-      last = kept ? index_of(s.token[kept - 1]) : -1;
-      if (alone && a.probs) {
-        uint64_t mass = 0;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) mass += 2 * tid + i < kept ? val[i] : 0;
-        mass = block_all<kWaves>(mass, s.part, Sum{});
-        const double inverse = unit / static_cast<double>(mass);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (2 * tid + i < kept)
-            a.probs[static_cast<int64_t>(row) * a.V + index_of(s.token[2 * tid + i])] = static_cast<float>(w[i] * inverse);
+    const auto in = [&](float v) {
+      const int b = bin_of(v, top);
+      return b >= lo && b <= hi;
+    };
+    const auto mass = [&](float v) { return integer(weigh(v)); };
+    const Taken taken{s, n};
+    if (mode == kTopP && certain > 0.0 && !(g > 0.0)) {  // what is certain reaches the goal
+      key = key_of(peak);
+      last = -1;
+    } else if (mode != kMinP) {
+      if (n <= kShort) cut_row(taken, s, set, ceiling(g), in, mass, key, last);
+      else cut_row(all, s, set, ceiling(g), in, mass, key, last);
+    }
+    const auto kept = [&](float v, int x) -> uint64_t {
+      const uint32_t k = key_of(v);
+      if (!(k > key || (k == key && x <= last))) return 0;
+      const double w = weigh(v);
+      return w >= least ? integer(w) : 0;
+    };
+    if (alone) {
+      // ---- all that is kept stands in s.token
+      uint64_t sum = 0;
+      taken.each([&](float v, int x) { sum += kept(v, x); });
+      sum = block_all<kWaves>(sum, s.part, Sum{});
+      if (a.probs) {
+        const double inverse = unit / static_cast<double>(sum);
+        taken.each([&](float v, int x) {
+          if (kept(v, x)) a.probs[static_cast<int64_t>(row) * a.V + x] = static_cast<float>(weigh(v) * inverse);
+        });
         if (tid == 0) a.state[row] = RowState{0, 0, m, 1, 0.0};
         return;
       }
-    } else if (none) {
-      key = key_of(peak);
-      last = -1;
-    } else {
-      // ---- selected by digits
-      const auto in = [&](float v) {
-        const int b = bin_of(v, top);
-        return b >= lo && b <= hi;
-      };
-      if (mode == kTopK) {
-        pick_border(all, s, static_cast<uint64_t>(set.k), [&](float, int) -> uint64_t { return 1; }, key, last);
-        if (set.p < 1.0) {
-          const uint32_t key_k = key;
-          const int last_k = last;
-          const auto value = [&](float v, int x) -> uint64_t {
-            const uint32_t k = key_of(v);
-            return k > key_k || (k == key_k && x <= last_k) ? integer(weight(v, mt, c2)) : 0;
-          };
-          uint64_t sum = 0;
-          all.each([&](float v, int x) { sum += value(v, x); });
-          sum = block_all<kWaves>(sum, s.part, Sum{});
-          __syncthreads();
-          pick_border(all, s, ceiling(set.p * static_cast<double>(sum)), value, key, last);
-        }
-      } else if (mode == kTopP) {
-        pick_border(all, s, ceiling(g), [&](float v, int) -> uint64_t { return in(v) ? integer(weight(v, mt, c2)) : 0; }, key, last);
+      // the first index at which the sum passes u times the total: digit by digit
+      uint64_t pass = static_cast<uint64_t>(fmin(fmax(static_cast<double>(a.uniforms[row]), 0.0), 1.0) * static_cast<double>(sum)) + 1;
+      uint32_t at = 0, mask = 0;
+#pragma unroll 1
+      for (int shift = 16; shift >= 0; shift -= 8) {
+        const uint32_t d = pick_digit<false>(s, pass, [&](auto add) {
+          taken.each([&](float v, int x) {
+            if ((static_cast<uint32_t>(x) & mask) == at) {
+              const uint64_t n = kept(v, x);
+              if (n) add((x >> shift) & 255, n);
+            }
+          });
+        });
+        at |= d << shift;
+        mask |= 255u << shift;
       }
-    }
-    if (alone) {
-      // ---- all that is kept stands in s.token: drawn from it, in index order
-      uint64_t t[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int at = 2 * tid + i;
-        t[i] = at < kept ? static_cast<uint64_t>(index_of(s.token[at])) << 32 | static_cast<uint32_t>(at) : 0;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (2 * tid + i < kept) s.token[2 * tid + i] = t[i];
-      __syncthreads();
-      sort_tokens<false>(s.token, kept);
-      uint64_t val[2], upto[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int at = 2 * tid + i;
-        val[i] = at < kept ? s.value[static_cast<uint32_t>(s.token[at])] : 0;
-      }
-      const uint64_t sum = block_scan2(val[0], val[1], s.part, upto[0], upto[1]);
-      const double pass = static_cast<double>(a.uniforms[row]) * static_cast<double>(sum);
-      int below = 0;  // that do not pass; the last one, should u be 1 or more
-#pragma unroll
-      for (int i = 0; i < 2; ++i) below += 2 * tid + i < kept && !(static_cast<double>(upto[i]) > pass);
-      below = block_all<kWaves>(below, reinterpret_cast<int*>(s.part), Sum{});
-      if (tid == 0) a.tokens[row] = static_cast<int64_t>(s.token[min(below, kept - 1)] >> 32);
+      if (tid == 0) a.tokens[row] = at;
       return;
     }
     // ---- the chunks' kept masses: what is certain, and the listed tokens up to the border
@@ -1069,7 +1057,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
         const uint32_t k = key_of(v);
         const int b = bin_of(v, top);
         if (b >= lo && b <= hi && (k > key || (k == key && x <= last))) {
-          const double w = weight(v, mt, c2);
+          const double w = weigh(v);
           if (w >= least) add_lds(s.extra + (x >> a.lg_chunk), max(static_cast<uint64_t>(w * units + 0.5), static_cast<uint64_t>(w > 0.0)));
         }
       });
@@ -1097,10 +1085,10 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
         if (some) {
           const int l = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
           chunk = c0 + l;
-          bar = goal - (__shfl(upto, l, 64) - __shfl(v, l, 64));
+          bar = goal - (lane_value(upto, l) - lane_value(v, l));
         }
         if (over) break;
-        run = __shfl(upto, 63, 64);
+        run = lane_value(upto, 63);
       }
       if (lane == 0) {
         s.chunk = chunk;
@@ -1132,7 +1120,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
       const uint32_t k = key_of(y);
       w[e] = 0.0;
       if (y != -INFINITY && (k > key || (k == key && x + e <= last))) {
-        const double ww = weight(y, mt, c2);
+        const double ww = weigh(y);
         w[e] = ww >= least ? ww : 0.0;
       }
       sum += w[e];
@@ -1179,6 +1167,7 @@ __global__ void __launch_bounds__(256) sample_write_kernel(SampleArgs a, int par
   if (st.done) return;
   const Settings& set = a.of(row);
   const float mt = tame(st.top);
+  const Weigh weigh(set, mt);
   const void* const src = row_of<DT>(a, row);
   for (int x = (part * 256 + static_cast<int>(threadIdx.x)) * 8; x < a.V; x += parts * 2048) {
     float v[8], out[8];
@@ -1189,7 +1178,7 @@ __global__ void __launch_bounds__(256) sample_write_kernel(SampleArgs a, int par
       const uint32_t k = key_of(y);
       out[e] = 0.f;
       if (y != -INFINITY && (k > st.key || (k == st.key && x + e <= st.last))) {
-        const double w = weight(y, mt, set.c);
+        const double w = weigh(y);
         out[e] = w >= set.m ? static_cast<float>(w * st.inverse) : 0.f;
       }
     }
