@@ -21,8 +21,8 @@
 //   select   (top-p, min-p) finds the bins that hold the row's border in the joined histograms, and lists what is
 //            kept (min-p), the tokens down to the border if they are few, or else those of its bins alone, with the
 //            mass of what is kept for certain above them
-//   finish   up to 64 listed tokens are ranked by one wave, among more (2048 of them in shared memory) the border
-//            is selected digit by digit; drawn from the list if it holds all that is kept, else by the chunks' masses
+//   finish   up to 64 listed tokens are ranked by one wave, 256 by the block, among more (5120 in shared memory) the
+//            border is selected digit by digit; drawn from the list if it holds all that is kept, else by the chunks' masses
 //   write    the probabilities of rows that keep many; the others' are few, in a row that the scan has cleared
 #include "tq_common.h"
 
@@ -32,7 +32,8 @@ constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of the finish
 constexpr int kScan = 512, kScanWaves = kScan / 64;     // of scan and select: a thread takes runs of 8 tokens
 constexpr int kBins = 512, kTail = kBins - 1;  // the last bin has everything below the others
 constexpr int kMaxChunks = 1024;
-constexpr int kShort = 2048;  // tokens that are taken into shared memory
+constexpr int kShort = 5120;  // tokens that are taken into shared memory
+constexpr int kRanked = 256;  // of them, tokens that are ranked one against the other
 constexpr int kFew = 1024;    // tokens down to the border that are listed with it
 constexpr double kUnit = 0x1p48;  // of a chunk's mass: at most 2^15 tokens of weight <= 1
 constexpr int kTiny = 49;         // a weight below 2^-49 is no unit
@@ -158,27 +159,45 @@ __device__ __forceinline__ uint32_t key_of(float v) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Eight logits from x on; what is not there is -inf.  NaN: as -inf (FIX), or as it is where every comparison leaves
-// it out.
-template <int DT, bool FIX = true>
-__device__ __forceinline__ void load_logits(const void* row, int x, int V, float (&v)[8]) {
-  if (x + 8 <= V) {
+// Eight logits from x on, as they are in memory; what is not there is -inf.
+template <int DT>
+struct Run {
+  uint32_t r[DT == TQ_F32 ? 8 : 4];
+  __device__ __forceinline__ void load(const void* row, int x, int V) {
     if constexpr (DT == TQ_F32) {
-      __builtin_memcpy(v, static_cast<const float*>(row) + x, 32);
+      if (x + 8 <= V) {
+        __builtin_memcpy(r, static_cast<const float*>(row) + x, 32);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = x + e < V ? static_cast<const uint32_t*>(row)[x + e] : 0xFF800000u;
+      }
     } else {
-      uint16_t r[8];
-      __builtin_memcpy(r, static_cast<const uint16_t*>(row) + x, 16);
+      constexpr uint32_t kLow = DT == TQ_F16 ? 0xFC00u : 0xFF80u;
+      if (x + 8 <= V) {
+        __builtin_memcpy(r, static_cast<const uint16_t*>(row) + x, 16);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = DT == TQ_F16 ? h2f(r[j]) : bf16_to_f32(r[j]);
+        for (int e = 0; e < 8; e += 2) {
+          const uint32_t lo = x + e < V ? static_cast<const uint16_t*>(row)[x + e] : kLow;
+          const uint32_t hi = x + e + 1 < V ? static_cast<const uint16_t*>(row)[x + e + 1] : kLow;
+          r[e / 2] = lo | hi << 16;
+        }
+      }
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = x + j < V ? load_act<DT>(row, x + j) : -INFINITY;
   }
-  if constexpr (FIX) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = fmaxf(v[j], -INFINITY);  // NaN: the other operand
+  __device__ __forceinline__ float operator[](int e) const {
+    if constexpr (DT == TQ_F32) return __uint_as_float(r[e]);
+    else if constexpr (DT == TQ_F16) return h2f(static_cast<uint16_t>(e & 1 ? r[e / 2] >> 16 : r[e / 2] & 0xFFFF));
+    else return __uint_as_float(e & 1 ? r[e / 2] & 0xFFFF0000u : r[e / 2] << 16);
   }
+};
+// eight logits, NaN as -inf
+template <int DT>
+__device__ __forceinline__ void load_logits(const void* row, int x, int V, float (&v)[8]) {
+  Run<DT> run;
+  run.load(row, x, V);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = fmaxf(run[e], -INFINITY);  // of a NaN the other operand
 }
 template <int DT>
 __device__ __forceinline__ const void* row_of(const SampleArgs& a, int row) {
@@ -273,11 +292,16 @@ __device__ __forceinline__ void each_run(const SampleArgs& a, int row, int chunk
   const void* const src = row_of<DT>(a, row);
   const int x0 = (chunk << a.lg_chunk) + static_cast<int>(threadIdx.x) * 8, runs = 1 << (a.lg_chunk - 12);
   static_assert(kScan * 8 == 1 << 12, "tokens of a block's run");
+  Run<DT> next;
+  next.load(src, x0, a.V);
 #pragma unroll 1
   for (int r = 0; r < runs; ++r) {
     const int x = x0 + r * (kScan * 8);
+    const Run<DT> run = next;
+    if (r + 1 < runs) next.load(src, x + kScan * 8, a.V);  // flies meanwhile
     float v[8];
-    load_logits<DT, false>(src, x, a.V, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = run[e];
     if (m == INFINITY) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = tame(v[e], m);
@@ -528,12 +552,15 @@ __global__ void __launch_bounds__(kScan) sample_select_kernel(SampleArgs a) {
       uint64_t h[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int k = i0 + i, b = k < a.C ? tid - s.off[k] : -1;
-        h[i] = b >= 0 && b < s.depth[min(k, a.C - 1)] && b < kTail ? a.hist[(at0 + k) * kBins + b] : 0;
+        const int k = min(i0 + i, a.C - 1);  // every load unconditional, so that they fly together
+        h[i] = a.hist[(at0 + k) * kBins + min(max(tid - s.off[k], 0), kTail)];
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i0 + i < a.C) share += static_cast<float>(h[i]) * 0x1p-48f * s.factor[i0 + i];
+      for (int i = 0; i < 8; ++i) {
+        const int k = min(i0 + i, a.C - 1), b = tid - s.off[k];
+        const bool in = i0 + i < a.C && b >= 0 && b < s.depth[k] && b < kTail;
+        share += in ? static_cast<float>(h[i]) * 0x1p-48f * s.factor[k] : 0.f;
+      }
     }
     s.bins[tid] = tid < kTail ? share * static_cast<float>(1.0 / total) : 0.f;
     __syncthreads();
@@ -595,10 +622,10 @@ constexpr int kSegments = 2048;  // runs of 64 listed tokens that the table hold
 
 struct FinishSmem {
   uint64_t token[kShort];  // key, then the complement of the index: larger ones rank first
-  uint64_t value[64];
+  uint64_t value[kRanked];
   uint32_t segment[kSegments];  // chunk, run of 64
   union {
-    uint64_t digits[256];
+    uint64_t digits[512];
     uint32_t bins[kBins];
   };
   uint64_t part[kWaves];
@@ -680,21 +707,21 @@ struct Taken {
   }
 };
 
-// Among some tokens: the digit in which the running sum of their values, from the largest digit down (FALL) or
+// Among some tokens: the digit (of 9 bits) in which the running sum of their values, from the largest digit down (FALL) or
 // from the smallest up, reaches goal; goal becomes what is left of it in front of that digit.  Where the sum never
 // reaches it: the last digit that holds any.
 template <bool FALL, class Each>
 __device__ __forceinline__ uint32_t pick_digit(FinishSmem& s, uint64_t& goal, Each each) {
   const int tid = threadIdx.x;
-  if (tid < 256) s.digits[tid] = 0;
+  if (tid < 512) s.digits[tid] = 0;
   __syncthreads();
   each([&](uint32_t digit, uint64_t value) { add_lds(s.digits + digit, value); });
   __syncthreads();
   if (tid < 64) {
-    uint64_t h[4], sum = 0;
+    uint64_t h[8], sum = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      h[i] = s.digits[FALL ? 255 - (4 * tid + i) : 4 * tid + i];
+    for (int i = 0; i < 8; ++i) {
+      h[i] = s.digits[FALL ? 511 - (8 * tid + i) : 8 * tid + i];
       sum += h[i];
     }
     const uint64_t upto = wave_scan(sum);
@@ -705,7 +732,7 @@ __device__ __forceinline__ uint32_t pick_digit(FinishSmem& s, uint64_t& goal, Ea
       int d = 0;
       bool done = false;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 8; ++i) {
         if (!done && h[i] != 0) {
           d = i;
           before = at;
@@ -713,8 +740,8 @@ __device__ __forceinline__ uint32_t pick_digit(FinishSmem& s, uint64_t& goal, Ea
         }
         at += h[i];
       }
-      const int pos = 4 * l + d;
-      s.digit = FALL ? 255 - pos : pos;
+      const int pos = 8 * l + d;
+      s.digit = FALL ? 511 - pos : pos;
       s.rest = goal > before ? goal - before : 0;
     }
   }
@@ -723,26 +750,47 @@ __device__ __forceinline__ uint32_t pick_digit(FinishSmem& s, uint64_t& goal, Ea
   return s.digit;
 }
 
+// The index at which the running sum of some tokens' values, in index order, reaches goal.  top_digit: shift of the
+// indices' highest digit.  each(fn(index, value)).
+template <class Each>
+__device__ __forceinline__ int pick_index(FinishSmem& s, uint64_t goal, int top_digit, Each each) {
+  uint32_t at = 0;
+#pragma unroll 1
+  for (int shift = top_digit; shift >= 0; shift -= 9) {
+    const uint32_t d = pick_digit<false>(s, goal, [&](auto add) {
+      each([&](int x, uint64_t n) {
+        if (static_cast<uint32_t>(x) >> shift >> 9 == at) add((x >> shift) & 511, n);
+      });
+    });
+    at = at << 9 | d;
+  }
+  return static_cast<int>(at);
+}
+
 // The border in rank among some tokens.  value: 1 (by rank) or the token's mass, 0: not one of them; kept are the
 // tokens whose predecessors' values sum to less than goal (>= 1).
-template <class Tokens, class Value>
-__device__ __forceinline__ void pick_border(const Tokens& all, FinishSmem& s, uint64_t goal, Value value, uint32_t& key, int& last) {
-  uint32_t prefix = 0, mask = 0;
+template <int DT, class Tokens, class Value>
+__device__ __forceinline__ void pick_border(const Tokens& all, FinishSmem& s, int top_digit, uint64_t goal, Value value, uint32_t& key,
+                                            int& last) {
+  // the bits in which floats of the type differ, from the top: 32, 19 (f16: sign, 8 of exponent, 10) or 16; those
+  // below are all zero, or of a negative float all one
+  constexpr int kBits = DT == TQ_F32 ? 32 : DT == TQ_F16 ? 19 : 16, kDigits = (kBits + 8) / 9, kLow = 32 - kBits;
+  uint32_t prefix = 0;
 #pragma unroll 1
-  for (int shift = 24; shift >= 0; shift -= 8) {
+  for (int shift = 9 * (kDigits - 1); shift >= 0; shift -= 9) {
     const uint32_t d = pick_digit<true>(s, goal, [&](auto add) {
       all.each([&](float v, int x) {
-        const uint32_t k = key_of(v);
-        if ((k & mask) == prefix) {
+        const uint32_t k = key_of(v) >> kLow;
+        if (static_cast<uint32_t>(static_cast<uint64_t>(k) >> (shift + 9)) == prefix) {
           const uint64_t n = value(v, x);
-          if (n) add((k >> shift) & 255, n);
+          if (n) add((k >> shift) & 511, n);
         }
       });
     });
-    prefix |= d << shift;
-    mask |= 255u << shift;
+    prefix = prefix << 9 | d;
   }
-  key = prefix;
+  key = prefix << kLow;
+  if (kLow && !(key & 0x80000000u)) key |= (1u << kLow) - 1;
   // equal logits have equal values: how many of them are kept, the first in index order
   if (threadIdx.x == 0) {
     s.one = 0;
@@ -764,25 +812,22 @@ __device__ __forceinline__ void pick_border(const Tokens& all, FinishSmem& s, ui
   if (keep < 1) keep = 1;
   last = 0x7FFFFFFF;
   if (keep >= s.ties) return;
-  uint32_t at = 0;
-  mask = 0;
-#pragma unroll 1
-  for (int shift = 16; shift >= 0; shift -= 8) {
-    const uint32_t d = pick_digit<false>(s, keep, [&](auto add) {
-      all.each([&](float v, int x) {
-        if (key_of(v) == key && (static_cast<uint32_t>(x) & mask) == at && value(v, x)) add((x >> shift) & 255, 1);
-      });
+  last = pick_index(s, keep, top_digit, [&](auto fn) {
+    all.each([&](float v, int x) {
+      if (key_of(v) == key && value(v, x)) fn(x, 1);
     });
-    at |= d << shift;
-    mask |= 255u << shift;
-  }
-  last = static_cast<int>(at);
+  });
+}
+
+__device__ __forceinline__ uint64_t ceiling(double g) {  // at least 1
+  return g >= 0x1p63 ? ~0ull : g >= 1.0 ? static_cast<uint64_t>(ceil(g)) : 1;
 }
 
 // The border of a row: by rank, then by mass
-template <class Tokens, class In, class Integer>
-__device__ __forceinline__ void cut_row(const Tokens& all, FinishSmem& s, const Settings& set, uint64_t mass_goal, In in, Integer integer, uint32_t& key, int& last) {
-  if (set.mode == kTopK) pick_border(all, s, static_cast<uint64_t>(set.k), [&](float, int) -> uint64_t { return 1; }, key, last);
+template <int DT, class Tokens, class In, class Integer>
+__device__ __forceinline__ void cut_row(const Tokens& all, FinishSmem& s, const Settings& set, int top_digit, uint64_t mass_goal, In in,
+                                        Integer integer, uint32_t& key, int& last) {
+  if (set.mode == kTopK) pick_border<DT>(all, s, top_digit, static_cast<uint64_t>(set.k), [&](float, int) -> uint64_t { return 1; }, key, last);
   if (set.p >= 1.0) return;
   const uint32_t key_k = key;
   const int last_k = last;
@@ -795,10 +840,84 @@ __device__ __forceinline__ void cut_row(const Tokens& all, FinishSmem& s, const 
     all.each([&](float v, int x) { sum += value(v, x); });
     sum = block_all<kWaves>(sum, s.part, Sum{});
     __syncthreads();
-    const double goal = ceil(set.p * static_cast<double>(sum));
-    mass_goal = goal >= 1.0 ? static_cast<uint64_t>(goal) : 1;
+    mass_goal = ceiling(set.p * static_cast<double>(sum));
   }
-  pick_border(all, s, mass_goal, value, key, last);
+  pick_border<DT>(all, s, top_digit, mass_goal, value, key, last);
+}
+
+// A row's whole list in s.token, n <= kRanked of them, or (ONE) at most 64 by one wave: a thread has a token, and meets
+// every other.
+template <bool ONE>
+__device__ __forceinline__ void rank_tokens(const SampleArgs& a, FinishSmem& s, const Settings& set, int row, float m, int n, double goal) {
+  const int tid = threadIdx.x;
+  const auto sync = [] {
+    if constexpr (ONE) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    else __syncthreads();
+  };
+  const auto sum_of = [&](uint64_t v) {
+    if constexpr (ONE) return wave_all(v, Sum{});
+    else {
+      __syncthreads();
+      return block_all<kWaves>(v, s.part, Sum{});
+    }
+  };
+  const Weigh weigh(set, tame(m));
+  const uint64_t t = tid < n ? s.token[tid] : 0;
+  const double w = tid < n ? weigh(logit_of(t)) : 0.0;
+  constexpr double unit = ONE ? 0x1p55 : 0x1p53;  // the maximum is among them
+  const uint64_t whole = static_cast<uint64_t>(w * unit + 0.5), val = w > 0.0 && !whole ? 1 : whole;
+  const int x = index_of(t), padded = (n + 7) & ~7;
+  if (tid < padded) {
+    s.token[tid] = t;
+    s.value[tid] = val;
+  }
+  sync();
+  int rank = 0;
+  uint64_t before = 0;
+  if (ONE || tid < n) {
+#pragma unroll 8
+    for (int j = 0; j < padded; ++j) {
+      const uint64_t v = s.value[j];
+      const bool ahead = s.token[j] > t;
+      rank += ahead;
+      before += ahead ? v : 0;
+    }
+  }
+  const bool in = tid < n && (set.mode != kTopK || rank < set.k);
+  uint64_t bar = ~0ull;  // predecessors of a kept token sum to less
+  if (set.mode == kTopP) bar = ceiling(goal * unit);
+  else if (set.mode == kTopK && set.p < 1.0) bar = ceiling(set.p * static_cast<double>(sum_of(in ? val : 0)));
+  const bool on = in && before < bar && w >= set.m;
+  const uint64_t sum = sum_of(on ? val : 0);
+  if (a.probs) {
+    if (on) a.probs[static_cast<int64_t>(row) * a.V + x] = static_cast<float>(w * (unit / static_cast<double>(sum)));
+    if (tid == 0) a.state[row] = RowState{0, 0, m, 1, 0.0};
+    return;
+  }
+  const double pass = static_cast<double>(a.uniforms[row]) * static_cast<double>(sum);
+  sync();
+  if (tid < padded) s.value[tid] = on ? val : 0;
+  sync();
+  uint64_t upto = 0;  // of the kept tokens at or before it
+  if (ONE || tid < n) {
+#pragma unroll 8
+    for (int j = 0; j < padded; ++j) {
+      const uint64_t v = s.value[j];
+      upto += index_of(s.token[j]) <= x ? v : 0;
+    }
+  }
+  // the first index that passes; the last one, should u be 1 or more
+  const bool over = on && static_cast<double>(upto) > pass;
+  int first = over ? -x : -0x7FFFFFFF, end = on ? x : -1;
+  if constexpr (ONE) {
+    first = wave_all(first, Max{});
+    end = wave_all(end, Max{});
+  } else {
+    first = block_all<kWaves>(first, reinterpret_cast<int*>(s.part), Max{});
+    __syncthreads();
+    end = block_all<kWaves>(end, reinterpret_cast<int*>(s.part), Max{});
+  }
+  if (tid == 0) a.tokens[row] = first > -0x7FFFFFFF ? -first : end;
 }
 
 template <int DT>
@@ -891,7 +1010,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
       return s.hi;
     };
     // every chunk listed its own first k: of them all, those down to the bin that k reach
-    const bool many = mode == kTopK && (s.raw || s.segments > kShort / 64);
+    const bool many = mode == kTopK && (s.raw || s.segments > 2 * kThreads / 64);
     if (many) {
       all.each([&](float v, int) { atomicAdd(s.bins + bin_of(v, top), 1u); });
       hi = reach_rank();
@@ -912,7 +1031,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
     });
     __syncthreads();
     int n = s.n;
-    if (mode == kTopK && !many && n > 64) {
+    if (mode == kTopK && !many && n > 64) {  // n <= 2048
       uint64_t t[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -934,57 +1053,19 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
     }
     const bool alone = n <= kShort && lo == 0;  // the tokens in s.token are all that can be kept
     const double goal = set.p * cut.total;
-    const auto ceiling = [](double g) -> uint64_t { return g >= 0x1p63 ? ~0ull : g >= 1.0 ? static_cast<uint64_t>(ceil(g)) : 1; };
     const auto integer = [&](double w) -> uint64_t {  // of listed tokens
       if (!(w > 0.0)) return 0;
       const uint64_t x = static_cast<uint64_t>(w * unit + 0.5);
       return x ? x : 1;
     };
 
-    if (n <= 64 && alone) {
-      // ---- ranked by one wave: lane i has token i, and meets every other
-      if (wave != 0) return;
-      const uint64_t t = lane < n ? s.token[lane] : 0;
-      const double w = lane < n ? weigh(logit_of(t)) : 0.0;
-      unit = 0x1p55;  // the maximum is among them
-      const uint64_t val = integer(w);
-      const int x = index_of(t);
-      s.token[lane] = t;
-      s.value[lane] = val;
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      int rank = 0;
-      uint64_t before = 0;
-#pragma unroll 8
-      for (int j = 0; j < ((n + 7) & ~7); ++j) {
-        const uint64_t v = s.value[j];
-        const bool ahead = s.token[j] > t;
-        rank += ahead;
-        before += ahead ? v : 0;
+    const int top_digit = 9 * ((31 - __builtin_clz(a.V - 1 | 1)) / 9);  // of an index
+    if (alone && n <= kRanked) {
+      if (n > 64) {
+        rank_tokens<false>(a, s, set, row, m, n, goal);
+      } else if (wave == 0) {
+        rank_tokens<true>(a, s, set, row, m, n, goal);
       }
-      const bool in = lane < n && (mode != kTopK || rank < set.k);
-      uint64_t bar = ~0ull;
-      if (mode == kTopP) bar = ceiling(goal * unit);
-      else if (mode == kTopK && set.p < 1.0) bar = ceiling(set.p * static_cast<double>(wave_all(in ? val : 0, Sum{})));
-      const bool on = in && before < bar && w >= least;
-      const uint64_t sum = wave_all(on ? val : 0, Sum{});
-      if (a.probs) {
-        if (on) a.probs[static_cast<int64_t>(row) * a.V + x] = static_cast<float>(w * (unit / static_cast<double>(sum)));
-        if (lane == 0) a.state[row] = RowState{0, 0, m, 1, 0.0};
-        return;
-      }
-      const double pass = static_cast<double>(a.uniforms[row]) * static_cast<double>(sum);
-      s.value[lane] = on ? val : 0;
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      uint64_t upto = 0;  // of the kept tokens at or before it
-#pragma unroll 8
-      for (int j = 0; j < ((n + 7) & ~7); ++j) {
-        const uint64_t v = s.value[j];
-        upto += index_of(s.token[j]) <= x ? v : 0;
-      }
-      // the first index that passes; the last one, should u be 1 or more
-      const bool over = on && static_cast<double>(upto) > pass;
-      const int first = -wave_all(over ? -x : -0x7FFFFFFF, Max{}), end = wave_all(on ? x : -1, Max{});
-      if (lane == 0) a.tokens[row] = first < 0x7FFFFFFF ? first : end;
       return;
     }
 
@@ -1008,8 +1089,8 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
       key = key_of(peak);
       last = -1;
     } else if (mode != kMinP) {
-      if (n <= kShort) cut_row(taken, s, set, ceiling(g), in, mass, key, last);
-      else cut_row(all, s, set, ceiling(g), in, mass, key, last);
+      if (n <= kShort) cut_row<DT>(taken, s, set, top_digit, ceiling(g), in, mass, key, last);
+      else cut_row<DT>(all, s, set, top_digit, ceiling(g), in, mass, key, last);
     }
     const auto kept = [&](float v, int x) -> uint64_t {
       const uint32_t k = key_of(v);
@@ -1031,21 +1112,13 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
         return;
       }
       // the first index at which the sum passes u times the total: digit by digit
-      uint64_t pass = static_cast<uint64_t>(fmin(fmax(static_cast<double>(a.uniforms[row]), 0.0), 1.0) * static_cast<double>(sum)) + 1;
-      uint32_t at = 0, mask = 0;
-#pragma unroll 1
-      for (int shift = 16; shift >= 0; shift -= 8) {
-        const uint32_t d = pick_digit<false>(s, pass, [&](auto add) {
-          taken.each([&](float v, int x) {
-            if ((static_cast<uint32_t>(x) & mask) == at) {
-              const uint64_t n = kept(v, x);
-              if (n) add((x >> shift) & 255, n);
-            }
-          });
+      const uint64_t pass = static_cast<uint64_t>(fmin(fmax(static_cast<double>(a.uniforms[row]), 0.0), 1.0) * static_cast<double>(sum)) + 1;
+      const int at = pick_index(s, pass, top_digit, [&](auto fn) {
+        taken.each([&](float v, int x) {
+          const uint64_t n = kept(v, x);
+          if (n) fn(x, n);
         });
-        at |= d << shift;
-        mask |= 255u << shift;
-      }
+      });
       if (tid == 0) a.tokens[row] = at;
       return;
     }
@@ -1204,7 +1277,7 @@ static SamplePlan plan_sample(int64_t N, int64_t V) {
   SamplePlan p{};
   p.lg_chunk = 15;
   const auto chunks = [&](int lg) { return (V + (int64_t(1) << lg) - 1) >> lg; };
-  while (p.lg_chunk > 12 && N * chunks(p.lg_chunk) < 1024 && chunks(p.lg_chunk - 1) <= kMaxChunks) --p.lg_chunk;
+  while (p.lg_chunk > 12 && N * chunks(p.lg_chunk) < 512 && chunks(p.lg_chunk - 1) <= kMaxChunks) --p.lg_chunk;
   p.C = static_cast<int>(chunks(p.lg_chunk));
   const int64_t n = N * p.C;
   int64_t at = 0;
