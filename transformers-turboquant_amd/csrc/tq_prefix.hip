@@ -10,9 +10,10 @@
 //
 // The work is a list of segments: a group's shared keys against a tile of 16 NTP of its columns, a
 // sequence's own keys against a tile of 16 NTO of its own.  As in tree attention their rounds (32 keys per wave of
-// a block) are dealt in equal stretches to as many blocks per kv head as the device holds at
-// once, from the lengths and groups that stand on the device; each (block, segment) part leaves a
-// record, and the merge joins those of the sequence's own segment and of the group's.
+// a block) are dealt in stretches to as many blocks per kv head as the device holds at once, from the
+// lengths and groups that stand on the device; each (block, segment) part leaves a record, and the merge joins those
+// of the sequence's own segment and of the group's.  The stretches are equal in time, not in rounds: a round weighs
+// what it takes, and a segment has a weight in front of its rounds for what a part takes besides them.
 #include "tq_tree.h"
 
 namespace tq {
@@ -31,21 +32,33 @@ constexpr int kSlab = 32;
 // A sequence's segments are those of the group it is the first of (pt tiles of pr rounds), then its
 // own (ot tiles of rounds(keys - start)).  The parts of block k in segment s have record k + s: walking
 // along the rounds, every step to the next part moves to the next block, to a later segment or both.
+//
+// Positions on the way along all segments count units of about 2000 cycles: kPart for a part (queries, first
+// slabs, join of the waves: 8 to 10 thousand cycles, as long as 2 rounds), then its rounds of 2 (one tile of columns, 4100
+// cycles) or 3 (two tiles, 5800).  A block does the rounds that begin in its stretch.  Without the weights a
+// block of four short sequences ends at 76 us where the others end at 51 (8 trees of 8 nodes on 16k keys of their
+// group).
+constexpr int kPart = 5;
 template <int RK, int WP, int WO>
 struct PrefixSplit {
+  static constexpr int UP = WP > 16 ? 3 : 2, UO = WO > 16 ? 3 : 2;  // units of a round
+  static constexpr int LEAST = WP > 16 ? 6 : 2;                     // of a block, no fewer than of a round
   struct Row {
     int start, keys;   // own positions [start, keys), keys = 0: none
     int pr, pt, cols;  // of the group it is the first of: rounds of a tile, tiles, columns
     int first;         // of the sequence's group, -1 without one
   };
   Row r0;           // sequence `lane`
-  int upto0, seg0;  // sums of rounds and segments up to it
+  int upto0, seg0;  // sums of units and segments up to it
   int ot;           // tiles of a sequence's own columns
   int total, blocks, each, extra;
 
   __device__ __forceinline__ static int rounds(int keys) { return static_cast<int>(static_cast<unsigned>(keys + RK - 1) / RK); }
   __device__ __forceinline__ int own_rounds(const Row& r) const { return r.keys ? rounds(r.keys - r.start) : 0; }
-  __device__ __forceinline__ int row_rounds(const Row& r) const { return r.pr * r.pt + own_rounds(r) * ot; }
+  // units of a tile of shared and of own keys (a sequence without a place has none), and of all of a sequence's
+  __device__ __forceinline__ static int shared_units(const Row& r) { return kPart + r.pr * UP; }
+  __device__ __forceinline__ int own_units(const Row& r) const { return r.keys ? kPart + own_rounds(r) * UO : 0; }
+  __device__ __forceinline__ int row_units(const Row& r) const { return shared_units(r) * r.pt + own_units(r) * ot; }
   __device__ __forceinline__ int row_segments(const Row& r) const { return r.pt + ot; }
 
   // sequence b0 + lane, by all lanes of a wave
@@ -78,21 +91,21 @@ struct PrefixSplit {
   }
   __device__ __forceinline__ PrefixSplit(const PrefixArgs& a, const Row& r) : r0(r) {
     ot = (a.C + WO - 1) / WO;
-    upto0 = scan64(row_rounds(r0));
+    upto0 = scan64(row_units(r0));
     seg0 = scan64(row_segments(r0));
     total = __builtin_amdgcn_readlane(upto0, 63);
     for (int b0 = 64; b0 < a.B; b0 += 64)
-      total += __builtin_amdgcn_readlane(scan64(row_rounds(load(a, b0))), 63);
-    blocks = min(a.slots, static_cast<int>((static_cast<unsigned>(total) + (1u << a.lg_least) - 1) >> a.lg_least));
+      total += __builtin_amdgcn_readlane(scan64(row_units(load(a, b0))), 63);
+    blocks = min(a.slots, static_cast<int>(static_cast<unsigned>(total) / LEAST));  // (total is 0, or more than LEAST)
     each = blocks ? static_cast<unsigned>(total) / static_cast<unsigned>(blocks) : 0;
     extra = total - each * blocks;
   }
   __device__ __forceinline__ int begin(int k) const { return k * each + min(k, extra); }
-  __device__ __forceinline__ int block_of(int round) const {
-    const unsigned big = extra * (each + 1), x = round;
+  __device__ __forceinline__ int block_of(int unit) const {
+    const unsigned big = extra * (each + 1), x = unit;
     return x < big ? x / static_cast<unsigned>(each + 1) : extra + (x - big) / static_cast<unsigned>(each);
   }
-  // a sequence as all lanes see it: its first round and segment, and its row
+  // a sequence as all lanes see it: its first unit and segment, and its row
   struct At {
     int first, segment;
     Row r;
@@ -105,11 +118,11 @@ struct PrefixSplit {
     at.r.pt = __builtin_amdgcn_readlane(r.pt, l);
     at.r.cols = __builtin_amdgcn_readlane(r.cols, l);
     at.r.first = __builtin_amdgcn_readlane(r.first, l);
-    at.first = __builtin_amdgcn_readlane(upto, l) - row_rounds(at.r);
+    at.first = __builtin_amdgcn_readlane(upto, l) - row_units(at.r);
     at.segment = __builtin_amdgcn_readlane(seg, l) - row_segments(at.r);
     return at;
   }
-  // the sequence of round x < total
+  // the sequence of unit x < total
   __device__ __forceinline__ At sequence_at(const PrefixArgs& a, int x, int& b) const {
     Row r = r0;
     int upto = upto0, seg = seg0;
@@ -134,7 +147,7 @@ struct PrefixSplit {
   __device__ __forceinline__ void next(const PrefixArgs& a, int b0, Row& r, int& upto, int& seg) const {
     const int run = __builtin_amdgcn_readlane(upto, 63), runs = __builtin_amdgcn_readlane(seg, 63);
     r = load(a, b0);
-    upto = scan64(row_rounds(r)) + run;
+    upto = scan64(row_units(r)) + run;
     seg = scan64(row_segments(r)) + runs;
   }
 };
@@ -163,13 +176,19 @@ prefix_attn_kernel(PrefixArgs a) {
   while (x < x_end) {
     int b;
     const typename Split::At at = split.sequence_at(a, x, b);
-    const int before = at.r.pr * at.r.pt;  // rounds of the shared keys' tiles, in front of the own ones'
+    const int before = Split::shared_units(at.r) * at.r.pt;  // the shared keys' tiles, in front of the own ones'
     const bool own = x - at.first >= before;
-    const int each = own ? split.own_rounds(at.r) : at.r.pr, from = at.first + (own ? before : 0);
-    const int tile = static_cast<int>(static_cast<unsigned>(x - from) / static_cast<unsigned>(each));
-    const int r0 = x - from - tile * each, r1 = min(r0 + x_end - x, each);
+    const int units = own ? split.own_units(at.r) : Split::shared_units(at.r), from = at.first + (own ? before : 0);
+    const int tile = static_cast<int>(static_cast<unsigned>(x - from) / static_cast<unsigned>(units));
+    const int u0 = x - from - tile * units, u1 = min(u0 + x_end - x, units);
+    const auto rounds_before = [&](int u) {  // rounds that begin in front of the segment's unit u
+      const unsigned v = max(u - kPart, 0);
+      return static_cast<int>(own ? (v + Split::UO - 1) / Split::UO : (v + Split::UP - 1) / Split::UP);
+    };
+    const int r0 = rounds_before(u0), r1 = rounds_before(u1);
     const int64_t rec = ((static_cast<int64_t>(blockIdx.x) + at.segment + tile + (own ? at.r.pt : 0)) * a.Hkv + hkv) * WP;
-    x += r1 - r0;
+    x += u1 - u0;
+    if (r0 == r1) continue;
     if (own) {
       const TreePart part{b, a.C, tile * WO, at.r.keys - a.T, at.r.start + r0 * RK, min(at.r.keys, at.r.start + r1 * RK), rec};
       tree_part<D, BITS, NTO, NW, false>(a, part, hkv, sm);
@@ -200,56 +219,80 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(PrefixArgs a) {
   const typename Split::At own = split.sequence(a, b);
   const typename Split::At head = own.r.first >= 0 && own.r.first != b ? split.sequence(a, own.r.first) : own;
   const int64_t step = static_cast<int64_t>(a.Hkv) * WP;  // columns between records
+  // a column's records: n1 of the group's tile from column at1 on, those of its own tile from at2 on, n in all
+  struct Records {
+    int64_t at1, at2;
+    int n1, n;
+  };
+  const auto records_of = [&](int c) {
+    Records rs{0, 0, 0, 0};
+    if (!own.r.keys) return rs;
+    const auto list = [&](int first, int units, int rounds, int segment, int col, int64_t& at) {
+      const int k0 = split.block_of(first + kPart), k1 = split.block_of(first + kPart + (rounds - 1) * units);
+      at = ((static_cast<int64_t>(k0) + segment) * a.Hkv + hkv) * WP + col;
+      return k1 - k0 + 1;
+    };
+    if (own.r.first >= 0) {
+      const int pc = (b - own.r.first) * a.C + c, tile = pc / WP;
+      rs.n1 = list(head.first + tile * Split::shared_units(head.r), Split::UP, head.r.pr, head.segment + tile, pc - tile * WP,
+                   rs.at1);
+    }
+    const int tile = c / WO;
+    rs.n = rs.n1 + list(own.first + Split::shared_units(own.r) * own.r.pt + tile * split.own_units(own.r), Split::UO,
+                        split.own_rounds(own.r), own.segment + own.r.pt + tile, c - tile * WO, rs.at2);
+    return rs;
+  };
+  const auto column = [&](const Records& rs, int q) { return q < rs.n1 ? rs.at1 + q * step : rs.at2 + (q - rs.n1) * step; };
+  // one memory round trip for the first NB records of all the wave's columns: partial O, and a record's
+  // maximum and sum per lane
+  Records rs[CW];
+  floatPL v0[CW][NB];
+  float m0[CW], l0[CW];
 #pragma unroll
   for (int k = 0; k < CW; ++k) {
-    const int cc = wave + 4 * k, c = c0 + cc;
+    rs[k] = records_of(min(c0 + wave + 4 * k, a.C - 1));
+#pragma unroll
+    for (int q = 0; q < NB; ++q)
+      v0[k][q] = q < rs[k].n ? *reinterpret_cast<const floatPL*>(a.part_o + column(rs[k], q) * D + PL * lane) : floatPL{};
+    m0[k] = lane < rs[k].n ? a.part_ml[column(rs[k], lane) * 2] : -INFINITY;
+    l0[k] = lane < rs[k].n ? a.part_ml[column(rs[k], lane) * 2 + 1] : 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < CW; ++k) {
+    const int cc = wave + 4 * k, c = c0 + cc, n = rs[k].n;
     floatPL o = floatPL{};
-    if (c < a.C && own.r.keys) {
-      // columns of the first record of both lists, and how many records they have
-      int64_t at1 = 0, at2;
-      int n1 = 0, n2;
-      const auto records = [&](int first, int rounds, int segment, int col, int64_t& at) {
-        const int k0 = split.block_of(first), k1 = split.block_of(first + rounds - 1);
-        at = ((static_cast<int64_t>(k0) + segment) * a.Hkv + hkv) * WP + col;
-        return k1 - k0 + 1;
-      };
-      if (own.r.first >= 0) {
-        const int pc = (b - own.r.first) * a.C + c, tile = pc / WP;
-        n1 = records(head.first + tile * head.r.pr, head.r.pr, head.segment + tile, pc - tile * WP, at1);
-      }
-      {
-        const int tile = c / WO, rounds = split.own_rounds(own.r);
-        n2 = records(own.first + own.r.pr * own.r.pt + tile * rounds, rounds, own.segment + own.r.pt + tile, c - tile * WO, at2);
-      }
-      const int n = n1 + n2;
-      const auto column = [&](int q) { return q < n1 ? at1 + q * step : at2 + (q - n1) * step; };
-      float mx = -INFINITY;
-      for (int r = lane; r < n; r += 64) mx = fmaxf(mx, a.part_ml[column(r) * 2]);
+    if (c < a.C) {
+      const auto ml = [&](int q) { return a.part_ml + column(rs[k], q) * 2; };
+      float mx = m0[k];
+      for (int q = lane + 64; q < n; q += 64) mx = fmaxf(mx, ml(q)[0]);
 #pragma unroll
       for (int sh = 32; sh >= 1; sh >>= 1) mx = fmaxf(mx, __shfl_xor(mx, sh, 64));
       float lsum = 0.f;
       for (int q0 = 0; q0 < n; q0 += 64) {
         float w = 0.f;
         if (q0 + lane < n) {
-          const float* const ml = a.part_ml + column(q0 + lane) * 2;
-          const float m = ml[0];
+          const float m = q0 == 0 ? m0[k] : ml(q0 + lane)[0];
           if (m != -INFINITY) {
             w = __builtin_amdgcn_exp2f(m - mx);
-            lsum += w * ml[1];
+            lsum += w * (q0 == 0 ? l0[k] : ml(q0 + lane)[1]);
           }
         }
-        const int nb = min(64, n - q0);
-        for (int u = 0; u < nb; u += NB) {
-          floatPL v[NB];
-#pragma unroll
-          for (int q = 0; q < NB; ++q)
-            v[q] = u + q < nb ? *reinterpret_cast<const floatPL*>(a.part_o + column(q0 + u + q) * D + PL * lane) : floatPL{};
+        const auto add = [&](const floatPL (&v)[NB], int u) {
 #pragma unroll
           for (int q = 0; q < NB; ++q) {
-            const float ww = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), (u + q) & 63));
+            const float ww = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), u + q));
 #pragma unroll
             for (int e = 0; e < PL; ++e) o[e] = fmaf(ww, v[q][e], o[e]);
           }
+        };
+        if (q0 == 0) add(v0[k], 0);
+        const int nb = min(64, n - q0);
+        for (int u = q0 == 0 ? NB : 0; u < nb; u += NB) {
+          floatPL v[NB];
+#pragma unroll
+          for (int q = 0; q < NB; ++q)
+            v[q] = u + q < nb ? *reinterpret_cast<const floatPL*>(a.part_o + column(rs[k], q0 + u + q) * D + PL * lane) : floatPL{};
+          add(v, u);
         }
       }
 #pragma unroll
@@ -268,7 +311,7 @@ using PrefixKernel = void (*)(PrefixArgs);
 struct PrefixPlan {
   PrefixKernel attend;
   int tiles, own_tiles;  // NTP, NTO
-  int slots, lg_least;
+  int slots;
   int64_t records, bytes;
 };
 
@@ -295,12 +338,11 @@ static PrefixPlan plan_prefix(int B, int Hq, int Hkv, int T, int64_t maxpos, int
   const int res = resident_blocks(reinterpret_cast<const void*>(p.attend), 256,
                                   resident[d == 128][bits - 2][p.tiles + p.own_tiles - 2]);
   p.slots = res / Hkv > 1 ? res / Hkv : 1;
-  p.lg_least = p.tiles == 2 ? 1 : 0;
   // a sequence's own tiles, and as many of its group's at most
   const int own = (C + 16 * p.own_tiles - 1) / (16 * p.own_tiles);
   const int64_t segments = 2 * static_cast<int64_t>(B) * own;
-  const int64_t most = segments * ((maxpos + 127) / 128);  // rounds
-  if (p.slots > most) p.slots = static_cast<int>(most);
+  const int64_t most = segments * (kPart + (maxpos + 127) / 128 * 3);  // units, of which a block has 2 or more
+  if (p.slots > most / 2) p.slots = static_cast<int>(most / 2);
   p.records = p.slots + segments;
   p.bytes = p.records * Hkv * (16 * p.tiles) * static_cast<int64_t>(d + 2) * 4;
   return p;
@@ -309,7 +351,7 @@ static PrefixPlan plan_prefix(int B, int Hq, int Hkv, int T, int64_t maxpos, int
 static bool prefix_shape(int B, int Hq, int Hkv, int T, int64_t maxpos, int d, int bits) {
   return B >= 1 && B <= 65535 && Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 && Hkv <= 65535 && T >= 1 && T <= 64 && maxpos >= T &&
          maxpos <= (int64_t(1) << 24) && (d == 64 || d == 128) && bits >= 2 && bits <= 4 &&
-         2 * static_cast<int64_t>(B) * ((static_cast<int64_t>(Hq / Hkv) * T + 15) / 16) * ((maxpos + 127) / 128) < (int64_t(1) << 31);
+         2 * static_cast<int64_t>(B) * ((static_cast<int64_t>(Hq / Hkv) * T + 15) / 16) * ((maxpos + 127) / 128) < (int64_t(1) << 28);
 }
 
 template <int D, int WP, int WO>
@@ -368,7 +410,7 @@ int tq_prefix_attention(const uint16_t* q_rot, const float* q_proj, const uint8_
   TQ_REQUIRE(out_dtype == TQ_F32 || out_dtype == TQ_F16 || out_dtype == TQ_BF16, "tq_prefix_attention: unknown dtype %d", out_dtype);
   if (B == 0) return TQ_OK;
   TQ_REQUIRE(prefix_shape(B, Hq, Hkv, T, maxpos, d, bits),
-             "tq_prefix_attention: at most 65535 sequences and kv heads, 2^24 positions a sequence and 2^31 (128 keys, 16 "
+             "tq_prefix_attention: at most 65535 sequences and kv heads, 2^24 positions a sequence and 2^31 / 8 (128 keys, 16 "
              "columns) blocks of work, got %d, %d and %lld", B, Hkv, (long long)maxpos);
   TQ_REQUIRE(q_rot && q_proj && key_codes && key_signs && key_rn && key_vn && key_centroids_f16 && val_codes && val_vn &&
                  val_centroids && val_pit_split && block_table && lengths && groups && out,
@@ -406,7 +448,6 @@ int tq_prefix_attention(const uint16_t* q_rot, const float* q_proj, const uint8_
   a.G = Hq / Hkv;
   a.C = a.G * T;
   a.slots = p.slots;
-  a.lg_least = p.lg_least;
   a.coeff = coeff;
   a.scale = scale;
   a.part_o = static_cast<float*>(workspace);
