@@ -41,6 +41,16 @@ inline int resident_blocks(const void* kernel, int threads, int* cache) {
   cache[dev] = per_cu * cus;
   return cache[dev];
 }
+// compute units of the current device
+inline int compute_units() {
+  static int cache[16] = {};
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 16) dev = 0;
+  if (cache[dev] > 0) return cache[dev];
+  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 1) cus = 1;
+  cache[dev] = cus;
+  return cus;
+}
 
 // ---------------------------------------------------------------- vector types
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));

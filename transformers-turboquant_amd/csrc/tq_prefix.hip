@@ -20,6 +20,7 @@ namespace tq {
 
 struct PrefixArgs : TreeArgs {
   const int32_t* groups;  // [B, 2]
+  int older;              // blocks of a kv head that come first on their compute unit, of two (0: more or fewer fit)
 };
 
 // A group ends with a lane's step of 64 sequences (behind it the same group begins anew): every sequence is in one
@@ -38,10 +39,11 @@ constexpr int kSlab = 32;
 // cycles) or 3 (two tiles, 5800).  A block does the rounds that begin in its stretch.  Without the weights a
 // block of four short sequences ends at 76 us where the others end at 51 (8 trees of 8 nodes on 16k keys of their
 // group).
-constexpr int kPart = 5;
 template <int RK, int WP, int WO>
 struct PrefixSplit {
+  static constexpr int kPart = WO > 16 ? 7 : 5;
   static constexpr int UP = WP > 16 ? 3 : 2, UO = WO > 16 ? 3 : 2;  // units of a round
+  static constexpr int kLead = 9;
   static constexpr int LEAST = WP > 16 ? 6 : 2;                     // of a block, no fewer than of a round
   struct Row {
     int start, keys;   // own positions [start, keys), keys = 0: none
@@ -51,7 +53,9 @@ struct PrefixSplit {
   Row r0;           // sequence `lane`
   int upto0, seg0;  // sums of units and segments up to it
   int ot;           // tiles of a sequence's own columns
-  int total, blocks, each, extra;
+  int total, blocks;
+  int older, most;  // blocks in front, and their units
+  int each, extra;  // units of the others, how many of them have one more
 
   __device__ __forceinline__ static int rounds(int keys) { return static_cast<int>(static_cast<unsigned>(keys + RK - 1) / RK); }
   __device__ __forceinline__ int own_rounds(const Row& r) const { return r.keys ? rounds(r.keys - r.start) : 0; }
@@ -98,12 +102,20 @@ struct PrefixSplit {
       total += __builtin_amdgcn_readlane(scan64(row_units(load(a, b0))), 63);
     blocks = min(a.slots, static_cast<int>(static_cast<unsigned>(total) / LEAST));  // (total is 0, or more than LEAST)
     each = blocks ? static_cast<unsigned>(total) / static_cast<unsigned>(blocks) : 0;
-    extra = total - each * blocks;
+    older = blocks == a.slots ? a.older : 0;
+    most = each + each * kLead / 64;
+    const int others = blocks - older, left = total - older * most;
+    each = others ? static_cast<unsigned>(left) / static_cast<unsigned>(others) : 0;
+    extra = left - each * others;
   }
-  __device__ __forceinline__ int begin(int k) const { return k * each + min(k, extra); }
+  __device__ __forceinline__ int begin(int k) const {
+    const int behind = max(k - older, 0);
+    return min(k, older) * most + behind * each + min(behind, extra);
+  }
   __device__ __forceinline__ int block_of(int unit) const {
-    const unsigned big = extra * (each + 1), x = unit;
-    return x < big ? x / static_cast<unsigned>(each + 1) : extra + (x - big) / static_cast<unsigned>(each);
+    if (unit < older * most) return static_cast<unsigned>(unit) / static_cast<unsigned>(most);
+    const unsigned x = unit - older * most, big = extra * (each + 1);
+    return older + (x < big ? x / static_cast<unsigned>(each + 1) : extra + (x - big) / static_cast<unsigned>(each));
   }
   // a sequence as all lanes see it: its first unit and segment, and its row
   struct At {
@@ -165,12 +177,12 @@ prefix_attn_kernel(PrefixArgs a) {
   constexpr int RK = 32 * NW, WP = 16 * NTP, WO = 16 * NTO;
   using Split = PrefixSplit<RK, WP, WO>;
   __shared__ __attribute__((aligned(16))) PrefixSmem<D, BITS, NTP, NW> sm;
-  const int tid = threadIdx.x, hkv = blockIdx.y;
+  const int tid = threadIdx.x, hkv = blockIdx.x, block = blockIdx.y;
   const TreeTables<BITS> tables(a, tid);
   const Split split(a, Split::load(a, 0));
-  if (static_cast<int>(blockIdx.x) >= split.blocks) return;  // block-uniform
-  int x = split.begin(blockIdx.x);
-  const int x_end = split.begin(blockIdx.x + 1);
+  if (block >= split.blocks) return;  // block-uniform
+  int x = split.begin(block);
+  const int x_end = split.begin(block + 1);
   tables.keys(sm.luts, tid);
   tables.values(sm.luts, tid);
   while (x < x_end) {
@@ -182,11 +194,11 @@ prefix_attn_kernel(PrefixArgs a) {
     const int tile = static_cast<int>(static_cast<unsigned>(x - from) / static_cast<unsigned>(units));
     const int u0 = x - from - tile * units, u1 = min(u0 + x_end - x, units);
     const auto rounds_before = [&](int u) {  // rounds that begin in front of the segment's unit u
-      const unsigned v = max(u - kPart, 0);
+      const unsigned v = max(u - Split::kPart, 0);
       return static_cast<int>(own ? (v + Split::UO - 1) / Split::UO : (v + Split::UP - 1) / Split::UP);
     };
     const int r0 = rounds_before(u0), r1 = rounds_before(u1);
-    const int64_t rec = ((static_cast<int64_t>(blockIdx.x) + at.segment + tile + (own ? at.r.pt : 0)) * a.Hkv + hkv) * WP;
+    const int64_t rec = ((static_cast<int64_t>(block) + at.segment + tile + (own ? at.r.pt : 0)) * a.Hkv + hkv) * WP;
     x += u1 - u0;
     if (r0 == r1) continue;
     if (own) {
@@ -228,7 +240,7 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(PrefixArgs a) {
     Records rs{0, 0, 0, 0};
     if (!own.r.keys) return rs;
     const auto list = [&](int first, int units, int rounds, int segment, int col, int64_t& at) {
-      const int k0 = split.block_of(first + kPart), k1 = split.block_of(first + kPart + (rounds - 1) * units);
+      const int k0 = split.block_of(first + Split::kPart), k1 = split.block_of(first + Split::kPart + (rounds - 1) * units);
       at = ((static_cast<int64_t>(k0) + segment) * a.Hkv + hkv) * WP + col;
       return k1 - k0 + 1;
     };
@@ -311,7 +323,7 @@ using PrefixKernel = void (*)(PrefixArgs);
 struct PrefixPlan {
   PrefixKernel attend;
   int tiles, own_tiles;  // NTP, NTO
-  int slots;
+  int slots, older;
   int64_t records, bytes;
 };
 
@@ -338,11 +350,12 @@ static PrefixPlan plan_prefix(int B, int Hq, int Hkv, int T, int64_t maxpos, int
   const int res = resident_blocks(reinterpret_cast<const void*>(p.attend), 256,
                                   resident[d == 128][bits - 2][p.tiles + p.own_tiles - 2]);
   p.slots = res / Hkv > 1 ? res / Hkv : 1;
+  p.older = res == 2 * compute_units() ? p.slots / 2 : 0;
   // a sequence's own tiles, and as many of its group's at most
   const int own = (C + 16 * p.own_tiles - 1) / (16 * p.own_tiles);
   const int64_t segments = 2 * static_cast<int64_t>(B) * own;
-  const int64_t most = segments * (kPart + (maxpos + 127) / 128 * 3);  // units, of which a block has 2 or more
-  if (p.slots > most / 2) p.slots = static_cast<int>(most / 2);
+  const int64_t most = segments * (7 + (maxpos + 127) / 128 * 3);  // units, of which a block has 2 or more
+  if (p.slots > most / 2) p.slots = static_cast<int>(most / 2), p.older = 0;
   p.records = p.slots + segments;
   p.bytes = p.records * Hkv * (16 * p.tiles) * static_cast<int64_t>(d + 2) * 4;
   return p;
@@ -366,7 +379,7 @@ static void launch_prefix_merge(const PrefixArgs& a, hipStream_t s) {
 
 template <int D>
 static void launch_prefix(const PrefixArgs& a, const PrefixPlan& p, hipStream_t s) {
-  p.attend<<<dim3(p.slots, a.Hkv), 256, 0, s>>>(a);
+  p.attend<<<dim3(a.Hkv, p.slots), 256, 0, s>>>(a);
   if (p.tiles == 1) launch_prefix_merge<D, 16, 16>(a, s);
   else if (p.own_tiles == 1) launch_prefix_merge<D, 32, 16>(a, s);
   else launch_prefix_merge<D, 32, 32>(a, s);
@@ -448,6 +461,7 @@ int tq_prefix_attention(const uint16_t* q_rot, const float* q_proj, const uint8_
   a.G = Hq / Hkv;
   a.C = a.G * T;
   a.slots = p.slots;
+  a.older = p.older;
   a.coeff = coeff;
   a.scale = scale;
   a.part_o = static_cast<float*>(workspace);
