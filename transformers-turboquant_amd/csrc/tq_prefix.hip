@@ -19,7 +19,6 @@
 namespace tq {
 
 struct PrefixArgs : TreeArgs {
-  const int32_t* groups;  // [B, 2]
   int older;              // blocks of a kv head that come first on their compute unit, of two (0: more or fewer fit)
 };
 
@@ -324,6 +323,7 @@ struct PrefixPlan {
   PrefixKernel attend;
   int tiles, own_tiles;  // NTP, NTO
   int slots, older;
+  bool apart;  // every sequence by itself, by tree attention
   int64_t records, bytes;
 };
 
@@ -344,11 +344,22 @@ static PrefixPlan plan_prefix(int B, int Hq, int Hkv, int T, int64_t maxpos, int
   static int resident[2][3][3][16] = {};  // per kernel, per device
   PrefixPlan p{};
   const int C = Hq / Hkv * T;
+  const auto rounds_of = [&](int columns) { return static_cast<int64_t>(B) * ((maxpos + 127) / 128) * Hkv * ((C + columns - 1) / columns); };
   p.tiles = static_cast<int64_t>(B) * C > 16 ? 2 : 1;
   p.own_tiles = C > 16 ? 2 : 1;
   p.attend = prefix_kernel(d, bits, p.tiles, p.own_tiles);
   const int res = resident_blocks(reinterpret_cast<const void*>(p.attend), 256,
                                   resident[d == 128][bits - 2][p.tiles + p.own_tiles - 2]);
+  // Sharing saves the reading of keys and columns that are idle in tree attention's tiles.  Where neither counts it
+  // is left out: a sequence's columns fill its two tiles (the matrix products bound both; 8 trees of 8 nodes on
+  // 16k shared keys, 32/8 heads, 79 us with tree attention against 80, 16 trees of 16 nodes 190 against 220; 7 nodes
+  // 120 against 115), or a block of the device has no more than one round to do (4 sequences of 1k, 12 heads of 64, 16.9
+  // against 20.8 us; 16 of 128, 32/8 heads, 20.0 against 24.3; 4 of 2k, 544 rounds to 512 blocks, 24.6 against 23.7).
+  p.apart = C % 32 == 0 || rounds_of(32) <= res;
+  if (p.apart) {
+    p.bytes = tree_workspace(B, Hq, Hkv, T, maxpos, d, bits);
+    return p;
+  }
   p.slots = res / Hkv > 1 ? res / Hkv : 1;
   p.older = res == 2 * compute_units() ? p.slots / 2 : 0;
   // a sequence's own tiles, and as many of its group's at most
@@ -460,12 +471,8 @@ int tq_prefix_attention(const uint16_t* q_rot, const float* q_proj, const uint8_
   a.T = T;
   a.G = Hq / Hkv;
   a.C = a.G * T;
-  a.slots = p.slots;
-  a.older = p.older;
   a.coeff = coeff;
   a.scale = scale;
-  a.part_o = static_cast<float*>(workspace);
-  a.part_ml = a.part_o + p.records * Hkv * (16 * p.tiles) * d;
   a.vpit = val_pit_split;
   a.out = out;
   a.out_dtype = out_dtype;
@@ -473,6 +480,14 @@ int tq_prefix_attention(const uint16_t* q_rot, const float* q_proj, const uint8_
   a.soh = soh;
   a.sos = sos;
   hipStream_t s = as_stream(stream);
+  if (p.apart) {
+    tree_attend(a, d, bits, workspace, s);
+    return launch_status("tq_prefix_attention");
+  }
+  a.slots = p.slots;
+  a.older = p.older;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.part_o + p.records * Hkv * (16 * p.tiles) * d;
   if (d == 64) launch_prefix<64>(a, p, s);
   else launch_prefix<128>(a, p, s);
   return launch_status("tq_prefix_attention");

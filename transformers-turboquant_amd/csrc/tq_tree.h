@@ -17,6 +17,7 @@ struct TreeArgs {
   const int32_t* table;
   int64_t ld_table;
   const int32_t* lengths;
+  const int32_t* groups;  // null, or [B, 2]: what a sequence shares with others, and is no shorter than (tq_prefix.hip)
   const int32_t* parents;
   int64_t ld_parents;
   int64_t num_pages;
@@ -33,8 +34,14 @@ struct TreeArgs {
 };
 
 // ---------------------------------------------------------------- the split of the keys
-// length of sequence b, -1 behind the last
-__device__ __forceinline__ int tree_length(const TreeArgs& a, int b) { return b < a.B ? a.lengths[b] : -1; }
+// length of sequence b, -1 behind the last and of one that is shorter than what it shares
+__device__ __forceinline__ int tree_length(const TreeArgs& a, int b) {
+  if (b >= a.B) return -1;
+  const int n = a.lengths[b];
+  if (!a.groups) return n;
+  const int32_t* const g = a.groups + static_cast<int64_t>(b) * 2;
+  return g[0] >= 0 && n < g[1] ? -1 : n;
+}
 // keys of a sequence of length n (cached and drafted), 0 where it does not fit its table
 __device__ __forceinline__ int tree_keys(const TreeArgs& a, int n) { return n >= 0 && n <= a.maxpos - a.T ? n + a.T : 0; }
 // Inclusive sum over the wave through DPP (shifts within rows of 16 lanes, then row 0's sum into
@@ -836,5 +843,9 @@ struct TreeFinish {
     }
   }
 };
+
+// Tree attention's workspace and launch; `a` holds what the caller gave (shapes, operands, output).
+int64_t tree_workspace(int B, int Hq, int Hkv, int T, int64_t maxpos, int d, int bits);
+void tree_attend(TreeArgs a, int d, int bits, void* workspace, hipStream_t s);
 
 }  // namespace tq

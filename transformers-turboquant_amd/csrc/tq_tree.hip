@@ -474,6 +474,20 @@ static void launch_tree(const TreeArgs& a, const TreePlan& p, hipStream_t s) {
   else tree_merge_kernel<D, 128, 1><<<grid(4), 256, 0, s>>>(a);
 }
 
+int64_t tree_workspace(int B, int Hq, int Hkv, int T, int64_t maxpos, int d, int bits) {
+  return plan_tree(B, Hq, Hkv, T, maxpos, d, bits).bytes;
+}
+
+void tree_attend(TreeArgs a, int d, int bits, void* workspace, hipStream_t s) {
+  const TreePlan p = plan_tree(a.B, a.Hq, a.Hkv, a.T, a.maxpos, d, bits);
+  a.slots = p.slots;
+  a.lg_least = p.lg_least;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.part_o + (static_cast<int64_t>(p.slots) + a.B) * a.Hkv * a.C * d;
+  if (d == 64) launch_tree<64>(a, p, s);
+  else launch_tree<128>(a, p, s);
+}
+
 }  // namespace tq
 
 using namespace tq;
@@ -483,7 +497,7 @@ extern "C" {
 int64_t tq_tree_workspace_size(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t table_width, int32_t page_size,
                                int32_t d, int32_t bits) {
   const int64_t maxpos = static_cast<int64_t>(table_width) * page_size;
-  return tree_shape(B, Hq, Hkv, T, maxpos, d, bits) ? plan_tree(B, Hq, Hkv, T, maxpos, d, bits).bytes : 0;
+  return tree_shape(B, Hq, Hkv, T, maxpos, d, bits) ? tree_workspace(B, Hq, Hkv, T, maxpos, d, bits) : 0;
 }
 
 int tq_tree_attention(const uint16_t* q_rot, const float* q_proj, const uint8_t* key_codes, const uint8_t* key_signs,
@@ -520,9 +534,9 @@ int tq_tree_attention(const uint16_t* q_rot, const float* q_proj, const uint8_t*
   for (const void* p : {static_cast<const void*>(q_rot), static_cast<const void*>(q_proj), static_cast<const void*>(key_codes),
                         static_cast<const void*>(key_signs), static_cast<const void*>(val_codes), static_cast<const void*>(val_pit_split)})
     TQ_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, "tq_tree_attention: queries, code planes and Pi_v must be 16-byte aligned");
-  const TreePlan p = plan_tree(B, Hq, Hkv, T, maxpos, d, bits);
-  TQ_REQUIRE(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= p.bytes,
-             "tq_tree_attention: the workspace must be 16-byte aligned and hold %lld bytes", (long long)p.bytes);
+  const int64_t bytes = tree_workspace(B, Hq, Hkv, T, maxpos, d, bits);
+  TQ_REQUIRE(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= bytes,
+             "tq_tree_attention: the workspace must be 16-byte aligned and hold %lld bytes", (long long)bytes);
   TreeArgs a{};
   a.q_rot = q_rot;
   a.q_proj = q_proj;
@@ -548,21 +562,15 @@ int tq_tree_attention(const uint16_t* q_rot, const float* q_proj, const uint8_t*
   a.T = T;
   a.G = Hq / Hkv;
   a.C = a.G * T;
-  a.slots = p.slots;
-  a.lg_least = p.lg_least;
   a.coeff = coeff;
   a.scale = scale;
-  a.part_o = static_cast<float*>(workspace);
-  a.part_ml = a.part_o + (static_cast<int64_t>(p.slots) + B) * Hkv * a.C * d;
   a.vpit = val_pit_split;
   a.out = out;
   a.out_dtype = out_dtype;
   a.sob = sob;
   a.soh = soh;
   a.sos = sos;
-  hipStream_t s = as_stream(stream);
-  if (d == 64) launch_tree<64>(a, p, s);
-  else launch_tree<128>(a, p, s);
+  tree_attend(a, d, bits, workspace, as_stream(stream));
   return launch_status("tq_tree_attention");
 }
 
