@@ -571,20 +571,25 @@ __global__ void __launch_bounds__(kScan) sample_select_kernel(SampleArgs a) {
       // sums of shares in float, off by less than 2^-18
       const float p = static_cast<float>(set.p);
       int lo = reach_bin(h, p - 0x1p-17f);
-      const int hi = reach_bin(h, p + 0x1p-17f);
+      int hi = reach_bin(h, p + 0x1p-17f);
+      double edge = 0.0, slack = 0.0;  // min-p's border below the maximum
+      if (least > 0.0) {  // nothing below it is kept, wherever top-p's may be
+        edge = log2(least) / c2;
+        slack = 1e-5 * (1.0 + fabs(edge) + fabs(static_cast<double>(mt)));
+        hi = min(hi, max(0, bin_of(static_cast<float>(fmax(mt + edge - slack, -3e38)), top)));
+      }
       // at most so many tokens down to there: a bin's mass over the least weight in it
       float few = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int b = 8 * lane + i;
-        const float edge = static_cast<float>((top - b) * 0.0625 - mt) * static_cast<float>(c2);
-        if (b <= hi && h[i] > 0.f) few += h[i] * static_cast<float>(total) / fmaxf(__builtin_amdgcn_exp2f(fmaxf(edge, -120.f)), 1e-30f);
+        const float y = static_cast<float>((top - b) * 0.0625 - mt) * static_cast<float>(c2);
+        if (b <= hi && h[i] > 0.f) few += h[i] * static_cast<float>(total) / fmaxf(__builtin_amdgcn_exp2f(fmaxf(y, -120.f)), 1e-30f);
       }
       few = wave_all(few, Sum{});
       if (hi < kTail && few < kFew) {
         lo = 0;
       } else if (least > 0.0) {  // what is certain is above min-p's border, too
-        const double edge = log2(least) / c2, slack = 1e-5 * (1.0 + fabs(edge) + fabs(static_cast<double>(mt)));
         lo = min(lo, max(0, bin_of(static_cast<float>(fmin(mt + edge + slack, 3e38)), top)));
       }
       if (lane == 0) {
@@ -768,10 +773,59 @@ __device__ __forceinline__ int pick_index(FinishSmem& s, uint64_t goal, int top_
 }
 
 // The border in rank among some tokens.  value: 1 (by rank) or the token's mass, 0: not one of them; kept are the
-// tokens whose predecessors' values sum to less than goal (>= 1).
+// tokens whose predecessors' values sum to less than goal (>= 1).  First the bin that holds it, then (not of the last
+// bin) 1/512 of that; as soon as no more than 64 tokens are left, a wave ranks them one against the other.  Among more,
+// as equal ones are, the digits of their logits select it, and an index.
 template <int DT, class Tokens, class Value>
-__device__ __forceinline__ void pick_border(const Tokens& all, FinishSmem& s, int top_digit, uint64_t goal, Value value, uint32_t& key,
-                                            int& last) {
+__device__ __forceinline__ void pick_border(const Tokens& all, FinishSmem& s, int top, int top_digit, uint64_t goal, Value value,
+                                            uint32_t& key, int& last) {
+  const int tid = threadIdx.x;
+  uint64_t rest = goal;
+  int bin = 0;
+#pragma unroll 1
+  for (int level = 0; level < 2 && (level == 0 || bin < kTail); ++level) {
+    const auto place = [&](float v) {
+      const int b = bin_of(v, top);
+      if (level == 0) return b;
+      const float x = fminf(fmaxf(v * 16.f, -0x1p27f), 0x1p27f);
+      return b == bin ? 511 - static_cast<int>((x - floorf(x)) * 512.f) : -1;
+    };
+    if (tid == 0) s.ties = 0;
+    const int at = pick_digit<false>(s, rest, [&](auto add) {
+      all.each([&](float v, int x) {
+        const int to = place(v);
+        const uint64_t n = to >= 0 ? value(v, x) : 0;
+        if (n) add(to, n);
+      });
+    });
+    all.each([&](float v, int x) {
+      if (place(v) != at) return;
+      const uint64_t n = value(v, x);
+      if (!n) return;
+      const uint32_t i = atomicAdd(&s.ties, 1u);
+      if (i < 64) {
+        s.value[i] = token_of(v, x);
+        s.value[64 + i] = n;
+      }
+    });
+    __syncthreads();
+    const int close = s.ties;
+    if (close <= 64 && tid < 64) {
+      const uint64_t t = tid < close ? s.value[tid] : 0;
+      uint64_t before = 0;
+      for (int j = 0; j < close; ++j) before += s.value[j] > t ? s.value[64 + j] : 0;
+      const uint64_t border = ~wave_all(tid < close && before < rest ? ~t : 0, Max{});
+      if (tid == 0) s.one = border;
+    }
+    __syncthreads();
+    if (close <= 64) {
+      key = close ? static_cast<uint32_t>(s.one >> 32) : 0;
+      last = close ? index_of(s.one) : 0x7FFFFFFF;  // none at all: none ends what is kept
+      __syncthreads();
+      return;
+    }
+    bin = at;
+  }
   // the bits in which floats of the type differ, from the top: 32, 19 (f16: sign, 8 of exponent, 10) or 16; those
   // below are all zero, or of a negative float all one
   constexpr int kBits = DT == TQ_F32 ? 32 : DT == TQ_F16 ? 19 : 16, kDigits = (kBits + 8) / 9, kLow = 32 - kBits;
@@ -825,9 +879,9 @@ __device__ __forceinline__ uint64_t ceiling(double g) {  // at least 1
 
 // The border of a row: by rank, then by mass
 template <int DT, class Tokens, class In, class Integer>
-__device__ __forceinline__ void cut_row(const Tokens& all, FinishSmem& s, const Settings& set, int top_digit, uint64_t mass_goal, In in,
+__device__ __forceinline__ void cut_row(const Tokens& all, FinishSmem& s, const Settings& set, int top, int top_digit, uint64_t mass_goal, In in,
                                         Integer integer, uint32_t& key, int& last) {
-  if (set.mode == kTopK) pick_border<DT>(all, s, top_digit, static_cast<uint64_t>(set.k), [&](float, int) -> uint64_t { return 1; }, key, last);
+  if (set.mode == kTopK) pick_border<DT>(all, s, top, top_digit, static_cast<uint64_t>(set.k), [&](float, int) -> uint64_t { return 1; }, key, last);
   if (set.p >= 1.0) return;
   const uint32_t key_k = key;
   const int last_k = last;
@@ -842,7 +896,7 @@ __device__ __forceinline__ void cut_row(const Tokens& all, FinishSmem& s, const 
     __syncthreads();
     mass_goal = ceiling(set.p * static_cast<double>(sum));
   }
-  pick_border<DT>(all, s, top_digit, mass_goal, value, key, last);
+  pick_border<DT>(all, s, top, top_digit, mass_goal, value, key, last);
 }
 
 // A row's whole list in s.token, n <= kRanked of them, or (ONE) at most 64 by one wave: a thread has a token, and meets
@@ -1089,8 +1143,8 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
       key = key_of(peak);
       last = -1;
     } else if (mode != kMinP) {
-      if (n <= kShort) cut_row<DT>(taken, s, set, top_digit, ceiling(g), in, mass, key, last);
-      else cut_row<DT>(all, s, set, top_digit, ceiling(g), in, mass, key, last);
+      if (n <= kShort) cut_row<DT>(taken, s, set, top, top_digit, ceiling(g), in, mass, key, last);
+      else cut_row<DT>(all, s, set, top, top_digit, ceiling(g), in, mass, key, last);
     }
     const auto kept = [&](float v, int x) -> uint64_t {
       const uint32_t k = key_of(v);
