@@ -77,6 +77,22 @@ def test_nested_forks_are_cut_where_it_saves_most():
     assert (cache._device_state[0][:2, :12] == cache._device_state[0][:1, :12]).all()
 
 
+def test_little_in_common_is_read_apart():
+    """A group is read as one while it saves a fifth of the pages."""
+    cache = sharing(pages=90)
+    step(cache, [list(range(64))])  # 2 pages
+    (a,) = cache.active
+    b = cache.fork(a)[0]
+    cache.use([a, b])
+    seen = []
+    for _ in range(8):
+        step(cache, [[1] * 32] * 2)  # a page more of each one's own
+        pages = sum(len(s) for s in (row[row >= 0] for row in cache._device_state[0]))
+        seen.append((5 * 2 >= pages, cache._groups is not None))
+    assert all(want == got for want, got in seen) and seen[0][1] and not seen[-1][1]
+    check(cache)
+
+
 def test_best_runs_against_every_cut():
     rng = random.Random(1)
     for n in list(range(1, 9)) * 12:

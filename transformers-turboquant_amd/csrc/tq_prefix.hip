@@ -102,7 +102,7 @@ struct PrefixSplit {
     blocks = min(a.slots, static_cast<int>(static_cast<unsigned>(total) / LEAST));  // (total is 0, or more than LEAST)
     each = blocks ? static_cast<unsigned>(total) / static_cast<unsigned>(blocks) : 0;
     older = blocks == a.slots ? a.older : 0;
-    most = each + each * kLead / 64;
+    most = each + static_cast<int>(static_cast<uint64_t>(each) * kLead >> 6);
     const int others = blocks - older, left = total - older * most;
     each = others ? static_cast<unsigned>(left) / static_cast<unsigned>(others) : 0;
     extra = left - each * others;
