@@ -164,6 +164,17 @@ struct PrefixSplit {
 };
 
 // ---------------------------------------------------------------- attention
+// A part is worked on as by tree attention (tree_part): a wave builds the matrix operands of 32 keys once and uses them for
+// 16 NTP columns, which here belong to several sequences.
+// 16 sequences of 32000 shared positions and 700 of their own, 32/8 heads, 3 bits (32 MB; 12.8 GFLOP, 11 us at a large library
+// product's rate): 38 us under a kernel trace, 49 the call with preparation (6) and merge (8).  Neither memory nor the matrix
+// unit ends it: of 76k cycles the VALU issues in 33k and the matrix unit is busy in 17k, over the two waves per
+// SIMD that two tiles' registers leave, and about 10k pass before the first of a block's nine rounds is done.
+// The blocks of a kv head are neighbours on one XCD (head along x), as they read the same rows at about the same time: 16
+// trees of 16 nodes on 16k positions miss the L2 in 0.35 million lines, with the head along y, where all XCDs
+// read all rows, in 3.5 million.
+// Of the two blocks on a compute unit the first has its instructions taken first: it ends at 30 us where the second ends at
+// 35, so that it is dealt 14% more (attention and merge 43 against 46 us, 64 sequences of 8k, 16/2 heads, 35 against 38).
 // NTP and NTO tiles of 16 columns to a segment of shared and of own keys (NTO <= NTP).  Records have 16 NTP columns.
 template <int D, int BITS, int NTP, int NW>
 struct PrefixSmem : TreeSmem<D, BITS, NTP, NW> {
@@ -213,7 +224,8 @@ prefix_attn_kernel(PrefixArgs a) {
 
 // ---------------------------------------------------------------- merge
 // One block per (sequence, kv head, 4 CW columns), as tree_merge_kernel: a column's records are those of its
-// tile of the group's shared keys, then those of its tile of the own ones.
+// tile of the group's shared keys, then those of its tile of the own ones.  8 us for 512 columns of 34 records (9 MB), 7 for 4096
+// of a few: three dependent round trips (lengths and groups, records, output).
 template <int D, int RK, int WP, int WO, int CW>
 __global__ void __launch_bounds__(256) prefix_merge_kernel(PrefixArgs a) {
   using Split = PrefixSplit<RK, WP, WO>;
