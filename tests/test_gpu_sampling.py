@@ -250,3 +250,39 @@ def test_graph_replays():
         torch.cuda.synchronize()
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1]), rep
         _check(logits, u, t, k, p, m)
+
+
+def test_probabilities_of_more_rows_than_a_step_of_their_writing():
+    """Rows that keep many among rows that keep few, over more than 2048 of them."""
+    N, V = 4500, 2100
+    logits, u = _logits(N, V, torch.bfloat16, 31)
+    g = torch.Generator(device=DEV).manual_seed(32)
+    k = torch.where(torch.rand(N, device=DEV, generator=g) < 0.7, 5, 0).to(torch.int32)  # without a k: all tokens
+    probs = filter_probs(logits, top_k=k)
+    some = torch.tensor([0, 1, 255, 256, 2046, 2047, 2048, 2049, 4095, 4096, 4097, N - 2, N - 1], device=DEV)
+    some = torch.cat([some, torch.randint(0, N, (40,), device=DEV, generator=g)])
+    p2, _ = _check(logits[some], u[some], 1.0, k[some])
+    assert (k[some] > 0).any() and (k[some] == 0).any()
+    assert ((probs[some] - p2).abs() <= p2 * (2.0 ** -23 + 2.0 ** -38)).all()  # one rounding each
+    assert (((probs > 0).sum(1) == 5) == (k == 5)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_min_p_above_and_below_the_border_of_top_p(dtype):
+    """The one that keeps less decides; with equal logits at either border."""
+    V = 30000
+    g = torch.Generator(device=DEV).manual_seed(41)
+    l = 1.5 * torch.randn(4, V, device=DEV, generator=g)
+    l[1] = (l[1] * 8).round() / 8
+    l[2, :3000] = 6.0
+    l[3] = (l[3] * 2).round() / 2 + 50
+    l, u = l.to(dtype), torch.rand(4, device=DEV, generator=g)
+    top = l.double().max(1, keepdim=True).values
+    for t in (0.5, 1.0, 2.5):
+        w = torch.exp((l.double() - top) / t)
+        for p in (0.05, 0.5, 0.9, 0.999):
+            for q in (0.2, 0.5, 0.8):  # a weight that some token has, so that min-p's border is one's own
+                m = w.flatten()[torch.argsort(w.flatten())[int(q * 4 * V)]].item()
+                for mm in (m * (1 - 1e-9), m * (1 + 1e-9)):
+                    print("case:", dtype, t, p, mm, flush=True)
+                    _check(l, u, t=t, p=p, m=mm)

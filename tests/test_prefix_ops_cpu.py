@@ -4,7 +4,7 @@ launch.  No GPU is touched."""
 import pytest
 import torch
 
-from test_draft_ops_cpu import B, D, F16, I32, I64, P, POOL, T, W, _append_args, _e, _refuses, _tree_args
+from test_draft_ops_cpu import B, D, F16, H, I32, I64, P, POOL, T, W, _append_args, _e, _refuses, _tree_args
 from turboquant_pytorch import _native, prefix_groups
 from turboquant_pytorch._ops import ops
 
@@ -47,6 +47,20 @@ def test_more_work_than_an_index_counts_is_refused_before_a_row_is_written():
     for args, fn in ((_append_args(), ops().prefix_page_attend), (_tree_args(True), ops().prefix_attend)):
         new = {k: _e(n, *args[k].shape[1:], dtype=args[k].dtype) for k in ("k", "v", "q") if k in args}
         _refuses(fn, _with_groups(args), {**new, **big}, "blocks of work")
+
+
+@pytest.mark.parametrize("positions", [1 << 16, 1 << 18, 1 << 22])
+def test_the_operators_refuse_what_the_library_does(positions):
+    n, args = 65535, _tree_args(True)
+    q = args["q"]
+    wide = dict(q=_e(n, *q.shape[1:], dtype=q.dtype), table=_e(n, positions // P, dtype=I32), lengths=_e(n, dtype=I32),
+                groups=_e(n, 2, dtype=I32))
+    size = _native.lib().tq_prefix_workspace_size(n, q.shape[1], H, q.shape[2], positions // P, P, D, args["bits"])
+    if size:
+        assert ops().prefix_attend(*dict(_with_groups(args), **wide).values()).shape[0] == n
+    else:
+        _refuses(ops().prefix_attend, _with_groups(args), wide, "blocks of work")
+    assert (size > 0) == (positions == 1 << 16)
 
 
 def test_groups():

@@ -869,7 +869,7 @@ __device__ __forceinline__ void pick_border(const Tokens& all, FinishSmem& s, in
   });
   __syncthreads();
   const uint64_t one = s.one;
-  uint64_t keep = one ? (goal + one - 1) / one : 1;
+  uint64_t keep = one ? goal / one + (goal % one != 0) : 1;  // (a goal that nothing reaches may be the largest integer)
   if (keep < 1) keep = 1;
   last = 0x7FFFFFFF;
   if (keep >= s.ties) return;

@@ -1028,8 +1028,8 @@ int64_t tree_workspace(const Tensor& q, const Tensor& kvn, const Tensor& table, 
 void check_groups(const Checker& c, const Tensor* groups, int64_t B, int64_t columns, int64_t positions) {
   if (!groups) return;
   check_index(c, *groups, "groups", {B, 2});
-  TORCH_CHECK(2 * B * ((columns + 15) / 16) * ((positions + 127) / 128) < (int64_t{1} << 31), c.op, ": ", B, " sequences of ",
-              columns, " query columns per kv head over tables of ", positions, " positions are more than 2^31 blocks of work");
+  TORCH_CHECK(2 * B * ((columns + 15) / 16) * ((positions + 127) / 128) < (int64_t{1} << 28), c.op, ": ", B, " sequences of ",
+              columns, " query columns per kv head over tables of ", positions, " positions are more than 2^31 / 8 blocks of work");
 }
 // out [B, T, Hq, D]; arguments checked
 void tree_launch(const uint16_t* q_rot, const float* q_proj, const Tensor& kcodes, const Tensor& ksigns, const Tensor& krn,
