@@ -423,8 +423,8 @@ int64_t tq_tree_workspace_size(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, in
 /* tq_tree_attention of sequences that share their first positions.  groups [B, 2] (int32, on the
  * device): sequences that follow one another with the same groups[b][0] >= 0 and the same
  * groups[b][1] have positions [0, groups[b][1]) in common, the same rows; they are read through the
- * table row of one of these sequences, once for all of them (up to the last multiple of 32 positions;
- * a batch is cut at every 64th sequence).  A sequence with a negative groups[b][0] or without shared
+ * table row of the first of these sequences that has a length, once for all of them (up to the last
+ * multiple of 32 positions; a batch is cut at every 64th sequence).  A sequence with a negative groups[b][0] or without shared
  * positions is attended alone; one that is shorter than its shared positions gets zeros.  Otherwise as
  * tq_tree_attention, with a workspace of tq_prefix_workspace_size bytes. */
 int tq_prefix_attention(const uint16_t* q_rot, const float* q_proj, const uint8_t* key_codes,

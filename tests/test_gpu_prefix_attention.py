@@ -257,3 +257,20 @@ def test_an_empty_batch_and_one_sequence():
     assert (out - alone).norm() <= 16 * 2.0 ** -10 * alone.norm()  # as tests/test_gpu_tree_attention.py derives it
     none = prefix_attention(q[:0], kc, vc, pool, 1, table[:0], lengths[:0], groups[:0])
     assert none.shape == (0, 1, 4, 64)
+
+
+@pytest.mark.parametrize("T,Hq,Hkv", [(1, 4, 2), (3, 8, 2), (20, 4, 2)])
+def test_a_group_that_begins_with_idle_rows(T, Hq, Hkv):
+    """Padding rows of a batch: no length, and pages that are not theirs or none."""
+    print("case:", T, Hq, Hkv, flush=True)
+    own = [-1, -1, 40, -1, 3, 200, -1, -1, -1, 7, -1]
+    kc, vc, pool, table, lengths, groups, q = _setup(128, 3, Hq, Hkv, T, [7, 1, 3], [500, 64, 160], own, 64, seed=17)
+    table[[0, 6, 7, 8]] = -1
+    table[1] = torch.arange(table.shape[1], dtype=torch.int32, device=DEV) % pool.num_pages  # another's rows
+    par = _tree(T, len(q), 3)
+    for parents in (par, None):
+        out = prefix_attention(q, kc, vc, pool, 1, table, lengths, groups, parents, out_dtype=torch.float32)
+        _check(out, kc, vc, pool, table, lengths, q, parents)
+    lengths[:7] = -1  # a whole group
+    out = prefix_attention(q, kc, vc, pool, 1, table, lengths, groups, par, out_dtype=torch.float32)
+    _check(out, kc, vc, pool, table, lengths, q, par)

@@ -48,6 +48,7 @@ struct PrefixSplit {
     int start, keys;   // own positions [start, keys), keys = 0: none
     int pr, pt, cols;  // of the group it is the first of: rounds of a tile, tiles, columns
     int first;         // of the sequence's group, -1 without one
+    int pages;         // the first sequence of the group that has a place: its table row is read
   };
   Row r0;           // sequence `lane`
   int upto0, seg0;  // sums of units and segments up to it
@@ -77,19 +78,23 @@ struct PrefixSplit {
     const int id1 = __shfl_up(id, 1, 64), shared1 = __shfl_up(shared, 1, 64);
     const bool on = grouped && lane > 0 && id1 == id && shared1 == shared;  // goes on with the group before it
     const uint64_t heads = __ballot(grouped && !on), ons = __ballot(on);
-    Row r{0, 0, 0, 0, 0, -1};
+    Row r{0, 0, 0, 0, 0, -1, b};
+    const int least = id >= 0 && shared > 0 ? shared : 0;
+    r.keys = n >= least && n <= a.maxpos - a.T ? n + a.T : 0;
+    const uint64_t runs = __ballot(r.keys != 0);
     if (grouped) {
       r.first = b0 + 63 - __builtin_clzll(heads & (~0ull >> (63 - lane)));
       r.start = shared & ~(kSlab - 1);
       if (!on) {
         const uint64_t behind = lane < 63 ? ons >> (lane + 1) : 0;
-        r.cols = (1 + __builtin_ctzll(~behind)) * a.C;
-        r.pt = (r.cols + WP - 1) / WP;
+        const int more = __builtin_ctzll(~behind);  // 63 at most
+        const uint64_t mine = (runs >> lane) & (~0ull >> (63 - more));
+        r.cols = (1 + more) * a.C;
+        r.pt = mine ? (r.cols + WP - 1) / WP : 0;
         r.pr = rounds(r.start);
+        r.pages = mine ? b + __builtin_ctzll(mine) : b;
       }
     }
-    const int least = id >= 0 && shared > 0 ? shared : 0;
-    r.keys = n >= least && n <= a.maxpos - a.T ? n + a.T : 0;
     return r;
   }
   __device__ __forceinline__ PrefixSplit(const PrefixArgs& a, const Row& r) : r0(r) {
@@ -129,6 +134,7 @@ struct PrefixSplit {
     at.r.pt = __builtin_amdgcn_readlane(r.pt, l);
     at.r.cols = __builtin_amdgcn_readlane(r.cols, l);
     at.r.first = __builtin_amdgcn_readlane(r.first, l);
+    at.r.pages = __builtin_amdgcn_readlane(r.pages, l);
     at.first = __builtin_amdgcn_readlane(upto, l) - row_units(at.r);
     at.segment = __builtin_amdgcn_readlane(seg, l) - row_segments(at.r);
     return at;
@@ -212,11 +218,11 @@ prefix_attn_kernel(PrefixArgs a) {
     x += u1 - u0;
     if (r0 == r1) continue;
     if (own) {
-      const TreePart part{b, a.C, tile * WO, at.r.keys - a.T, at.r.start + r0 * RK, min(at.r.keys, at.r.start + r1 * RK), rec};
+      const TreePart part{b, b, a.C, tile * WO, at.r.keys - a.T, at.r.start + r0 * RK, min(at.r.keys, at.r.start + r1 * RK), rec};
       tree_part<D, BITS, NTO, NW, false>(a, part, hkv, sm);
     } else {
       const int end = min(at.r.start, r1 * RK);
-      const TreePart part{b, at.r.cols, tile * WP, end, r0 * RK, end, rec};
+      const TreePart part{b, at.r.pages, at.r.cols, tile * WP, end, r0 * RK, end, rec};
       tree_part<D, BITS, NTP, NW, true>(a, part, hkv, sm);
     }
   }

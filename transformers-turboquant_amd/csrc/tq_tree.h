@@ -123,7 +123,8 @@ struct TreeSplit {
 
 // What a block works on at a time: some columns of a kv head against a run of keys.
 struct TreePart {
-  int row;         // the sequence whose table row gives the pages
+  int row;         // the sequence of column 0
+  int pages;       // the one whose table row gives the pages
   int cols, ct0;   // the part's columns are those of [ct0, cols) that fit its tiles
   int nctx;        // key positions below nctx are cached, drafted tokens behind
   int kbeg, kend;  // positions
@@ -412,7 +413,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const TreePart& p, 
   // parents, the first slabs' pages and the queries come in one round trip
   int par = -1;
   if constexpr (!SHARED) par = tree_parent(a, b);
-  const ST stream(a, b, hkv, kend);
+  const ST stream(a, p.pages, hkv, kend);
   const int k0w = kbeg + wave * NK;
   int nrows[R], pages[R];
 #pragma unroll

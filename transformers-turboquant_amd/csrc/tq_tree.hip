@@ -43,7 +43,7 @@ tree_attn_kernel(TreeArgs a) {
     int b, first, nkeys;
     split.sequence_at(a, x, b, first, nkeys);
     const int rec = static_cast<int>(blockIdx.x) + b, last = min(x_end, first + split.rounds(nkeys));
-    const TreePart part{b, a.C, ct0, nkeys - a.T, (x - first) * RK, min(nkeys, (last - first) * RK),
+    const TreePart part{b, b, a.C, ct0, nkeys - a.T, (x - first) * RK, min(nkeys, (last - first) * RK),
                         (static_cast<int64_t>(rec) * a.Hkv + hkv) * a.C + ct0};
     x = last;
     tree_part<D, BITS, NT, NW, false>(a, part, hkv, sm);

@@ -38,8 +38,8 @@ def prefix_attention(queries: torch.Tensor, key_compressor: TurboQuantCompressor
 
     groups int32 [B, 2] on the GPU: sequences that follow one another with the same id ``groups[b, 0] >= 0`` and
     the same ``groups[b, 1]`` have the rows of positions ``[0, groups[b, 1])`` in common (`prefix_groups` makes it); an id of
-    -1 or 0 shared positions: alone.  The shared rows are read through the block table of one sequence of the
-    group, whole slabs of 32 positions of them once for all its sequences (64 at most: a batch is cut at every
+    -1 or 0 shared positions: alone.  The shared rows are read through the block table of the group's first sequence
+    that has a length, whole slabs of 32 positions of them once for all its sequences (64 at most: a batch is cut at every
     64th sequence).  A sequence shorter than what it shares gets zeros, as one without room for its tokens does."""
     tk, tv = _both_tables(key_compressor, val_compressor, queries.device)
     args = _tree_args(tk, tv, queries.shape[-1], key_compressor, val_compressor, pool, layer, block_table, lengths, parents,
