@@ -21,8 +21,9 @@
 //   select   (top-p, min-p) finds the bins that hold the row's border in the joined histograms, and lists what is
 //            kept (min-p), the tokens down to the border if they are few, or else those of its bins alone, with the
 //            mass of what is kept for certain above them
-//   finish   up to 64 listed tokens are ranked by one wave, 256 by the block, among more (5120 in shared memory) the
-//            border is selected digit by digit; drawn from the list if it holds all that is kept, else by the chunks' masses
+//   finish   up to 64 listed tokens are ranked by one wave, 256 by the block; among more (5120 in shared memory) the border is
+//            found in its bin, and there by rank or, of many equal ones, digit by digit; drawn from the list if it holds
+//            all that is kept, else by the chunks' masses
 //   write    the probabilities of rows that keep many; the others' are few, in a row that the scan has cleared
 #include "tq_common.h"
 
