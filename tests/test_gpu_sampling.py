@@ -286,3 +286,16 @@ def test_min_p_above_and_below_the_border_of_top_p(dtype):
                 for mm in (m * (1 - 1e-9), m * (1 + 1e-9)):
                     print("case:", dtype, t, p, mm, flush=True)
                     _check(l, u, t=t, p=p, m=mm)
+
+
+def test_top_p_keeps_no_more_of_equal_logits_than_top_k():
+    """top_k ends among many equal logits and top_p behind them, or just in front of the last."""
+    g = torch.Generator(device=DEV).manual_seed(51)
+    for V, step in ((2747, 0.25), (9000, 0.5), (40001, 0.125)):
+        l = ((0.5 * torch.randn(3, V, device=DEV, generator=g)) / step).round() * step
+        u = torch.rand(3, device=DEV, generator=g)
+        for k in (100, 300, 1200, V - 5):
+            for p in (0.5, 0.99, 1 - 1e-4, 1 - 1e-9):
+                print("case:", V, step, k, p, flush=True)
+                _check(l, u, t=20.0, k=k, p=p)
+                _check(l.half(), u, t=3.0, k=k, p=p, m=1e-4)

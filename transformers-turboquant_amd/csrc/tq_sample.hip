@@ -905,6 +905,10 @@ __device__ __forceinline__ void cut_row(const Tokens& all, FinishSmem& s, const 
     mass_goal = ceiling(set.p * static_cast<double>(sum));
   }
   pick_border<DT>(all, s, top, top_digit, mass_goal, value, key, last);
+  if (key < key_k || (key == key_k && last > last_k)) {  // all that the rank keeps
+    key = key_k;
+    last = last_k;
+  }
 }
 
 // A row's whole list in s.token, n <= kRanked of them, or (ONE) at most 64 by one wave: a thread has a token, and meets
