@@ -11,7 +11,8 @@
 //
 // What is kept is decided by a comparison of sums over up to 10^5 terms, and a draw lies next to a border once
 // in a few thousand tokens if sums are off by 10^-7; so weights are float64 (2^f by its Taylor series, 2 10^-13), and
-// sums are float64 in a fixed order or integers, which have none.
+// sums are float64 in a fixed order or integers, which have none (of n listed tokens in units of 2^-61 n of the heaviest: 4
+// 10^4 tokens' roundings add up to 2^-39 of it).
 //
 // A row is never sorted.  It is cut into chunks, one per block, and then finished by one block:
 //   scan     the chunk's maximum; without filters its mass; for top-p its mass, and a histogram of it over bins of
