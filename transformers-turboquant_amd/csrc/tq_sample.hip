@@ -797,7 +797,8 @@ __device__ __forceinline__ void pick_border(const Tokens& all, FinishSmem& s, in
       const int b = bin_of(v, top);
       if (level == 0) return b;
       const float x = fminf(fmaxf(v * 16.f, -0x1p27f), 0x1p27f);
-      return b == bin ? 511 - static_cast<int>((x - floorf(x)) * 512.f) : -1;
+      // (of x from -2^-25 up to 0 the difference rounds to 1)
+      return b == bin ? 511 - min(static_cast<int>((x - floorf(x)) * 512.f), 511) : -1;
     };
     if (tid == 0) s.ties = 0;
     const int at = pick_digit<false>(s, rest, [&](auto add) {
