@@ -24,3 +24,14 @@ def test_logits_just_below_zero(dtype):
     for kw in (dict(k=50), dict(k=300), dict(k=400, p=0.5), dict(p=0.3), dict(p=0.6), dict(k=700, m=0.9), dict(t=3.0, p=0.4)):
         print("case:", dtype, kw, flush=True)
         _check(l, u, **kw)
+
+
+@pytest.mark.parametrize("light,p", [(-1.54, 1 - 1e-6), (-1.54, 1 - 2e-6), (-1.6, 1 - 1e-6)])
+def test_top_p_over_hundreds_of_chunks(light, p):
+    """598 chunks with the same masses, whose float32 sums over the chunks would all be rounded to one side."""
+    V = 598 * 4096
+    l = torch.full((1, V), light, device=DEV)
+    l[0, ::4096] = 0.0
+    print("case:", light, p, flush=True)
+    probs, _ = _check(l, torch.full((1,), 0.999999, device=DEV), p=p)
+    assert int((probs > 0).sum()) < V

@@ -556,7 +556,7 @@ __global__ void __launch_bounds__(kScan) sample_select_kernel(SampleArgs a) {
       s.depth[i] = in ? a.depth[at0 + i] : 0;
     }
     const double total = block_all<kScanWaves>(mine, s.total, Sum{});  // in a fixed order
-    float share = 0.f;
+    double share = 0.0;  // in float, equal shares of hundreds of chunks are all rounded to one side: 2^-16.8 at 598 of them
     for (int i0 = 0; i0 < a.C; i0 += 8) {
       float h[8];
 #pragma unroll
@@ -568,16 +568,17 @@ __global__ void __launch_bounds__(kScan) sample_select_kernel(SampleArgs a) {
       for (int i = 0; i < 8; ++i) {
         const int k = min(i0 + i, a.C - 1), b = tid - s.off[k];
         const bool in = i0 + i < a.C && b >= 0 && b < s.depth[k] && b < kTail;
-        share += in ? h[i] * s.factor[k] : 0.f;
+        share += in ? static_cast<double>(h[i] * s.factor[k]) : 0.0;
       }
     }
-    s.bins[tid] = tid < kTail ? share * static_cast<float>(1.0 / total) : 0.f;
+    s.bins[tid] = tid < kTail ? static_cast<float>(share * (1.0 / total)) : 0.f;
     __syncthreads();
     if (wave == 0) {
       float h[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) h[i] = s.bins[8 * lane + i];
-      // sums of shares in float, off by less than 2^-18
+      // Off by less than 2^-19: a share by four roundings of 2^-24 of it (histogram, factor, their product, itself), the sum
+      // up to a bin by some 20 of 2^-25.
       const float p = static_cast<float>(set.p);
       int lo = reach_bin(h, p - 0x1p-17f);
       int hi = reach_bin(h, p + 0x1p-17f);
