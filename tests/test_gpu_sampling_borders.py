@@ -1,12 +1,31 @@
-"""Borders of sampling that a rounding could move."""
+"""Borders of sampling that a rounding could move: where what is kept or drawn ends within 2^-30 of the total beside a token's edge.
+
+Rows of a few levels, each of many equal logits, so that every sum is a product: a level's tokens times their weight, off by a
+few 2^-53 of itself.  Borders are set on either side of an edge, further from it than 2^-40 of the total: the weights'
+series is off by 3e-13 (2^-41.6), sums by less."""
+
+import math
 
 import pytest
 import torch
 
 from test_gpu_sampling import _check
+from turboquant_pytorch import filter_probs, sample_tokens
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+
+
+def _near_edges(first, last, weight, total, least, most, count):
+    """(uniforms, tokens): u total lies `least` to `most` beside the edge between tokens j - 1 and j of a row that begins with
+    equal tokens; the draw is j where it lies behind the edge, else j - 1."""
+    j = torch.arange(first, last, dtype=torch.float64)
+    u = (j * weight / total).float()
+    off = u.double() * total - j * weight
+    take = torch.nonzero((off.abs() >= least) & (off.abs() <= most))[:, 0]
+    take = take[torch.randperm(len(take), generator=torch.Generator().manual_seed(1))[:count]]
+    assert len(take) == count and (off[take] > 0).any() and (off[take] < 0).any()
+    return u[take].to(DEV), (j[take].long() - (off[take] < 0).long()).to(DEV)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -35,3 +54,29 @@ def test_top_p_over_hundreds_of_chunks(light, p):
     print("case:", light, p, flush=True)
     probs, _ = _check(l, torch.full((1,), 0.999999, device=DEV), p=p)
     assert int((probs > 0).sum()) < V
+
+
+def test_draws_between_light_tokens_under_min_p():
+    n, at = 150000, -16.4716796875
+    w = math.exp(at)
+    u, want = _near_edges(60000, n, w, 1 + n * w, 4e-12, 1e-10, 48)
+    l = torch.full((1, n + 1), at, device=DEV)
+    l[0, n] = 0.0
+    assert torch.equal(sample_tokens(l.expand(48, -1), u, min_p=1e-8), want)
+    for i in range(4):  # a row by itself is cut into other chunks
+        assert torch.equal(sample_tokens(l, u[i:i + 1], min_p=1e-8), want[i:i + 1])
+
+
+@pytest.mark.parametrize("off", [2e-11, -2e-11])
+def test_top_p_ends_among_light_tokens_below_light_ones(off):
+    """60000 tokens that are kept for certain above the level in which the border lies."""
+    n, a, b = 60000, -11.0439453125, -11.2939453125
+    wa, wb = math.exp(a), math.exp(b)
+    l = torch.full((1, 2 * n + 1), a, device=DEV)
+    l[0, 1::2] = b
+    l[0, 7000] = 0.0  # in place of one of the upper level, which has n + 1 places
+    for j in (20000, 47000):
+        p = (1 + n * wa + j * wb + off) / (1 + n * wa + n * wb)
+        print("case:", j, p, flush=True)
+        probs = filter_probs(l, top_p=p)
+        assert int((probs > 0).sum()) == 1 + n + j + (off > 0)

@@ -37,7 +37,6 @@ constexpr int kMaxChunks = 1024;
 constexpr int kShort = 5120;  // tokens that are taken into shared memory
 constexpr int kRanked = 256;  // of them, tokens that are ranked one against the other
 constexpr int kFew = 1024;    // tokens down to the border that are listed with it
-constexpr double kUnit = 0x1p48;  // of a chunk's mass: at most 2^15 tokens of weight <= 1
 constexpr int kTiny = 49;         // a weight below 2^-49 is no unit
 
 enum Mode { kAll, kMinP, kTopP, kTopK };
@@ -495,8 +494,7 @@ struct SelectSmem {
   float factor[kMaxChunks];  // of a chunk's units: shares of the row's mass
   int off[kMaxChunks];       // its first bin among the row's
   int depth[kMaxChunks];
-  double total[kScanWaves];
-  uint64_t part[kScanWaves];
+  double total[kScanWaves], sum[kScanWaves];
   int listed, lo, hi;
 };
 
@@ -526,7 +524,10 @@ __global__ void __launch_bounds__(kScan) sample_select_kernel(SampleArgs a) {
   const Weigh weigh(set, mt);
   const double c2 = set.c, least = set.m;
   const int top = grid_of(mt);
-  uint64_t sum = 0, on = 0;
+  // Of what is kept for certain: in 64-bit floats, as rounded to 2^-48 of the maximum equal weights would all err to one
+  // side, 150000 tokens of 2^-24 by 2^-32 of the total.
+  double sum = 0.0;
+  uint64_t on = 0;
   if (mode == kMinP) {
     __syncthreads();
     const float x1 = mt - set.far, far = fmaxf(-3.4028235e38f, x1 - 2e-7f * (fabsf(mt) + fabsf(x1)));
@@ -537,8 +538,7 @@ __global__ void __launch_bounds__(kScan) sample_select_kernel(SampleArgs a) {
         if (__any(take)) {
           const double w = weigh(v[e]);
           take = take && w >= least;
-          const uint64_t n = units_of(w);
-          sum += !take ? 0 : n ? n : 1;
+          sum += take ? w : 0.0;
           on |= static_cast<uint64_t>(take) << (8 * r + e);
         }
       }
@@ -617,17 +617,17 @@ __global__ void __launch_bounds__(kScan) sample_select_kernel(SampleArgs a) {
         for (int e = 0; e < 8; ++e) {
           const bool certain = v[e] >= sure;
           if (__any(certain)) {
-            const uint64_t n = units_of(weigh(v[e]));
-            sum += certain ? n : 0;
+            const double w = weigh(v[e]);
+            sum += certain ? w : 0.0;
           }
           on |= static_cast<uint64_t>(v[e] >= edge && !certain) << (8 * r + e);
         }
       });
   }
   list_tokens<DT>(a, row, c, m, on, &s.listed);
-  sum = block_all<kScanWaves>(sum, s.part, Sum{});
+  sum = block_all<kScanWaves>(sum, s.sum, Sum{});
   if (tid == 0) {
-    a.kept[at] = static_cast<double>(sum) * (1.0 / kUnit);
+    a.kept[at] = sum;
     a.listed[at] = s.listed;
   }
 }
