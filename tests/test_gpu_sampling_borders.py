@@ -80,3 +80,15 @@ def test_top_p_ends_among_light_tokens_below_light_ones(off):
         print("case:", j, p, flush=True)
         probs = filter_probs(l, top_p=p)
         assert int((probs > 0).sum()) == 1 + n + j + (off > 0)
+
+
+@pytest.mark.parametrize("off", [3e-10, -3e-10])
+def test_top_p_counts_tokens_that_weigh_almost_nothing(off):
+    """A million tokens of 2^-49.1 each weigh 1.7e-9 together, beside 256 of weight 1 (2^-40 of the total is 2.3e-10)."""
+    V, at = 1 << 20, -34.0625
+    l = torch.full((1, V), at, device=DEV)
+    l[0, ::4096] = 0.0
+    for j in (150, 220):
+        p = (j + off) / (256 + (V - 256) * math.exp(at))
+        print("case:", j, p, flush=True)
+        assert int((filter_probs(l, top_p=p) > 0).sum()) == j + (off > 0)

@@ -37,7 +37,6 @@ constexpr int kMaxChunks = 1024;
 constexpr int kShort = 5120;  // tokens that are taken into shared memory
 constexpr int kRanked = 256;  // of them, tokens that are ranked one against the other
 constexpr int kFew = 1024;    // tokens down to the border that are listed with it
-constexpr int kTiny = 49;         // a weight below 2^-49 is no unit
 
 enum Mode { kAll, kMinP, kTopP, kTopK };
 
@@ -48,7 +47,7 @@ struct Settings {
   double low;   // a logit this far below the maximum weighs nothing (2^-1200)
   double p, m;
   float far;    // kept tokens' logits are down to this far from the maximum (top-p, min-p)
-  float tiny;   // weights are units down to this far
+  float tiny;   // what is further weighs less than 2^-46 of the maximum together (top-p)
 
   // t: NaN and what is not positive count as 0
   __host__ __device__ Settings(int V, double t, int k_, double p_, double m_) : k(k_), p(p_), m(m_) {
@@ -66,7 +65,7 @@ struct Settings {
     if (mode == kTopP) y = fmax(y, log2((1.0 - p) / V) - 1.0);
     const double d = (0.001 - y) / c;
     far = d < 3e38 ? static_cast<float>(d * 1.000001) : INFINITY;
-    const double z = (kTiny + 0.01) / c;
+    const double z = (46.01 + log2(static_cast<double>(V))) / c;
     tiny = z < 3e38 ? static_cast<float>(z * 1.000001) : INFINITY;
   }
 };
