@@ -92,3 +92,24 @@ def test_top_p_counts_tokens_that_weigh_almost_nothing(off):
         p = (j + off) / (256 + (V - 256) * math.exp(at))
         print("case:", j, p, flush=True)
         assert int((filter_probs(l, top_p=p) > 0).sum()) == j + (off > 0)
+
+
+@pytest.mark.parametrize("off", [1e-10, -1e-10])
+def test_top_p_of_many_ranked_tokens(off):
+    n, at = 100000, -11.494140625
+    w = math.exp(at)
+    l = torch.full((1, 150001), at, device=DEV)
+    l[0, 140000] = 0.0
+    for j in (30000, 50000):
+        p = (1 + j * w + off) / (1 + n * w)
+        probs = filter_probs(l, top_k=n + 1, top_p=p)
+        assert int((probs > 0).sum()) == 1 + j + (off > 0)
+
+
+def test_draws_between_many_ranked_tokens():
+    n, at = 100000, -11.494140625
+    w = math.exp(at)
+    u, want = _near_edges(20000, 90000, w, 1 + n * w, 2e-11, 4e-10, 16)
+    l = torch.full((1, 150001), at, device=DEV)
+    l[0, 150000] = 0.0
+    assert torch.equal(sample_tokens(l.expand(16, -1), u, top_k=n + 1), want)

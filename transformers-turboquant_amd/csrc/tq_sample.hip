@@ -10,9 +10,10 @@
 // w_0 + ... + w_x > u (the kept tokens' total).
 //
 // What is kept is decided by a comparison of sums over up to 10^5 terms, and a draw lies next to a border once
-// in a few thousand tokens if sums are off by 10^-7; so weights are float64 (2^f by its Taylor series, 2 10^-13), and
-// sums are float64 in a fixed order or integers, which have none (of n listed tokens in units of 2^-61 n of the heaviest: 4
-// 10^4 tokens' roundings add up to 2^-39 of it).
+// in a few thousand tokens if sums are off by 10^-7; so weights are float64 (2^f by its Taylor series, 3 10^-13, 2^-41.6), and
+// sums are float64 in a fixed order or integers, which have none (of listed tokens in units of at most 2^-62 of the total, each
+// off by less than a unit, so n of them by n 2^-62).  Both together: less than 2^-40 of the total for up to 2^20 tokens, 2^-37
+// for 2^24.
 //
 // A row is never sorted.  It is cut into chunks, one per block, and then finished by one block:
 //   scan     the chunk's maximum; without filters its mass; for top-p its mass, and a histogram of it over bins of
@@ -117,7 +118,7 @@ struct SampleArgs {
 };
 
 // Weights under a maximum: exp((v - top) / t) = 2^y as 2^n 2^f, n = rint(y): 2^f, |f| <= 1/2, by the series of
-// exp(f ln 2) up to the 10th power (2 10^-13).  Adding 1.5 2^52 leaves n in the low word.  -inf weighs 0.
+// exp(f ln 2) up to the 10th power (3 10^-13).  Adding 1.5 2^52 leaves n in the low word.  -inf weighs 0.
 struct Weigh {
   double top, c, low;  // top: of finite logits, or one that v is not above
   __device__ __forceinline__ Weigh(const Settings& set, float m) : top(m), c(set.c), low(set.low) {}
@@ -1145,17 +1146,29 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
       for (int c = 0; c < a.C; ++c) certain += s.mass[c];
     peak = block_all<kWaves>(peak, reinterpret_cast<float*>(s.part), Max{});
     __syncthreads();
-    // the heaviest is 2^(61 - bits of their number)
-    const double big = peak == -INFINITY ? 1.0 : weigh(peak);
-    unit = big > 0.0 ? ldexp(1.0, 30 + __builtin_clz(n | 1)) / big : 0.0;
-    if (!(unit < INFINITY)) unit = 0.0;
-    const double g = (goal - certain) * unit;
     const auto in = [&](float v) {
       const int b = bin_of(v, top);
       return b >= lo && b <= hi;
     };
     const auto mass = [&](float v) { return integer(weigh(v)); };
     const Taken taken{s, n};
+    // The unit has the total, the row's or the listed tokens', at 2^62 to 2^63 (of up to 2^24 integers, each less than one
+    // off): next to n times the heaviest, equal light tokens' roundings would add up, to 2^-29 of the total at 150000.
+    if (mode == kTopP) {
+      int bits;
+      frexp(cut.total, &bits);
+      unit = ldexp(1.0, 63 - bits);
+    } else if (mode == kTopK || alone) {  // the heaviest, of weight 1, is listed
+      unit = ldexp(1.0, 30 + __builtin_clz(n));
+      uint64_t sum = 0;
+      const auto add = [&](float v, int) { sum += in(v) ? mass(v) : 0; };
+      if (n <= kShort) taken.each(add);
+      else all.each(add);
+      sum = block_all<kWaves>(sum, s.part, Sum{});
+      __syncthreads();
+      unit = ldexp(unit, __builtin_clzll(sum + n) - 1);
+    }
+    const double g = (goal - certain) * unit;
     if (mode == kTopP && certain > 0.0 && !(g > 0.0)) {  // what is certain reaches the goal
       key = key_of(peak);
       last = -1;
@@ -1195,18 +1208,16 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a) {
     }
     // ---- the chunks' kept masses: what is certain, and the listed tokens up to the border
     if (mode != kMinP) {
-      const double fine = ldexp(1.0, 30 + __builtin_clz(a.V | 1)) / big;
-      const double units = fine < INFINITY ? fine : 0.0;
       all.each([&](float v, int x) {
         const uint32_t k = key_of(v);
         const int b = bin_of(v, top);
         if (b >= lo && b <= hi && (k > key || (k == key && x <= last))) {
           const double w = weigh(v);
-          if (w >= least) add_lds(s.extra + (x >> a.lg_chunk), max(static_cast<uint64_t>(w * units + 0.5), static_cast<uint64_t>(w > 0.0)));
+          if (w >= least) add_lds(s.extra + (x >> a.lg_chunk), integer(w));
         }
       });
       __syncthreads();
-      for (int c = tid; c < a.C; c += kThreads) s.mass[c] += units > 0.0 ? static_cast<double>(s.extra[c]) / units : 0.0;
+      for (int c = tid; c < a.C; c += kThreads) s.mass[c] += static_cast<double>(s.extra[c]) / unit;
       __syncthreads();
     }
   }

@@ -21,9 +21,9 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
     """A token of every row: int64 [...] from logits [..., V] and uniforms float32 [...] in [0, 1).
 
     The first token x, in index order, at which the kept tokens' weights up to x exceed the uniform times their
-    total; -1 for a row without a logit above -inf.  Weights are float64 (2e-13) and sums integers of 2^-45 of the
-    heaviest or finer: what is kept and drawn is that of the exact distribution, unless a border lies within 2^-38 of the
-    total of a token's edge, and a call gives the same tokens every time."""
+    total; -1 for a row without a logit above -inf.  Weights are float64 (3e-13), sums float64 or integers of 2^-62 of
+    the total: what is kept and drawn is that of the exact distribution, unless a border lies within 2^-40 of the total of a
+    token's edge (2^-37 for more than 2^20 tokens), and a call gives the same tokens every time."""
     if uniforms.shape != logits.shape[:-1]:
         raise ValueError(f"uniforms must be {list(logits.shape[:-1])}, one per row of the logits, got {list(uniforms.shape)}")
     settings = _settings(logits, temperature, top_k, top_p, min_p)
