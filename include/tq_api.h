@@ -475,8 +475,8 @@ int64_t tq_verify_workspace_size(int32_t B, int32_t V);
  * the tokens at it are equally likely.  A setting's array (one value per row, on the device) stands in
  * place of the number where it is not NULL; there temperatures <= 0 or NaN count as 0, top_k <= 0
  * as 0, top_p NaN as 1, min_p outside [0, 1] as its nearer end.  Weights and sums are float64 or 64-bit
- * integers: the same call gives the same tokens.  V <= 2^24; a 16-byte aligned workspace of
- * tq_sample_workspace_size bytes. */
+ * integers: the same call gives the same tokens.  V <= 2^24, N < 2^22 and fewer than 2^23 chunks of
+ * 2^15 tokens; a 16-byte aligned workspace of tq_sample_workspace_size bytes. */
 int tq_sample_tokens(const void* logits, int32_t dtype, int64_t ld, int32_t N, int32_t V,
                      const float* uniforms, const float* temperatures, double temperature,
                      const int32_t* top_ks, int32_t top_k, const float* top_ps, double top_p,

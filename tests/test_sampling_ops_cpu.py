@@ -87,3 +87,23 @@ def test_c_entries_refuse():
     assert lib.tq_filter_probs(16, 0, 10, 1, 10, none, 1.0, none, 0, none, 1.0, none, 0.0, none, 16, 1 << 30, none) == -1
     assert lib.tq_sample_workspace_size(0, 10) == 0 and lib.tq_sample_workspace_size(1, (1 << 24) + 1) == 0
     assert lib.tq_sample_workspace_size(1, 1) > 0
+
+
+@pytest.mark.parametrize("n,v,taken", [((1 << 22) - 1, 10, True), (1 << 22, 10, False), ((1 << 22) - 1, 1 << 15, True),
+                                       ((1 << 22) - 1, (1 << 15) + 1, True), ((1 << 22) - 1, (1 << 16) + 1, False),
+                                       (1 << 14, 1 << 24, False), ((1 << 14) - 1, 1 << 24, True), ((1 << 31) - 1, 1, False)])
+def test_no_more_rows_and_chunks_than_a_launch_has_threads_for(n, v, taken):
+    """A grid of HIP has fewer than 2^32 threads along x: 1024 work on a row, 512 on a chunk of 2^15 tokens."""
+    lib, none = _native.lib(), None
+    assert (lib.tq_sample_workspace_size(n, v) > 0) == taken
+    args = [dict(_args(True), logits=_e(n, v, dtype=torch.bfloat16), u=_e(n)), dict(_args(False), logits=_e(n, v, dtype=torch.bfloat16))]
+    for fn, a in zip((ops().sample_tokens, ops().filter_probs), args):
+        if taken:
+            assert fn(*a.values()).shape[0] == n
+        else:
+            with pytest.raises(RuntimeError, match="fewer than 2\\^22 rows"):
+                fn(*a.values())
+    if not taken:
+        for call in (lambda: lib.tq_sample_tokens(16, 0, v, n, v, 16, none, 1.0, none, 0, none, 1.0, none, 0.0, 16, 16, 1 << 50, none),
+                     lambda: lib.tq_filter_probs(16, 0, v, n, v, none, 1.0, none, 0, none, 1.0, none, 0.0, 16, 16, 1 << 50, none)):
+            assert call() == -1 and b"fewer than 2^22 rows" in lib.tq_last_error()

@@ -1422,8 +1422,10 @@ static SamplePlan plan_sample(int64_t N, int64_t V) {
   p.bytes = at;
   return p;
 }
+// A launch has fewer than 2^32 threads: kThreads to a row in the finish, kScan to a chunk in the scan
 static bool sample_shape(int64_t N, int64_t V) {
-  return N >= 1 && V >= 1 && V <= (int64_t(1) << 24) && N < (int64_t(1) << 31) && N * ((V + 2047) / 2048) < (int64_t(1) << 31);
+  return N >= 1 && V >= 1 && V <= (int64_t(1) << 24) && N < (int64_t(1) << 32) / kThreads &&
+         N * plan_sample(N, V).C < (int64_t(1) << 32) / kScan;
 }
 
 template <int DT>
@@ -1447,7 +1449,8 @@ static int run_sample(const char* what, SampleArgs& a, int32_t dtype, double tem
   TQ_REQUIRE(temperature >= 0.0 && top_k >= 0 && top_p >= 0.0 && min_p >= 0.0,
              "%s: temperature, top_k, top_p and min_p must not be negative", what);
   if (a.N == 0) return TQ_OK;
-  TQ_REQUIRE(sample_shape(a.N, a.V), "%s: at most 2^24 tokens and 2^31 tiles of 2048, got %d rows of %d", what, a.N, a.V);
+  TQ_REQUIRE(sample_shape(a.N, a.V), "%s: at most 2^24 tokens, fewer than 2^22 rows and 2^23 chunks of 2^15 tokens, got %d rows of %d",
+             what, a.N, a.V);
   TQ_REQUIRE(a.logits && (a.probs || (a.tokens && a.uniforms)), "%s: null pointer", what);
   const SamplePlan p = plan_sample(a.N, a.V);
   TQ_REQUIRE(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && bytes >= p.bytes,

@@ -1328,8 +1328,8 @@ void check_logits(const Checker& c, const Tensor& logits, const OptTensor& tempe
   TORCH_CHECK(logits.dim() == 2 && is_act(logits.scalar_type()), c.op, ": logits must be float32, float16 or bfloat16 [N, V], got ",
               logits.scalar_type(), " ", logits.sizes());
   const int64_t N = logits.size(0), V = logits.size(1);
-  TORCH_CHECK(V >= 1 && V <= (int64_t{1} << 24) && N < (int64_t{1} << 31) && N * ((V + 2047) / 2048) < (int64_t{1} << 31), c.op,
-              ": 1 to 2^24 tokens and fewer than 2^31 tiles of 2048, got ", logits.sizes());
+  TORCH_CHECK(V >= 1 && V <= (int64_t{1} << 24) && N < (int64_t{1} << 31) && (N == 0 || tq_sample_workspace_size(i32(N), i32(V)) > 0),
+              c.op, ": 1 to 2^24 tokens, fewer than 2^22 rows and 2^23 chunks of 2^15 tokens, got ", logits.sizes());
   TORCH_CHECK(V == 1 || logits.stride(1) == 1, c.op, ": logits must be contiguous along the vocabulary");
   check_setting(c, temperatures, "temperature", at::kFloat, N);
   check_setting(c, top_ks, "top_k", at::kInt, N);
