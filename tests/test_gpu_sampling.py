@@ -299,3 +299,15 @@ def test_top_p_keeps_no_more_of_equal_logits_than_top_k():
                 print("case:", V, step, k, p, flush=True)
                 _check(l, u, t=20.0, k=k, p=p)
                 _check(l.half(), u, t=3.0, k=k, p=p, m=1e-4)
+
+
+def test_logits_that_are_strided_along_the_vocabulary():
+    g = torch.Generator(device=DEV).manual_seed(71)
+    u = torch.rand(6, device=DEV, generator=g)
+    x = torch.randn(2006, 6, device=DEV, generator=g).to(torch.bfloat16)
+    for l in (x.t(), x.reshape(6, -1)[:, ::2], x.t().reshape(6, 1, -1)[..., ::3], x.reshape(1003, 2, 6).permute(2, 1, 0)):
+        v = u[:, None].expand(l.shape[:-1]) if l.dim() == 3 else u
+        assert l.stride(-1) != 1
+        for kw in (dict(top_k=9), dict(top_p=0.7)):
+            assert torch.equal(sample_tokens(l, v, **kw), sample_tokens(l.contiguous(), v, **kw))
+            assert torch.equal(filter_probs(l, **kw), filter_probs(l.contiguous(), **kw))

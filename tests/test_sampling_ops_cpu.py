@@ -107,3 +107,9 @@ def test_no_more_rows_and_chunks_than_a_launch_has_threads_for(n, v, taken):
         for call in (lambda: lib.tq_sample_tokens(16, 0, v, n, v, 16, none, 1.0, none, 0, none, 1.0, none, 0.0, 16, 16, 1 << 50, none),
                      lambda: lib.tq_filter_probs(16, 0, v, n, v, none, 1.0, none, 0, none, 1.0, none, 0.0, 16, 16, 1 << 50, none)):
             assert call() == -1 and b"fewer than 2^22 rows" in lib.tq_last_error()
+
+
+def test_logits_that_are_strided_along_the_vocabulary():
+    for x in (_e(V, N).t(), _e(N, 2 * V)[:, ::2], _e(N, 1, 3 * V)[..., ::3], _e(V, 2, N).permute(2, 1, 0)):
+        assert sample_tokens(x, _e(*x.shape[:-1]), top_k=3).shape == x.shape[:-1]
+        assert filter_probs(x, top_p=0.5).shape == x.shape

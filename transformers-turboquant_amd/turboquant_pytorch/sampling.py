@@ -28,18 +28,22 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
         raise ValueError(f"uniforms must be {list(logits.shape[:-1])}, one per row of the logits, got {list(uniforms.shape)}")
     settings = _settings(logits, temperature, top_k, top_p, min_p)
     if logits.dim() == 2:
-        return ops().sample_tokens(logits, uniforms.contiguous(), *settings)
-    rows = logits.reshape(-1, logits.shape[-1])
-    return ops().sample_tokens(rows, uniforms.reshape(-1).contiguous(), *settings).reshape(logits.shape[:-1])
+        return ops().sample_tokens(_rows(logits), uniforms.contiguous(), *settings)
+    return ops().sample_tokens(_rows(logits), uniforms.reshape(-1).contiguous(), *settings).reshape(logits.shape[:-1])
 
 
 def filter_probs(logits: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> torch.Tensor:
     """The distributions that `sample_tokens` draws from, float32 [..., V]: zero where a token is not kept (a whole
     row of zeros where no logit is above -inf).  `verify_drafts` takes them as target or draft probabilities."""
     settings = _settings(logits, temperature, top_k, top_p, min_p)
-    if logits.dim() == 2:
-        return ops().filter_probs(logits, *settings)
-    return ops().filter_probs(logits.reshape(-1, logits.shape[-1]), *settings).reshape(logits.shape)
+    probs = ops().filter_probs(_rows(logits), *settings)
+    return probs if logits.dim() == 2 else probs.reshape(logits.shape)
+
+
+def _rows(logits):
+    """Logits as [N, V], copied where they are strided along the vocabulary."""
+    rows = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
+    return rows if rows.stride(1) == 1 else rows.contiguous()
 
 
 def _settings(logits, temperature, top_k, top_p, min_p):
