@@ -422,10 +422,13 @@ int64_t tq_tree_workspace_size(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, in
 
 /* tq_tree_attention of sequences that share their first positions.  groups [B, 2] (int32, on the
  * device): sequences that follow one another with the same groups[b][0] >= 0 and the same
- * groups[b][1] have positions [0, groups[b][1]) in common, the same rows; they are read through the
- * table row of the first of these sequences that has a length, once for all of them (up to the last
- * multiple of 32 positions; a batch is cut at every 64th sequence).  A sequence with a negative groups[b][0] or without shared
- * positions is attended alone; one that is shorter than its shared positions gets zeros.  Otherwise as
+ * groups[b][1] have positions [0, groups[b][1]) in common, the same rows.  The table row of every one
+ * of them that has a length holds pages with these rows: which of the table rows a shared position is
+ * read through depends on the shape (that of the first such sequence, for 16 or 32 query columns of
+ * the group at a time, up to the last multiple of 32 positions and cut at every 64th sequence; or each
+ * sequence's own).  Without a length a sequence's table row may hold anything.  A sequence with a
+ * negative groups[b][0] or without shared positions is attended alone; one that is shorter than its
+ * shared positions gets zeros.  Otherwise as
  * tq_tree_attention, with a workspace of tq_prefix_workspace_size bytes. */
 int tq_prefix_attention(const uint16_t* q_rot, const float* q_proj, const uint8_t* key_codes,
                         const uint8_t* key_signs, const uint16_t* key_rn, const uint16_t* key_vn,

@@ -5,8 +5,8 @@
 // the same shared have positions [0, shared) in common.  The softmax over a sequence's keys is that over its parts,
 // joined by their maxima and sums:
 //   m = max(m1, m2), l = l1 2^(m1 - m) + l2 2^(m2 - m), O = O1 2^(m1 - m) + O2 2^(m2 - m),
-// so the shared rows are read and decoded once for all queries of the group (rows x T x G columns of a kv
-// head), and each sequence's own rows for its T x G.
+// so the shared rows are read and decoded for 16 or 32 columns of the group at a time (it has rows x T x G of a kv head;
+// another tile of them decodes them again), and each sequence's own rows for its T x G.
 //
 // The work is a list of segments: a group's shared keys against a tile of 16 NTP of its columns, a
 // sequence's own keys against a tile of 16 NTO of its own.  As in tree attention their rounds (32 keys per wave of
@@ -171,7 +171,8 @@ struct PrefixSplit {
 
 // ---------------------------------------------------------------- attention
 // A part is worked on as by tree attention (tree_part): a wave builds the matrix operands of 32 keys once and uses them for
-// 16 NTP columns, which here belong to several sequences.
+// 16 NTP columns, which here belong to several sequences.  As there, weights times value norms and the value centroids (scaled
+// so that they lose least) are f16 and sums f32: 1.0 to 1.6e-4 of an output's norm from float64, before its own rounding.
 // 16 sequences of 32000 shared positions and 700 of their own, 32/8 heads, 3 bits (32 MB; 12.8 GFLOP, 11 us at a large library
 // product's rate): 38 us under a kernel trace, 49 the call with preparation (6) and merge (8).  Neither memory nor the matrix
 // unit ends it: of 76k cycles the VALU issues in 33k and the matrix unit is busy in 17k, over the two waves per
@@ -369,10 +370,12 @@ static PrefixPlan plan_prefix(int B, int Hq, int Hkv, int T, int64_t maxpos, int
   const int res = resident_blocks(reinterpret_cast<const void*>(p.attend), 256,
                                   resident[d == 128][bits - 2][p.tiles + p.own_tiles - 2]);
   // Sharing saves the reading of keys and columns that are idle in tree attention's tiles.  Where neither counts it
-  // is left out: a sequence's columns fill its two tiles (the matrix products bound both; 8 trees of 8 nodes on
-  // 16k shared keys, 32/8 heads, 79 us with tree attention against 80, 16 trees of 16 nodes 190 against 220; 7 nodes
-  // 120 against 115), or a block of the device has no more than one round to do (4 sequences of 1k, 12 heads of 64, 16.9
-  // against 20.8 us; 16 of 128, 32/8 heads, 20.0 against 24.3; 4 of 2k, 544 rounds to 512 blocks, 24.6 against 23.7).
+  // is left out: a sequence's columns fill its two tiles, which decode the keys for themselves either way (8 trees of 8 nodes on
+  // 16k shared keys, 32/8 heads, 79 us with tree attention against 80, no difference; 16 trees of 16 nodes 190 against 220; 7
+  // nodes, 28 columns, 120 against 115; other numbers of full tiles are not measured), or a block of the device has no more
+  // than one round to do (4 sequences of 1k, 12 heads of 64, 16.9 against 20.8 us; 16 of 128, 32/8 heads, 20.0 against 24.3;
+  // 4 of 2k, 544 rounds to 512 blocks, 24.6 against 23.7).  The rounds are those of full tables, as lengths are the device's: short
+  // sequences over tables of many more entries take the slower form.
   p.apart = C % 32 == 0 || rounds_of(32) <= res;
   if (p.apart) {
     p.bytes = tree_workspace(B, Hq, Hkv, T, maxpos, d, bits);

@@ -19,7 +19,10 @@
 //   scan     the chunk's maximum; without filters its mass; for top-p its mass, and a histogram of it over bins of
 //            1/16 below the maximum, as far down as tokens can be kept (all those of weight below (1 - p) / V of the
 //            largest together weigh less than (1 - p) of the total, so p of it stands before them); for
-//            top-k a list of the tokens down to the bin that k threads' own maxima reach
+//            top-k a list of the tokens down to the bin that k threads' own maxima reach.  From k = 513 on, a block having 512
+//            threads, and from about 460 on in chunks of 4096 that is every token: the list, of a quarter of the chunk, does not hold
+//            them, and the finish reads the row again (64 rows of 128256: k 50 16.6 us, 400 30, 512 74, 1000 92, 20000
+//            325; one row: 400 42, 500 100)
 //   select   (top-p, min-p) finds the bins that hold the row's border in the joined histograms, and lists what is
 //            kept (min-p), the tokens down to the border if they are few, or else those of its bins alone, with the
 //            mass of what is kept for certain above them
@@ -1392,7 +1395,8 @@ struct SamplePlan {
   int64_t rows, state, cut, top, mass, kept, listed, depth, hist, list, bytes;  // offsets
 };
 
-// The chunks of a row, and the workspace.
+// The chunks of a row, and the workspace: whatever the settings, which may be the rows' own, 2 bytes a token for lists and 2 KB
+// a chunk for its histogram.
 static SamplePlan plan_sample(int64_t N, int64_t V) {
   SamplePlan p{};
   p.lg_chunk = 15;

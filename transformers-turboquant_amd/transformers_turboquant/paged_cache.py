@@ -7,7 +7,7 @@ Where :class:`TurboQuantCache` holds capacity planes of one length for a whole b
   rows are;
 * a fork (``fork``, beam search's ``reorder_cache``) shares its pages with the sequence it came from; a
   shared page is copied before a position in it is written; with ``shared_prefix=True`` attention reads the pages
-  that active sequences next to one another share once for all of them;
+  that active sequences next to one another share for several of them together;
 * drafted tokens (``draft``) are appended as a tree that is not part of the text yet; after verification
   ``accept`` keeps one path of it, moved down behind the cached positions, and frees the rest.
 

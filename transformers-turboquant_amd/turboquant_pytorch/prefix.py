@@ -1,8 +1,8 @@
 """Attention of sequences that share a long prefix, over pages of a compressed cache.
 
-Sequences that were forked from one prompt have the prompt's pages in common.  Tree attention reads them once per
-sequence; the operators here once for all sequences of a group: the shared positions against the queries of the
-whole group, each sequence's own positions against its own, and both joined.  No counterpart in the
+Sequences that were forked from one prompt have the prompt's pages in common.  Tree attention reads them for every
+sequence; the operators here for up to 32 query columns of a group at a time: the shared positions against the queries of
+several sequences, each sequence's own positions against its own, and both joined.  No counterpart in the
 reference, which keeps no cache between steps (patch.py:81).
 """
 
@@ -38,9 +38,10 @@ def prefix_attention(queries: torch.Tensor, key_compressor: TurboQuantCompressor
 
     groups int32 [B, 2] on the GPU: sequences that follow one another with the same id ``groups[b, 0] >= 0`` and
     the same ``groups[b, 1]`` have the rows of positions ``[0, groups[b, 1])`` in common (`prefix_groups` makes it); an id of
-    -1 or 0 shared positions: alone.  The shared rows are read through the block table of the group's first sequence
-    that has a length, whole slabs of 32 positions of them once for all its sequences (64 at most: a batch is cut at every
-    64th sequence).  A sequence shorter than what it shares gets zeros, as one without room for its tokens does."""
+    -1 or 0 shared positions: alone.  The table row of every sequence of a group that has a length holds pages with the
+    shared rows; through which of these table rows they are read depends on the shape.  Whole slabs of 32 shared positions are
+    read for several sequences together (64 at most: a batch is cut at every 64th sequence).  A sequence shorter than what it
+    shares gets zeros, as one without room for its tokens does."""
     tk, tv = _both_tables(key_compressor, val_compressor, queries.device)
     args = _tree_args(tk, tv, queries.shape[-1], key_compressor, val_compressor, pool, layer, block_table, lengths, parents,
                       scale, out_dtype or queries.dtype)

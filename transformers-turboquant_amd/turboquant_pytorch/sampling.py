@@ -23,7 +23,8 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
     The first token x, in index order, at which the kept tokens' weights up to x exceed the uniform times their
     total; -1 for a row without a logit above -inf.  Weights are float64 (3e-13), sums float64 or integers of 2^-62 of
     the total: what is kept and drawn is that of the exact distribution, unless a border lies within 2^-40 of the total of a
-    token's edge (2^-37 for more than 2^20 tokens), and a call gives the same tokens every time."""
+    token's edge (2^-37 for more than 2^20 tokens) or min_p within 3e-13 of a weight, and a call gives the same tokens every
+    time."""
     if uniforms.shape != logits.shape[:-1]:
         raise ValueError(f"uniforms must be {list(logits.shape[:-1])}, one per row of the logits, got {list(uniforms.shape)}")
     settings = _settings(logits, temperature, top_k, top_p, min_p)
