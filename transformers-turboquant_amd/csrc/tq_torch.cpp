@@ -1152,12 +1152,13 @@ Tensor prefix_attend(const Tensor& q, const Tensor& pi_split, const Tensor& s_ef
 
 // A layer's decoding or speculation step in one call: the new tokens' keys and values compressed into
 // their pages (positions lengths[b] + i) and the queries prepared in one launch, then tree attention.
-Tensor append_attend_meta(const char* op, const Tensor& k, const Tensor& v, const Tensor& q, const Tensor& kpi, const Tensor& kseff,
-                        const Tensor& kcent, const Tensor& kbounds, const Tensor& vpi, const Tensor& vbounds,
-                        const Tensor& kseff16, const Tensor& kcodes, const Tensor& ksigns, const Tensor& krn,
-                        const Tensor& kvn, const Tensor& kcent16, int64_t bits, const Tensor& vcodes, const Tensor& vvn,
-                        const Tensor& vcent32, const Tensor& vpit, const Tensor& table, const Tensor& lengths,
-                          const Tensor* groups, const c10::optional<Tensor>& parents, at::ScalarType out_dtype) {
+Tensor append_attend_meta(const char* op, const Tensor& k, const Tensor& v, const Tensor& q, const Tensor& kpi,
+                          const Tensor& kseff, const Tensor& kcent, const Tensor& kbounds, const Tensor& vpi,
+                          const Tensor& vbounds, const Tensor& kseff16, const Tensor& kcodes, const Tensor& ksigns,
+                          const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits, const Tensor& vcodes,
+                          const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit, const Tensor& table,
+                          const Tensor& lengths, const Tensor* groups, const c10::optional<Tensor>& parents,
+                          at::ScalarType out_dtype) {
   const Checker c{op, q.device()};
   Pool pool{&kcodes, &ksigns, &krn, &kvn, &vcodes, &vvn};
   Tensor out = check_tree(c, q, pool, kcent16, bits, vcent32, vpit, table, lengths, parents, out_dtype);
@@ -1179,14 +1180,15 @@ Tensor append_attend_meta(const char* op, const Tensor& k, const Tensor& v, cons
   return out;
 }
 
-Tensor append_attend(const char* op, const Tensor& k_in, const Tensor& v_in, const Tensor& q_in, const Tensor& kpi, const Tensor& kseff,
-                   const Tensor& kcent, const Tensor& kbounds, const Tensor& vpi, const Tensor& vbounds,
-                   const Tensor& kseff16, const Tensor& kcodes, const Tensor& ksigns, const Tensor& krn, const Tensor& kvn,
-                   const Tensor& kcent16, int64_t bits, const Tensor& vcodes, const Tensor& vvn, const Tensor& vcent32,
-                   const Tensor& vpit, const Tensor& table, const Tensor& lengths, const Tensor* groups,
-                     const c10::optional<Tensor>& parents, double coeff, double scale, at::ScalarType out_dtype) {
-  Tensor out = append_attend_meta(op, k_in, v_in, q_in, kpi, kseff, kcent, kbounds, vpi, vbounds, kseff16, kcodes, ksigns, krn, kvn,
-                                kcent16, bits, vcodes, vvn, vcent32, vpit, table, lengths, groups, parents, out_dtype);
+Tensor append_attend(const char* op, const Tensor& k_in, const Tensor& v_in, const Tensor& q_in, const Tensor& kpi,
+                     const Tensor& kseff, const Tensor& kcent, const Tensor& kbounds, const Tensor& vpi,
+                     const Tensor& vbounds, const Tensor& kseff16, const Tensor& kcodes, const Tensor& ksigns,
+                     const Tensor& krn, const Tensor& kvn, const Tensor& kcent16, int64_t bits, const Tensor& vcodes,
+                     const Tensor& vvn, const Tensor& vcent32, const Tensor& vpit, const Tensor& table,
+                     const Tensor& lengths, const Tensor* groups, const c10::optional<Tensor>& parents, double coeff,
+                     double scale, at::ScalarType out_dtype) {
+  Tensor out = append_attend_meta(op, k_in, v_in, q_in, kpi, kseff, kcent, kbounds, vpi, vbounds, kseff16, kcodes, ksigns, krn,
+                                  kvn, kcent16, bits, vcodes, vvn, vcent32, vpit, table, lengths, groups, parents, out_dtype);
   const c10::DeviceGuard g(q_in.device());
   Tensor k = activation(k_in), v = activation(v_in), q = activation(q_in);
   if (v.scalar_type() != k.scalar_type() || q.scalar_type() != k.scalar_type()) {

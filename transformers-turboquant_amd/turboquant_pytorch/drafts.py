@@ -66,7 +66,8 @@ def _both_tables(key_compressor, val_compressor, dev):
     return _tables(key_compressor, dev, with_qjl=True), _tables(val_compressor, dev, with_qjl=False)
 
 
-def _tree_args(tk, tv, D, key_compressor, val_compressor, pool, layer, block_table, lengths, parents, scale, out_dtype):
+def _tree_args(tk, tv, D, key_compressor, val_compressor, pool, layer, block_table, lengths, parents, scale, out_dtype, groups=()):
+    """Operands from the pool's planes on; groups: (the groups,) of sequences that share their first positions."""
     if key_compressor.S.shape[0] != D:
         raise ValueError("tree attention needs a square QJL matrix")
     if val_compressor.bits != key_compressor.mse_bits + 1:
@@ -77,7 +78,7 @@ def _tree_args(tk, tv, D, key_compressor, val_compressor, pool, layer, block_tab
     if out_dtype not in (torch.float32, torch.float16, torch.bfloat16):
         out_dtype = torch.float32
     return (kcodes, ksigns, krn, kvn, tk.cent16, val_compressor.bits, vcodes, vvn, vcent, vpit, block_table,
-            lengths, parents, math.sqrt(math.pi / 2) / key_compressor.S.shape[0],
+            lengths, *groups, parents, math.sqrt(math.pi / 2) / key_compressor.S.shape[0],
             float(scale if scale is not None else 1.0 / math.sqrt(D)), out_dtype)
 
 

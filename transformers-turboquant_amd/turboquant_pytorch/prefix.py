@@ -44,8 +44,8 @@ def prefix_attention(queries: torch.Tensor, key_compressor: TurboQuantCompressor
     shares gets zeros, as one without room for its tokens does."""
     tk, tv = _both_tables(key_compressor, val_compressor, queries.device)
     args = _tree_args(tk, tv, queries.shape[-1], key_compressor, val_compressor, pool, layer, block_table, lengths, parents,
-                      scale, out_dtype or queries.dtype)
-    return ops().prefix_attend(queries, tk.pi_split, tk.s_eff16, *_with_groups(args, groups))
+                      scale, out_dtype or queries.dtype, (groups,))
+    return ops().prefix_attend(queries, tk.pi_split, tk.s_eff16, *args)
 
 
 def append_prefix_attention(k: torch.Tensor, v: torch.Tensor, queries: torch.Tensor, key_compressor, val_compressor,
@@ -56,12 +56,6 @@ def append_prefix_attention(k: torch.Tensor, v: torch.Tensor, queries: torch.Ten
     [B, Hkv, T, D] into their pages (positions ``lengths[b] + i``, none of them shared), then prefix_attention."""
     tk, tv = _both_tables(key_compressor, val_compressor, queries.device)
     args = _tree_args(tk, tv, queries.shape[-1], key_compressor, val_compressor, pool, layer, block_table, lengths, parents,
-                      scale, out_dtype or queries.dtype)
+                      scale, out_dtype or queries.dtype, (groups,))
     return ops().prefix_page_attend(k, v, queries, tk.pi_split, tk.seff_split, tk.cent32, tk.bounds32, tv.pi_split,
-                                    tv.bounds32, tk.s_eff16, *_with_groups(args, groups))
-
-
-def _with_groups(args: tuple, groups: torch.Tensor) -> tuple:
-    """The operands of tree attention with the groups behind the lengths."""
-    at = len(args) - 4  # parents, coeff, scale, out_dtype
-    return (*args[:at], groups, *args[at:])
+                                    tv.bounds32, tk.s_eff16, *args)
